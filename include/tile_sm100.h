@@ -45,7 +45,8 @@ enum {
 enum {
   TSM100_F32 = 0,
   TSM100_F16 = 1,
-  TSM100_BF16 = 2
+  TSM100_BF16 = 2,
+  TSM100_I8 = 3 /* whole numbers -127 .. 127 with an f32 step per row; only where an operator says so */
 };
 
 typedef struct tsm100_device_s* tsm100_device_t; /* opaque */
@@ -75,7 +76,8 @@ int32_t tsm100_mem_info(tsm100_device_t dev, size_t* free_bytes, size_t* total_b
 int32_t tsm100_device_sm_count(tsm100_device_t dev, int32_t* sms);
 /* Synchronises `stream`, then reads and clears the device's kernel status word:
  * 0, or 0x1000|site when a kernel gave up one of its bounded waits (mbarrier,
- * tensor-core completion); a site number belongs to one kernel source file.  The reference has no device-side error channel;
+ * tensor-core completion), 0x2000|site when one met a page, a position or a sequence outside
+ * what its call described (tsm100_paged_batch); a site number belongs to one kernel source file.  The reference has no device-side error channel;
  * check_cu (crates/tile_hal/src/cuda.rs:124-130) sees driver codes only. */
 int32_t tsm100_device_status(tsm100_device_t dev, void* stream, uint32_t* status);
 
@@ -364,6 +366,94 @@ typedef struct {
 } tsm100_attention_decode_desc;
 int32_t tsm100_attention_decode(tsm100_device_t dev, const tsm100_attention_decode_desc* desc, const void* q,
                                 const void* k_cache, const void* v_cache, void* o, void* stream);
+
+/* ---- serving: residual norm, 4-bit weights, paged KV cache -------------- */
+/* The steps of a decoder layer around the intrinsics above; none has a counterpart in the
+ * reference, whose norm, matmul and KV cache (tile.rs:2063, :192-193, :2113-2136) these go beside.
+ *
+ * Values in 8 bits are whole numbers q in -127 .. 127 with an f32 step per row, x ~ q * step: step =
+ * max|x| / 127, q = x / step rounded to nearest even; a row of zeros has step 0. */
+
+/* RMS normalisation with the residual's addition, a weight, and an output in storage type or 8 bits:
+ *   h = x + residual;  sum = h;  y[r,c] = h[r,c] * rsqrt(mean_c(h[r,:]^2) + eps) * weight[c]
+ * in f32, each result rounded once (the norm goes on with the unrounded h).  residual, sum and weight may be
+ * NULL (no addition; h not kept; all ones).  sum may be x or residual, y may be x or residual unless sum is the same buffer;
+ * no other overlap.  out_dtype TSM100_I8: y holds whole numbers and
+ * scales[rows] their steps.  The numbers are taken from h * weight before the common factor of the row,
+ * so they do not depend on the order in which the squares are summed.  Rows are packed and may start anywhere. */
+typedef struct {
+  int32_t dtype;     /* of x, residual, sum and weight: TSM100_F32 | TSM100_F16 | TSM100_BF16 */
+  int32_t out_dtype; /* of y: dtype | TSM100_I8 */
+  int64_t rows;
+  int64_t cols;
+  float eps;
+} tsm100_add_rms_norm_desc;
+int32_t tsm100_add_rms_norm(tsm100_device_t dev, const tsm100_add_rms_norm_desc* desc, const void* x, const void* residual, void* sum,
+                            const void* weight, void* y, float* scales, void* stream);
+
+/* Product with 4-bit weights, C[M,N] = A[M,K] * W^T, W[n,k] = (q[n,k] - zero[n, k/group]) * w_scales[n, k/group]:
+ * w is [N][K/2] bytes, the even k in the low half; w_scales [N][K/group] of type dtype; w_zeros [N][K/group] bytes (0 .. 15), or
+ * NULL for 8 everywhere.  A is of type dtype, or TSM100_I8 with the steps of its rows in a_scales[M] (what
+ * tsm100_add_rms_norm leaves).  C is of type dtype.  Products are exact, sums f32, C is rounded once, up to 64 rows; with
+ * more rows the weights times their scales are rounded to dtype once each, for the tensor-core GEMM. */
+typedef struct {
+  int32_t dtype;   /* of w_scales, C, and A unless a_dtype says otherwise: TSM100_F16 | TSM100_BF16 */
+  int32_t a_dtype; /* dtype | TSM100_I8 */
+  int32_t group;   /* 32 | 64 | 128; K is a multiple of it */
+  int64_t m, n, k;
+} tsm100_gemm_w4_desc;
+int32_t tsm100_gemm_w4(tsm100_device_t dev, const tsm100_gemm_w4_desc* desc, const void* a, const float* a_scales, const uint8_t* w,
+                       const void* w_scales, const uint8_t* w_zeros, void* c, void* stream);
+
+/* A KV cache in pages: k, v are [pages][heads_kv][page_size][head_dim], with dtype TSM100_I8 the steps of the rows in
+ * k_scales, v_scales [pages][heads_kv][page_size] (else NULL). */
+typedef struct {
+  int32_t dtype; /* TSM100_F16 | TSM100_BF16 | TSM100_I8 */
+  int32_t heads_kv;
+  int32_t head_dim;  /* a multiple of 16, up to 256 */
+  int32_t page_size; /* positions of a page, 1 .. 4096 */
+  int64_t pages;
+  void* k;
+  void* v;
+  float* k_scales;
+  float* v_scales;
+} tsm100_paged_kv;
+
+/* Sequences of uneven length, side by side: tokens starts[b] .. starts[b+1]-1 of the call are the last ones of sequence b, which has
+ * lens[b] positions with them; position p of it lies in page table[b][p / page_size].  The arrays are in device memory and are read when the call's
+ * kernels run.  A table entry outside 0 .. pages-1, a position outside the table's row, a sequence with more than
+ * max_new tokens, or more tokens than positions, is left out (nothing is read or written for it) and reported by the next
+ * tsm100_stream_synchronize as TSM100_ERR_INVALID (status 0x2000|site).  Tokens from starts[batch] on belong to no sequence and are left alone. */
+typedef struct {
+  int32_t batch;
+  int32_t tokens;      /* of the call: rows of its token-major arrays, starts[batch] or more */
+  int32_t max_new;     /* no sequence has more tokens in this call */
+  int32_t max_len;     /* how long sequences get, for planning; 0: as long as the table's rows allow */
+  int32_t table_pitch; /* entries of a row of the table */
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* starts; /* batch + 1 */
+} tsm100_paged_batch;
+
+/* Writes new tokens into the pages: position p of head h, k and v being [tokens][heads_kv][head_dim] of type dtype (F16 | BF16).  A cache of 16
+ * bits has the same type and gets the same bits; TSM100_I8 is quantised row by row on the way. */
+int32_t tsm100_kv_page_append(tsm100_device_t dev, const tsm100_paged_kv* kv, const tsm100_paged_batch* batch, int32_t dtype, const void* k,
+                              const void* v, void* stream);
+/* The other way: the tokens of the call read back from the pages into k, v [tokens][heads_kv][head_dim]; q * step rounded to dtype.  With
+ * starts counting all positions (starts[b+1] - starts[b] = lens[b]) whole sequences come out. */
+int32_t tsm100_kv_page_read(tsm100_device_t dev, const tsm100_paged_kv* kv, const tsm100_paged_batch* batch, int32_t dtype, void* k, void* v,
+                            void* stream);
+
+/* Attention of the call's tokens, already appended, over their sequences' pages: a token at position p sees positions 0 .. p,
+ *   o[t,h,:] = softmax_j(q[t,h,:] . K[j,g,:] / sqrt(d)) V[j,g,:],  j <= p,  g = h / (heads_q / heads_kv).
+ * q, o are token-major [tokens][heads_q][head_dim] of type dtype; a cache of 16 bits has the same type.  Positions a sequence does not
+ * have are never used, whatever the page holds there.  head_dim 64 or 128; buffers 16-byte aligned. */
+typedef struct {
+  int32_t dtype; /* TSM100_F16 | TSM100_BF16 */
+  int32_t heads_q;
+} tsm100_attention_paged_desc;
+int32_t tsm100_attention_paged(tsm100_device_t dev, const tsm100_paged_kv* kv, const tsm100_paged_batch* batch,
+                               const tsm100_attention_paged_desc* desc, const void* q, void* o, void* stream);
 
 /* The path a tile_hal host program takes per kernel: alloc_from_slice ->
  * launch -> copy_to_host (crates/tile_hal/src/cuda.rs:348-371, :245-288,

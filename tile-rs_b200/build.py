@@ -25,7 +25,7 @@ LIB_PATH = PKG_DIR / "libtile_sm100.so"
 # the operators for CPython without ctypes (csrc/python.cpp); absent where there are no CPython headers
 FAST_PATH = PKG_DIR / ("_tile_sm100" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
-CUDA_SOURCES = ["runtime.cu", "capi_ops.cu", "multi.cu"]
+CUDA_SOURCES = ["runtime.cu", "capi_ops.cu", "serving.cu", "multi.cu"]
 CXX_SOURCES = ["inputs.cpp", "emit.cpp"]
 
 NVCC_FLAGS = [

@@ -15,8 +15,8 @@ from . import build as _build
 
 OK, ERR_INVALID, ERR_NO_DEVICE, ERR_MEMORY, ERR_LAUNCH = 0, 1, 2, 3, 4
 ERR_STREAM, ERR_RUNTIME, ERR_TIMEOUT, ERR_BUFFER, ERR_EMIT = 5, 6, 7, 8, 9
-F32, F16, BF16 = 0, 1, 2
-DTYPE_SIZE = {F32: 4, F16: 2, BF16: 2}
+F32, F16, BF16, I8 = 0, 1, 2, 3
+DTYPE_SIZE = {F32: 4, F16: 2, BF16: 2, I8: 1}
 
 c_i32, c_i64, c_u32, c_u64, c_sz, c_vp = C.c_int32, C.c_int64, C.c_uint32, C.c_uint64, C.c_size_t, C.c_void_p
 
@@ -68,6 +68,28 @@ class AttentionDecodeDesc(C.Structure):
 class AttentionDesc(C.Structure):
     _fields_ = [("dtype", c_i32), ("causal", c_i32), ("batch", c_i32), ("heads_q", c_i32),
                 ("heads_kv", c_i32), ("seq", c_i32), ("head_dim", c_i32)]
+
+
+class AddRmsNormDesc(C.Structure):
+    _fields_ = [("dtype", c_i32), ("out_dtype", c_i32), ("rows", c_i64), ("cols", c_i64), ("eps", C.c_float)]
+
+
+class GemmW4Desc(C.Structure):
+    _fields_ = [("dtype", c_i32), ("a_dtype", c_i32), ("group", c_i32), ("m", c_i64), ("n", c_i64), ("k", c_i64)]
+
+
+class PagedKv(C.Structure):
+    _fields_ = [("dtype", c_i32), ("heads_kv", c_i32), ("head_dim", c_i32), ("page_size", c_i32), ("pages", c_i64), ("k", c_vp), ("v", c_vp),
+                ("k_scales", c_vp), ("v_scales", c_vp)]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [("batch", c_i32), ("tokens", c_i32), ("max_new", c_i32), ("max_len", c_i32), ("table_pitch", c_i32), ("table", c_vp), ("lens", c_vp),
+                ("starts", c_vp)]
+
+
+class AttentionPagedDesc(C.Structure):
+    _fields_ = [("dtype", c_i32), ("heads_q", c_i32)]
 
 
 OP_SOFTMAX, OP_GEMM, OP_ATTENTION = 0, 1, 2
@@ -129,6 +151,11 @@ PROTOTYPES = {
     "tsm100_kv_cache_update": (c_i32, [c_vp, P(KvCacheUpdateDesc), c_vp, c_vp, c_vp]),
     "tsm100_attention_prefill": (c_i32, [c_vp, P(AttentionPrefillDesc), c_vp, c_vp, c_vp, c_vp, c_vp]),
     "tsm100_attention_decode": (c_i32, [c_vp, P(AttentionDecodeDesc), c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "tsm100_add_rms_norm": (c_i32, [c_vp, P(AddRmsNormDesc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "tsm100_gemm_w4": (c_i32, [c_vp, P(GemmW4Desc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "tsm100_kv_page_append": (c_i32, [c_vp, P(PagedKv), P(PagedBatch), c_i32, c_vp, c_vp, c_vp]),
+    "tsm100_kv_page_read": (c_i32, [c_vp, P(PagedKv), P(PagedBatch), c_i32, c_vp, c_vp, c_vp]),
+    "tsm100_attention_paged": (c_i32, [c_vp, P(PagedKv), P(PagedBatch), P(AttentionPagedDesc), c_vp, c_vp, c_vp]),
     "tsm100_softmax_host": (c_i32, [c_vp, P(SoftmaxDesc), c_vp, c_vp]),
     "tsm100_gemm_host": (c_i32, [c_vp, P(GemmDesc), c_vp, c_vp, c_vp]),
     "tsm100_attention_host": (c_i32, [c_vp, P(AttentionDesc), c_vp, c_vp, c_vp, c_vp]),
@@ -175,7 +202,8 @@ class _ThroughCtypes:
 
 
 _FAST = None
-FAST_ENTRIES = ("softmax", "rms_norm", "silu_mul", "gemm", "attention", "rope", "kv_cache_update", "attention_prefill", "attention_decode")
+FAST_ENTRIES = ("softmax", "rms_norm", "silu_mul", "gemm", "attention", "rope", "kv_cache_update", "attention_prefill", "attention_decode",
+                "add_rms_norm", "gemm_w4", "kv_page_append", "kv_page_read", "attention_paged")
 
 
 def fast():

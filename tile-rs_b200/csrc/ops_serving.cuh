@@ -1,0 +1,204 @@
+// Host-side launch logic of the serving operators (residual norm, 4-bit weights, paged KV cache and its attention): argument checks, kernel
+// selection, launch.  As in ops.cuh nothing here synchronises and every function answers a TSM100_* status with a message in *err.
+#pragma once
+
+#include <cmath>
+
+#include "add_rms_norm.cuh"
+#include "attention_paged.cuh"
+#include "gemm_w4.cuh"
+#include "kv_pages.cuh"
+#include "launch.cuh"
+
+namespace tsm100 {
+namespace ops {
+
+inline bool dtype_16bit(int32_t dtype) { return dtype == TSM100_F16 || dtype == TSM100_BF16; }
+
+// ---------------------------------------------------------------------------
+// residual norm
+// ---------------------------------------------------------------------------
+template <typename T>
+inline int32_t add_rms_norm_typed(std::string* err, const tsm100_add_rms_norm_desc* d, const void* x, const void* residual, void* sum, const void* weight,
+                                  void* y, float* scales, cudaStream_t s) {
+  addnorm::Params<T> p;
+  p.x = static_cast<const T*>(x);
+  p.residual = static_cast<const T*>(residual);
+  p.sum = static_cast<T*>(sum);
+  p.weight = static_cast<const T*>(weight);
+  p.y = y;
+  p.scales = scales;
+  p.rows = d->rows;
+  p.cols = static_cast<int32_t>(d->cols);
+  p.eps = d->eps;
+  const unsigned grid = static_cast<unsigned>(d->rows);
+  if (d->out_dtype == TSM100_I8) addnorm::add_rms_norm_kernel<T, true><<<grid, addnorm::kThreads, 0, s>>>(p);
+  else addnorm::add_rms_norm_kernel<T, false><<<grid, addnorm::kThreads, 0, s>>>(p);
+  return cuda_ok(err, cudaGetLastError(), "add_rms_norm launch");
+}
+
+inline int32_t add_rms_norm(std::string* err, const tsm100_add_rms_norm_desc* d, const void* x, const void* residual, void* sum, const void* weight, void* y,
+                            float* scales, void* stream) {
+  if (!d) return op_fail(err, TSM100_ERR_INVALID, "add_rms_norm: null descriptor");
+  if (!dtype_valid(d->dtype)) return op_fail(err, TSM100_ERR_INVALID, "add_rms_norm: unknown dtype");
+  if (d->out_dtype != d->dtype && d->out_dtype != TSM100_I8) return op_fail(err, TSM100_ERR_INVALID, "add_rms_norm: out_dtype must be dtype or TSM100_I8");
+  if (d->rows < 0 || d->cols < 0 || d->rows > 0x7fffffff || d->cols > 0x7fffffff) return op_fail(err, TSM100_ERR_INVALID, "add_rms_norm: bad shape");
+  if (d->rows == 0 || d->cols == 0) return TSM100_OK;
+  if (!x || !y) return op_fail(err, TSM100_ERR_INVALID, "add_rms_norm: null buffer");
+  if (d->out_dtype == TSM100_I8 && !scales) return op_fail(err, TSM100_ERR_INVALID, "add_rms_norm: an output in 8 bits needs scales");
+  if (sum && sum == y) return op_fail(err, TSM100_ERR_INVALID, "add_rms_norm: sum and y are the same buffer");
+  if (d->out_dtype == TSM100_I8 && (y == x || y == residual)) return op_fail(err, TSM100_ERR_INVALID, "add_rms_norm: y in 8 bits cannot be x or residual");
+  const size_t mask = dtype_size(d->dtype) - 1;
+  for (const void* q : {x, residual, static_cast<const void*>(sum), weight, d->out_dtype == TSM100_I8 ? nullptr : static_cast<const void*>(y)})
+    if (reinterpret_cast<uintptr_t>(q) & mask) return op_fail(err, TSM100_ERR_INVALID, "add_rms_norm: a buffer does not start on an element boundary");
+  if (reinterpret_cast<uintptr_t>(scales) & 3u) return op_fail(err, TSM100_ERR_INVALID, "add_rms_norm: scales do not start on an element boundary");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (d->dtype) {
+    case TSM100_F32: return add_rms_norm_typed<float>(err, d, x, residual, sum, weight, y, scales, s);
+    case TSM100_BF16: return add_rms_norm_typed<__nv_bfloat16>(err, d, x, residual, sum, weight, y, scales, s);
+    default: return add_rms_norm_typed<__half>(err, d, x, residual, sum, weight, y, scales, s);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 4-bit weights
+// ---------------------------------------------------------------------------
+template <typename T>
+inline int32_t gemm_w4_typed(std::string* err, const tsm100_gemm_w4_desc* d, const w4::Params& p, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>((d->m * d->n + 7) / 8);
+  if (d->a_dtype == TSM100_I8) w4::gemm_w4_kernel<T, int8_t><<<grid, 256, 0, s>>>(p);
+  else w4::gemm_w4_kernel<T, T><<<grid, 256, 0, s>>>(p);
+  return cuda_ok(err, cudaGetLastError(), "gemm_w4 launch");
+}
+
+inline int32_t gemm_w4(std::string* err, const tsm100_gemm_w4_desc* d, const void* a, const float* a_scales, const uint8_t* w, const void* w_scales,
+                       const uint8_t* w_zeros, void* c, void* stream) {
+  if (!d) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: null descriptor");
+  if (!dtype_16bit(d->dtype)) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: dtype must be TSM100_F16 or TSM100_BF16");
+  if (d->a_dtype != d->dtype && d->a_dtype != TSM100_I8) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: a_dtype must be dtype or TSM100_I8");
+  if (d->group != 32 && d->group != 64 && d->group != 128) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: group must be 32, 64 or 128");
+  if (d->m < 0 || d->n < 0 || d->k < 0 || d->m > 0x7fffffff || d->n > 0x7fffffff || d->k > 0x7fffffff)
+    return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: bad shape");
+  if (d->k % d->group != 0) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: k must be a multiple of group");
+  if (d->m == 0 || d->n == 0) return TSM100_OK;
+  if (d->m * d->n / 8 >= 0x7fffffff) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: too many outputs for one launch");
+  if (!c || (d->k > 0 && (!a || !w || !w_scales))) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: null buffer");
+  if (d->a_dtype == TSM100_I8 && !a_scales) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: rows in 8 bits need a_scales");
+  if (!aligned16(a) || !aligned16(w)) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: a and w must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(w_scales) | reinterpret_cast<uintptr_t>(c)) & 1u || reinterpret_cast<uintptr_t>(a_scales) & 3u)
+    return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: a buffer does not start on an element boundary");
+  w4::Params p;
+  p.a = a;
+  p.a_scales = d->a_dtype == TSM100_I8 ? a_scales : nullptr;
+  p.w = w;
+  p.scales = w_scales;
+  p.zeros = w_zeros;
+  p.c = c;
+  p.m = d->m, p.n = d->n;
+  p.k = static_cast<int32_t>(d->k), p.group = d->group;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return d->dtype == TSM100_BF16 ? gemm_w4_typed<__nv_bfloat16>(err, d, p, s) : gemm_w4_typed<__half>(err, d, p, s);
+}
+
+// ---------------------------------------------------------------------------
+// paged KV cache
+// ---------------------------------------------------------------------------
+// What every operator on pages asks of its descriptors.  *nothing: there are no tokens.
+inline int32_t paged_args(std::string* err, const char* op, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, int32_t dtype, pages::Cache* c,
+                          pages::Batch* s, bool* nothing) {
+  auto no = [&](const char* what) { return op_fail(err, TSM100_ERR_INVALID, std::string(op) + ": " + what); };
+  *nothing = false;
+  if (!kv || !b) return no("null descriptor");
+  if (!dtype_16bit(dtype)) return no("dtype must be TSM100_F16 or TSM100_BF16");
+  if (kv->dtype != dtype && kv->dtype != TSM100_I8) return no("the cache must hold dtype or TSM100_I8");
+  if (kv->heads_kv <= 0 || kv->page_size <= 0 || kv->page_size > 4096 || kv->pages < 0 || kv->pages > 0x7fffffff) return no("bad cache shape");
+  if (kv->head_dim <= 0 || kv->head_dim > 256 || kv->head_dim % 16 != 0) return no("head_dim must be a multiple of 16, up to 256");
+  if (static_cast<int64_t>(kv->heads_kv) * kv->pages > 0x7fffffff) return no("too many pages times heads");
+  if (b->batch < 0 || b->tokens < 0 || b->max_new < 0 || b->max_len < 0 || b->table_pitch < 0) return no("bad batch shape");
+  if (static_cast<int64_t>(b->table_pitch) * kv->page_size > 0x7fffffff) return no("a row of the table covers too many positions");
+  if (b->batch == 0 || b->tokens == 0 || b->max_new == 0) {
+    *nothing = true;
+    return TSM100_OK;
+  }
+  if (!b->table || !b->lens || !b->starts) return no("null table, lens or starts");
+  if ((reinterpret_cast<uintptr_t>(b->table) | reinterpret_cast<uintptr_t>(b->lens) | reinterpret_cast<uintptr_t>(b->starts)) & 3u)
+    return no("table, lens or starts do not start on an element boundary");
+  if (!kv->k || !kv->v) return no("null cache");
+  if (!aligned16(kv->k) || !aligned16(kv->v)) return no("the cache must be 16-byte aligned");
+  if (kv->dtype == TSM100_I8 && (!kv->k_scales || !kv->v_scales)) return no("a cache of 8 bits needs scales");
+  if ((reinterpret_cast<uintptr_t>(kv->k_scales) | reinterpret_cast<uintptr_t>(kv->v_scales)) & 3u) return no("scales do not start on an element boundary");
+  c->heads = kv->heads_kv, c->d = kv->head_dim, c->page_size = kv->page_size, c->pages = kv->pages;
+  c->kv[0] = kv->k, c->kv[1] = kv->v;
+  c->scales[0] = kv->k_scales, c->scales[1] = kv->v_scales;
+  s->batch = b->batch, s->tokens = b->tokens, s->max_new = b->max_new, s->pitch = b->table_pitch;
+  s->table = b->table, s->lens = b->lens, s->starts = b->starts;
+  return TSM100_OK;
+}
+
+template <typename T, bool kRead>
+inline cudaError_t kv_page_rows_launch(const pages::Cache& c, const pages::Batch& b, bool i8, void* k, void* v, uint32_t* status, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(b.tokens) * 2 * c.heads + 7) / 8);
+  if (i8) pages::kv_page_rows_kernel<T, true, kRead><<<grid, 256, 0, s>>>(c, b, static_cast<T*>(k), static_cast<T*>(v), status);
+  else pages::kv_page_rows_kernel<T, false, kRead><<<grid, 256, 0, s>>>(c, b, static_cast<T*>(k), static_cast<T*>(v), status);
+  return cudaGetLastError();
+}
+
+template <bool kRead>
+inline int32_t kv_page_rows(std::string* err, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, int32_t dtype, void* k, void* v, uint32_t* status,
+                            void* stream) {
+  const char* op = kRead ? "kv_page_read" : "kv_page_append";
+  pages::Cache c;
+  pages::Batch step;
+  bool nothing;
+  const int32_t st = paged_args(err, op, kv, b, dtype, &c, &step, &nothing);
+  if (st != TSM100_OK || nothing) return st;
+  if (!k || !v) return op_fail(err, TSM100_ERR_INVALID, std::string(op) + ": null buffer");
+  if (!aligned16(k) || !aligned16(v)) return op_fail(err, TSM100_ERR_INVALID, std::string(op) + ": k and v must be 16-byte aligned");
+  if (static_cast<int64_t>(step.tokens) * 2 * c.heads / 8 >= 0x7fffffff) return op_fail(err, TSM100_ERR_INVALID, std::string(op) + ": too many tokens for one launch");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool i8 = kv->dtype == TSM100_I8;
+  return cuda_ok(err, dtype == TSM100_BF16 ? kv_page_rows_launch<__nv_bfloat16, kRead>(c, step, i8, k, v, status, s)
+                                           : kv_page_rows_launch<__half, kRead>(c, step, i8, k, v, status, s), op);
+}
+
+// ---------------------------------------------------------------------------
+// attention over pages
+// ---------------------------------------------------------------------------
+template <typename T, bool kI8, int D>
+inline cudaError_t attention_paged_launch(const paged::Params& p, const void* q, void* o, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(p.step.tokens) * p.heads_q + 7) / 8);
+  paged::attention_paged_kernel<T, kI8, D><<<grid, 256, 0, s>>>(static_cast<const T*>(q), static_cast<T*>(o), p);
+  return cudaGetLastError();
+}
+
+template <typename T>
+inline cudaError_t attention_paged_typed(const paged::Params& p, bool i8, const void* q, void* o, cudaStream_t s) {
+  if (p.cache.d == 128) return i8 ? attention_paged_launch<T, true, 128>(p, q, o, s) : attention_paged_launch<T, false, 128>(p, q, o, s);
+  return i8 ? attention_paged_launch<T, true, 64>(p, q, o, s) : attention_paged_launch<T, false, 64>(p, q, o, s);
+}
+
+inline int32_t attention_paged(std::string* err, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, const tsm100_attention_paged_desc* d, const void* q,
+                               void* o, uint32_t* status, void* stream) {
+  if (!d) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: null descriptor");
+  paged::Params p;
+  bool nothing;
+  const int32_t st = paged_args(err, "attention_paged", kv, b, d->dtype, &p.cache, &p.step, &nothing);
+  if (st != TSM100_OK) return st;
+  if (kv->head_dim != 64 && kv->head_dim != 128) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: head_dim must be 64 or 128");
+  if (d->heads_q <= 0 || d->heads_q % kv->heads_kv != 0)
+    return op_fail(err, TSM100_ERR_INVALID, "attention_paged: heads_q must be a positive multiple of heads_kv");
+  if (nothing) return TSM100_OK;
+  if (!q || !o) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: null buffer");
+  if (!aligned16(q) || !aligned16(o)) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: q and o must be 16-byte aligned");
+  if (static_cast<int64_t>(b->tokens) * d->heads_q / 8 >= 0x7fffffff) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: too many tokens for one launch");
+  p.heads_q = d->heads_q;
+  p.scale_log2 = static_cast<float>((1.0 / std::sqrt(static_cast<double>(kv->head_dim))) * 1.4426950408889634);
+  p.status = status;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool i8 = kv->dtype == TSM100_I8;
+  return cuda_ok(err, d->dtype == TSM100_BF16 ? attention_paged_typed<__nv_bfloat16>(p, i8, q, o, s) : attention_paged_typed<__half>(p, i8, q, o, s),
+                 "attention_paged launch");
+}
+
+}  // namespace ops
+}  // namespace tsm100

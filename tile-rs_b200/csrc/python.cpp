@@ -13,7 +13,7 @@
 
 namespace {
 
-enum Entry { kSoftmax, kRmsNorm, kSiluMul, kGemm, kAttention, kRope, kKvCacheUpdate, kPrefill, kDecode, kEntries };
+enum Entry { kSoftmax, kRmsNorm, kSiluMul, kGemm, kAttention, kRope, kKvCacheUpdate, kPrefill, kDecode, kAddRmsNorm, kGemmW4, kPageAppend, kPageRead, kPaged, kEntries };
 void* g_entry[kEntries] = {};
 
 // Walks through the arguments; `ok` turns false at the first that does not fit.
@@ -167,10 +167,66 @@ PyObject* attention_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
   void *q = a.ptr(), *k = a.ptr(), *v = a.ptr(), *o = a.ptr(), *s = a.ptr();
   return call<decltype(&tsm100_attention_decode)>(a, kDecode, dev, &d, q, k, v, o, s);
 }
+// (device, dtype, out_dtype, rows, cols, eps, x, residual, sum, weight, y, scales, stream)
+PyObject* add_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 13, kAddRmsNorm);
+  auto* dev = a.ptr<tsm100_device_s>();
+  tsm100_add_rms_norm_desc d = {};
+  d.dtype = a.i32(), d.out_dtype = a.i32(), d.rows = a.i64(), d.cols = a.i64(), d.eps = a.f32();
+  void *x = a.ptr(), *residual = a.ptr(), *sum = a.ptr(), *weight = a.ptr(), *y = a.ptr();
+  float* scales = a.ptr<float>();
+  void* s = a.ptr();
+  return call<decltype(&tsm100_add_rms_norm)>(a, kAddRmsNorm, dev, &d, x, residual, sum, weight, y, scales, s);
+}
+// (device, dtype, a_dtype, group, m, n, k, a, a_scales, w, w_scales, w_zeros, c, stream)
+PyObject* gemm_w4(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 14, kGemmW4);
+  auto* dev = a.ptr<tsm100_device_s>();
+  tsm100_gemm_w4_desc d = {};
+  d.dtype = a.i32(), d.a_dtype = a.i32(), d.group = a.i32(), d.m = a.i64(), d.n = a.i64(), d.k = a.i64();
+  void* x = a.ptr();
+  const float* x_scales = a.ptr<float>();
+  const uint8_t* w = a.ptr<uint8_t>();
+  void* scales = a.ptr();
+  const uint8_t* zeros = a.ptr<uint8_t>();
+  void *c = a.ptr(), *s = a.ptr();
+  return call<decltype(&tsm100_gemm_w4)>(a, kGemmW4, dev, &d, x, x_scales, w, scales, zeros, c, s);
+}
+// (device, cache, batch, dtype, k, v, stream); cache and batch: addresses of their descriptors
+PyObject* kv_page_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 7, kPageAppend);
+  auto* dev = a.ptr<tsm100_device_s>();
+  auto* kv = a.ptr<tsm100_paged_kv>();
+  auto* batch = a.ptr<tsm100_paged_batch>();
+  const int32_t dtype = a.i32();
+  void *k = a.ptr(), *v = a.ptr(), *s = a.ptr();
+  return call<decltype(&tsm100_kv_page_append)>(a, kPageAppend, dev, kv, batch, dtype, k, v, s);
+}
+PyObject* kv_page_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 7, kPageRead);
+  auto* dev = a.ptr<tsm100_device_s>();
+  auto* kv = a.ptr<tsm100_paged_kv>();
+  auto* batch = a.ptr<tsm100_paged_batch>();
+  const int32_t dtype = a.i32();
+  void *k = a.ptr(), *v = a.ptr(), *s = a.ptr();
+  return call<decltype(&tsm100_kv_page_read)>(a, kPageRead, dev, kv, batch, dtype, k, v, s);
+}
+// (device, cache, batch, dtype, heads_q, q, o, stream)
+PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 8, kPaged);
+  auto* dev = a.ptr<tsm100_device_s>();
+  auto* kv = a.ptr<tsm100_paged_kv>();
+  auto* batch = a.ptr<tsm100_paged_batch>();
+  tsm100_attention_paged_desc d = {};
+  d.dtype = a.i32(), d.heads_q = a.i32();
+  void *q = a.ptr(), *o = a.ptr(), *s = a.ptr();
+  return call<decltype(&tsm100_attention_paged)>(a, kPaged, dev, kv, batch, &d, q, o, s);
+}
 
 #define TSM_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {TSM_METHOD(bind), TSM_METHOD(softmax), TSM_METHOD(rms_norm), TSM_METHOD(silu_mul), TSM_METHOD(gemm), TSM_METHOD(attention),
                            TSM_METHOD(rope), TSM_METHOD(kv_cache_update), TSM_METHOD(attention_prefill), TSM_METHOD(attention_decode),
+                           TSM_METHOD(add_rms_norm), TSM_METHOD(gemm_w4), TSM_METHOD(kv_page_append), TSM_METHOD(kv_page_read), TSM_METHOD(attention_paged),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_tile_sm100", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

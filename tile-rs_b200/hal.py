@@ -319,6 +319,25 @@ class KernelLauncher:
             pass
 
 
+# ---- paged KV caches -----------------------------------------------------------
+class PagedKv:
+    """A KV cache in pages of device memory (tsm100_paged_kv): k, v [pages, heads_kv, page_size, head_dim]; with dtype capi.I8 the steps of the
+    rows, f32 [pages, heads_kv, page_size].  Pointers as ints; the memory stays the caller's."""
+
+    def __init__(self, dtype: int, heads_kv: int, head_dim: int, page_size: int, pages: int, k: int, v: int, k_scales: int = 0, v_scales: int = 0):
+        self.desc = capi.PagedKv(dtype, heads_kv, head_dim, page_size, pages, k or None, v or None, k_scales or None, v_scales or None)
+        self.address = C.addressof(self.desc)
+
+
+class PagedBatch:
+    """The sequences of a call (tsm100_paged_batch): table [batch, table_pitch], lens [batch] and starts [batch + 1] are int32 arrays in device
+    memory.  No sequence has more than max_new tokens in the call; max_len is for planning (0: unknown)."""
+
+    def __init__(self, batch: int, tokens: int, max_new: int, max_len: int, table_pitch: int, table: int, lens: int, starts: int):
+        self.desc = capi.PagedBatch(batch, tokens, max_new, max_len, table_pitch, table or None, lens or None, starts or None)
+        self.address = C.addressof(self.desc)
+
+
 # ---- device (device.rs:25-57) -------------------------------------------------
 class CudaSm100Device:
     def __init__(self, ordinal: int):
@@ -468,6 +487,55 @@ class CudaSm100Device:
         if st is None:
             d = capi.AttentionDecodeDesc(dtype, batch, heads_q, heads_kv, seq_len, max_seq, head_dim)
             check(capi.lib().tsm100_attention_decode(self._h, C.byref(d), q, k_cache, v_cache, o, stream or None))
+        elif st:
+            check(st)
+
+    def add_rms_norm(self, dtype: int, rows: int, cols: int, eps: float, x: int, residual: int, sum_out: int, weight: int, y: int, *,
+                     out_dtype: Optional[int] = None, scales: int = 0, stream: int = 0) -> None:
+        """h = x + residual; sum_out = h; y = h * rsqrt(mean(h^2) + eps) * weight.  residual, sum_out and weight may be 0.  With out_dtype
+        capi.I8, y holds whole numbers and scales[rows] their f32 steps."""
+        out_dtype = dtype if out_dtype is None else out_dtype
+        st = self._fast.add_rms_norm(self._raw, dtype, out_dtype, rows, cols, eps, x, residual or 0, sum_out or 0, weight or 0, y, scales or 0, stream)
+        if st is None:
+            d = capi.AddRmsNormDesc(dtype, out_dtype, rows, cols, eps)
+            check(capi.lib().tsm100_add_rms_norm(self._h, C.byref(d), x, residual or None, sum_out or None, weight or None, y, scales or None, stream or None))
+        elif st:
+            check(st)
+
+    def gemm_w4(self, dtype: int, m: int, n: int, k: int, group: int, a: int, w: int, w_scales: int, c: int, *, a_dtype: Optional[int] = None,
+                a_scales: int = 0, w_zeros: int = 0, stream: int = 0) -> None:
+        """C = A * W^T with 4-bit W [n, k/2] (even k in the low half) = (q - zero) * scale, a scale per group of k; w_zeros 0: 8 everywhere.
+        a_dtype capi.I8 takes the whole numbers and steps that add_rms_norm leaves."""
+        a_dtype = dtype if a_dtype is None else a_dtype
+        st = self._fast.gemm_w4(self._raw, dtype, a_dtype, group, m, n, k, a, a_scales or 0, w, w_scales, w_zeros or 0, c, stream)
+        if st is None:
+            d = capi.GemmW4Desc(dtype, a_dtype, group, m, n, k)
+            check(capi.lib().tsm100_gemm_w4(self._h, C.byref(d), a, a_scales or None, w, w_scales, w_zeros or None, c, stream or None))
+        elif st:
+            check(st)
+
+    def kv_page_append(self, kv: PagedKv, batch: PagedBatch, dtype: int, k: int, v: int, stream: int = 0) -> None:
+        """Writes the call's tokens k, v [tokens, heads_kv, d] into their sequences' pages, quantised on the way if the cache holds 8 bits."""
+        st = self._fast.kv_page_append(self._raw, kv.address, batch.address, dtype, k, v, stream)
+        if st is None:
+            check(capi.lib().tsm100_kv_page_append(self._h, C.byref(kv.desc), C.byref(batch.desc), dtype, k, v, stream or None))
+        elif st:
+            check(st)
+
+    def kv_page_read(self, kv: PagedKv, batch: PagedBatch, dtype: int, k: int, v: int, stream: int = 0) -> None:
+        """The call's tokens read back from the pages into k, v [tokens, heads_kv, d]."""
+        st = self._fast.kv_page_read(self._raw, kv.address, batch.address, dtype, k, v, stream)
+        if st is None:
+            check(capi.lib().tsm100_kv_page_read(self._h, C.byref(kv.desc), C.byref(batch.desc), dtype, k, v, stream or None))
+        elif st:
+            check(st)
+
+    def attention_paged(self, kv: PagedKv, batch: PagedBatch, dtype: int, heads_q: int, q: int, o: int, stream: int = 0) -> None:
+        """Causal attention of the call's tokens q [tokens, heads_q, d], already appended, over their sequences' pages."""
+        st = self._fast.attention_paged(self._raw, kv.address, batch.address, dtype, heads_q, q, o, stream)
+        if st is None:
+            d = capi.AttentionPagedDesc(dtype, heads_q)
+            check(capi.lib().tsm100_attention_paged(self._h, C.byref(kv.desc), C.byref(batch.desc), C.byref(d), q, o, stream or None))
         elif st:
             check(st)
 
