@@ -1,57 +1,603 @@
-// Attention of new tokens over the pages of their sequences: a token at position p sees positions 0 .. p.
+// Attention of a few new tokens over the pages of their sequences (single tokens above all): a token at position p sees positions 0 .. p.
+//
+//   o[t,h] = sum_j w_j V[j] / sum_j w_j,   w_j = 2^(s_j - m),   s_j = (q[t,h] . K[j]) log2(e) / sqrt(d),   m = max_j s_j
+//
+// in one pass over the keys: a running (m, sum, O), rescaled when m grows; parts of a sequence that different warps or CTAs have seen are joined
+// by their maxima.
+//
+// Bound: HBM, the cache is read once; at sixteen rows a tile the arithmetic is a third of what the SMs give.  So the tiles of
+// all (sequence, KV head) pairs are numbered through and every SM takes an equal, contiguous share of them, which may begin and end inside a
+// pair: how uneven the sequences are does not matter, and no grid has to be planned from lengths that only the device knows.  A pair's new tokens
+// times the heads of its group are the rows of mma.sync tiles, up to sixteen at a time; more rows are further passes over the pair's keys.
+//
+// A CTA has eight warps and each takes every eighth tile of the share: K and V come by TMA, a box per page or part of one (128-byte
+// swizzle, no multicast), into slots of its own.  Pages that are no multiple of eight positions are fetched row by row with cp.async instead.
+//
+// 8 bits: whole numbers become f16 exactly (a byte behind 0x64 is 1024 + byte), K's step multiplies the score and V's the probability, over the
+// largest step so far (the accumulator is rescaled when that grows), so that only the probability is rounded.  bf16 queries are brought to f16 by a power of two per row.
 #pragma once
 
+#include "attention_decode.cuh"
 #include "kv_pages.cuh"
 #include "ptx.cuh"
 
 namespace tsm100 {
 namespace paged {
 
+namespace mma = attn_decode::mma;
+
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kRows = 16;
+constexpr int kMaxCtas = 1024;
+template <bool kI8, int D>
+struct Tile {
+  static constexpr int kBytes = kI8 ? 4096 : 8192;        // of K or of V
+  static constexpr int kRowBytes = kI8 ? D : 2 * D;
+  static constexpr int kPos = kBytes / kRowBytes;         // 32 or 64 positions
+  static constexpr int kSlots = kI8 ? 5 : 3;              // per warp
+  static constexpr int kRec = D + 4;                      // floats of a row's record: O, maximum, sum; 16-byte rows
+  static constexpr int kScales = kI8 ? kPos * 4 : 0;      // bytes beside a slot
+  static constexpr int kSmem = kWarps * kSlots * (kBytes + kScales) + kWarps * 8 * kRec * 4 + kWarps * kSlots * 8 + 64 + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory budget of one CTA");
+};
+
 struct Params {
   pages::Cache cache;
   pages::Batch step;
-  int32_t heads_q;
-  float scale_log2;  // log2(e) / sqrt(d)
+  int32_t heads_q, group;
+  int32_t run_log2;   // positions a copy brings: a power of two that divides the page (kTma), else the whole tile
+  float scale_log2;   // log2(e) / sqrt(d)
+  float* part;        // [CTA][2][kRows][kRec]: of a pair that began in an earlier share, of one that goes on in the next
+  int4* info;         // [CTA]: 1 if a pair of earlier shares ends in this one, 2 if it goes on; sequence and unit of the pair that goes on in the next, or -1
   uint32_t* status;
 };
 
-// A warp per (token, head), a position at a time.
-template <typename T, bool kI8, int D>
-__global__ void __launch_bounds__(256)
-attention_paged_kernel(const T* __restrict__ q, T* __restrict__ o, const Params p) {
-  constexpr int N = D / 32;
-  using H = typename std::conditional<kI8, int8_t, T>::type;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (i >= static_cast<int64_t>(p.step.tokens) * p.heads_q) return;
-  const int head = static_cast<int>(i % p.heads_q), token = static_cast<int>(i / p.heads_q), g = head / (p.heads_q / p.cache.heads);
-  const int b = pages::sequence_of(p.step, token);
-  int first, count, len;
-  if (b < 0 || !pages::sequence(p.step, p.cache.page_size, b, first, count, len, p.status, 3)) return;
-  const int last = len - count + token - first;
-  float qv[N], acc[N] = {}, m = -INFINITY, l = 0.f;
+// A sequence's place in the stream of tiles.
+struct Seq {
+  int b, first, count, len;
+  int tiles;      // of a unit: the keys of one KV head for up to kRows rows
+  int passes;     // units of a KV head
+  int64_t base;   // tiles before it
+  int64_t end;    // and with it
+};
+template <int kPos>
+__device__ __forceinline__ int64_t sequence_tiles(const Params& p, int b, Seq& s, uint32_t* status) {
+  if (!pages::sequence(p.step, p.cache.page_size, b, s.first, s.count, s.len, status, 143)) return 0;
+  s.tiles = (s.len + kPos - 1) / kPos;
+  s.passes = static_cast<int>((static_cast<int64_t>(s.count) * p.group + kRows - 1) / kRows);
+  return static_cast<int64_t>(s.tiles) * s.passes * p.cache.heads;
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(bar)), "r"(0), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int32_t y, int32_t w) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %3, %5}], [%2];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(bar)), "r"(0), "r"(y), "r"(w)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(ptx::smem_u32(bar))
+               : "memory");
+}
+// Two of the four whole numbers of x, as f16: bytes 0 and 1, 2 and 3, 0 and 2 or 1 and 3 (the selector says which, 4 stands for 0x64).
+__device__ __forceinline__ uint32_t i8_pair(uint32_t biased, uint32_t selector) {
+  const uint32_t h = __byte_perm(biased, 0x64646464u, selector);  // 1024 + 128 + q
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T, bool kI8, int D, bool kTma>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const T* __restrict__ q, T* __restrict__ o,
+                       const __grid_constant__ Params p) {
+  using L = Tile<kI8, D>;
+  constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
+  constexpr bool kMmaBf16 = kIsBf16 && !kI8;
+  constexpr int TP = L::kPos, N8 = TP / 8, KSTEPS = D / 16, REC = L::kRec, kSlots = L::kSlots, kChunks = L::kRowBytes / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* records = reinterpret_cast<float*>(smem + kWarps * kSlots * (L::kBytes + L::kScales));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(records + kWarps * 8 * REC);
+  __shared__ int64_t scan[kWarps + 2];
+  __shared__ uint32_t abort_word;
+  __shared__ int first_seq;
+  volatile uint32_t* abort_flag = &abort_word;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tq = lane & 3;
+  if (tid == 0) {
+    for (int i = 0; i < kWarps * kSlots; ++i) ptx::mbar_init(&bars[i], 1);
+    abort_word = 0;
+    first_seq = p.step.batch;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&tmap_k);
+    ptx::prefetch_tensormap(&tmap_v);
+  }
+  ptx::launch_dependents();
+  q = ptx::wait_prior_grid(q);
+
+  // The stream: how long it is, and the sequence in which this CTA's share begins.
+  const int batch = p.step.batch;
+  auto block_scan = [&](int64_t v, int64_t& before) {  // of all threads; answers the total
+    int64_t x = v;
 #pragma unroll
-  for (int j = 0; j < N; ++j) qv[j] = softmax::Elem<T>::load1(q + i * D + j * 32 + lane) * p.scale_log2;
-  for (int pos = 0; pos <= last; ++pos) {
-    const int page = pages::page_of(p.cache, p.step, b, pos, p.status, 4);
-    if (page < 0) return;
-    const int64_t row = (static_cast<int64_t>(page) * p.cache.heads + g) * p.cache.page_size + pos % p.cache.page_size;
-    const H* k = static_cast<const H*>(p.cache.kv[0]) + row * D;
-    const H* v = static_cast<const H*>(p.cache.kv[1]) + row * D;
-    float s = 0.f;
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, off);
+      if (lane >= off) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) scan[warp] = x;
+    __syncthreads();
+    int64_t total = 0;
+    before = x - v;
 #pragma unroll
-    for (int j = 0; j < N; ++j) s = fmaf(qv[j], static_cast<float>(k[j * 32 + lane]), s);
-    s = softmax::warp_sum(s);
-    if (kI8) s *= p.cache.scales[0][row];
-    const float n = fmaxf(m, s), a = ptx::ex2_approx(m - n), w = ptx::ex2_approx(s - n);
-    l = fmaf(l, a, w);
-    m = n;
-    const float wv = kI8 ? w * p.cache.scales[1][row] : w;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    return total;
+  };
+  int64_t total = 0, before = 0, own = 0;
+  for (int base = 0; base < batch; base += kThreads) {
+    Seq s;
+    own = base + tid < batch ? sequence_tiles<TP>(p, base + tid, s, p.status) : 0;
+    total += block_scan(own, before);
+  }
+  // whole rounds of the eight warps, so that none has a tile more than another without need
+  const int64_t per = ((total + gridDim.x - 1) / gridDim.x + kWarps - 1) / kWarps * kWarps;
+  const int64_t t0 = min(total, blockIdx.x * per), t1 = min(total, t0 + per);
+  if (t0 < t1) {
+    if (batch <= kThreads) {
+      if (before <= t0 && t0 < before + own) first_seq = tid, scan[kWarps] = before;
+    } else {
+      int64_t sum = 0;
+      for (int base = 0; base < batch; base += kThreads) {
+        Seq s;
+        own = base + tid < batch ? sequence_tiles<TP>(p, base + tid, s, nullptr) : 0;
+        const int64_t here = block_scan(own, before);
+        if (sum + before <= t0 && t0 < sum + before + own) first_seq = base + tid, scan[kWarps] = sum + before;
+        sum += here;
+      }
+    }
+  }
+  __syncthreads();
+  if (t0 >= t1) {
+    if (tid == 0) p.info[blockIdx.x] = make_int4(0, -1, -1, 0);
+    return;
+  }
+  auto open = [&](Seq& s, int b, int64_t base) {  // the first sequence from b on that has tiles; there is one
+    int64_t n = 0;
+    for (; b < batch; ++b)
+      if ((n = sequence_tiles<TP>(p, b, s, nullptr)) > 0) break;
+    s.b = b;
+    s.base = base;
+    s.end = base + n;
+  };
+  Seq seq, ahead;
+  open(seq, first_seq, scan[kWarps]);
+  ahead = seq;
+
+  const uint32_t slots = ptx::smem_u32(smem) + warp * (kSlots * L::kBytes);
+  const uint32_t steps = ptx::smem_u32(smem) + kWarps * kSlots * L::kBytes + warp * (kSlots * L::kScales);
+  const float* steps_at = reinterpret_cast<const float*>(smem + kWarps * kSlots * L::kBytes + warp * (kSlots * L::kScales));
+  uint64_t* full = bars + warp * kSlots;
+  const int heads = p.cache.heads, ps = p.cache.page_size;
+  const int lb = p.run_log2, run = 1 << lb;  // of the tile's rows, what lies together: see at()
+  // where 16 bytes `chunk` of position `pos` of a tile are in its slot
+  auto at = [&](int pos, int chunk) -> uint32_t {
+    if constexpr (L::kRowBytes == 256) return ((pos >> lb) << (lb + 8)) + ((chunk >> 3) << (lb + 7)) + ((pos & (run - 1)) << 7) + (((chunk & 7) ^ (pos & 7)) << 4);
+    else if constexpr (L::kRowBytes == 128) return (pos << 7) + ((chunk ^ (pos & 7)) << 4);
+    else return (pos << 6) + ((chunk ^ ((pos >> 1) & 3)) << 4);
+  };
+
+  // The warp's tiles, ahead of their use: K and V of a tile in turn.
+  int64_t t_ahead = t0 + warp;
+  int load_slot = 0, page = 0, tile_ahead = 0, head_ahead = 0;
+  bool load_v = false, more = false;
+  auto settle = [&]() {  // on to tile t_ahead: where it is, and (lane i) the page of its i-th run
+    more = t_ahead < t1;
+    if (!more) return;
+    while (t_ahead >= ahead.end && ahead.b < batch) open(ahead, ahead.b + 1, ahead.end);
+    if (!(more = ahead.b < batch)) return;
+    const int64_t in_seq = t_ahead - ahead.base;
+    const int unit = static_cast<int>(in_seq / ahead.tiles);
+    tile_ahead = static_cast<int>(in_seq - static_cast<int64_t>(unit) * ahead.tiles);
+    head_ahead = unit / ahead.passes;
+    if (kTma) {
+      const int pos = tile_ahead * TP + (lane << lb);
+      page = 0;
+      if ((lane << lb) < TP && pos < ahead.len) page = max(0, pages::page_of(p.cache, p.step, ahead.b, pos, p.status, 144));
+    }
+  };
+  auto issue = [&]() {
+    if (!more) {
+      if (!kTma) mma::cp_async_commit();
+      return;
+    }
+    const int pos0 = tile_ahead * TP, here = min(TP, ahead.len - pos0);
+    const uint32_t dst = slots + load_slot * L::kBytes, dst_steps = steps + load_slot * L::kScales;
+    if constexpr (kTma) {
+      const int runs = (here + run - 1) >> lb;
+      if (lane == 0) ptx::mbar_arrive_expect_tx(&full[load_slot], runs * (run * (L::kRowBytes + (kI8 ? 4 : 0))));
+      __syncwarp();
+      if (lane < runs) {
+        const int in_page = (pos0 + (lane << lb)) % ps;
+        const CUtensorMap* map = load_v ? &tmap_v : &tmap_k;
+        const uint32_t to = dst + ((lane << lb) * L::kRowBytes);
+        const int row = page * heads + head_ahead;
+        if constexpr (L::kRowBytes == 256) tma_load_4d(to, map, &full[load_slot], in_page, row);
+        else tma_load_3d(to, map, &full[load_slot], in_page, row);
+        if constexpr (kI8) bulk_load(dst_steps + (lane << lb) * 4, p.cache.scales[load_v] + static_cast<int64_t>(row) * ps + in_page, run * 4, &full[load_slot]);
+      }
+    } else {
+      for (int i = lane; i < TP * kChunks; i += 32) {
+        const int r = i / kChunks, c = i % kChunks, pos = pos0 + r;
+        const bool ok = r < here;
+        const int pg = ok ? max(0, pages::page_of(p.cache, p.step, ahead.b, pos, p.status, 144)) : 0;
+        const int64_t row = (static_cast<int64_t>(pg) * heads + head_ahead) * ps + (ok ? pos % ps : 0);
+        mma::cp_async_16(dst + at(r, c), static_cast<const uint8_t*>(p.cache.kv[load_v]) + row * L::kRowBytes + c * 16, ok);
+        if (kI8 && c == 0) ptx::cp_async_4(dst_steps + r * 4, p.cache.scales[load_v] + row, ok);
+      }
+      mma::cp_async_commit();
+    }
+    if (load_v) {
+      t_ahead += kWarps;
+      settle();
+    }
+    load_v = !load_v;
+    load_slot = load_slot + 1 == kSlots ? 0 : load_slot + 1;
+  };
+  settle();
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = fmaf(acc[j], a, wv * static_cast<float>(v[j * 32 + lane]));
+  for (int i = 0; i < kSlots; ++i) issue();
+
+  int slot = 0;
+  uint32_t phase = 0;
+  bool alive = true;
+  auto arrived = [&]() {
+    if constexpr (kTma) {
+      alive = alive && __all_sync(0xffffffffu, ptx::mbar_wait(&full[slot], phase, abort_flag, p.status, 131));
+    } else {
+      mma::cp_async_wait<kSlots - 1>();
+      __syncwarp();
+    }
+    return alive;
+  };
+  auto release = [&]() {  // every lane has read the slot: it is filled again
+    __syncwarp();
+    if (++slot == kSlots) slot = 0, phase ^= 1u;
+    issue();
+  };
+  uint32_t qa[KSTEPS][4];
+  float q_factor[2];  // what the rows of Q were divided by
+  const int k_row = (lane & 7) + ((lane >> 4) & 1) * 8, v_row = (lane & 7) + ((lane >> 3) & 1) * 8;
+  int head_state = 0, tail_b = -1, tail_unit = -1;
+  for (int64_t t = t0; t < t1;) {
+    while (t >= seq.end && seq.b < batch) open(seq, seq.b + 1, seq.end);
+    if (seq.b >= batch) break;
+    const int unit = static_cast<int>((t - seq.base) / seq.tiles);
+    const int begin = static_cast<int>(t - seq.base - static_cast<int64_t>(unit) * seq.tiles);
+    const int end = static_cast<int>(min(static_cast<int64_t>(seq.tiles), begin + (t1 - t)));
+    const int head = unit / seq.passes, row0 = unit % seq.passes * kRows;
+    const int rows = min(kRows, seq.count * p.group - row0);
+    // rows gr and gr + 8: their Q as A fragments, and the last position each sees
+    int limit[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bool ok = gr + 8 * e < rows;
+      const int r = row0 + (ok ? gr + 8 * e : 0), token = r / p.group;
+      limit[e] = seq.len - seq.count + token;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(q + (static_cast<int64_t>(seq.first + token) * p.heads_q + head * p.group + r % p.group) * D);
+#pragma unroll
+      for (int kk = 0; kk < KSTEPS; ++kk) {
+        if (kI8) {  // the four numbers of a fragment lie together in a row of the cache
+          const uint2 x = ok ? __ldg(reinterpret_cast<const uint2*>(src + kk * 8 + 2 * tq)) : make_uint2(0u, 0u);
+          qa[kk][e] = x.x, qa[kk][2 + e] = x.y;
+        } else {
+          qa[kk][e] = ok ? __ldg(src + kk * 8 + tq) : 0u;
+          qa[kk][2 + e] = ok ? __ldg(src + kk * 8 + tq + 4) : 0u;
+        }
+      }
+      q_factor[e] = 1.f;
+      if constexpr (kI8 && kIsBf16) {
+        float top = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x = qa[kk][2 * i + e];
+            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x << 16)), fabsf(__uint_as_float(x & 0xffff0000u))));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the power of two below the largest magnitude: what lies 2^24 under that is lost, which f32 sums would lose too
+        const int ex = min(max(static_cast<int>(__float_as_uint(top) >> 23), 20), 250) - 127;
+        q_factor[e] = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
+        const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t& x = qa[kk][2 * i + e];
+            x = mma::pack2<false>(__uint_as_float(x << 16) * inv, __uint_as_float(x & 0xffff0000u) * inv);
+          }
+      }
+    }
+    const int least = seq.len - seq.count + row0 / p.group;  // the first row's last position: tiles up to it need no masks
+    float oacc[2 * KSTEPS][4];
+#pragma unroll
+    for (int j = 0; j < 2 * KSTEPS; ++j) oacc[j][0] = oacc[j][1] = oacc[j][2] = oacc[j][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float v_top = 0x1p-100f;  // 8 bits: the largest step of V so far, oacc is in units of it; far smaller steps count as zero
+    for (int tile = begin + static_cast<int>((warp - (t - t0)) & (kWarps - 1)); tile < end; tile += kWarps) {
+      if (!arrived()) break;
+      const uint32_t ks = slots + slot * L::kBytes;
+      float s[N8][4];
+#pragma unroll
+      for (int j = 0; j < N8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < N8 / 2; ++j) {
+        if constexpr (!kI8) {
+#pragma unroll
+          for (int kk = 0; kk < KSTEPS; ++kk) {
+            uint32_t kb[4];  // (positions 0-7, k lo), (0-7, k hi), (8-15, k lo), (8-15, k hi)
+            mma::ldmatrix_x4(ks + at(j * 16 + k_row, kk * 2 + ((lane >> 3) & 1)), kb);
+            mma::mma_16816<kMmaBf16>(s[2 * j], qa[kk], kb[0], kb[1]);
+            mma::mma_16816<kMmaBf16>(s[2 * j + 1], qa[kk], kb[2], kb[3]);
+          }
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < KSTEPS; kk += 2) {
+            uint32_t kb[4];  // (positions 0-7, 16 numbers), (0-7, the next 16), (8-15, 16), (8-15, the next)
+            mma::ldmatrix_x4(ks + at(j * 16 + k_row, kk + ((lane >> 3) & 1)), kb);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t x = kb[i] ^ 0x80808080u;
+              mma::mma_16816<false>(s[2 * j + (i >> 1)], qa[kk + (i & 1)], i8_pair(x, 0x4140), i8_pair(x, 0x4342));
+            }
+          }
+        }
+      }
+      const int pos = tile * TP + 2 * tq;
+      const bool masked = (tile + 1) * TP - 1 > least;
+      if constexpr (kI8) {
+        const float* kst = steps_at + slot * TP + 2 * tq;
+#pragma unroll
+        for (int j = 0; j < N8; ++j) {
+          const float2 st = *reinterpret_cast<const float2*>(kst + j * 8);
+          const float a = st.x * p.scale_log2, b = st.y * p.scale_log2;
+          s[j][0] *= a * q_factor[0], s[j][1] *= b * q_factor[0];
+          s[j][2] *= a * q_factor[1], s[j][3] *= b * q_factor[1];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < N8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[j][e] *= p.scale_log2;
+      }
+      release();
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < N8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (pos + j * 8 + (e & 1) > limit[e >> 1]) s[j][e] = -INFINITY;
+      }
+      float a[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < N8; ++j) top = fmaxf(top, fmaxf(s[j][2 * e], s[j][2 * e + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float n = fmaxf(m[e], top), base = n == -INFINITY ? 0.f : n;  // a row may see nothing of this warp's first tiles
+        a[e] = ptx::ex2_approx(m[e] - base);
+        m[e] = n;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < N8; ++j) {
+          s[j][2 * e] = ptx::ex2_approx(s[j][2 * e] - base);
+          s[j][2 * e + 1] = ptx::ex2_approx(s[j][2 * e + 1] - base);
+          sum += s[j][2 * e] + s[j][2 * e + 1];
+        }
+        l[e] = fmaf(l[e], a[e], sum);
+      }
+      if (!arrived()) break;
+      const uint32_t vs = slots + slot * L::kBytes;
+      const bool ragged = (tile + 1) * TP > seq.len;
+      if constexpr (kI8) {
+        const float* vst = steps_at + slot * TP + 2 * tq;
+        float2 st[N8];
+        float top = v_top;
+#pragma unroll
+        for (int j = 0; j < N8; ++j) {
+          st[j] = *reinterpret_cast<const float2*>(vst + j * 8);
+          if (ragged) {  // behind the last position may be anything
+            if (pos + j * 8 >= seq.len) st[j].x = 0.f;
+            if (pos + j * 8 + 1 >= seq.len) st[j].y = 0.f;
+          }
+          top = fmaxf(top, fmaxf(st[j].x, st[j].y));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float inv = 1.f / top;
+        a[0] *= v_top * inv, a[1] *= v_top * inv;
+        v_top = top;
+#pragma unroll
+        for (int j = 0; j < N8; ++j) {
+          const float x = st[j].x * inv, y = st[j].y * inv;
+          s[j][0] *= x, s[j][1] *= y, s[j][2] *= x, s[j][3] *= y;
+        }
+      }
+      uint32_t pa[N8 / 2][4];
+#pragma unroll
+      for (int j = 0; j < N8 / 2; ++j) {
+        pa[j][0] = mma::pack2<kMmaBf16>(s[2 * j][0], s[2 * j][1]);
+        pa[j][1] = mma::pack2<kMmaBf16>(s[2 * j][2], s[2 * j][3]);
+        pa[j][2] = mma::pack2<kMmaBf16>(s[2 * j + 1][0], s[2 * j + 1][1]);
+        pa[j][3] = mma::pack2<kMmaBf16>(s[2 * j + 1][2], s[2 * j + 1][3]);
+      }
+#pragma unroll
+      for (int j = 0; j < 2 * KSTEPS; ++j) oacc[j][0] *= a[0], oacc[j][1] *= a[0], oacc[j][2] *= a[1], oacc[j][3] *= a[1];
+      if (!kI8 && ragged) {
+        // what lies behind the last position weighs nothing, but may be anything
+        for (int i = lane; i < TP * kChunks; i += 32)
+          if (tile * TP + i / kChunks >= seq.len) ptx::st_shared_v4(vs + at(i / kChunks, i % kChunks), 0u, 0u, 0u, 0u);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int j = 0; j < N8 / 2; ++j) {
+          uint32_t vb[4];
+          if constexpr (!kI8) {
+            // (positions 0-7, d lo), (8-15, d lo), (0-7, d hi), (8-15, d hi), transposed on load
+            mma::ldmatrix_x4_trans(vs + at(j * 16 + v_row, c * 2 + ((lane >> 4) & 1)), vb);
+            mma::mma_16816<kMmaBf16>(oacc[2 * c], pa[j], vb[0], vb[1]);
+            mma::mma_16816<kMmaBf16>(oacc[2 * c + 1], pa[j], vb[2], vb[3]);
+          } else if (c % 2 == 0) {
+            // the same of pairs of numbers: two positions of column 2 gr and of column 2 gr + 1 in a register
+            mma::ldmatrix_x4_trans(vs + at(j * 16 + v_row, c + ((lane >> 4) & 1)), vb);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t x = vb[2 * i] ^ 0x80808080u, y = vb[2 * i + 1] ^ 0x80808080u;
+              mma::mma_16816<false>(oacc[2 * (c + i)], pa[j], i8_pair(x, 0x4240), i8_pair(y, 0x4240));
+              mma::mma_16816<false>(oacc[2 * (c + i) + 1], pa[j], i8_pair(x, 0x4341), i8_pair(y, 0x4341));
+            }
+          }
+        }
+      if (!kI8 && ragged && kTma) ptx::fence_proxy_async_smem();  // the zeros before the slot's next copy
+      release();
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+    }
+
+    // the warps' records, eight rows at a time
+    const bool whole = begin == 0 && end == seq.tiles;
+    for (int half = 0; half * 8 < rows; ++half) {
+      __syncthreads();  // the records before have been read
+      {
+        float* rec = records + (warp * 8 + gr) * REC;
+        const float f = kI8 ? v_top : 1.f;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          const float x0 = (half ? oacc[2 * c][2] : oacc[2 * c][0]) * f, x1 = (half ? oacc[2 * c][3] : oacc[2 * c][1]) * f;
+          const float y0 = (half ? oacc[2 * c + 1][2] : oacc[2 * c + 1][0]) * f, y1 = (half ? oacc[2 * c + 1][3] : oacc[2 * c + 1][1]) * f;
+          if (kI8) {
+            *reinterpret_cast<float4*>(rec + c * 16 + 4 * tq) = make_float4(x0, y0, x1, y1);
+          } else {
+            *reinterpret_cast<float2*>(rec + c * 16 + 2 * tq) = make_float2(x0, x1);
+            *reinterpret_cast<float2*>(rec + c * 16 + 8 + 2 * tq) = make_float2(y0, y1);
+          }
+        }
+        if (tq == 0) *reinterpret_cast<float2*>(rec + D) = half ? make_float2(m[1], l[1]) : make_float2(m[0], l[0]);
+      }
+      __syncthreads();
+      for (int i = tid; i < min(8, rows - half * 8) * (D / 4); i += kThreads) {
+        const int rr = i / (D / 4), dd = i % (D / 4) * 4;
+        const float* rec = records + rr * REC;
+        float2 ml[kWarps];
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          ml[w] = *reinterpret_cast<const float2*>(rec + w * 8 * REC + D);
+          mm = fmaxf(mm, ml[w].x);
+        }
+        float ll = 0.f;
+        float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          // a warp that has seen nothing weighs nothing; it is added all the same, because one of NaN scores has that maximum too
+          const float wgt = ml[w].x == -INFINITY ? 0.f : ptx::ex2_approx(ml[w].x - mm);
+          const float4 x = *reinterpret_cast<const float4*>(rec + w * 8 * REC + dd);
+          ll = fmaf(ml[w].y, wgt, ll);
+          oo.x = fmaf(x.x, wgt, oo.x), oo.y = fmaf(x.y, wgt, oo.y), oo.z = fmaf(x.z, wgt, oo.z), oo.w = fmaf(x.w, wgt, oo.w);
+        }
+        const int r = half * 8 + rr;
+        if (whole) {
+          const int token = (row0 + r) / p.group, h = head * p.group + (row0 + r) % p.group;
+          const float inv = 1.f / ll;
+          *reinterpret_cast<uint2*>(o + (static_cast<int64_t>(seq.first + token) * p.heads_q + h) * D + dd) =
+              make_uint2(mma::pack2<kIsBf16>(oo.x * inv, oo.y * inv), mma::pack2<kIsBf16>(oo.z * inv, oo.w * inv));
+        } else {
+          float* out = p.part + ((static_cast<int64_t>(blockIdx.x) * 2 + (begin == 0 ? 1 : 0)) * kRows + r) * REC;
+          *reinterpret_cast<float4*>(out + dd) = oo;
+          if (dd == 0) *reinterpret_cast<float2*>(out + D) = make_float2(mm, ll);
+        }
+      }
+    }
+    if (begin > 0) head_state = end == seq.tiles ? 1 : 2;
+    else if (end < seq.tiles) tail_b = seq.b, tail_unit = unit;
+    t += end - begin;
+  }
+  if (tid == 0) p.info[blockIdx.x] = make_int4(head_state, tail_b, tail_unit, 0);
+  if constexpr (!kTma) mma::cp_async_wait<0>();
+  if (*abort_flag != 0u) {
+    // a wait gave up: copies in flight land before the shared memory is released
+    const unsigned long long since = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - since < 1000000ull) {
+    }
+    __syncthreads();
+  }
+}
+
+// The records of a pair that several shares have a part of, in order; a warp per row, CTA (x, y) rows 4 y .. of the pair that goes on behind share x.
+template <typename T, int D>
+__global__ void __launch_bounds__(128)
+attention_paged_merge_kernel(T* __restrict__ o, const __grid_constant__ Params p) {
+  constexpr int REC = D + 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 4 + warp;
+  ptx::launch_dependents();
+  ptx::wait_prior_grid();
+  const int4 mine = __ldcg(p.info + blockIdx.x);
+  if (mine.y < 0) return;
+  int n = 1;  // records: this share's second, and the first of the shares behind it
+  while (blockIdx.x + n < gridDim.x) {
+    const int state = __ldcg(p.info + blockIdx.x + n).x;
+    ++n;
+    if (state != 2) break;
+  }
+  const int first = p.step.starts[mine.y], count = p.step.starts[mine.y + 1] - first;
+  const int passes = static_cast<int>((static_cast<int64_t>(count) * p.group + kRows - 1) / kRows), head = mine.z / passes, row = mine.z % passes * kRows + r;
+  if (row >= count * p.group) return;
+  auto record = [&](int i) { return p.part + ((static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + r) * REC; };
+  float mm = -INFINITY;
+  for (int i = lane; i < n; i += 32) mm = fmaxf(mm, __ldcg(record(i) + D));
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
+  float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+  float ll = 0.f;
+  for (int base = 0; base < n; base += 32) {
+    float w = 0.f;
+    if (base + lane < n) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(record(base + lane) + D));
+      w = ml.x == -INFINITY ? 0.f : ptx::ex2_approx(ml.x - mm);
+      ll = fmaf(ml.y, w, ll);
+    }
+    const int here = min(32, n - base);
+#pragma unroll 8
+    for (int i = 0; i < here; ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      if (lane < D / 4) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(record(base + i)) + lane);
+        oo.x = fmaf(x.x, wi, oo.x), oo.y = fmaf(x.y, wi, oo.y), oo.z = fmaf(x.z, wi, oo.z), oo.w = fmaf(x.w, wi, oo.w);
+      }
+    }
   }
 #pragma unroll
-  for (int j = 0; j < N; ++j) softmax::Elem<T>::store1(o + i * D + j * 32 + lane, acc[j] / l);
+  for (int off = 16; off > 0; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
+  if (lane < D / 4) {
+    const float inv = 1.f / ll;
+    constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
+    *reinterpret_cast<uint2*>(o + (static_cast<int64_t>(first + row / p.group) * p.heads_q + head * p.group + row % p.group) * D + lane * 4) =
+        make_uint2(mma::pack2<kIsBf16>(oo.x * inv, oo.y * inv), mma::pack2<kIsBf16>(oo.z * inv, oo.w * inv));
+  }
 }
 
 }  // namespace paged

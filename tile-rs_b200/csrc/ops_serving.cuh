@@ -2,6 +2,7 @@
 // selection, launch.  As in ops.cuh nothing here synchronises and every function answers a TSM100_* status with a message in *err.
 #pragma once
 
+#include <algorithm>
 #include <cmath>
 
 #include "add_rms_norm.cuh"
@@ -123,6 +124,7 @@ inline int32_t paged_args(std::string* err, const char* op, const tsm100_paged_k
   if (!b->table || !b->lens || !b->starts) return no("null table, lens or starts");
   if ((reinterpret_cast<uintptr_t>(b->table) | reinterpret_cast<uintptr_t>(b->lens) | reinterpret_cast<uintptr_t>(b->starts)) & 3u)
     return no("table, lens or starts do not start on an element boundary");
+  if (kv->pages == 0) return no("the cache has no pages");
   if (!kv->k || !kv->v) return no("null cache");
   if (!aligned16(kv->k) || !aligned16(kv->v)) return no("the cache must be 16-byte aligned");
   if (kv->dtype == TSM100_I8 && (!kv->k_scales || !kv->v_scales)) return no("a cache of 8 bits needs scales");
@@ -164,17 +166,62 @@ inline int32_t kv_page_rows(std::string* err, const tsm100_paged_kv* kv, const t
 // ---------------------------------------------------------------------------
 // attention over pages
 // ---------------------------------------------------------------------------
+// The tiles of all sequences' caches dealt out evenly over the SMs, and what several of them have a part of merged (attention_paged.cuh).
 template <typename T, bool kI8, int D>
-inline cudaError_t attention_paged_launch(const paged::Params& p, const void* q, void* o, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(p.step.tokens) * p.heads_q + 7) / 8);
-  paged::attention_paged_kernel<T, kI8, D><<<grid, 256, 0, s>>>(static_cast<const T*>(q), static_cast<T*>(o), p);
-  return cudaGetLastError();
+inline int32_t attention_paged_launch(std::string* err, paged::Params p, const void* q, void* o, cudaStream_t s) {
+  using L = paged::Tile<kI8, D>;
+  int sms = 0;
+  int32_t st = sm_count(err, &sms);
+  if (st != TSM100_OK) return st;
+  const unsigned ctas = static_cast<unsigned>(std::min(sms, paged::kMaxCtas));
+  const int64_t rows = std::min<int64_t>(paged::kRows, static_cast<int64_t>(p.step.max_new) * p.group);
+  const size_t part = static_cast<size_t>(ctas) * 2 * paged::kRows * L::kRec * sizeof(float);
+  st = take_scratch(err, reinterpret_cast<void**>(&p.part), part + ctas * sizeof(int4), s);
+  if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged: no device memory for partial results");
+  if (st != TSM100_OK) return st;
+  p.info = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(p.part) + part);
+  // boxes of a power of two of positions that a page is a multiple of; 8-bit steps come by copies of 16 bytes and more
+  int run_log2 = 0;
+  while ((2 << run_log2) <= L::kPos && p.cache.page_size % (2 << run_log2) == 0) ++run_log2;
+  const bool boxes = run_log2 >= 3 && (!kI8 || (aligned16(p.cache.scales[0]) && aligned16(p.cache.scales[1])));
+  p.run_log2 = boxes ? run_log2 : L::kPos == 32 ? 5 : 6;
+  CUtensorMap map[2];
+  std::memset(map, 0, sizeof map);
+  for (int i = 0; i < 2 && boxes && st == TSM100_OK; ++i) {
+    TmapKey key;
+    std::memset(&key, 0, sizeof key);
+    constexpr bool kTwo = L::kRowBytes == 256;  // rows of two 128-byte groups
+    key.base = p.cache.kv[i];
+    const uint64_t rows = static_cast<uint64_t>(p.cache.page_size), units = static_cast<uint64_t>(p.cache.pages) * p.cache.heads;
+    if (kTwo) {
+      key.dim[0] = 64, key.dim[1] = rows, key.dim[2] = 2, key.dim[3] = units;
+      key.stride[0] = 256, key.stride[1] = 128, key.stride[2] = rows * 256;
+      key.box[0] = 64, key.box[1] = 1u << run_log2, key.box[2] = 2, key.box[3] = 1;
+    } else {
+      key.dim[0] = kI8 ? D : 64, key.dim[1] = rows, key.dim[2] = units;
+      key.stride[0] = L::kRowBytes, key.stride[1] = rows * L::kRowBytes;
+      key.box[0] = kI8 ? D : 64, key.box[1] = 1u << run_log2, key.box[2] = 1;
+    }
+    key.dtype = static_cast<int32_t>(kI8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+    key.rank = kTwo ? 4 : 3;
+    st = make_tmap(err, &map[i], key, kI8 ? 1 : 2);
+  }
+  if (st == TSM100_OK) {
+    auto kern = boxes ? paged::attention_paged_kernel<T, kI8, D, true> : paged::attention_paged_kernel<T, kI8, D, false>;
+    cudaError_t e = set_dyn_smem_once(kern, L::kSmem);
+    if (e == cudaSuccess) e = launch_chained(kern, ctas, paged::kThreads, L::kSmem, s, 0, map[0], map[1], static_cast<const T*>(q), static_cast<T*>(o), p);
+    if (e == cudaSuccess) e = launch_chained(paged::attention_paged_merge_kernel<T, D>, dim3(ctas, static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, 0, static_cast<T*>(o), p);
+    st = cuda_ok(err, e, "attention_paged_kernel launch");
+  }
+  const cudaError_t e = cudaFreeAsync(p.part, s);
+  if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
+  return st;
 }
 
 template <typename T>
-inline cudaError_t attention_paged_typed(const paged::Params& p, bool i8, const void* q, void* o, cudaStream_t s) {
-  if (p.cache.d == 128) return i8 ? attention_paged_launch<T, true, 128>(p, q, o, s) : attention_paged_launch<T, false, 128>(p, q, o, s);
-  return i8 ? attention_paged_launch<T, true, 64>(p, q, o, s) : attention_paged_launch<T, false, 64>(p, q, o, s);
+inline int32_t attention_paged_typed(std::string* err, const paged::Params& p, bool i8, const void* q, void* o, cudaStream_t s) {
+  if (p.cache.d == 128) return i8 ? attention_paged_launch<T, true, 128>(err, p, q, o, s) : attention_paged_launch<T, false, 128>(err, p, q, o, s);
+  return i8 ? attention_paged_launch<T, true, 64>(err, p, q, o, s) : attention_paged_launch<T, false, 64>(err, p, q, o, s);
 }
 
 inline int32_t attention_paged(std::string* err, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, const tsm100_attention_paged_desc* d, const void* q,
@@ -190,14 +237,14 @@ inline int32_t attention_paged(std::string* err, const tsm100_paged_kv* kv, cons
   if (nothing) return TSM100_OK;
   if (!q || !o) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: null buffer");
   if (!aligned16(q) || !aligned16(o)) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: q and o must be 16-byte aligned");
-  if (static_cast<int64_t>(b->tokens) * d->heads_q / 8 >= 0x7fffffff) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: too many tokens for one launch");
+  if (static_cast<int64_t>(b->tokens) * d->heads_q > 0x7fffffff) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: too many tokens times heads");
   p.heads_q = d->heads_q;
+  p.group = d->heads_q / kv->heads_kv;
   p.scale_log2 = static_cast<float>((1.0 / std::sqrt(static_cast<double>(kv->head_dim))) * 1.4426950408889634);
   p.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool i8 = kv->dtype == TSM100_I8;
-  return cuda_ok(err, d->dtype == TSM100_BF16 ? attention_paged_typed<__nv_bfloat16>(p, i8, q, o, s) : attention_paged_typed<__half>(p, i8, q, o, s),
-                 "attention_paged launch");
+  return d->dtype == TSM100_BF16 ? attention_paged_typed<__nv_bfloat16>(err, p, i8, q, o, s) : attention_paged_typed<__half>(err, p, i8, q, o, s);
 }
 
 }  // namespace ops
