@@ -32,7 +32,7 @@ int32_t tsm100_add_rms_norm(tsm100_device_t dev, const tsm100_add_rms_norm_desc*
 
 int32_t tsm100_gemm_w4(tsm100_device_t dev, const tsm100_gemm_w4_desc* desc, const void* a, const float* a_scales, const uint8_t* w, const void* w_scales,
                        const uint8_t* w_zeros, void* c, void* stream) {
-  return on_device(dev, [&](std::string* err) { return ops::gemm_w4(err, desc, a, a_scales, w, w_scales, w_zeros, c, stream); });
+  return on_device(dev, [&](std::string* err) { return ops::gemm_w4(err, desc, a, a_scales, w, w_scales, w_zeros, c, dev->status, stream); });
 }
 
 int32_t tsm100_kv_page_append(tsm100_device_t dev, const tsm100_paged_kv* kv, const tsm100_paged_batch* batch, int32_t dtype, const void* k, const void* v,
