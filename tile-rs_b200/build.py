@@ -25,7 +25,7 @@ LIB_PATH = PKG_DIR / "libtile_sm100.so"
 # the operators for CPython without ctypes (csrc/python.cpp); absent where there are no CPython headers
 FAST_PATH = PKG_DIR / ("_tile_sm100" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
-CUDA_SOURCES = ["runtime.cu", "capi_ops.cu", "serving.cu", "multi.cu"]
+CUDA_SOURCES = ["runtime.cu", "capi_ops.cu", "serving_w4_bf16.cu", "serving_w4_f16.cu", "serving.cu", "multi.cu"]
 CXX_SOURCES = ["inputs.cpp", "emit.cpp"]
 
 NVCC_FLAGS = [
@@ -96,7 +96,7 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     if not force and LIB_PATH.exists() and stamp.exists() and stamp.read_text() == digest:
         _compile_fast(digest)
         return LIB_PATH
-    with ThreadPoolExecutor(max_workers=4) as pool:
+    with ThreadPoolExecutor(max_workers=8) as pool:
         objs = list(pool.map(_compile, CUDA_SOURCES + CXX_SOURCES))
     cmd = [nvcc(), "-shared", "-o", str(LIB_PATH), *map(str, objs), "-cudart", "static", "-Xcompiler", "-fopenmp", "-ldl"]
     r = subprocess.run(cmd, capture_output=True, text=True)

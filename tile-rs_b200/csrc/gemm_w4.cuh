@@ -116,6 +116,12 @@ __device__ __forceinline__ uint32_t i8_to_16(uint32_t lo, uint32_t hi, int j) {
   return ptx::pack_bf16x2(x, y);
 }
 
+// A whole warp's bounded wait: one vote where the barrier's phase has passed already.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* status, uint32_t site) {
+  if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag, status, site));
+}
+
 template <int X>
 __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[X]) {
   if constexpr (X == 32) ptx::tmem_ld_32x32b_x32(at, r);
@@ -125,7 +131,7 @@ __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[X]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(at) : "memory");
 }
 
-template <typename T, int N, int GC, bool kScaled>
+template <typename T, int N, int GC, bool kScaled, bool kEight>
 __global__ void __launch_bounds__(kThreads, Shape<N, GC, kScaled>::kTwo ? 2 : 1)
 gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
   using S = Shape<N, GC, kScaled>;
@@ -180,7 +186,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
     int b = 0;
     for (int i = 0; i < chunks; ++i) {
       const int d = i & 1;
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&bars->ready[d], (i >> 1) & 1u, abort_flag, p.status, 136))) break;
+      if (!warp_wait(&bars->ready[d], (i >> 1) & 1u, abort_flag, p.status, 136)) break;
       ptx::tcgen05_fence_after_thread_sync();
       if (ptx::elect_one_sync()) {
         const uint32_t act = ptx::smem_u32(smem + S::kActOff + b * S::kActBytes);
@@ -211,7 +217,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
     auto fetch_row = [&](int i, uint16_t (&to)[GC], uint32_t& zero) {
 #pragma unroll
       for (int j = 0; j < GC; ++j) to[j] = 0;
-      zero = 0x08080808u;
+      if (zero_at) zero = 0x08080808u;
       if (together) {
         if (i * GC < groups_left) {
           if constexpr (GC == 4) {
@@ -234,38 +240,31 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
           }
       }
     };
-    const bool eight = p.a_scales != nullptr;
-    const int e8 = tid % 16 * 8, k_left = min(p.k - first * kChunkK, chunks * kChunkK);
+    using Vec = typename std::conditional<kEight, uint2, uint4>::type;  // eight numbers of A
+    const int e8 = tid % 16 * 8, rows_left = min(p.m - token0, p.tokens) - tid / 16;
     const int64_t act_row = static_cast<int64_t>(token0 + tid / 16) * p.k + first * kChunkK + e8;
-    const uint8_t* act_at = static_cast<const uint8_t*>(p.a) + act_row * (eight ? 1 : 2);
-    const int64_t act_pitch = static_cast<int64_t>(p.k) * (eight ? 16 : 32);  // of sixteen rows
-    const int rows_left = min(p.m - token0, p.tokens) - tid / 16;
-    uint4 act[kAhead][S::kVecs];
-    auto fetch_act = [&](int i, uint4 (&to)[S::kVecs]) {
-      const bool inside = i * kChunkK + e8 < k_left;
-      const uint8_t* from = act_at + static_cast<int64_t>(i) * (eight ? kChunkK : 2 * kChunkK);
+    const Vec* act_at = reinterpret_cast<const Vec*>(static_cast<const uint8_t*>(p.a) + act_row * (kEight ? 1 : 2));
+    const int64_t act_pitch = static_cast<int64_t>(p.k) * 2;  // vectors of sixteen rows
+    // chunks in which this thread has something to fetch
+    const int act_chunks = rows_left > 0 ? min(chunks, (p.k - first * kChunkK - e8 + kChunkK - 1) / kChunkK) : 0;
+    Vec act[kAhead][S::kVecs];
+    auto fetch_act = [&](int i, Vec (&to)[S::kVecs]) {
 #pragma unroll
       for (int v = 0; v < S::kVecs; ++v) {
-        to[v] = make_uint4(0u, 0u, 0u, 0u);
-        if (inside && v * 16 < rows_left) {
-          if (eight) {
-            const uint2 x = *reinterpret_cast<const uint2*>(from + v * act_pitch);
-            to[v].x = x.x, to[v].y = x.y;
-          } else {
-            to[v] = *reinterpret_cast<const uint4*>(from + v * act_pitch);
-          }
-        }
+        to[v] = Vec{};
+        if (i < act_chunks && (v == 0 || v * 16 < rows_left)) to[v] = act_at[i * (kChunkK / 8) + v * act_pitch];
       }
     };
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
+      zp[b] = 0x08080808u;
       fetch_row(b, sc[b], zp[b]);
       if (b < kAhead) fetch_act(b, act[b]);
     }
     uint16_t sc_of[2][GC];  // of the two chunks whose sums are still out
     bool ok = true;
     auto wait_done = [&](int i) {
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->done[i & 1], (i >> 1) & 1u, abort_flag, p.status, 137));
+      ok = warp_wait(&bars->done[i & 1], (i >> 1) & 1u, abort_flag, p.status, 137);
       ptx::tcgen05_fence_after_thread_sync();
     };
     auto collect = [&](int i, auto which) {  // chunk i's products are done; its sums, times their scales
@@ -340,16 +339,11 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
       if (d == 1 || i == chunks - 1) ptx::mbar_arrive(&bars->empty[slot]);
 #pragma unroll
       for (int v = 0; v < S::kVecs; ++v) {
-        uint4 x = act[from][v];
-        if (eight) {
-          uint32_t y[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = i8_to_16<T>(x.x, x.y, j);
-          x = make_uint4(y[0], y[1], y[2], y[3]);
-        } else {
-          x = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
-        }
-        *reinterpret_cast<uint4*>(act_to + b * S::kActBytes + v * 2048) = x;
+        const Vec x = act[from][v];
+        uint4 y;
+        if constexpr (kEight) y = make_uint4(i8_to_16<T>(x.x, x.y, 0), i8_to_16<T>(x.x, x.y, 1), i8_to_16<T>(x.x, x.y, 2), i8_to_16<T>(x.x, x.y, 3));
+        else y = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+        *reinterpret_cast<uint4*>(act_to + b * S::kActBytes + v * 2048) = y;
       }
       fetch_act(i + kAhead, act[from]);
       if (i >= 2) collect(i - 2, which);  // frees its sums for this chunk, and its operands for the next
@@ -359,7 +353,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
       b = b + 1 == kBuffers ? 0 : b + 1;
     };
     for (int i = 0; i < chunks && ok; i += 2) {
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->full[slot], full_phase, abort_flag, p.status, 138));
+      ok = warp_wait(&bars->full[slot], full_phase, abort_flag, p.status, 138);
       if (!ok) break;
       chunk(i, std::integral_constant<int, 0>{});
       if (ok && i + 1 < chunks) chunk(i + 1, std::integral_constant<int, 1>{});
@@ -409,7 +403,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
       for (int i = 0; i < NH; ++i) {
         const int t = wg * NH + i;
         if (t < here)
-          softmax::Elem<T>::store1(out + static_cast<int64_t>(token0 + t) * p.n + row_base + row, p.a_scales ? acc[i] * p.a_scales[token0 + t] : acc[i]);
+          softmax::Elem<T>::store1(out + static_cast<int64_t>(token0 + t) * p.n + row_base + row, kEight ? acc[i] * p.a_scales[token0 + t] : acc[i]);
       }
     }
     return;
@@ -428,7 +422,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
     float sum = 0.f;
 #pragma unroll 4
     for (int q = 0; q < p.splits; ++q) sum += ptx::ld_shared_cluster_f32(ptx::mapa_shared(ptx::smem_u32(red + i), q));
-    softmax::Elem<T>::store1(out + static_cast<int64_t>(t) * p.n + r, p.a_scales ? sum * p.a_scales[t] : sum);
+    softmax::Elem<T>::store1(out + static_cast<int64_t>(t) * p.n + r, kEight ? sum * p.a_scales[t] : sum);
   }
   ptx::cluster_sync_all();  // the others have read this CTA's sums
 }

@@ -5,6 +5,7 @@
 
 #include <type_traits>
 
+#include "ptx.cuh"
 #include "softmax.cuh"
 
 namespace tsm100 {
@@ -59,36 +60,97 @@ __device__ __forceinline__ int sequence_of(const Batch& s, int token) {
   return lo > 0 && token < s.starts[lo] ? lo - 1 : -1;
 }
 
-// A warp per row of a token: (token, k or v, head).
-template <typename T, bool kI8, bool kRead>
-__global__ void __launch_bounds__(256)
+// Rows of tokens, numbered (token, k or v, head): LANES threads have a row, eight numbers each (LANES times 8 is d or the next power of two), and kPasses rows in
+// turn, all of whose loads are on their way before the first is used.
+// Bound: HBM.  A search for its first token's sequence is all that a CTA does besides; the tokens behind it are a step or two away.
+constexpr int kThreads = 256, kPasses = 4;
+
+template <typename T, bool kI8, bool kRead, int LANES>
+__global__ void __launch_bounds__(kThreads)
 kv_page_rows_kernel(const Cache c, const Batch s, T* k, T* v, uint32_t* status) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (i >= static_cast<int64_t>(s.tokens) * 2 * c.heads) return;
-  const int head = static_cast<int>(i % c.heads), which = static_cast<int>(i / c.heads & 1), token = static_cast<int>(i / c.heads / 2);
-  const int b = sequence_of(s, token);
-  int first, count, len;
-  if (b < 0 || !sequence(s, c.page_size, b, first, count, len, status, 1)) return;
-  const int pos = len - count + token - first;
-  const int page = page_of(c, s, b, pos, status, 2);
-  if (page < 0) return;
-  T* mine = (which ? v : k) + (static_cast<int64_t>(token) * c.heads + head) * c.d;
-  const int64_t row = (static_cast<int64_t>(page) * c.heads + head) * c.page_size + pos % c.page_size;
+  constexpr int kRows = kThreads / LANES;  // of a pass
+  using softmax::Elem;
+  using softmax::Vec16;
+  ptx::launch_dependents_if_few();
+  ptx::wait_prior_grid();
+  const int lane = threadIdx.x % LANES, e = lane * 8, per_token = 2 * c.heads;
+  const int64_t first_row = static_cast<int64_t>(blockIdx.x) * (kRows * kPasses);
+  int b = -1;
+  {
+    __shared__ int found;
+    if (threadIdx.x == 0) found = sequence_of(s, static_cast<int>(first_row / per_token));
+    __syncthreads();
+    b = found;
+  }
+  const bool inside = e < c.d;
+  T* mine[kPasses];
+  int64_t row[kPasses];  // of the cache; -1: none
+  int which[kPasses];
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int64_t r = first_row + i * kRows + threadIdx.x / LANES;
+    row[i] = -1;
+    mine[i] = nullptr;
+    which[i] = 0;
+    const int64_t token = r / per_token;
+    if (b < 0 || token >= s.tokens) continue;  // no sequence starts at a CTA's first token or before: none does at a later one unless starts run backwards
+    const int in_token = static_cast<int>(r - token * per_token), head = in_token % c.heads;
+    which[i] = in_token / c.heads;
+    while (b + 1 < s.batch && token >= s.starts[b + 1]) ++b;
+    int first, count, len;
+    if (token >= s.starts[b + 1] || !sequence(s, c.page_size, b, first, count, len, status, 141)) continue;
+    const int pos = len - count + static_cast<int>(token) - first;
+    const int page = page_of(c, s, b, pos, status, 142);
+    if (page < 0) continue;
+    row[i] = (static_cast<int64_t>(page) * c.heads + head) * c.page_size + pos % c.page_size;
+    mine[i] = (which[i] ? v : k) + (token * c.heads + head) * c.d + e;
+  }
+  auto held = [&](int i) { return static_cast<uint8_t*>(which[i] ? c.kv[1] : c.kv[0]) + (row[i] * c.d + e) * (kI8 ? 1 : 2); };
+  auto step_at = [&](int i) { return (which[i] ? c.scales[1] : c.scales[0]) + row[i]; };
   if constexpr (!kI8) {
-    T* held = static_cast<T*>(c.kv[which]) + row * c.d;
-    for (int j = lane; j < c.d; j += 32) (kRead ? mine : held)[j] = (kRead ? held : mine)[j];
+    Vec16 x[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i)
+      if (row[i] >= 0 && inside) x[i] = softmax::ld_stream(kRead ? reinterpret_cast<const Vec16*>(held(i)) : reinterpret_cast<const Vec16*>(mine[i]));
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i)
+      if (row[i] >= 0 && inside) *(kRead ? reinterpret_cast<Vec16*>(mine[i]) : reinterpret_cast<Vec16*>(held(i))) = x[i];
+  } else if constexpr (kRead) {
+    uint2 x[kPasses];
+    float step[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i)
+      if (row[i] >= 0 && inside) x[i] = __ldcs(reinterpret_cast<const uint2*>(held(i))), step[i] = *step_at(i);
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      if (row[i] < 0 || !inside) continue;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = static_cast<float>(static_cast<int8_t>((j < 4 ? x[i].x : x[i].y) >> (8 * (j & 3)))) * step[i];
+      softmax::st_stream(reinterpret_cast<Vec16*>(mine[i]), Elem<T>::pack(f));
+    }
   } else {
-    int8_t* held = static_cast<int8_t*>(c.kv[which]) + row * c.d;
-    if constexpr (kRead) {
-      const float step = c.scales[which][row];
-      for (int j = lane; j < c.d; j += 32) softmax::Elem<T>::store1(mine + j, held[j] * step);
-    } else {
-      float top = 0.f;
-      for (int j = lane; j < c.d; j += 32) top = fmaxf(top, fabsf(softmax::Elem<T>::load1(mine + j)));
-      const float step = softmax::warp_max(top) * static_cast<float>(1.0 / 127.0);
-      for (int j = lane; j < c.d; j += 32) held[j] = static_cast<int8_t>(step > 0.f ? __float2int_rn(softmax::Elem<T>::load1(mine + j) / step) : 0);
-      if (lane == 0) c.scales[which][row] = step;
+    Vec16 x[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      x[i] = Vec16{};
+      if (row[i] >= 0 && inside) x[i] = softmax::ld_stream(reinterpret_cast<const Vec16*>(mine[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      float f[8], top = 0.f;
+      Elem<T>::unpack(x[i], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j]));
+#pragma unroll
+      for (int off = LANES / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      if (row[i] < 0 || !inside) continue;
+      const float step = top * static_cast<float>(1.0 / 127.0);
+      uint32_t q[2] = {0u, 0u};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j >> 2] |= (static_cast<uint32_t>(step > 0.f ? __float2int_rn(f[j] / step) : 0) & 0xffu) << (8 * (j & 3));
+      *reinterpret_cast<uint2*>(held(i)) = make_uint2(q[0], q[1]);
+      if (lane == 0) *step_at(i) = step;
     }
   }
 }

@@ -46,6 +46,7 @@ inline int32_t take_scratch(std::string* err, void** ws, size_t bytes, cudaStrea
 
 inline size_t dtype_size(int32_t dtype) { return dtype == TSM100_F32 ? 4 : 2; }
 inline bool dtype_valid(int32_t dtype) { return dtype == TSM100_F32 || dtype == TSM100_F16 || dtype == TSM100_BF16; }
+inline bool dtype_16bit(int32_t dtype) { return dtype == TSM100_F16 || dtype == TSM100_BF16; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---------------------------------------------------------------------------

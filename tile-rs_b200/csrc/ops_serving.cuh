@@ -1,4 +1,4 @@
-// Host-side launch logic of the serving operators (residual norm, 4-bit weights, paged KV cache and its attention): argument checks, kernel
+// Host-side launch logic of the serving operators (residual norm, paged KV cache and its attention): argument checks, kernel
 // selection, launch.  As in ops.cuh nothing here synchronises and every function answers a TSM100_* status with a message in *err.
 #pragma once
 
@@ -7,18 +7,43 @@
 
 #include "add_rms_norm.cuh"
 #include "attention_paged.cuh"
-#include "gemm_w4.cuh"
 #include "kv_pages.cuh"
 #include "launch.cuh"
 
 namespace tsm100 {
 namespace ops {
 
-inline bool dtype_16bit(int32_t dtype) { return dtype == TSM100_F16 || dtype == TSM100_BF16; }
-
 // ---------------------------------------------------------------------------
 // residual norm
 // ---------------------------------------------------------------------------
+template <typename T, bool kI8>
+inline cudaError_t add_rms_norm_launch(const addnorm::Params<T>& p, cudaStream_t s) {
+  namespace an = addnorm;
+  constexpr int PV = softmax::Elem<T>::kPerVec;
+  const int64_t vecs = p.cols / PV;
+  bool vec = p.cols % PV == 0 && vecs <= 8 * an::kThreads;
+  for (const void* q : {static_cast<const void*>(p.x), static_cast<const void*>(p.residual), static_cast<const void*>(p.sum), static_cast<const void*>(p.weight)})
+    vec = vec && aligned16(q);
+  vec = vec && (kI8 ? reinterpret_cast<uintptr_t>(p.y) % PV == 0 : aligned16(p.y));
+  const unsigned rows = static_cast<unsigned>(p.rows);
+  auto go = [&](auto kern, unsigned grid) { return launch_chained(kern, grid, an::kThreads, 0, s, 0, p); };
+  if (vec) {
+    // a warp a row as long as that is four vectors a lane, and there are rows for its lanes
+    const unsigned warps = (rows + 7) / 8;
+    if (vecs <= 32) return go(an::add_rms_norm_vec_kernel<T, kI8, 32, 1>, warps);
+    if (vecs <= 64) return go(an::add_rms_norm_vec_kernel<T, kI8, 32, 2>, warps);
+    if (vecs <= 128) return go(an::add_rms_norm_vec_kernel<T, kI8, 32, 4>, warps);
+    if (vecs <= an::kThreads) return go(an::add_rms_norm_vec_kernel<T, kI8, an::kThreads, 1>, rows);
+    if (vecs <= 2 * an::kThreads) return go(an::add_rms_norm_vec_kernel<T, kI8, an::kThreads, 2>, rows);
+    if (vecs <= 4 * an::kThreads) return go(an::add_rms_norm_vec_kernel<T, kI8, an::kThreads, 4>, rows);
+    return go(an::add_rms_norm_vec_kernel<T, kI8, an::kThreads, 8>, rows);
+  }
+  if (p.cols <= 4 * an::kThreads) return go(an::add_rms_norm_any_kernel<T, kI8, 4>, rows);
+  if (p.cols <= 12 * an::kThreads) return go(an::add_rms_norm_any_kernel<T, kI8, 12>, rows);
+  if (p.cols <= 32 * an::kThreads) return go(an::add_rms_norm_any_kernel<T, kI8, 32>, rows);
+  return go(an::add_rms_norm_any_kernel<T, kI8, 0>, rows);
+}
+
 template <typename T>
 inline int32_t add_rms_norm_typed(std::string* err, const tsm100_add_rms_norm_desc* d, const void* x, const void* residual, void* sum, const void* weight,
                                   void* y, float* scales, cudaStream_t s) {
@@ -32,10 +57,7 @@ inline int32_t add_rms_norm_typed(std::string* err, const tsm100_add_rms_norm_de
   p.rows = d->rows;
   p.cols = static_cast<int32_t>(d->cols);
   p.eps = d->eps;
-  const unsigned grid = static_cast<unsigned>(d->rows);
-  if (d->out_dtype == TSM100_I8) addnorm::add_rms_norm_kernel<T, true><<<grid, addnorm::kThreads, 0, s>>>(p);
-  else addnorm::add_rms_norm_kernel<T, false><<<grid, addnorm::kThreads, 0, s>>>(p);
-  return cuda_ok(err, cudaGetLastError(), "add_rms_norm launch");
+  return cuda_ok(err, d->out_dtype == TSM100_I8 ? add_rms_norm_launch<T, true>(p, s) : add_rms_norm_launch<T, false>(p, s), "add_rms_norm launch");
 }
 
 inline int32_t add_rms_norm(std::string* err, const tsm100_add_rms_norm_desc* d, const void* x, const void* residual, void* sum, const void* weight, void* y,
@@ -59,83 +81,6 @@ inline int32_t add_rms_norm(std::string* err, const tsm100_add_rms_norm_desc* d,
     case TSM100_BF16: return add_rms_norm_typed<__nv_bfloat16>(err, d, x, residual, sum, weight, y, scales, s);
     default: return add_rms_norm_typed<__half>(err, d, x, residual, sum, weight, y, scales, s);
   }
-}
-
-// ---------------------------------------------------------------------------
-// 4-bit weights
-// ---------------------------------------------------------------------------
-// CTAs of a cluster along K: until the GPU has its `places`, each with two steps of K or more.
-inline int gemm_w4_splits(int64_t n, int64_t k, int64_t token_blocks, int64_t places) {
-  const int64_t steps = (k + w4::kStepK - 1) / w4::kStepK, tiles = (n + w4::kRows - 1) / w4::kRows * token_blocks;
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= places && steps / (2 * splits) >= 2) splits *= 2;
-  return splits;
-}
-
-template <typename T, int N, int GC, bool kScaled = false>
-inline int32_t gemm_w4_launch(std::string* err, const CUtensorMap& map, w4::Params p, int sms, cudaStream_t s) {
-  using S = w4::Shape<N, GC, kScaled>;
-  const int blocks = (p.m + N - 1) / N;
-  p.tokens = ((p.m + blocks - 1) / blocks + 15) / 16 * 16;
-  p.splits = gemm_w4_splits(p.n, p.k, blocks, S::kTwo ? 2ll * sms : sms);
-  auto kern = w4::gemm_w4_kernel<T, N, GC, kScaled>;
-  cudaError_t e = set_dyn_smem_once(kern, S::kSmem);
-  const dim3 grid(static_cast<unsigned>((p.n + w4::kRows - 1) / w4::kRows * p.splits), static_cast<unsigned>((p.m + p.tokens - 1) / p.tokens));
-  if (e == cudaSuccess) e = launch_chained(kern, grid, w4::kThreads, S::kSmem, s, p.splits > 1 ? p.splits : 0, map, p);
-  return cuda_ok(err, e, "gemm_w4_kernel launch");
-}
-template <typename T, int GC>
-inline int32_t gemm_w4_grouped(std::string* err, const CUtensorMap& map, const w4::Params& p, int sms, cudaStream_t s) {
-  if (p.m <= 16) return gemm_w4_launch<T, 16, GC>(err, map, p, sms, s);
-  if (p.m > w4::kExactTokens) return gemm_w4_launch<T, 128, GC, true>(err, map, p, sms, s);
-  if constexpr (GC <= 2)
-    if (p.m > 32) return gemm_w4_launch<T, 64, GC>(err, map, p, sms, s);
-  return gemm_w4_launch<T, 32, GC>(err, map, p, sms, s);
-}
-template <typename T>
-inline int32_t gemm_w4_typed(std::string* err, const tsm100_gemm_w4_desc* d, const uint8_t* w, const w4::Params& p, cudaStream_t s) {
-  int sms = 0;
-  int32_t st = sm_count(err, &sms);
-  if (st != TSM100_OK) return st;
-  if (d->k == 0) return cuda_ok(err, cudaMemsetAsync(p.c, 0, static_cast<size_t>(d->m) * d->n * sizeof(T), s), "cudaMemsetAsync");
-  CUtensorMap map;
-  st = make_tmap_3d(err, &map, w, d->k / 2, d->n, 1, d->k / 2, static_cast<uint64_t>(d->n) * (d->k / 2), w4::kStepK / 2, w4::kRows,
-                    CU_TENSOR_MAP_DATA_TYPE_UINT8, 1);
-  if (st != TSM100_OK) return st;
-  switch (d->group) {
-    case 32: return gemm_w4_grouped<T, 4>(err, map, p, sms, s);
-    case 64: return gemm_w4_grouped<T, 2>(err, map, p, sms, s);
-    default: return gemm_w4_grouped<T, 1>(err, map, p, sms, s);
-  }
-}
-
-inline int32_t gemm_w4(std::string* err, const tsm100_gemm_w4_desc* d, const void* a, const float* a_scales, const uint8_t* w, const void* w_scales,
-                       const uint8_t* w_zeros, void* c, uint32_t* status, void* stream) {
-  if (!d) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: null descriptor");
-  if (!dtype_16bit(d->dtype)) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: dtype must be TSM100_F16 or TSM100_BF16");
-  if (d->a_dtype != d->dtype && d->a_dtype != TSM100_I8) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: a_dtype must be dtype or TSM100_I8");
-  if (d->group != 32 && d->group != 64 && d->group != 128) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: group must be 32, 64 or 128");
-  if (d->m < 0 || d->n < 0 || d->k < 0 || d->m > 0x7fffffff || d->n > 0x7fffffff || d->k > 0x7fffffff)
-    return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: bad shape");
-  if (d->k % d->group != 0) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: k must be a multiple of group");
-  if (d->m == 0 || d->n == 0) return TSM100_OK;
-  if (d->m > 64 * 65535) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: too many rows for one launch");
-  if (!c || (d->k > 0 && (!a || !w || !w_scales))) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: null buffer");
-  if (d->a_dtype == TSM100_I8 && !a_scales) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: rows in 8 bits need a_scales");
-  if (!aligned16(a) || !aligned16(w)) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: a and w must be 16-byte aligned");
-  if ((reinterpret_cast<uintptr_t>(w_scales) | reinterpret_cast<uintptr_t>(c)) & 1u || reinterpret_cast<uintptr_t>(a_scales) & 3u)
-    return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: a buffer does not start on an element boundary");
-  w4::Params p;
-  p.a = a;
-  p.a_scales = d->a_dtype == TSM100_I8 ? a_scales : nullptr;
-  p.scales = w_scales;
-  p.zeros = w_zeros;
-  p.c = c;
-  p.m = static_cast<int32_t>(d->m), p.n = static_cast<int32_t>(d->n), p.k = static_cast<int32_t>(d->k);
-  p.groups = static_cast<int32_t>(d->k / d->group);
-  p.status = status;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return d->dtype == TSM100_BF16 ? gemm_w4_typed<__nv_bfloat16>(err, d, w, p, s) : gemm_w4_typed<__half>(err, d, w, p, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -174,12 +119,18 @@ inline int32_t paged_args(std::string* err, const char* op, const tsm100_paged_k
   return TSM100_OK;
 }
 
+template <typename T, bool kI8, bool kRead, int LANES>
+inline cudaError_t kv_page_rows_launch(const pages::Cache& c, const pages::Batch& b, T* k, T* v, uint32_t* status, cudaStream_t s) {
+  if constexpr (LANES < 32)
+    if (c.d > 8 * LANES) return kv_page_rows_launch<T, kI8, kRead, 2 * LANES>(c, b, k, v, status, s);
+  constexpr int64_t kRows = pages::kThreads / LANES * pages::kPasses;  // of a CTA
+  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(b.tokens) * 2 * c.heads + kRows - 1) / kRows);
+  return launch_chained(pages::kv_page_rows_kernel<T, kI8, kRead, LANES>, grid, pages::kThreads, 0, s, 0, c, b, k, v, status);
+}
 template <typename T, bool kRead>
-inline cudaError_t kv_page_rows_launch(const pages::Cache& c, const pages::Batch& b, bool i8, void* k, void* v, uint32_t* status, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(b.tokens) * 2 * c.heads + 7) / 8);
-  if (i8) pages::kv_page_rows_kernel<T, true, kRead><<<grid, 256, 0, s>>>(c, b, static_cast<T*>(k), static_cast<T*>(v), status);
-  else pages::kv_page_rows_kernel<T, false, kRead><<<grid, 256, 0, s>>>(c, b, static_cast<T*>(k), static_cast<T*>(v), status);
-  return cudaGetLastError();
+inline cudaError_t kv_page_rows_typed(const pages::Cache& c, const pages::Batch& b, bool i8, void* k, void* v, uint32_t* status, cudaStream_t s) {
+  return i8 ? kv_page_rows_launch<T, true, kRead, 2>(c, b, static_cast<T*>(k), static_cast<T*>(v), status, s)
+            : kv_page_rows_launch<T, false, kRead, 2>(c, b, static_cast<T*>(k), static_cast<T*>(v), status, s);
 }
 
 template <bool kRead>
@@ -196,8 +147,8 @@ inline int32_t kv_page_rows(std::string* err, const tsm100_paged_kv* kv, const t
   if (static_cast<int64_t>(step.tokens) * 2 * c.heads / 8 >= 0x7fffffff) return op_fail(err, TSM100_ERR_INVALID, std::string(op) + ": too many tokens for one launch");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool i8 = kv->dtype == TSM100_I8;
-  return cuda_ok(err, dtype == TSM100_BF16 ? kv_page_rows_launch<__nv_bfloat16, kRead>(c, step, i8, k, v, status, s)
-                                           : kv_page_rows_launch<__half, kRead>(c, step, i8, k, v, status, s), op);
+  return cuda_ok(err, dtype == TSM100_BF16 ? kv_page_rows_typed<__nv_bfloat16, kRead>(c, step, i8, k, v, status, s)
+                                           : kv_page_rows_typed<__half, kRead>(c, step, i8, k, v, status, s), op);
 }
 
 // ---------------------------------------------------------------------------

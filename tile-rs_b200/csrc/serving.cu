@@ -1,6 +1,7 @@
 // C-ABI operators around the intrinsics in a serving step: tsm100_add_rms_norm / _gemm_w4 / _kv_page_append / _kv_page_read / _attention_paged.
 #include "common.hpp"
 #include "ops_serving.cuh"
+#include "ops_w4.cuh"
 
 using namespace tsm100;
 
