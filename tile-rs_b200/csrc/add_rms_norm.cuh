@@ -8,6 +8,7 @@
 // time from the caches.
 #pragma once
 
+#include "quantise.cuh"
 #include "softmax.cuh"
 
 namespace tsm100 {
@@ -44,9 +45,6 @@ __device__ __forceinline__ float2 row_sum_max(float2 v, float2* red) {
   for (int w = 1; w < LANES / 32; ++w) v.x += red[w].x, v.y = fmaxf(v.y, red[w].y);
   return v;
 }
-__device__ __forceinline__ float step_of(float top) { return top * static_cast<float>(1.0 / 127.0); }
-__device__ __forceinline__ uint32_t quantised(float z, float step) { return static_cast<uint32_t>(step > 0.f ? __float2int_rn(z / step) : 0) & 0xffu; }
-
 // Every buffer and row on 16-byte boundaries (y in 8 bits: on as many bytes as a vector has elements); VPT vectors a thread.
 template <typename T, bool kI8, int LANES, int VPT>
 __global__ void __launch_bounds__(kThreads)
@@ -99,7 +97,8 @@ add_rms_norm_vec_kernel(const Params<T> p) {
     }
   }
   acc = row_sum_max<LANES>(acc, red);
-  const float r = rsqrtf(acc.x / p.cols + p.eps), step = step_of(acc.y);
+  const float r = rsqrtf(acc.x / p.cols + p.eps);
+  const quant::Step step = kI8 ? quant::step_of(acc.y) : quant::Step{};
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
     const int i = k * LANES + lane;
@@ -107,8 +106,7 @@ add_rms_norm_vec_kernel(const Params<T> p) {
     if constexpr (kI8) {
       uint32_t q[PV / 4];
 #pragma unroll
-      for (int j = 0; j < PV / 4; ++j)
-        q[j] = quantised(h[k][4 * j], step) | quantised(h[k][4 * j + 1], step) << 8 | quantised(h[k][4 * j + 2], step) << 16 | quantised(h[k][4 * j + 3], step) << 24;
+      for (int j = 0; j < PV / 4; ++j) q[j] = quant::quantise4(h[k] + 4 * j, step);
       uint8_t* to = static_cast<uint8_t*>(p.y) + row * p.cols + static_cast<int64_t>(i) * PV;
       if constexpr (PV == 8) *reinterpret_cast<uint2*>(to) = make_uint2(q[0], q[PV / 4 - 1]);
       else *reinterpret_cast<uint32_t*>(to) = q[0];
@@ -118,7 +116,7 @@ add_rms_norm_vec_kernel(const Params<T> p) {
       softmax::st_stream(reinterpret_cast<Vec16*>(static_cast<T*>(p.y) + row * p.cols) + i, Elem<T>::pack(h[k]));
     }
   }
-  if (kI8 && lane == 0) p.scales[row] = step * r;
+  if (kI8 && lane == 0) p.scales[row] = step.step * r;
 }
 
 // Rows that start anywhere.  EPT > 0: that many elements a thread in registers; 0: any width, read twice (sum is written on the second way, so that it may be x or
@@ -138,7 +136,17 @@ add_rms_norm_any_kernel(const Params<T> p) {
 #pragma unroll
     for (int k = 0; k < EPT; ++k) {
       const int c = k * kThreads + threadIdx.x;
-      h[k] = c < p.cols ? h_of(c) : 0.f;
+      h[k] = c < p.cols ? Elem<T>::load1(p.x + at + c) : 0.f;
+    }
+    if (p.residual) {
+      float b[EPT];
+#pragma unroll
+      for (int k = 0; k < EPT; ++k) {
+        const int c = k * kThreads + threadIdx.x;
+        b[k] = c < p.cols ? Elem<T>::load1(p.residual + at + c) : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < EPT; ++k) h[k] += b[k];
     }
 #pragma unroll
     for (int k = 0; k < EPT; ++k) {
@@ -157,9 +165,10 @@ add_rms_norm_any_kernel(const Params<T> p) {
     }
   }
   acc = row_sum_max<kThreads>(acc, red);
-  const float r = rsqrtf(acc.x / p.cols + p.eps), step = step_of(acc.y);
+  const float r = rsqrtf(acc.x / p.cols + p.eps);
+  const quant::Step step = kI8 ? quant::step_of(acc.y) : quant::Step{};
   auto put = [&](int c, float z) {
-    if (kI8) static_cast<uint8_t*>(p.y)[at + c] = static_cast<uint8_t>(quantised(z, step));
+    if (kI8) static_cast<int8_t*>(p.y)[at + c] = static_cast<int8_t>(step.step > 0.f ? __float2int_rn(z / step.step) : 0);
     else Elem<T>::store1(static_cast<T*>(p.y) + at + c, z * r);
   };
   if constexpr (EPT > 0) {
@@ -175,7 +184,7 @@ add_rms_norm_any_kernel(const Params<T> p) {
       put(c, z);
     }
   }
-  if (kI8 && threadIdx.x == 0) p.scales[blockIdx.x] = step * r;
+  if (kI8 && threadIdx.x == 0) p.scales[blockIdx.x] = step.step * r;
 }
 
 }  // namespace addnorm

@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "ptx.cuh"
+#include "quantise.cuh"
 #include "softmax.cuh"
 
 namespace tsm100 {
@@ -60,97 +61,96 @@ __device__ __forceinline__ int sequence_of(const Batch& s, int token) {
   return lo > 0 && token < s.starts[lo] ? lo - 1 : -1;
 }
 
-// Rows of tokens, numbered (token, k or v, head): LANES threads have a row, eight numbers each (LANES times 8 is d or the next power of two), and kPasses rows in
-// turn, all of whose loads are on their way before the first is used.
-// Bound: HBM.  A search for its first token's sequence is all that a CTA does besides; the tokens behind it are a step or two away.
-constexpr int kThreads = 256, kPasses = 4;
+// A CTA has `per_cta` tokens.  Where those lie is found first, a token to a thread; then LANES threads have a row of a token (k or v, head), eight numbers each
+// (LANES times 8 is d or the next power of two), and kPasses rows in turn, all of whose loads are on their way before the first is used.
+// Bound: HBM.
+constexpr int kThreads = 256, kPasses = 4, kMaxTokens = 32;
 
 template <typename T, bool kI8, bool kRead, int LANES>
 __global__ void __launch_bounds__(kThreads)
-kv_page_rows_kernel(const Cache c, const Batch s, T* k, T* v, uint32_t* status) {
+kv_page_rows_kernel(const Cache c, const Batch s, T* k, T* v, int32_t per_cta, uint32_t* status) {
   constexpr int kRows = kThreads / LANES;  // of a pass
   using softmax::Elem;
   using softmax::Vec16;
+  __shared__ int64_t place[kMaxTokens];    // of a token in its page's first head, in rows of the cache; -1: it has none
   ptx::launch_dependents_if_few();
   ptx::wait_prior_grid();
-  const int lane = threadIdx.x % LANES, e = lane * 8, per_token = 2 * c.heads;
-  const int64_t first_row = static_cast<int64_t>(blockIdx.x) * (kRows * kPasses);
-  int b = -1;
-  {
-    __shared__ int found;
-    if (threadIdx.x == 0) found = sequence_of(s, static_cast<int>(first_row / per_token));
-    __syncthreads();
-    b = found;
-  }
-  const bool inside = e < c.d;
-  T* mine[kPasses];
-  int64_t row[kPasses];  // of the cache; -1: none
-  int which[kPasses];
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int64_t r = first_row + i * kRows + threadIdx.x / LANES;
-    row[i] = -1;
-    mine[i] = nullptr;
-    which[i] = 0;
-    const int64_t token = r / per_token;
-    if (b < 0 || token >= s.tokens) continue;  // no sequence starts at a CTA's first token or before: none does at a later one unless starts run backwards
-    const int in_token = static_cast<int>(r - token * per_token), head = in_token % c.heads;
-    which[i] = in_token / c.heads;
-    while (b + 1 < s.batch && token >= s.starts[b + 1]) ++b;
+  const int token0 = static_cast<int>(blockIdx.x) * per_cta;
+  if (static_cast<int>(threadIdx.x) < per_cta) {
+    const int token = token0 + threadIdx.x;
+    int64_t at = -1;
+    const int b = token < s.tokens ? sequence_of(s, token) : -1;
     int first, count, len;
-    if (token >= s.starts[b + 1] || !sequence(s, c.page_size, b, first, count, len, status, 141)) continue;
-    const int pos = len - count + static_cast<int>(token) - first;
-    const int page = page_of(c, s, b, pos, status, 142);
-    if (page < 0) continue;
-    row[i] = (static_cast<int64_t>(page) * c.heads + head) * c.page_size + pos % c.page_size;
-    mine[i] = (which[i] ? v : k) + (token * c.heads + head) * c.d + e;
+    if (b >= 0 && sequence(s, c.page_size, b, first, count, len, status, 141)) {
+      const int pos = len - count + token - first, page = page_of(c, s, b, pos, status, 142);
+      if (page >= 0) at = static_cast<int64_t>(page) * c.heads * c.page_size + pos % c.page_size;
+    }
+    place[threadIdx.x] = at;
   }
-  auto held = [&](int i) { return static_cast<uint8_t*>(which[i] ? c.kv[1] : c.kv[0]) + (row[i] * c.d + e) * (kI8 ? 1 : 2); };
-  auto step_at = [&](int i) { return (which[i] ? c.scales[1] : c.scales[0]) + row[i]; };
-  if constexpr (!kI8) {
-    Vec16 x[kPasses];
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i)
-      if (row[i] >= 0 && inside) x[i] = softmax::ld_stream(kRead ? reinterpret_cast<const Vec16*>(held(i)) : reinterpret_cast<const Vec16*>(mine[i]));
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i)
-      if (row[i] >= 0 && inside) *(kRead ? reinterpret_cast<Vec16*>(mine[i]) : reinterpret_cast<Vec16*>(held(i))) = x[i];
-  } else if constexpr (kRead) {
-    uint2 x[kPasses];
-    float step[kPasses];
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i)
-      if (row[i] >= 0 && inside) x[i] = __ldcs(reinterpret_cast<const uint2*>(held(i))), step[i] = *step_at(i);
+  __syncthreads();
+  const int lane = threadIdx.x % LANES, e = lane * 8, per_token = 2 * c.heads;
+  const bool inside = e < c.d;
+  int row = threadIdx.x / LANES, token = row / per_token;  // of the CTA's
+  row -= token * per_token;
+  const int rounds = (per_cta * per_token + kRows * kPasses - 1) / (kRows * kPasses);
+  for (int round = 0; round < rounds; ++round) {
+    T* mine[kPasses];
+    int64_t at[kPasses];  // -1: none
+    bool second[kPasses];
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      if (row[i] < 0 || !inside) continue;
-      float f[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = static_cast<float>(static_cast<int8_t>((j < 4 ? x[i].x : x[i].y) >> (8 * (j & 3)))) * step[i];
-      softmax::st_stream(reinterpret_cast<Vec16*>(mine[i]), Elem<T>::pack(f));
+      at[i] = token < per_cta ? place[token] : -1;
+      second[i] = row >= c.heads;
+      const int head = second[i] ? row - c.heads : row;
+      if (at[i] >= 0) at[i] += static_cast<int64_t>(head) * c.page_size;
+      mine[i] = (second[i] ? v : k) + (static_cast<int64_t>(token0 + token) * c.heads + head) * c.d + e;
+      row += kRows;
+      while (row >= per_token) row -= per_token, ++token;
     }
-  } else {
-    Vec16 x[kPasses];
+    auto held = [&](int i) { return static_cast<uint8_t*>(second[i] ? c.kv[1] : c.kv[0]) + (at[i] * c.d + e) * (kI8 ? 1 : 2); };
+    auto step_at = [&](int i) { return (second[i] ? c.scales[1] : c.scales[0]) + at[i]; };
+    if constexpr (!kI8) {
+      Vec16 x[kPasses];
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      x[i] = Vec16{};
-      if (row[i] >= 0 && inside) x[i] = softmax::ld_stream(reinterpret_cast<const Vec16*>(mine[i]));
-    }
+      for (int i = 0; i < kPasses; ++i)
+        if (at[i] >= 0 && inside) x[i] = softmax::ld_stream(kRead ? reinterpret_cast<const Vec16*>(held(i)) : reinterpret_cast<const Vec16*>(mine[i]));
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      float f[8], top = 0.f;
-      Elem<T>::unpack(x[i], f);
+      for (int i = 0; i < kPasses; ++i)
+        if (at[i] >= 0 && inside) *(kRead ? reinterpret_cast<Vec16*>(mine[i]) : reinterpret_cast<Vec16*>(held(i))) = x[i];
+    } else if constexpr (kRead) {
+      uint2 x[kPasses];
+      float step[kPasses];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j]));
+      for (int i = 0; i < kPasses; ++i)
+        if (at[i] >= 0 && inside) x[i] = __ldcs(reinterpret_cast<const uint2*>(held(i))), step[i] = *step_at(i);
 #pragma unroll
-      for (int off = LANES / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      if (row[i] < 0 || !inside) continue;
-      const float step = top * static_cast<float>(1.0 / 127.0);
-      uint32_t q[2] = {0u, 0u};
+      for (int i = 0; i < kPasses; ++i) {
+        if (at[i] < 0 || !inside) continue;
+        float f[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q[j >> 2] |= (static_cast<uint32_t>(step > 0.f ? __float2int_rn(f[j] / step) : 0) & 0xffu) << (8 * (j & 3));
-      *reinterpret_cast<uint2*>(held(i)) = make_uint2(q[0], q[1]);
-      if (lane == 0) *step_at(i) = step;
+        for (int j = 0; j < 8; ++j) f[j] = quant::number(j < 4 ? x[i].x : x[i].y, j & 3) * step[i];
+        softmax::st_stream(reinterpret_cast<Vec16*>(mine[i]), Elem<T>::pack(f));
+      }
+    } else {
+      Vec16 x[kPasses];
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        x[i] = Vec16{};
+        if (at[i] >= 0 && inside) x[i] = softmax::ld_stream(reinterpret_cast<const Vec16*>(mine[i]));
+      }
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        float f[8], top = 0.f;
+        Elem<T>::unpack(x[i], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j]));
+#pragma unroll
+        for (int off = LANES / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        if (at[i] < 0 || !inside) continue;
+        const quant::Step step = quant::step_of(top);
+        *reinterpret_cast<uint2*>(held(i)) = make_uint2(quant::quantise4(f, step), quant::quantise4(f + 4, step));
+        if (lane == 0) *step_at(i) = step.step;
+      }
     }
   }
 }

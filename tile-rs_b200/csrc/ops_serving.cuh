@@ -40,6 +40,7 @@ inline cudaError_t add_rms_norm_launch(const addnorm::Params<T>& p, cudaStream_t
   }
   if (p.cols <= 4 * an::kThreads) return go(an::add_rms_norm_any_kernel<T, kI8, 4>, rows);
   if (p.cols <= 12 * an::kThreads) return go(an::add_rms_norm_any_kernel<T, kI8, 12>, rows);
+  if (p.cols <= 20 * an::kThreads) return go(an::add_rms_norm_any_kernel<T, kI8, 20>, rows);
   if (p.cols <= 32 * an::kThreads) return go(an::add_rms_norm_any_kernel<T, kI8, 32>, rows);
   return go(an::add_rms_norm_any_kernel<T, kI8, 0>, rows);
 }
@@ -123,9 +124,13 @@ template <typename T, bool kI8, bool kRead, int LANES>
 inline cudaError_t kv_page_rows_launch(const pages::Cache& c, const pages::Batch& b, T* k, T* v, uint32_t* status, cudaStream_t s) {
   if constexpr (LANES < 32)
     if (c.d > 8 * LANES) return kv_page_rows_launch<T, kI8, kRead, 2 * LANES>(c, b, k, v, status, s);
-  constexpr int64_t kRows = pages::kThreads / LANES * pages::kPasses;  // of a CTA
-  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(b.tokens) * 2 * c.heads + kRows - 1) / kRows);
-  return launch_chained(pages::kv_page_rows_kernel<T, kI8, kRead, LANES>, grid, pages::kThreads, 0, s, 0, c, b, k, v, status);
+  // eight rounds of rows to a CTA, so that finding their places counts for little, unless that left SMs without one
+  constexpr int kRows = pages::kThreads / LANES * pages::kPasses;
+  int sms = 148;
+  (void)sm_count(nullptr, &sms);
+  const int per_cta = std::max(1, std::min({pages::kMaxTokens, (8 * kRows + 2 * c.heads - 1) / (2 * c.heads), b.tokens / (4 * sms)}));
+  return launch_chained(pages::kv_page_rows_kernel<T, kI8, kRead, LANES>, static_cast<unsigned>((b.tokens + per_cta - 1) / per_cta), pages::kThreads, 0, s, 0, c, b, k, v,
+                        static_cast<int32_t>(per_cta), status);
 }
 template <typename T, bool kRead>
 inline cudaError_t kv_page_rows_typed(const pages::Cache& c, const pages::Batch& b, bool i8, void* k, void* v, uint32_t* status, cudaStream_t s) {

@@ -1,0 +1,46 @@
+// Rows of f32 as whole numbers of steps of their largest magnitude: step = max|x| * (1/127), q = x / step rounded to nearest even (the quotient in f32).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace tsm100 {
+namespace quant {
+
+struct Step {
+  float step, inv;
+};
+__device__ __forceinline__ Step step_of(float top) {
+  Step s;
+  s.step = top * static_cast<float>(1.0 / 127.0);
+  // NaN where the reciprocal is no use (zero, far from 1, not finite): every number then takes the division
+  s.inv = s.step >= 0x1p-120f && s.step <= 0x1p120f ? 1.f / s.step : __uint_as_float(0x7fffffffu);
+  return s;
+}
+// Four numbers as bytes.  A product with the reciprocal is within 4e-5 of the quotient, so both round alike unless that ends near a half; only then is it divided
+// (a tenth of the warps; dividing always made the append of 8192 tokens of 8 heads of 128 a third longer).  Adding 1.5 * 2^23 rounds to nearest
+// even and leaves the number in the low byte.
+__device__ __forceinline__ uint32_t quantise4(const float* x, const Step& s) {
+  constexpr float kMagic = 12582912.f;
+  float u[4];
+  bool divide = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float t = x[i] * s.inv;
+    u[i] = t + kMagic;
+    divide |= !(fabsf(t - (u[i] - kMagic)) <= 0.4999f);
+  }
+  if (divide) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = (s.step > 0.f ? x[i] / s.step : 0.f) + kMagic;
+  }
+  const uint32_t lo = __byte_perm(__float_as_uint(u[0]), __float_as_uint(u[1]), 0x0040), hi = __byte_perm(__float_as_uint(u[2]), __float_as_uint(u[3]), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+// Byte i of x, a whole number, as f32: behind 0x4b0000 it is 2^23 + 128 + q.
+__device__ __forceinline__ float number(uint32_t x, int i) {
+  return __uint_as_float(__byte_perm(x ^ 0x80808080u, 0x4b000000u, 0x7540 + i)) - 8388736.f;
+}
+
+}  // namespace quant
+}  // namespace tsm100
