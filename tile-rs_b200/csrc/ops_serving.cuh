@@ -7,6 +7,7 @@
 
 #include "add_rms_norm.cuh"
 #include "attention_paged.cuh"
+#include "attention_paged_tc.cuh"
 #include "kv_pages.cuh"
 #include "launch.cuh"
 
@@ -159,10 +160,78 @@ inline int32_t kv_page_rows(std::string* err, const tsm100_paged_kv* kv, const t
 // ---------------------------------------------------------------------------
 // attention over pages
 // ---------------------------------------------------------------------------
+// Positions that a TMA box of a page may have, as a power of two: one that the page is a multiple of, at most 2^top.
+inline int page_run_log2(int page_size, int top) {
+  int n = 0;
+  while (n < top && page_size % (2 << n) == 0) ++n;
+  return n;
+}
+// Boxes of 64 columns and 2^run_log2 positions of the pages.
+inline int32_t page_tmap(std::string* err, CUtensorMap* map, const pages::Cache& c, const void* base, int run_log2, bool is_bf16) {
+  const uint64_t d = static_cast<uint64_t>(c.d), rows = static_cast<uint64_t>(c.page_size);
+  return make_tmap_16bit_3d(err, map, base, d, rows, static_cast<uint64_t>(c.pages) * c.heads, d, rows * d, 64, 1u << run_log2, is_bf16);
+}
+
+// Chunks of tokens: tcgen05 (attention_paged_tc.cuh).
+template <typename T, bool kI8, int D>
+inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& base, int run_log2, const void* q, void* o, cudaStream_t s) {
+  namespace tc = paged::tc;
+  constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
+  using S = tc::Shape<kI8, D>;
+  int sms = 0;
+  int32_t st = sm_count(err, &sms);
+  if (st != TSM100_OK) return st;
+  const unsigned ctas = static_cast<unsigned>(sms);
+  tc::Params p;
+  p.cache = base.cache, p.step = base.step;
+  p.heads_q = base.heads_q, p.group = base.group;
+  p.tokens = tc::kTileRows / base.group;
+  p.run_log2 = run_log2;
+  p.scale_log2 = base.scale_log2;
+  p.status = base.status;
+  CUtensorMap tq, tk, tv;
+  TmapKey key;
+  std::memset(&key, 0, sizeof key);
+  key.base = q;
+  key.dim[0] = D, key.dim[1] = static_cast<uint64_t>(p.heads_q), key.dim[2] = static_cast<uint64_t>(p.step.tokens);
+  key.stride[0] = D * 2, key.stride[1] = static_cast<uint64_t>(p.heads_q) * D * 2;
+  key.box[0] = 64, key.box[1] = static_cast<uint32_t>(p.group), key.box[2] = static_cast<uint32_t>(p.tokens);
+  key.dtype = static_cast<int32_t>(kIsBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16), key.rank = 3;
+  st = make_tmap(err, &tq, key, 2);
+  if (kI8) {
+    tk = tv = tq;  // not used
+  } else {
+    if (st == TSM100_OK) st = page_tmap(err, &tk, p.cache, p.cache.kv[0], run_log2, kIsBf16);
+    if (st == TSM100_OK) st = page_tmap(err, &tv, p.cache, p.cache.kv[1], run_log2, kIsBf16);
+  }
+  if (st != TSM100_OK) return st;
+  const size_t rows = static_cast<size_t>(ctas) * 2 * 256, part = rows * D * sizeof(float), ml = rows * sizeof(float2);
+  uint8_t* ws = nullptr;
+  st = take_scratch(err, reinterpret_cast<void**>(&ws), part + ml + ctas * sizeof(int4), s);
+  if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged: no device memory for partial results");
+  if (st != TSM100_OK) return st;
+  p.part = reinterpret_cast<float4*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + part);
+  p.info = reinterpret_cast<int4*>(ws + part + ml);
+  auto kern = tc::attention_paged_tc_kernel<kIsBf16, kI8, D>;
+  constexpr int smem = tc::smem_bytes<kI8, D>();
+  cudaError_t e = set_dyn_smem_once(kern, smem);
+  if (e == cudaSuccess) e = launch_chained(kern, ctas, S::kThreads, smem, s, 0, tq, tk, tv, static_cast<uint16_t*>(o), p);
+  if (e == cudaSuccess) e = launch_chained(tc::attention_paged_tc_merge_kernel<kIsBf16, D>, dim3(ctas, D / 16), 256, 0, s, 0, static_cast<uint16_t*>(o), p);
+  st = cuda_ok(err, e, "attention_paged_tc_kernel launch");
+  e = cudaFreeAsync(ws, s);
+  if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
+  return st;
+}
+
 // The tiles of all sequences' caches dealt out evenly over the SMs, and what several of them have a part of merged (attention_paged.cuh).
 template <typename T, bool kI8, int D>
 inline int32_t attention_paged_launch(std::string* err, paged::Params p, const void* q, void* o, cudaStream_t s) {
   using L = paged::Tile<kI8, D>;
+  // more rows than a tile of mma.sync has would go over their keys again: tcgen05, as long as a group's heads fit a tile and boxes of eight positions a page
+  const int wide = page_run_log2(p.cache.page_size, 7);
+  if (static_cast<int64_t>(p.step.max_new) * p.group > paged::kRows && p.group <= paged::tc::kMaxGroup && (kI8 || wide >= 3))
+    return attention_paged_tc_launch<T, kI8, D>(err, p, wide, q, o, s);
   int sms = 0;
   int32_t st = sm_count(err, &sms);
   if (st != TSM100_OK) return st;
@@ -174,8 +243,7 @@ inline int32_t attention_paged_launch(std::string* err, paged::Params p, const v
   if (st != TSM100_OK) return st;
   p.info = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(p.part) + part);
   // boxes of a power of two of positions that a page is a multiple of; 8-bit steps come by copies of 16 bytes and more
-  int run_log2 = 0;
-  while ((2 << run_log2) <= L::kPos && p.cache.page_size % (2 << run_log2) == 0) ++run_log2;
+  const int run_log2 = page_run_log2(p.cache.page_size, L::kPos == 32 ? 5 : 6);
   const bool boxes = run_log2 >= 3 && (!kI8 || (aligned16(p.cache.scales[0]) && aligned16(p.cache.scales[1])));
   p.run_log2 = boxes ? run_log2 : L::kPos == 32 ? 5 : 6;
   CUtensorMap map[2];
