@@ -5,7 +5,7 @@
 //   * The rows of a tile are tokens times the heads of a group (row = token * group + head), so that a group's heads read K and V once and a chunk of a few tokens
 //     still fills a tile.  One TMA box brings them: 64 columns x group x tokens.
 //   * The work is one stream, dealt out evenly: blocks of up to two tiles are numbered through (sequence, KV head, block) with the keys they see as their length
-//     (times 3, or 2 where a block has one tile: 3240 and 2060 clocks a step), and every SM takes an equal, contiguous share of it, to the step.  Lengths are only
+//     (times 3, or 2 where a block has one tile: 3240 and 2060 clocks a step in attention_tc.cuh), and every SM takes an equal, contiguous share of it, to the step.  Lengths are only
 //     known on the device, prompts and single tokens come in one call, and 64 blocks over 148 SMs would leave half of them idle.  A block that is cut leaves (maximum, sum, O)
 //     for a merging kernel.
 //   * K and V come by pages: boxes of a power of two of positions (8 and more), a lane each.  What a page holds behind the sequence's end is
@@ -26,12 +26,14 @@ namespace tc {
 
 constexpr int kTileRows = 128, kKeys = 128;
 constexpr int kMaxGroup = 128;
+constexpr int kBlockCost = 3 * kKeys;      // beginning and ending a block, as a length: about a step of two tiles
 constexpr int kMinShare = 4 * 3 * kKeys;   // a share's length at least: four steps of two tiles
 template <bool kI8, int D>
 struct Shape {
   static constexpr int kThreads = kI8 ? 512 : 384;   // warps 0..3 softmax A, 4..7 softmax B, 8 TMA, 9 Q K^T, 10 P V, 11 idle, 12..15 conversion
   // registers after setmaxnreg; the shares of a block add up to what it was launched with
-  static constexpr int kRegsSoftmax = kI8 ? 192 : 216, kRegsOther = kI8 ? 56 : 72, kRegsConvert = 72;
+  static constexpr int kRegsSoftmax = kI8 ? 184 : 216, kRegsOther = kI8 ? 48 : 72, kRegsConvert = 96;
+  static constexpr int kLoneWeight = kI8 ? 3 : 2;     // a step of a block of one tile, against 3 of two: conversion takes as long for either
   static constexpr int kHalves = D / 64;
   static constexpr int kHalfBytes = 128 * 128;        // 128 rows x 64 columns
   static constexpr int kTileBytes = kHalves * kHalfBytes;
@@ -41,7 +43,7 @@ struct Shape {
   static constexpr int kStepTiles = kI8 ? (D == 128 ? 3 : 8) : 0;
   static constexpr int kPOff = 2 * kTileBytes, kRingOff = kPOff + 2 * kPBytes, kStepsOff = kRingOff + kRing * kTileBytes, kBarsOff = kStepsOff + kStepTiles * 512;
 };
-static_assert(256 * 192 + 128 * 56 + 128 * 72 <= 512 * 128 && 256 * 216 + 128 * 72 <= 384 * 168, "registers of a block at launch");
+static_assert(256 * 184 + 128 * 48 + 128 * 96 <= 512 * 128 && 256 * 216 + 128 * 72 <= 384 * 168, "registers of a block at launch");
 
 struct alignas(8) Barriers {
   uint64_t q_full, q_free;
@@ -64,6 +66,7 @@ struct Params {
   pages::Batch step;
   int32_t heads_q, group;
   int32_t tokens;      // of a tile: 128 / group
+  int32_t lone_weight; // Shape::kLoneWeight
   int32_t run_log2;    // positions of a page's box
   float scale_log2;
   float4* part;        // [CTA][2][D / 4][256 rows]: of a block that began in an earlier share, of one that goes on in the next
@@ -72,7 +75,7 @@ struct Params {
   uint32_t* status;
 };
 
-// The stream of blocks.  A block's length is the keys that its last token sees, times its weight.
+// The stream of blocks.  A block's length is the keys that its last token sees, times its weight, and kBlockCost.
 struct Seq {
   int b, first, count, len, blocks;
   int64_t per_head, base, end;
@@ -86,13 +89,13 @@ struct Work {
 };
 __device__ __forceinline__ int64_t full_blocks(const Params& p, const Seq& s, int64_t i) {  // the length of the first i blocks, which have two tiles
   const int64_t two = 2 * p.tokens;
-  return 3 * (i * (s.len - s.count) + two * (i * (i + 1) / 2));
+  return 3 * (i * (s.len - s.count) + two * (i * (i + 1) / 2)) + i * kBlockCost;
 }
-__device__ __forceinline__ int last_weight(const Params& p, const Seq& s) { return s.count - (s.blocks - 1) * 2 * p.tokens <= p.tokens ? 2 : 3; }
+__device__ __forceinline__ int last_weight(const Params& p, const Seq& s) { return s.count - (s.blocks - 1) * 2 * p.tokens <= p.tokens ? p.lone_weight : 3; }
 __device__ __forceinline__ int64_t sequence_length(const Params& p, int b, Seq& s, uint32_t* status) {
   if (!pages::sequence(p.step, p.cache.page_size, b, s.first, s.count, s.len, status, 145)) return 0;
   s.blocks = (s.count + 2 * p.tokens - 1) / (2 * p.tokens);
-  s.per_head = full_blocks(p, s, s.blocks - 1) + static_cast<int64_t>(s.len) * last_weight(p, s);
+  s.per_head = full_blocks(p, s, s.blocks - 1) + static_cast<int64_t>(s.len) * last_weight(p, s) + kBlockCost;
   return s.per_head * p.cache.heads;
 }
 struct Stream {
@@ -123,11 +126,13 @@ struct Stream {
       w.token0 = lo * 2 * p.tokens;
       const int keys = seq.len - seq.count + min(seq.count, w.token0 + 2 * p.tokens);
       w.steps = (keys + kKeys - 1) / kKeys;
-      const int64_t step = static_cast<int64_t>(weight) * kKeys, stop = min(to, in_head + (end - at));
-      w.begin = static_cast<int>((in_head - from + step - 1) / step);
-      w.n = static_cast<int>((stop - from + step - 1) / step) - w.begin;
+      const int step = weight * kKeys;  // a block's length fits 32 bits
+      const int64_t stop = min(to, in_head + (end - at));
+      auto steps_to = [&](int64_t x) { return static_cast<int>((static_cast<uint32_t>(max(x - from - kBlockCost, static_cast<int64_t>(0))) + step - 1) / step); };
+      w.begin = steps_to(in_head);
+      w.n = steps_to(stop) - w.begin;
       w.b = seq.b, w.first = seq.first, w.count = seq.count, w.len = seq.len, w.block = lo;
-      w.lone = weight == 2;
+      w.lone = last && seq.count - w.token0 <= p.tokens;
       const int keys_a = seq.len - seq.count + min(seq.count, w.token0 + p.tokens);
       w.n_a = max(0, min(w.n, (keys_a + kKeys - 1) / kKeys - w.begin));
       at += stop - in_head;
@@ -397,62 +402,76 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       int idx0 = 0;
       bool ok = true;
       while (ok && stream.next(p, w)) {
+        // A tile's page is asked for three tiles ahead, its steps two and its rows one, so that none of these loads is waited for.
         const int total = 2 * w.n;
-        auto step_of = [&](int i, bool& is_v) {
-          is_v = i == total - 1 || (i >= 2 && (i & 1) == 0);
-          return i == 0 ? 0 : i == total - 1 ? w.n - 1 : is_v ? (i >> 1) - 1 : (i + 1) >> 1;
+        auto second = [&](int i) { return i == total - 1 || (i >= 2 && (i & 1) == 0); };  // V
+        auto pos_of = [&](int i) { return (w.begin + (i == 0 ? 0 : i == total - 1 ? w.n - 1 : (i & 1) == 0 ? (i >> 1) - 1 : (i + 1) >> 1)) * kKeys + my_row; };
+        int32_t page = -1;        // of this lane's row of a tile
+        int64_t row_at = -1;      // -1: behind the sequence's end
+        float step_at = 0.f, step_next = 0.f;
+        uint4 next[kVecs];
+        auto ask_page = [&](int i) {
+          const int pos = pos_of(i);
+          page = i < total && pos < w.len ? p.step.table[static_cast<int64_t>(w.b) * p.step.pitch + pos / ps] : 0;
         };
-        int64_t at_row = -1;
-        float step_row = 0.f;
-        auto locate = [&](int i) {  // this lane's row of tile i, a tile ahead
-          bool is_v;
-          const int pos = (w.begin + step_of(i, is_v)) * kKeys + my_row;
-          at_row = -1;
-          step_row = 0.f;
+        auto ask_step = [&](int i) {
+          const int pos = pos_of(i);
+          row_at = -1;
+          step_at = 0.f;
           if (i < total && pos < w.len) {
-            const int page = max(0, pages::page_of(p.cache, p.step, w.b, pos, p.status, 146));
-            at_row = (static_cast<int64_t>(page) * p.cache.heads + w.head) * ps + pos % ps;
-            step_row = (is_v ? p.cache.scales[1] : p.cache.scales[0])[at_row];
+            if (page < 0 || page >= p.cache.pages) {
+              pages::report(p.status, 146);
+              page = 0;
+            }
+            row_at = (static_cast<int64_t>(page) * p.cache.heads + w.head) * ps + pos % ps;
+            step_at = (second(i) ? p.cache.scales[1] : p.cache.scales[0])[row_at];
           }
         };
-        locate(0);
-        for (int i = 0; i < total && ok; ++i) {
-          bool is_v;
-          const int step_i = step_of(i, is_v);
-          const uint8_t* from = static_cast<const uint8_t*>(is_v ? p.cache.kv[1] : p.cache.kv[0]);
-          uint4 x[kVecs];
-          const float step_now = step_row;
+        auto ask_rows = [&](int i) {
+          step_next = step_at;
+          const uint8_t* from = static_cast<const uint8_t*>(second(i) ? p.cache.kv[1] : p.cache.kv[0]);
 #pragma unroll
           for (int v = 0; v < kVecs; ++v) {
-            const int64_t at = __shfl_sync(0xffffffffu, at_row, v * kOwn + lane / kVecs);
-            x[v] = make_uint4(0u, 0u, 0u, 0u);
-            if (at >= 0) x[v] = __ldg(reinterpret_cast<const uint4*>(from + at * D) + lane % kVecs);
+            const int64_t at = __shfl_sync(0xffffffffu, row_at, v * kOwn + lane / kVecs);
+            next[v] = make_uint4(0u, 0u, 0u, 0u);
+            if (at >= 0) next[v] = __ldg(reinterpret_cast<const uint4*>(from + at * D) + lane % kVecs);
           }
-          locate(i + 1);
+        };
+        ask_page(0);
+        ask_step(0);
+        ask_page(1);
+        ask_rows(0);
+        ask_step(1);
+        ask_page(2);
+        for (int i = 0; i < total; ++i) {
+          uint4 x[kVecs];
+#pragma unroll
+          for (int v = 0; v < kVecs; ++v) x[v] = next[v];
+          const float step_now = step_next;
+          ask_rows(i + 1);
+          ask_step(i + 2);
+          ask_page(i + 3);
           const int slot = (idx0 + i) % S::kRing;
           if (!(ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->kv_empty[slot], (((idx0 + i) / S::kRing) & 1u) ^ 1u, abort_flag, p.status, 164)))) break;
-          const uint32_t tile = ptx::smem_u32(smem_kv + slot * S::kTileBytes);
+          const uint32_t to = ptx::smem_u32(smem_kv + slot * S::kTileBytes);
+          const bool is_v = second(i);
+          const float mine = is_v ? step_now : 1.f;  // K stays whole numbers
 #pragma unroll
           for (int v = 0; v < kVecs; ++v) {
-            const float st = __shfl_sync(0xffffffffu, step_now, v * kOwn + lane / kVecs);
+            const float st = __shfl_sync(0xffffffffu, mine, v * kOwn + lane / kVecs);
             const int row = v * kRowsAt + cw * kOwn + lane / kVecs;
             const uint32_t in[4] = {x[v].x, x[v].y, x[v].z, x[v].w};
             uint32_t out[8];
-            if (is_v) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                out[e] = attn::pack16x2<kIsBf16>(quant::number(in[e >> 1], 2 * (e & 1)) * st, quant::number(in[e >> 1], 2 * (e & 1) + 1) * st);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) out[e] = quant::pair_of<kIsBf16>(in[e >> 1], 2 * (e & 1));
-            }
+            for (int e = 0; e < 8; ++e)
+              out[e] = attn::pack16x2<kIsBf16>(quant::number(in[e >> 1], 2 * (e & 1)) * st, quant::number(in[e >> 1], 2 * (e & 1) + 1) * st);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int chunk = lane % kVecs * 2 + h;
-              ptx::st_shared_v4(tile + (chunk >> 3) * S::kHalfBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), out[4 * h], out[4 * h + 1], out[4 * h + 2], out[4 * h + 3]);
+              ptx::st_shared_v4(to + (chunk >> 3) * S::kHalfBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), out[4 * h], out[4 * h + 1], out[4 * h + 2], out[4 * h + 3]);
             }
           }
-          if (!is_v) reinterpret_cast<float*>(smem + S::kStepsOff)[(idx0 / 2 + step_i) % S::kStepTiles * kKeys + my_row] = step_now;
+          if (!is_v) reinterpret_cast<float*>(smem + S::kStepsOff)[(idx0 / 2 + (i + 1) / 2) % S::kStepTiles * kKeys + my_row] = step_now;
           ptx::fence_proxy_async_smem();
           ptx::mbar_arrive(&bars->kv_full[slot]);
         }
