@@ -10,8 +10,9 @@
 // pair: how uneven the sequences are does not matter, and no grid has to be planned from lengths that only the device knows.  A pair's new tokens
 // times the heads of its group are the rows of mma.sync tiles, up to sixteen at a time; more rows are further passes over the pair's keys.
 //
-// A CTA has eight warps and each takes every eighth tile of the share: K and V come by TMA, a box per page or part of one (128-byte
-// swizzle, no multicast), into slots of its own.  Pages that are no multiple of eight positions are fetched row by row with cp.async instead.
+// Up to eight rows (kRows8) leave half of a tile's registers unused: then a CTA has twelve warps, which hide each other's latencies, instead of eight.  Each takes
+// every twelfth or eighth tile of the share: K and V come by TMA, a box per page or part of one (128-byte swizzle, no multicast), into slots of its own.
+// Pages that are no multiple of eight positions are fetched row by row with cp.async instead.
 //
 // 8 bits: whole numbers become f16 exactly (a byte behind 0x64 is 1024 + byte), K's step multiplies the score and V's the probability, over the
 // largest step so far (the accumulator is rescaled when that grows), so that only the probability is rounded.  bf16 queries are brought to f16 by a power of two per row.
@@ -26,19 +27,21 @@ namespace paged {
 
 namespace mma = attn_decode::mma;
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kRows = 16;
 constexpr int kMaxCtas = 1024;
-template <bool kI8, int D>
+constexpr int kUnitCost = 6;  // what beginning and ending a pair costs, in tiles: shares are as long in tiles and these
+template <bool kI8, int D, bool kRows8>
 struct Tile {
-  static constexpr int kBytes = kI8 ? 4096 : 8192;        // of K or of V
+  static constexpr int kWarps = kRows8 ? 12 : 8, kThreads = kWarps * 32;
+  static constexpr int kHeld = kRows8 ? 8 : 16;           // rows of a tile that exist
+  static constexpr int kBytes = kI8 || kRows8 ? 4096 : 8192;  // of K or of V
   static constexpr int kRowBytes = kI8 ? D : 2 * D;
-  static constexpr int kPos = kBytes / kRowBytes;         // 32 or 64 positions
-  static constexpr int kSlots = kI8 ? 5 : 3;              // per warp
+  static constexpr int kPos = kBytes / kRowBytes;         // 16, 32 or 64 positions
+  static constexpr int kSlots = kI8 && !kRows8 ? 5 : 3;   // per warp
   static constexpr int kRec = D + 4;                      // floats of a row's record: O, maximum, sum; 16-byte rows
   static constexpr int kScales = kI8 ? kPos * 4 : 0;      // bytes beside a slot
-  static constexpr int kSmem = kWarps * kSlots * (kBytes + kScales) + kWarps * 8 * kRec * 4 + kWarps * kSlots * 8 + 64 + 1024;
-  static_assert(kSmem <= 227 * 1024, "shared memory budget of one CTA");
+  static constexpr int kSmem = kWarps * kSlots * (kBytes + kScales) + kWarps * 8 * kRec * 4 + kWarps * kSlots * 8 + 1024;
+  static_assert(kSmem + 224 + 72 * kWarps <= 227 * 1024, "shared memory of one CTA, with what is declared in the kernel");
 };
 
 struct Params {
@@ -47,25 +50,33 @@ struct Params {
   int32_t heads_q, group;
   int32_t run_log2;   // positions a copy brings: a power of two that divides the page (kTma), else the whole tile
   float scale_log2;   // log2(e) / sqrt(d)
-  float* part;        // [CTA][2][kRows][kRec]: of a pair that began in an earlier share, of one that goes on in the next
+  float* part;        // [CTA][2][kHeld][kRec]: of a pair that began in an earlier share, of one that goes on in the next
   int4* info;         // [CTA]: 1 if a pair of earlier shares ends in this one, 2 if it goes on; sequence and unit of the pair that goes on in the next, or -1
   uint32_t* status;
 };
 
-// A sequence's place in the stream of tiles.
+// A sequence's place in the stream.  Its units, the keys of one KV head for up to kHeld rows, are kUnitCost and their tiles long.
 struct Seq {
   int b, first, count, len;
-  int tiles;      // of a unit: the keys of one KV head for up to kRows rows
+  int tiles;      // of a unit
   int passes;     // units of a KV head
-  int64_t base;   // tiles before it
-  int64_t end;    // and with it
+  int units;
+  int64_t base;   // where it begins
 };
-template <int kPos>
+// A unit, or a share's part of it.
+struct Part {
+  Seq seq;
+  int unit, begin, end;  // tiles
+  int64_t start;         // where the unit begins
+  bool there;
+};
+template <int kPos, int kHeld>
 __device__ __forceinline__ int64_t sequence_tiles(const Params& p, int b, Seq& s, uint32_t* status) {
   if (!pages::sequence(p.step, p.cache.page_size, b, s.first, s.count, s.len, status, 143)) return 0;
   s.tiles = (s.len + kPos - 1) / kPos;
-  s.passes = static_cast<int>((static_cast<int64_t>(s.count) * p.group + kRows - 1) / kRows);
-  return static_cast<int64_t>(s.tiles) * s.passes * p.cache.heads;
+  s.passes = static_cast<int>((static_cast<int64_t>(s.count) * p.group + kHeld - 1) / kHeld);
+  s.units = s.passes * p.cache.heads;
+  return static_cast<int64_t>(s.tiles + kUnitCost) * s.units;
 }
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int32_t y, int32_t z) {
@@ -90,11 +101,34 @@ __device__ __forceinline__ uint32_t i8_pair(uint32_t biased, uint32_t selector) 
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-template <typename T, bool kI8, int D, bool kTma>
-__global__ void __launch_bounds__(kThreads, 1)
+// A 16 x 8 tile, or its first eight rows with the others zero.
+template <bool kIsBf16, int E>
+__device__ __forceinline__ void mma_rows(float (&d)[E], const uint32_t (&a)[E], uint32_t b0, uint32_t b1) {
+  if constexpr (E == 4) {
+    if (kIsBf16)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    float u, v;
+    if (kIsBf16)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %6, %5, %6}, {%7, %8}, {%0, %1, %9, %9};"
+                   : "+f"(d[0]), "+f"(d[1]), "=f"(u), "=f"(v) : "r"(a[0]), "r"(a[1]), "r"(0u), "r"(b0), "r"(b1), "f"(0.f));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %6, %5, %6}, {%7, %8}, {%0, %1, %9, %9};"
+                   : "+f"(d[0]), "+f"(d[1]), "=f"(u), "=f"(v) : "r"(a[0]), "r"(a[1]), "r"(0u), "r"(b0), "r"(b1), "f"(0.f));
+  }
+}
+
+template <typename T, bool kI8, int D, bool kTma, bool kRows8>
+__global__ void __launch_bounds__((Tile<kI8, D, kRows8>::kThreads), 1)
 attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const T* __restrict__ q, T* __restrict__ o,
                        const __grid_constant__ Params p) {
-  using L = Tile<kI8, D>;
+  using L = Tile<kI8, D, kRows8>;
+  constexpr int kWarps = L::kWarps, kThreads = L::kThreads, kHeld = L::kHeld;
+  constexpr int E = kRows8 ? 2 : 4, R = kRows8 ? 1 : 2;  // values of a fragment, rows of a lane
   constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
   constexpr bool kMmaBf16 = kIsBf16 && !kI8;
   constexpr int TP = L::kPos, N8 = TP / 8, KSTEPS = D / 16, REC = L::kRec, kSlots = L::kSlots, kChunks = L::kRowBytes / 16;
@@ -102,7 +136,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* records = reinterpret_cast<float*>(smem + kWarps * kSlots * (L::kBytes + L::kScales));
   uint64_t* bars = reinterpret_cast<uint64_t*>(records + kWarps * 8 * REC);
-  __shared__ int64_t scan[kWarps + 2];
+  __shared__ int64_t scan[kWarps + 1];
   __shared__ uint32_t abort_word;
   __shared__ int first_seq;
   volatile uint32_t* abort_flag = &abort_word;
@@ -142,11 +176,10 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   int64_t total = 0, before = 0, own = 0;
   for (int base = 0; base < batch; base += kThreads) {
     Seq s;
-    own = base + tid < batch ? sequence_tiles<TP>(p, base + tid, s, p.status) : 0;
+    own = base + tid < batch ? sequence_tiles<TP, kHeld>(p, base + tid, s, p.status) : 0;
     total += block_scan(own, before);
   }
-  // whole rounds of the eight warps, so that none has a tile more than another without need
-  const int64_t per = ((total + gridDim.x - 1) / gridDim.x + kWarps - 1) / kWarps * kWarps;
+  const int64_t per = (total + gridDim.x - 1) / gridDim.x;
   const int64_t t0 = min(total, blockIdx.x * per), t1 = min(total, t0 + per);
   if (t0 < t1) {
     if (batch <= kThreads) {
@@ -155,7 +188,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       int64_t sum = 0;
       for (int base = 0; base < batch; base += kThreads) {
         Seq s;
-        own = base + tid < batch ? sequence_tiles<TP>(p, base + tid, s, nullptr) : 0;
+        own = base + tid < batch ? sequence_tiles<TP, kHeld>(p, base + tid, s, nullptr) : 0;
         const int64_t here = block_scan(own, before);
         if (sum + before <= t0 && t0 < sum + before + own) first_seq = base + tid, scan[kWarps] = sum + before;
         sum += here;
@@ -167,17 +200,39 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     if (tid == 0) p.info[blockIdx.x] = make_int4(0, -1, -1, 0);
     return;
   }
-  auto open = [&](Seq& s, int b, int64_t base) {  // the first sequence from b on that has tiles; there is one
-    int64_t n = 0;
-    for (; b < batch; ++b)
-      if ((n = sequence_tiles<TP>(p, b, s, nullptr)) > 0) break;
-    s.b = b;
-    s.base = base;
-    s.end = base + n;
+  auto cut = [&](Part& x) {  // what the share has of the unit, from its beginning on
+    x.begin = 0;
+    x.end = static_cast<int>(min(static_cast<int64_t>(x.seq.tiles), max(t1 - x.start - kUnitCost, static_cast<int64_t>(0))));
+    x.there = x.end > 0;
   };
-  Seq seq, ahead;
-  open(seq, first_seq, scan[kWarps]);
-  ahead = seq;
+  auto open = [&](Part& x, int b, int64_t base) {  // the first sequence from b on that has units
+    for (; b < batch; ++b)
+      if (sequence_tiles<TP, kHeld>(p, b, x.seq, nullptr) > 0) break;
+    x.seq.b = b, x.seq.base = base;
+    x.unit = 0, x.start = base;
+  };
+  auto next = [&](Part& x) {
+    x.start += x.seq.tiles + kUnitCost;
+    if (++x.unit == x.seq.units) open(x, x.seq.b + 1, x.start);
+    if (x.start >= t1 || x.seq.b >= batch) x.there = false;
+    else cut(x);
+  };
+  // Parts live in shared memory: the CTA's, the one that its thread 0 finds while the warps work on that, and each warp's that its loads have come to.
+  __shared__ Part parts[2], parts_ahead[kWarps];
+  if (tid == 0) {
+    Part x;
+    open(x, first_seq, scan[kWarps]);
+    x.unit = static_cast<int>((t0 - x.start) / (x.seq.tiles + kUnitCost));
+    x.start += static_cast<int64_t>(x.unit) * (x.seq.tiles + kUnitCost);
+    cut(x);
+    x.begin = static_cast<int>(max(t0 - x.start - kUnitCost, static_cast<int64_t>(0)));
+    x.there = x.end > x.begin;
+    if (!x.there) next(x);
+    parts[0] = x;
+    for (int i = 0; i < kWarps; ++i) parts_ahead[i] = x;
+  }
+  __syncthreads();
+  Part& ahead = parts_ahead[warp];
 
   const uint32_t slots = ptx::smem_u32(smem) + warp * (kSlots * L::kBytes);
   const uint32_t steps = ptx::smem_u32(smem) + kWarps * kSlots * L::kBytes + warp * (kSlots * L::kScales);
@@ -192,23 +247,29 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     else return (pos << 6) + ((chunk ^ ((pos >> 1) & 3)) << 4);
   };
 
-  // The warp's tiles, ahead of their use: K and V of a tile in turn.
-  int64_t t_ahead = t0 + warp;
-  int load_slot = 0, page = 0, tile_ahead = 0, head_ahead = 0;
-  bool load_v = false, more = false;
-  auto settle = [&]() {  // on to tile t_ahead: where it is, and (lane i) the page of its i-th run
-    more = t_ahead < t1;
+  // The warp's tiles, ahead of their use: K and V of a tile in turn.  Tiles are dealt to the warps in turn, across units.
+  int load_slot = 0, page = 0, tile_ahead = ahead.begin + warp, end_ahead = ahead.end, head_ahead = 0, turn_ahead = 0, b_ahead = 0, len_ahead = 0;
+  bool load_v = false, more = ahead.there;
+  auto look = [&]() {
+    b_ahead = ahead.seq.b, len_ahead = ahead.seq.len, end_ahead = ahead.end;
+    head_ahead = ahead.seq.passes == 1 ? ahead.unit : ahead.unit / ahead.seq.passes;
+  };
+  look();
+  auto settle = [&]() {  // on to the first unit that has tile_ahead for this warp, and (lane i) the page of the tile's i-th run
+    while (more && tile_ahead >= end_ahead) {
+      turn_ahead = (turn_ahead + end_ahead - ahead.begin) % kWarps;
+      __syncwarp();
+      if (lane == 0) next(ahead);
+      __syncwarp();
+      more = ahead.there;
+      look();
+      tile_ahead = ahead.begin + (warp >= turn_ahead ? warp - turn_ahead : warp + kWarps - turn_ahead);
+    }
     if (!more) return;
-    while (t_ahead >= ahead.end && ahead.b < batch) open(ahead, ahead.b + 1, ahead.end);
-    if (!(more = ahead.b < batch)) return;
-    const int64_t in_seq = t_ahead - ahead.base;
-    const int unit = static_cast<int>(in_seq / ahead.tiles);
-    tile_ahead = static_cast<int>(in_seq - static_cast<int64_t>(unit) * ahead.tiles);
-    head_ahead = unit / ahead.passes;
     if (kTma) {
       const int pos = tile_ahead * TP + (lane << lb);
       page = 0;
-      if ((lane << lb) < TP && pos < ahead.len) page = max(0, pages::page_of(p.cache, p.step, ahead.b, pos, p.status, 144));
+      if ((lane << lb) < TP && pos < len_ahead) page = max(0, pages::page_of(p.cache, p.step, b_ahead, pos, p.status, 144));
     }
   };
   auto issue = [&]() {
@@ -216,7 +277,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       if (!kTma) mma::cp_async_commit();
       return;
     }
-    const int pos0 = tile_ahead * TP, here = min(TP, ahead.len - pos0);
+    const int pos0 = tile_ahead * TP, here = min(TP, len_ahead - pos0);
     const uint32_t dst = slots + load_slot * L::kBytes, dst_steps = steps + load_slot * L::kScales;
     if constexpr (kTma) {
       const int runs = (here + run - 1) >> lb;
@@ -235,7 +296,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       for (int i = lane; i < TP * kChunks; i += 32) {
         const int r = i / kChunks, c = i % kChunks, pos = pos0 + r;
         const bool ok = r < here;
-        const int pg = ok ? max(0, pages::page_of(p.cache, p.step, ahead.b, pos, p.status, 144)) : 0;
+        const int pg = ok ? max(0, pages::page_of(p.cache, p.step, b_ahead, pos, p.status, 144)) : 0;
         const int64_t row = (static_cast<int64_t>(pg) * heads + head_ahead) * ps + (ok ? pos % ps : 0);
         mma::cp_async_16(dst + at(r, c), static_cast<const uint8_t*>(p.cache.kv[load_v]) + row * L::kRowBytes + c * 16, ok);
         if (kI8 && c == 0) ptx::cp_async_4(dst_steps + r * 4, p.cache.scales[load_v] + row, ok);
@@ -243,7 +304,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       mma::cp_async_commit();
     }
     if (load_v) {
-      t_ahead += kWarps;
+      tile_ahead += kWarps;
       settle();
     }
     load_v = !load_v;
@@ -270,22 +331,36 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     if (++slot == kSlots) slot = 0, phase ^= 1u;
     issue();
   };
-  uint32_t qa[KSTEPS][4];
-  float q_factor[2];  // what the rows of Q were divided by
-  const int k_row = (lane & 7) + ((lane >> 4) & 1) * 8, v_row = (lane & 7) + ((lane >> 3) & 1) * 8;
-  int head_state = 0, tail_b = -1, tail_unit = -1;
-  for (int64_t t = t0; t < t1;) {
-    while (t >= seq.end && seq.b < batch) open(seq, seq.b + 1, seq.end);
-    if (seq.b >= batch) break;
-    const int unit = static_cast<int>((t - seq.base) / seq.tiles);
-    const int begin = static_cast<int>(t - seq.base - static_cast<int64_t>(unit) * seq.tiles);
-    const int end = static_cast<int>(min(static_cast<int64_t>(seq.tiles), begin + (t1 - t)));
-    const int head = unit / seq.passes, row0 = unit % seq.passes * kRows;
-    const int rows = min(kRows, seq.count * p.group - row0);
-    // rows gr and gr + 8: their Q as A fragments, and the last position each sees
-    int limit[2];
+  uint32_t qa[KSTEPS][E];  // (row gr, k lo), [(row gr + 8, k lo),] (gr, k hi) [, (gr + 8, k hi)]
+  float q_factor[R];       // what the rows of Q were divided by
+  // What this lane's ldmatrix addresses start from, in a slot: 16 positions, chunk 0 or 1.  A pair of chunks further is the same with bits 5 and 6 turned (no row starts
+  // inside them), eight chunks further the run's next 128-byte group.
+  uint32_t k_from[N8 / 2], v_from[N8 / 2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+  for (int j = 0; j < N8 / 2; ++j) {
+    k_from[j] = at(j * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, (lane >> 3) & 1);
+    v_from[j] = at(j * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, (lane >> 4) & 1);
+  }
+  const uint32_t group = L::kRowBytes == 256 ? 1u << (lb + 7) : 0u;
+  auto pair_of = [&](uint32_t from, int pair) -> uint32_t { return (from ^ ((pair & 3) << 5)) + (pair >= 4 ? group : 0u); };
+  int head_state = 0, tail_b = -1, tail_unit = -1, turn = 0;
+  for (int which = 0; parts[which].there; which ^= 1) {
+    const Part& now = parts[which];
+    const int unit = now.unit, begin = now.begin, end = now.end;
+    struct {
+      int b, first, count, len, tiles, passes;
+    } const seq = {now.seq.b, now.seq.first, now.seq.count, now.seq.len, now.seq.tiles, now.seq.passes};
+    if (tid == 0) {  // the others look at it when they have met at the records
+      Part x = now;
+      next(x);
+      parts[which ^ 1] = x;
+    }
+    const int head = seq.passes == 1 ? unit : unit / seq.passes, row0 = (unit - head * seq.passes) * kHeld;
+    const int rows = min(kHeld, seq.count * p.group - row0);
+    // rows gr and gr + 8: their Q as A fragments, and the last position each sees
+    int limit[R];
+#pragma unroll
+    for (int e = 0; e < R; ++e) {
       const bool ok = gr + 8 * e < rows;
       const int r = row0 + (ok ? gr + 8 * e : 0), token = r / p.group;
       limit[e] = seq.len - seq.count + token;
@@ -294,10 +369,10 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       for (int kk = 0; kk < KSTEPS; ++kk) {
         if (kI8) {  // the four numbers of a fragment lie together in a row of the cache
           const uint2 x = ok ? __ldg(reinterpret_cast<const uint2*>(src + kk * 8 + 2 * tq)) : make_uint2(0u, 0u);
-          qa[kk][e] = x.x, qa[kk][2 + e] = x.y;
+          qa[kk][e] = x.x, qa[kk][R + e] = x.y;
         } else {
           qa[kk][e] = ok ? __ldg(src + kk * 8 + tq) : 0u;
-          qa[kk][2 + e] = ok ? __ldg(src + kk * 8 + tq + 4) : 0u;
+          qa[kk][R + e] = ok ? __ldg(src + kk * 8 + tq + 4) : 0u;
         }
       }
       q_factor[e] = 1.f;
@@ -307,7 +382,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         for (int kk = 0; kk < KSTEPS; ++kk)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint32_t x = qa[kk][2 * i + e];
+            const uint32_t x = qa[kk][R * i + e];
             top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x << 16)), fabsf(__uint_as_float(x & 0xffff0000u))));
           }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -320,44 +395,52 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         for (int kk = 0; kk < KSTEPS; ++kk)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            uint32_t& x = qa[kk][2 * i + e];
+            uint32_t& x = qa[kk][R * i + e];
             x = mma::pack2<false>(__uint_as_float(x << 16) * inv, __uint_as_float(x & 0xffff0000u) * inv);
           }
       }
     }
     const int least = seq.len - seq.count + row0 / p.group;  // the first row's last position: tiles up to it need no masks
-    float oacc[2 * KSTEPS][4];
+    float oacc[2 * KSTEPS][E];
 #pragma unroll
-    for (int j = 0; j < 2 * KSTEPS; ++j) oacc[j][0] = oacc[j][1] = oacc[j][2] = oacc[j][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int j = 0; j < 2 * KSTEPS; ++j)
+#pragma unroll
+      for (int e = 0; e < E; ++e) oacc[j][e] = 0.f;
+    float m[R], l[R];
+#pragma unroll
+    for (int e = 0; e < R; ++e) m[e] = -INFINITY, l[e] = 0.f;
     float v_top = 0x1p-100f;  // 8 bits: the largest step of V so far, oacc is in units of it; far smaller steps count as zero
-    for (int tile = begin + static_cast<int>((warp - (t - t0)) & (kWarps - 1)); tile < end; tile += kWarps) {
+    for (int tile = begin + (warp >= turn ? warp - turn : warp + kWarps - turn); tile < end; tile += kWarps) {
       if (!arrived()) break;
       const uint32_t ks = slots + slot * L::kBytes;
-      float s[N8][4];
+      float s[N8][E];
 #pragma unroll
-      for (int j = 0; j < N8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+      for (int j = 0; j < N8; ++j)
 #pragma unroll
-      for (int j = 0; j < N8 / 2; ++j) {
-        if constexpr (!kI8) {
+        for (int e = 0; e < E; ++e) s[j][e] = 0.f;
+      if constexpr (!kI8) {
 #pragma unroll
-          for (int kk = 0; kk < KSTEPS; ++kk) {
+        for (int kk = 0; kk < KSTEPS; ++kk)
+#pragma unroll
+          for (int j = 0; j < N8 / 2; ++j) {
             uint32_t kb[4];  // (positions 0-7, k lo), (0-7, k hi), (8-15, k lo), (8-15, k hi)
-            mma::ldmatrix_x4(ks + at(j * 16 + k_row, kk * 2 + ((lane >> 3) & 1)), kb);
-            mma::mma_16816<kMmaBf16>(s[2 * j], qa[kk], kb[0], kb[1]);
-            mma::mma_16816<kMmaBf16>(s[2 * j + 1], qa[kk], kb[2], kb[3]);
+            mma::ldmatrix_x4(pair_of(ks + k_from[j], kk), kb);
+            mma_rows<kMmaBf16>(s[2 * j], qa[kk], kb[0], kb[1]);
+            mma_rows<kMmaBf16>(s[2 * j + 1], qa[kk], kb[2], kb[3]);
           }
-        } else {
+      } else {
 #pragma unroll
-          for (int kk = 0; kk < KSTEPS; kk += 2) {
-            uint32_t kb[4];  // (positions 0-7, 16 numbers), (0-7, the next 16), (8-15, 16), (8-15, the next)
-            mma::ldmatrix_x4(ks + at(j * 16 + k_row, kk + ((lane >> 3) & 1)), kb);
+        for (int kk = 0; kk < KSTEPS; kk += 2) {
+          uint32_t kb[N8 / 2][4];  // (positions 0-7, 16 numbers), (0-7, the next 16), (8-15, 16), (8-15, the next)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t x = kb[i] ^ 0x80808080u;
-              mma::mma_16816<false>(s[2 * j + (i >> 1)], qa[kk + (i & 1)], i8_pair(x, 0x4140), i8_pair(x, 0x4342));
+          for (int j = 0; j < N8 / 2; ++j) mma::ldmatrix_x4(pair_of(ks + k_from[j], kk / 2), kb[j]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < N8; ++j) {
+              const uint32_t x = kb[j / 2][2 * (j & 1) + i] ^ 0x80808080u;
+              mma_rows<false>(s[j], qa[kk + i], i8_pair(x, 0x4140), i8_pair(x, 0x4342));
             }
-          }
         }
       }
       const int pos = tile * TP + 2 * tq;
@@ -368,26 +451,26 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         for (int j = 0; j < N8; ++j) {
           const float2 st = *reinterpret_cast<const float2*>(kst + j * 8);
           const float a = st.x * p.scale_log2, b = st.y * p.scale_log2;
-          s[j][0] *= a * q_factor[0], s[j][1] *= b * q_factor[0];
-          s[j][2] *= a * q_factor[1], s[j][3] *= b * q_factor[1];
+#pragma unroll
+          for (int e = 0; e < R; ++e) s[j][2 * e] *= a * q_factor[e], s[j][2 * e + 1] *= b * q_factor[e];
         }
       } else {
 #pragma unroll
         for (int j = 0; j < N8; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[j][e] *= p.scale_log2;
+          for (int e = 0; e < E; ++e) s[j][e] *= p.scale_log2;
       }
       release();
       if (masked) {
 #pragma unroll
         for (int j = 0; j < N8; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < E; ++e)
             if (pos + j * 8 + (e & 1) > limit[e >> 1]) s[j][e] = -INFINITY;
       }
-      float a[2];
+      float a[R];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < R; ++e) {
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < N8; ++j) top = fmaxf(top, fmaxf(s[j][2 * e], s[j][2 * e + 1]));
@@ -424,24 +507,28 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const float inv = 1.f / top;
-        a[0] *= v_top * inv, a[1] *= v_top * inv;
+#pragma unroll
+        for (int e = 0; e < R; ++e) a[e] *= v_top * inv;
         v_top = top;
 #pragma unroll
         for (int j = 0; j < N8; ++j) {
           const float x = st[j].x * inv, y = st[j].y * inv;
-          s[j][0] *= x, s[j][1] *= y, s[j][2] *= x, s[j][3] *= y;
+#pragma unroll
+          for (int e = 0; e < R; ++e) s[j][2 * e] *= x, s[j][2 * e + 1] *= y;
         }
       }
-      uint32_t pa[N8 / 2][4];
+      uint32_t pa[N8 / 2][E];
 #pragma unroll
-      for (int j = 0; j < N8 / 2; ++j) {
-        pa[j][0] = mma::pack2<kMmaBf16>(s[2 * j][0], s[2 * j][1]);
-        pa[j][1] = mma::pack2<kMmaBf16>(s[2 * j][2], s[2 * j][3]);
-        pa[j][2] = mma::pack2<kMmaBf16>(s[2 * j + 1][0], s[2 * j + 1][1]);
-        pa[j][3] = mma::pack2<kMmaBf16>(s[2 * j + 1][2], s[2 * j + 1][3]);
-      }
+      for (int j = 0; j < N8 / 2; ++j)
 #pragma unroll
-      for (int j = 0; j < 2 * KSTEPS; ++j) oacc[j][0] *= a[0], oacc[j][1] *= a[0], oacc[j][2] *= a[1], oacc[j][3] *= a[1];
+        for (int e = 0; e < R; ++e) {
+          pa[j][e] = mma::pack2<kMmaBf16>(s[2 * j][2 * e], s[2 * j][2 * e + 1]);
+          pa[j][R + e] = mma::pack2<kMmaBf16>(s[2 * j + 1][2 * e], s[2 * j + 1][2 * e + 1]);
+        }
+#pragma unroll
+      for (int j = 0; j < 2 * KSTEPS; ++j)
+#pragma unroll
+        for (int e = 0; e < R; ++e) oacc[j][2 * e] *= a[e], oacc[j][2 * e + 1] *= a[e];
       if (!kI8 && ragged) {
         // what lies behind the last position weighs nothing, but may be anything
         for (int i = lane; i < TP * kChunks; i += 32)
@@ -455,17 +542,17 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           uint32_t vb[4];
           if constexpr (!kI8) {
             // (positions 0-7, d lo), (8-15, d lo), (0-7, d hi), (8-15, d hi), transposed on load
-            mma::ldmatrix_x4_trans(vs + at(j * 16 + v_row, c * 2 + ((lane >> 4) & 1)), vb);
-            mma::mma_16816<kMmaBf16>(oacc[2 * c], pa[j], vb[0], vb[1]);
-            mma::mma_16816<kMmaBf16>(oacc[2 * c + 1], pa[j], vb[2], vb[3]);
+            mma::ldmatrix_x4_trans(pair_of(vs + v_from[j], c), vb);
+            mma_rows<kMmaBf16>(oacc[2 * c], pa[j], vb[0], vb[1]);
+            mma_rows<kMmaBf16>(oacc[2 * c + 1], pa[j], vb[2], vb[3]);
           } else if (c % 2 == 0) {
             // the same of pairs of numbers: two positions of column 2 gr and of column 2 gr + 1 in a register
-            mma::ldmatrix_x4_trans(vs + at(j * 16 + v_row, c + ((lane >> 4) & 1)), vb);
+            mma::ldmatrix_x4_trans(pair_of(vs + v_from[j], c / 2), vb);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint32_t x = vb[2 * i] ^ 0x80808080u, y = vb[2 * i + 1] ^ 0x80808080u;
-              mma::mma_16816<false>(oacc[2 * (c + i)], pa[j], i8_pair(x, 0x4240), i8_pair(y, 0x4240));
-              mma::mma_16816<false>(oacc[2 * (c + i) + 1], pa[j], i8_pair(x, 0x4341), i8_pair(y, 0x4341));
+              mma_rows<false>(oacc[2 * (c + i)], pa[j], i8_pair(x, 0x4240), i8_pair(y, 0x4240));
+              mma_rows<false>(oacc[2 * (c + i) + 1], pa[j], i8_pair(x, 0x4341), i8_pair(y, 0x4341));
             }
           }
         }
@@ -473,7 +560,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       release();
     }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < R; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
     }
@@ -487,8 +574,9 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const float f = kI8 ? v_top : 1.f;
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
-          const float x0 = (half ? oacc[2 * c][2] : oacc[2 * c][0]) * f, x1 = (half ? oacc[2 * c][3] : oacc[2 * c][1]) * f;
-          const float y0 = (half ? oacc[2 * c + 1][2] : oacc[2 * c + 1][0]) * f, y1 = (half ? oacc[2 * c + 1][3] : oacc[2 * c + 1][1]) * f;
+          constexpr int H = kRows8 ? 0 : 2;  // the other row's
+          const float x0 = (half ? oacc[2 * c][H] : oacc[2 * c][0]) * f, x1 = (half ? oacc[2 * c][H + 1] : oacc[2 * c][1]) * f;
+          const float y0 = (half ? oacc[2 * c + 1][H] : oacc[2 * c + 1][0]) * f, y1 = (half ? oacc[2 * c + 1][H + 1] : oacc[2 * c + 1][1]) * f;
           if (kI8) {
             *reinterpret_cast<float4*>(rec + c * 16 + 4 * tq) = make_float4(x0, y0, x1, y1);
           } else {
@@ -496,7 +584,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             *reinterpret_cast<float2*>(rec + c * 16 + 8 + 2 * tq) = make_float2(y0, y1);
           }
         }
-        if (tq == 0) *reinterpret_cast<float2*>(rec + D) = half ? make_float2(m[1], l[1]) : make_float2(m[0], l[0]);
+        if (tq == 0) *reinterpret_cast<float2*>(rec + D) = half ? make_float2(m[R - 1], l[R - 1]) : make_float2(m[0], l[0]);
       }
       __syncthreads();
       for (int i = tid; i < min(8, rows - half * 8) * (D / 4); i += kThreads) {
@@ -526,7 +614,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           *reinterpret_cast<uint2*>(o + (static_cast<int64_t>(seq.first + token) * p.heads_q + h) * D + dd) =
               make_uint2(mma::pack2<kIsBf16>(oo.x * inv, oo.y * inv), mma::pack2<kIsBf16>(oo.z * inv, oo.w * inv));
         } else {
-          float* out = p.part + ((static_cast<int64_t>(blockIdx.x) * 2 + (begin == 0 ? 1 : 0)) * kRows + r) * REC;
+          float* out = p.part + ((static_cast<int64_t>(blockIdx.x) * 2 + (begin == 0 ? 1 : 0)) * kHeld + r) * REC;
           *reinterpret_cast<float4*>(out + dd) = oo;
           if (dd == 0) *reinterpret_cast<float2*>(out + D) = make_float2(mm, ll);
         }
@@ -534,7 +622,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     }
     if (begin > 0) head_state = end == seq.tiles ? 1 : 2;
     else if (end < seq.tiles) tail_b = seq.b, tail_unit = unit;
-    t += end - begin;
+    turn = (turn + end - begin) % kWarps;
   }
   if (tid == 0) p.info[blockIdx.x] = make_int4(head_state, tail_b, tail_unit, 0);
   if constexpr (!kTma) mma::cp_async_wait<0>();
@@ -548,7 +636,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 }
 
 // The records of a pair that several shares have a part of, in order; a warp per row, CTA (x, y) rows 4 y .. of the pair that goes on behind share x.
-template <typename T, int D>
+template <typename T, int D, int kHeld>
 __global__ void __launch_bounds__(128)
 attention_paged_merge_kernel(T* __restrict__ o, const __grid_constant__ Params p) {
   constexpr int REC = D + 4;
@@ -564,9 +652,9 @@ attention_paged_merge_kernel(T* __restrict__ o, const __grid_constant__ Params p
     if (state != 2) break;
   }
   const int first = p.step.starts[mine.y], count = p.step.starts[mine.y + 1] - first;
-  const int passes = static_cast<int>((static_cast<int64_t>(count) * p.group + kRows - 1) / kRows), head = mine.z / passes, row = mine.z % passes * kRows + r;
-  if (row >= count * p.group) return;
-  auto record = [&](int i) { return p.part + ((static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + r) * REC; };
+  const int passes = static_cast<int>((static_cast<int64_t>(count) * p.group + kHeld - 1) / kHeld), head = mine.z / passes, row = mine.z % passes * kHeld + r;
+  if (r >= kHeld || row >= count * p.group) return;
+  auto record = [&](int i) { return p.part + ((static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kHeld + r) * REC; };
   float mm = -INFINITY;
   for (int i = lane; i < n; i += 32) mm = fmaxf(mm, __ldcg(record(i) + D));
 #pragma unroll

@@ -226,27 +226,24 @@ inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& 
 }
 
 // The tiles of all sequences' caches dealt out evenly over the SMs, and what several of them have a part of merged (attention_paged.cuh).
-template <typename T, bool kI8, int D>
-inline int32_t attention_paged_launch(std::string* err, paged::Params p, const void* q, void* o, cudaStream_t s) {
-  using L = paged::Tile<kI8, D>;
-  // more rows than a tile of mma.sync has would go over their keys again: tcgen05, as long as a group's heads fit a tile and boxes of eight positions a page
-  const int wide = page_run_log2(p.cache.page_size, 7);
-  if (static_cast<int64_t>(p.step.max_new) * p.group > paged::kRows && p.group <= paged::tc::kMaxGroup && (kI8 || wide >= 3))
-    return attention_paged_tc_launch<T, kI8, D>(err, p, wide, q, o, s);
+template <typename T, bool kI8, int D, bool kRows8>
+inline int32_t attention_paged_few_launch(std::string* err, paged::Params p, const void* q, void* o, cudaStream_t s) {
+  using L = paged::Tile<kI8, D, kRows8>;
   int sms = 0;
   int32_t st = sm_count(err, &sms);
   if (st != TSM100_OK) return st;
   const unsigned ctas = static_cast<unsigned>(std::min(sms, paged::kMaxCtas));
-  const int64_t rows = std::min<int64_t>(paged::kRows, static_cast<int64_t>(p.step.max_new) * p.group);
-  const size_t part = static_cast<size_t>(ctas) * 2 * paged::kRows * L::kRec * sizeof(float);
+  const int64_t rows = std::min<int64_t>(L::kHeld, static_cast<int64_t>(p.step.max_new) * p.group);
+  const size_t part = static_cast<size_t>(ctas) * 2 * L::kHeld * L::kRec * sizeof(float);
   st = take_scratch(err, reinterpret_cast<void**>(&p.part), part + ctas * sizeof(int4), s);
   if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged: no device memory for partial results");
   if (st != TSM100_OK) return st;
   p.info = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(p.part) + part);
   // boxes of a power of two of positions that a page is a multiple of; 8-bit steps come by copies of 16 bytes and more
-  const int run_log2 = page_run_log2(p.cache.page_size, L::kPos == 32 ? 5 : 6);
+  constexpr int kTop = L::kPos == 16 ? 4 : L::kPos == 32 ? 5 : 6;
+  const int run_log2 = page_run_log2(p.cache.page_size, kTop);
   const bool boxes = run_log2 >= 3 && (!kI8 || (aligned16(p.cache.scales[0]) && aligned16(p.cache.scales[1])));
-  p.run_log2 = boxes ? run_log2 : L::kPos == 32 ? 5 : 6;
+  p.run_log2 = boxes ? run_log2 : kTop;
   CUtensorMap map[2];
   std::memset(map, 0, sizeof map);
   for (int i = 0; i < 2 && boxes && st == TSM100_OK; ++i) {
@@ -269,15 +266,24 @@ inline int32_t attention_paged_launch(std::string* err, paged::Params p, const v
     st = make_tmap(err, &map[i], key, kI8 ? 1 : 2);
   }
   if (st == TSM100_OK) {
-    auto kern = boxes ? paged::attention_paged_kernel<T, kI8, D, true> : paged::attention_paged_kernel<T, kI8, D, false>;
+    auto kern = boxes ? paged::attention_paged_kernel<T, kI8, D, true, kRows8> : paged::attention_paged_kernel<T, kI8, D, false, kRows8>;
     cudaError_t e = set_dyn_smem_once(kern, L::kSmem);
-    if (e == cudaSuccess) e = launch_chained(kern, ctas, paged::kThreads, L::kSmem, s, 0, map[0], map[1], static_cast<const T*>(q), static_cast<T*>(o), p);
-    if (e == cudaSuccess) e = launch_chained(paged::attention_paged_merge_kernel<T, D>, dim3(ctas, static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, 0, static_cast<T*>(o), p);
+    if (e == cudaSuccess) e = launch_chained(kern, ctas, L::kThreads, L::kSmem, s, 0, map[0], map[1], static_cast<const T*>(q), static_cast<T*>(o), p);
+    if (e == cudaSuccess) e = launch_chained(paged::attention_paged_merge_kernel<T, D, L::kHeld>, dim3(ctas, static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, 0, static_cast<T*>(o), p);
     st = cuda_ok(err, e, "attention_paged_kernel launch");
   }
   const cudaError_t e = cudaFreeAsync(p.part, s);
   if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
   return st;
+}
+
+// More rows than a tile of mma.sync has would go over their keys again: those take tcgen05, as long as a group's heads fit a tile and boxes of eight positions a page.
+template <typename T, bool kI8, int D>
+inline int32_t attention_paged_launch(std::string* err, const paged::Params& p, const void* q, void* o, cudaStream_t s) {
+  const int64_t rows = static_cast<int64_t>(p.step.max_new) * p.group;
+  const int wide = page_run_log2(p.cache.page_size, 7);
+  if (rows > paged::kRows && p.group <= paged::tc::kMaxGroup && (kI8 || wide >= 3)) return attention_paged_tc_launch<T, kI8, D>(err, p, wide, q, o, s);
+  return rows <= 8 ? attention_paged_few_launch<T, kI8, D, true>(err, p, q, o, s) : attention_paged_few_launch<T, kI8, D, false>(err, p, q, o, s);
 }
 
 template <typename T>
