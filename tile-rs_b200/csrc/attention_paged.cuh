@@ -5,13 +5,13 @@
 // in one pass over the keys: a running (m, sum, O), rescaled when m grows; parts of a sequence that different warps or CTAs have seen are joined
 // by their maxima.
 //
-// Bound: HBM, the cache is read once; at sixteen rows a tile the arithmetic is a third of what the SMs give.  So the tiles of
-// all (sequence, KV head) pairs are numbered through and every SM takes an equal, contiguous share of them, which may begin and end inside a
-// pair: how uneven the sequences are does not matter, and no grid has to be planned from lengths that only the device knows.  A pair's new tokens
-// times the heads of its group are the rows of mma.sync tiles, up to sixteen at a time; more rows are further passes over the pair's keys.
+// Bound: HBM, the cache is read once.  So the tiles of all (sequence, KV head) pairs are numbered through and every SM takes an equal, contiguous share of
+// them, which may begin and end inside a pair: how uneven the sequences are does not matter, and no grid has to be planned from lengths that only the device knows.
+// A pair's new tokens times the heads of its group are its rows, up to eight (kWide: sixteen) at a time; more rows are further passes over the pair's keys.
 //
-// Up to eight rows (kRows8) leave half of a tile's registers unused: then a CTA has twelve warps, which hide each other's latencies, instead of eight.  Each takes
-// every twelfth or eighth tile of the share: K and V come by TMA, a box per page or part of one (128-byte swizzle, no multicast), into slots of its own.
+// The products are mma.sync tiles with the keys, and V's columns, on the side of sixteen and the rows on the side of eight, S^T = K Q^T and O^T = V^T P^T, so that a
+// group of eight heads or fewer leaves none of them idle: half the products, and half the registers, of tiles with the rows on the other side.  P^T is transposed between the two by movmatrix.
+// A CTA's warps take the tiles of its share in turn: K and V come by TMA, a box per page or part of one (128-byte swizzle, no multicast), into slots of a warp's own.
 // Pages that are no multiple of eight positions are fetched row by row with cp.async instead.
 //
 // 8 bits: whole numbers become f16 exactly (a byte behind 0x64 is 1024 + byte), K's step multiplies the score and V's the probability, over the
@@ -27,17 +27,17 @@ namespace paged {
 
 namespace mma = attn_decode::mma;
 
-constexpr int kRows = 16;
+constexpr int kRows = 16;     // of a pass, at most
 constexpr int kMaxCtas = 1024;
 constexpr int kUnitCost = 6;  // what beginning and ending a pair costs, in tiles: shares are as long in tiles and these
-template <bool kI8, int D, bool kRows8>
+template <bool kI8, int D, bool kWide>
 struct Tile {
-  static constexpr int kWarps = kRows8 ? 12 : 8, kThreads = kWarps * 32;
-  static constexpr int kHeld = kRows8 ? 8 : 16;           // rows of a tile that exist
-  static constexpr int kBytes = kI8 || kRows8 ? 4096 : 8192;  // of K or of V
+  static constexpr int kWarps = kWide ? 8 : 12, kThreads = kWarps * 32;
+  static constexpr int kHeld = kWide ? 16 : 8;            // rows
+  static constexpr int kBytes = 4096;                     // of K or of V
   static constexpr int kRowBytes = kI8 ? D : 2 * D;
   static constexpr int kPos = kBytes / kRowBytes;         // 16, 32 or 64 positions
-  static constexpr int kSlots = kI8 && !kRows8 ? 5 : 3;   // per warp
+  static constexpr int kSlots = kWide ? 5 : 3;            // per warp
   static constexpr int kRec = D + 4;                      // floats of a row's record: O, maximum, sum; 16-byte rows
   static constexpr int kScales = kI8 ? kPos * 4 : 0;      // bytes beside a slot
   static constexpr int kSmem = kWarps * kSlots * (kBytes + kScales) + kWarps * 8 * kRec * 4 + kWarps * kSlots * 8 + 1024;
@@ -101,37 +101,31 @@ __device__ __forceinline__ uint32_t i8_pair(uint32_t biased, uint32_t selector) 
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// A 16 x 8 tile, or its first eight rows with the others zero.
-template <bool kIsBf16, int E>
-__device__ __forceinline__ void mma_rows(float (&d)[E], const uint32_t (&a)[E], uint32_t b0, uint32_t b1) {
-  if constexpr (E == 4) {
-    if (kIsBf16)
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  } else {
-    float u, v;
-    if (kIsBf16)
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %6, %5, %6}, {%7, %8}, {%0, %1, %9, %9};"
-                   : "+f"(d[0]), "+f"(d[1]), "=f"(u), "=f"(v) : "r"(a[0]), "r"(a[1]), "r"(0u), "r"(b0), "r"(b1), "f"(0.f));
-    else
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %6, %5, %6}, {%7, %8}, {%0, %1, %9, %9};"
-                   : "+f"(d[0]), "+f"(d[1]), "=f"(u), "=f"(v) : "r"(a[0]), "r"(a[1]), "r"(0u), "r"(b0), "r"(b1), "f"(0.f));
-  }
+template <bool kIsBf16>
+__device__ __forceinline__ void mma_tile(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (kIsBf16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {  // an 8 x 8 tile of 16-bit numbers
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 
-template <typename T, bool kI8, int D, bool kTma, bool kRows8>
-__global__ void __launch_bounds__((Tile<kI8, D, kRows8>::kThreads), 1)
+template <typename T, bool kI8, int D, bool kTma, bool kWide>
+__global__ void __launch_bounds__((Tile<kI8, D, kWide>::kThreads), 1)
 attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const T* __restrict__ q, T* __restrict__ o,
                        const __grid_constant__ Params p) {
-  using L = Tile<kI8, D, kRows8>;
+  using L = Tile<kI8, D, kWide>;
   constexpr int kWarps = L::kWarps, kThreads = L::kThreads, kHeld = L::kHeld;
-  constexpr int E = kRows8 ? 2 : 4, R = kRows8 ? 1 : 2;  // values of a fragment, rows of a lane
+  constexpr int NB = kWide ? 2 : 1;  // eights of rows
   constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
   constexpr bool kMmaBf16 = kIsBf16 && !kI8;
-  constexpr int TP = L::kPos, N8 = TP / 8, KSTEPS = D / 16, REC = L::kRec, kSlots = L::kSlots, kChunks = L::kRowBytes / 16;
+  constexpr int TP = L::kPos, N16 = TP / 16, KSTEPS = D / 16, REC = L::kRec, kSlots = L::kSlots, kChunks = L::kRowBytes / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* records = reinterpret_cast<float*>(smem + kWarps * kSlots * (L::kBytes + L::kScales));
@@ -331,18 +325,20 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     if (++slot == kSlots) slot = 0, phase ^= 1u;
     issue();
   };
-  uint32_t qa[KSTEPS][E];  // (row gr, k lo), [(row gr + 8, k lo),] (gr, k hi) [, (gr + 8, k hi)]
-  float q_factor[R];       // what the rows of Q were divided by
   // What this lane's ldmatrix addresses start from, in a slot: 16 positions, chunk 0 or 1.  A pair of chunks further is the same with bits 5 and 6 turned (no row starts
   // inside them), eight chunks further the run's next 128-byte group.
-  uint32_t k_from[N8 / 2], v_from[N8 / 2];
+  uint32_t k_from[N16], v_from[N16];
 #pragma unroll
-  for (int j = 0; j < N8 / 2; ++j) {
-    k_from[j] = at(j * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, (lane >> 3) & 1);
-    v_from[j] = at(j * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, (lane >> 4) & 1);
+  for (int j = 0; j < N16; ++j) {
+    k_from[j] = at(j * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, (lane >> 4) & 1);  // (positions 0-7, chunk 0), (8-15, 0), (0-7, 1), (8-15, 1)
+    v_from[j] = at(j * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, (lane >> 3) & 1);  // (positions 0-7, chunk 0), (0-7, 1), (8-15, 0), (8-15, 1)
   }
   const uint32_t group = L::kRowBytes == 256 ? 1u << (lb + 7) : 0u;
   auto pair_of = [&](uint32_t from, int pair) -> uint32_t { return (from ^ ((pair & 3) << 5)) + (pair >= 4 ? group : 0u); };
+  uint32_t qb[NB][KSTEPS][2];  // row gr of an eight: its Q as B fragments
+  // of rows 2 tq and 2 tq + 1 of an eight, whose scores this lane has at positions gr and gr + 8 of a sixteen
+  float q_factor[NB][2];       // what the row of Q was divided by
+  int limit[NB][2];            // the last position it sees
   int head_state = 0, tail_b = -1, tail_unit = -1, turn = 0;
   for (int which = 0; parts[which].there; which ^= 1) {
     const Part& now = parts[which];
@@ -357,178 +353,176 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     }
     const int head = seq.passes == 1 ? unit : unit / seq.passes, row0 = (unit - head * seq.passes) * kHeld;
     const int rows = min(kHeld, seq.count * p.group - row0);
-    // rows gr and gr + 8: their Q as A fragments, and the last position each sees
-    int limit[R];
 #pragma unroll
-    for (int e = 0; e < R; ++e) {
-      const bool ok = gr + 8 * e < rows;
-      const int r = row0 + (ok ? gr + 8 * e : 0), token = r / p.group;
-      limit[e] = seq.len - seq.count + token;
+    for (int n = 0; n < NB; ++n) {
+      const bool ok = n * 8 + gr < rows;
+      const int r = row0 + (ok ? n * 8 + gr : 0), token = r / p.group;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(q + (static_cast<int64_t>(seq.first + token) * p.heads_q + head * p.group + r % p.group) * D);
 #pragma unroll
       for (int kk = 0; kk < KSTEPS; ++kk) {
         if (kI8) {  // the four numbers of a fragment lie together in a row of the cache
           const uint2 x = ok ? __ldg(reinterpret_cast<const uint2*>(src + kk * 8 + 2 * tq)) : make_uint2(0u, 0u);
-          qa[kk][e] = x.x, qa[kk][R + e] = x.y;
+          qb[n][kk][0] = x.x, qb[n][kk][1] = x.y;
         } else {
-          qa[kk][e] = ok ? __ldg(src + kk * 8 + tq) : 0u;
-          qa[kk][R + e] = ok ? __ldg(src + kk * 8 + tq + 4) : 0u;
+          qb[n][kk][0] = ok ? __ldg(src + kk * 8 + tq) : 0u;
+          qb[n][kk][1] = ok ? __ldg(src + kk * 8 + tq + 4) : 0u;
         }
       }
-      q_factor[e] = 1.f;
+      float factor = 1.f;
       if constexpr (kI8 && kIsBf16) {
         float top = 0.f;
 #pragma unroll
         for (int kk = 0; kk < KSTEPS; ++kk)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t x = qa[kk][R * i + e];
-            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x << 16)), fabsf(__uint_as_float(x & 0xffff0000u))));
-          }
+          for (int i = 0; i < 2; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(qb[n][kk][i] << 16)), fabsf(__uint_as_float(qb[n][kk][i] & 0xffff0000u))));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // the power of two below the largest magnitude: what lies 2^24 under that is lost, which f32 sums would lose too
         const int ex = min(max(static_cast<int>(__float_as_uint(top) >> 23), 20), 250) - 127;
-        q_factor[e] = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
+        factor = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
         const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
 #pragma unroll
         for (int kk = 0; kk < KSTEPS; ++kk)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            uint32_t& x = qa[kk][R * i + e];
+            uint32_t& x = qb[n][kk][i];
             x = mma::pack2<false>(__uint_as_float(x << 16) * inv, __uint_as_float(x & 0xffff0000u) * inv);
           }
       }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        q_factor[n][e] = __shfl_sync(0xffffffffu, factor, (2 * tq + e) * 4) * p.scale_log2;
+        const int mine = row0 + min(n * 8 + 2 * tq + e, rows - 1);
+        limit[n][e] = seq.len - seq.count + mine / p.group;
+      }
     }
     const int least = seq.len - seq.count + row0 / p.group;  // the first row's last position: tiles up to it need no masks
-    float oacc[2 * KSTEPS][E];
+    float oacc[KSTEPS][NB][4];
 #pragma unroll
-    for (int j = 0; j < 2 * KSTEPS; ++j)
+    for (int c = 0; c < KSTEPS; ++c)
 #pragma unroll
-      for (int e = 0; e < E; ++e) oacc[j][e] = 0.f;
-    float m[R], l[R];
+      for (int n = 0; n < NB; ++n) oacc[c][n][0] = oacc[c][n][1] = oacc[c][n][2] = oacc[c][n][3] = 0.f;
+    float m[NB][2], l[NB][2];
 #pragma unroll
-    for (int e = 0; e < R; ++e) m[e] = -INFINITY, l[e] = 0.f;
+    for (int n = 0; n < NB; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
     float v_top = 0x1p-100f;  // 8 bits: the largest step of V so far, oacc is in units of it; far smaller steps count as zero
     for (int tile = begin + (warp >= turn ? warp - turn : warp + kWarps - turn); tile < end; tile += kWarps) {
       if (!arrived()) break;
       const uint32_t ks = slots + slot * L::kBytes;
-      float s[N8][E];
+      float s[N16][NB][4];
 #pragma unroll
-      for (int j = 0; j < N8; ++j)
+      for (int j = 0; j < N16; ++j)
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[j][e] = 0.f;
+        for (int n = 0; n < NB; ++n) s[j][n][0] = s[j][n][1] = s[j][n][2] = s[j][n][3] = 0.f;
       if constexpr (!kI8) {
 #pragma unroll
         for (int kk = 0; kk < KSTEPS; ++kk)
 #pragma unroll
-          for (int j = 0; j < N8 / 2; ++j) {
-            uint32_t kb[4];  // (positions 0-7, k lo), (0-7, k hi), (8-15, k lo), (8-15, k hi)
-            mma::ldmatrix_x4(pair_of(ks + k_from[j], kk), kb);
-            mma_rows<kMmaBf16>(s[2 * j], qa[kk], kb[0], kb[1]);
-            mma_rows<kMmaBf16>(s[2 * j + 1], qa[kk], kb[2], kb[3]);
+          for (int j = 0; j < N16; ++j) {
+            uint32_t ka[4];
+            mma::ldmatrix_x4(pair_of(ks + k_from[j], kk), ka);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) mma_tile<kMmaBf16>(s[j][n], ka[0], ka[1], ka[2], ka[3], qb[n][kk][0], qb[n][kk][1]);
           }
       } else {
 #pragma unroll
-        for (int kk = 0; kk < KSTEPS; kk += 2) {
-          uint32_t kb[N8 / 2][4];  // (positions 0-7, 16 numbers), (0-7, the next 16), (8-15, 16), (8-15, the next)
+        for (int kk = 0; kk < KSTEPS; kk += 2)
 #pragma unroll
-          for (int j = 0; j < N8 / 2; ++j) mma::ldmatrix_x4(pair_of(ks + k_from[j], kk / 2), kb[j]);
+          for (int j = 0; j < N16; ++j) {
+            uint32_t kx[4];
+            mma::ldmatrix_x4(pair_of(ks + k_from[j], kk / 2), kx);
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t x = kx[2 * i] ^ 0x80808080u, y = kx[2 * i + 1] ^ 0x80808080u;
+              const uint32_t a0 = i8_pair(x, 0x4140), a1 = i8_pair(y, 0x4140), a2 = i8_pair(x, 0x4342), a3 = i8_pair(y, 0x4342);
 #pragma unroll
-            for (int j = 0; j < N8; ++j) {
-              const uint32_t x = kb[j / 2][2 * (j & 1) + i] ^ 0x80808080u;
-              mma_rows<false>(s[j], qa[kk + i], i8_pair(x, 0x4140), i8_pair(x, 0x4342));
+              for (int n = 0; n < NB; ++n) mma_tile<false>(s[j][n], a0, a1, a2, a3, qb[n][kk + i][0], qb[n][kk + i][1]);
             }
-        }
+          }
       }
-      const int pos = tile * TP + 2 * tq;
+      const int pos = tile * TP + gr;
       const bool masked = (tile + 1) * TP - 1 > least;
-      if constexpr (kI8) {
-        const float* kst = steps_at + slot * TP + 2 * tq;
 #pragma unroll
-        for (int j = 0; j < N8; ++j) {
-          const float2 st = *reinterpret_cast<const float2*>(kst + j * 8);
-          const float a = st.x * p.scale_log2, b = st.y * p.scale_log2;
+      for (int j = 0; j < N16; ++j)
 #pragma unroll
-          for (int e = 0; e < R; ++e) s[j][2 * e] *= a * q_factor[e], s[j][2 * e + 1] *= b * q_factor[e];
+        for (int h = 0; h < 2; ++h) {
+          const float step = kI8 ? steps_at[slot * TP + j * 16 + h * 8 + gr] : 1.f;
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[j][n][2 * h + e] *= kI8 ? step * q_factor[n][e] : p.scale_log2;
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < N8; ++j)
-#pragma unroll
-          for (int e = 0; e < E; ++e) s[j][e] *= p.scale_log2;
-      }
       release();
       if (masked) {
 #pragma unroll
-        for (int j = 0; j < N8; ++j)
+        for (int j = 0; j < N16; ++j)
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (pos + j * 8 + (e & 1) > limit[e >> 1]) s[j][e] = -INFINITY;
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (pos + j * 16 + (e >> 1) * 8 > limit[n][e & 1]) s[j][n][e] = -INFINITY;
       }
-      float a[R];
+      float a[NB][2];
 #pragma unroll
-      for (int e = 0; e < R; ++e) {
-        float top = -INFINITY;
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int j = 0; j < N8; ++j) top = fmaxf(top, fmaxf(s[j][2 * e], s[j][2 * e + 1]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float n = fmaxf(m[e], top), base = n == -INFINITY ? 0.f : n;  // a row may see nothing of this warp's first tiles
-        a[e] = ptx::ex2_approx(m[e] - base);
-        m[e] = n;
-        float sum = 0.f;
+        for (int e = 0; e < 2; ++e) {
+          float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < N8; ++j) {
-          s[j][2 * e] = ptx::ex2_approx(s[j][2 * e] - base);
-          s[j][2 * e + 1] = ptx::ex2_approx(s[j][2 * e + 1] - base);
-          sum += s[j][2 * e] + s[j][2 * e + 1];
+          for (int j = 0; j < N16; ++j) top = fmaxf(top, fmaxf(s[j][n][e], s[j][n][2 + e]));
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          const float most = fmaxf(m[n][e], top), base = most == -INFINITY ? 0.f : most;  // a row may see nothing of this warp's first tiles
+          a[n][e] = ptx::ex2_approx(m[n][e] - base);
+          m[n][e] = most;
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < N16; ++j) {
+            s[j][n][e] = ptx::ex2_approx(s[j][n][e] - base);
+            s[j][n][2 + e] = ptx::ex2_approx(s[j][n][2 + e] - base);
+            sum += s[j][n][e] + s[j][n][2 + e];
+          }
+          l[n][e] = fmaf(l[n][e], a[n][e], sum);
         }
-        l[e] = fmaf(l[e], a[e], sum);
-      }
       if (!arrived()) break;
       const uint32_t vs = slots + slot * L::kBytes;
       const bool ragged = (tile + 1) * TP > seq.len;
       if constexpr (kI8) {
-        const float* vst = steps_at + slot * TP + 2 * tq;
-        float2 st[N8];
-        float top = v_top;
+        float st[N16][2], top = v_top;
 #pragma unroll
-        for (int j = 0; j < N8; ++j) {
-          st[j] = *reinterpret_cast<const float2*>(vst + j * 8);
-          if (ragged) {  // behind the last position may be anything
-            if (pos + j * 8 >= seq.len) st[j].x = 0.f;
-            if (pos + j * 8 + 1 >= seq.len) st[j].y = 0.f;
+        for (int j = 0; j < N16; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            st[j][h] = steps_at[slot * TP + j * 16 + h * 8 + gr];
+            if (ragged && pos + j * 16 + h * 8 >= seq.len) st[j][h] = 0.f;  // behind the last position may be anything
+            top = fmaxf(top, st[j][h]);
           }
-          top = fmaxf(top, fmaxf(st[j].x, st[j].y));
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         const float inv = 1.f / top;
 #pragma unroll
-        for (int e = 0; e < R; ++e) a[e] *= v_top * inv;
+        for (int n = 0; n < NB; ++n) a[n][0] *= v_top * inv, a[n][1] *= v_top * inv;
         v_top = top;
 #pragma unroll
-        for (int j = 0; j < N8; ++j) {
-          const float x = st[j].x * inv, y = st[j].y * inv;
+        for (int j = 0; j < N16; ++j)
 #pragma unroll
-          for (int e = 0; e < R; ++e) s[j][2 * e] *= x, s[j][2 * e + 1] *= y;
-        }
+          for (int h = 0; h < 2; ++h) {
+            const float x = st[j][h] * inv;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) s[j][n][2 * h] *= x, s[j][n][2 * h + 1] *= x;
+          }
       }
-      uint32_t pa[N8 / 2][E];
+      uint32_t pb[N16][NB][2];
 #pragma unroll
-      for (int j = 0; j < N8 / 2; ++j)
+      for (int j = 0; j < N16; ++j)
 #pragma unroll
-        for (int e = 0; e < R; ++e) {
-          pa[j][e] = mma::pack2<kMmaBf16>(s[2 * j][2 * e], s[2 * j][2 * e + 1]);
-          pa[j][R + e] = mma::pack2<kMmaBf16>(s[2 * j + 1][2 * e], s[2 * j + 1][2 * e + 1]);
-        }
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int j = 0; j < 2 * KSTEPS; ++j)
+          for (int h = 0; h < 2; ++h) pb[j][n][h] = transposed(mma::pack2<kMmaBf16>(s[j][n][2 * h], s[j][n][2 * h + 1]));
 #pragma unroll
-        for (int e = 0; e < R; ++e) oacc[j][2 * e] *= a[e], oacc[j][2 * e + 1] *= a[e];
+      for (int c = 0; c < KSTEPS; ++c)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) oacc[c][n][0] *= a[n][0], oacc[c][n][1] *= a[n][1], oacc[c][n][2] *= a[n][0], oacc[c][n][3] *= a[n][1];
       if (!kI8 && ragged) {
         // what lies behind the last position weighs nothing, but may be anything
         for (int i = lane; i < TP * kChunks; i += 32)
@@ -536,23 +530,24 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         __syncwarp();
       }
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c)
+      for (int c = 0; c < KSTEPS; ++c)
 #pragma unroll
-        for (int j = 0; j < N8 / 2; ++j) {
-          uint32_t vb[4];
+        for (int j = 0; j < N16; ++j) {
+          uint32_t va[4];
           if constexpr (!kI8) {
-            // (positions 0-7, d lo), (8-15, d lo), (0-7, d hi), (8-15, d hi), transposed on load
-            mma::ldmatrix_x4_trans(pair_of(vs + v_from[j], c), vb);
-            mma_rows<kMmaBf16>(oacc[2 * c], pa[j], vb[0], vb[1]);
-            mma_rows<kMmaBf16>(oacc[2 * c + 1], pa[j], vb[2], vb[3]);
+            // transposed on load: (d 0-7, positions 0-7), (d 8-15, 0-7), (d 0-7, 8-15), (d 8-15, 8-15)
+            mma::ldmatrix_x4_trans(pair_of(vs + v_from[j], c), va);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) mma_tile<kMmaBf16>(oacc[c][n], va[0], va[1], va[2], va[3], pb[j][n][0], pb[j][n][1]);
           } else if (c % 2 == 0) {
-            // the same of pairs of numbers: two positions of column 2 gr and of column 2 gr + 1 in a register
-            mma::ldmatrix_x4_trans(pair_of(vs + v_from[j], c / 2), vb);
+            // the same of pairs of numbers: two positions of column 2 gr and of column 2 gr + 1 in a register, which become rows gr and gr + 8
+            mma::ldmatrix_x4_trans(pair_of(vs + v_from[j], c / 2), va);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const uint32_t x = vb[2 * i] ^ 0x80808080u, y = vb[2 * i + 1] ^ 0x80808080u;
-              mma_rows<false>(oacc[2 * (c + i)], pa[j], i8_pair(x, 0x4240), i8_pair(y, 0x4240));
-              mma_rows<false>(oacc[2 * (c + i) + 1], pa[j], i8_pair(x, 0x4341), i8_pair(y, 0x4341));
+              const uint32_t x = va[i] ^ 0x80808080u, y = va[2 + i] ^ 0x80808080u;
+              const uint32_t a0 = i8_pair(x, 0x4240), a1 = i8_pair(x, 0x4341), a2 = i8_pair(y, 0x4240), a3 = i8_pair(y, 0x4341);
+#pragma unroll
+              for (int n = 0; n < NB; ++n) mma_tile<false>(oacc[c + i][n], a0, a1, a2, a3, pb[j][n][0], pb[j][n][1]);
             }
           }
         }
@@ -560,31 +555,38 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       release();
     }
 #pragma unroll
-    for (int e = 0; e < R; ++e) {
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-    }
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], off);
 
     // the warps' records, eight rows at a time
     const bool whole = begin == 0 && end == seq.tiles;
     for (int half = 0; half * 8 < rows; ++half) {
       __syncthreads();  // the records before have been read
       {
-        float* rec = records + (warp * 8 + gr) * REC;
+        float* rec = records + (warp * 8 + 2 * tq) * REC;
         const float f = kI8 ? v_top : 1.f;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          constexpr int H = kRows8 ? 0 : 2;  // the other row's
-          const float x0 = (half ? oacc[2 * c][H] : oacc[2 * c][0]) * f, x1 = (half ? oacc[2 * c][H + 1] : oacc[2 * c][1]) * f;
-          const float y0 = (half ? oacc[2 * c + 1][H] : oacc[2 * c + 1][0]) * f, y1 = (half ? oacc[2 * c + 1][H + 1] : oacc[2 * c + 1][1]) * f;
-          if (kI8) {
-            *reinterpret_cast<float4*>(rec + c * 16 + 4 * tq) = make_float4(x0, y0, x1, y1);
-          } else {
-            *reinterpret_cast<float2*>(rec + c * 16 + 2 * tq) = make_float2(x0, x1);
-            *reinterpret_cast<float2*>(rec + c * 16 + 8 + 2 * tq) = make_float2(y0, y1);
+        for (int n = 0; n < NB; ++n) {
+          if (n != half) continue;
+#pragma unroll
+          for (int c = 0; c < KSTEPS; ++c)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (kI8) {
+                *reinterpret_cast<float2*>(rec + e * REC + c * 16 + 2 * gr) = make_float2(oacc[c][n][e] * f, oacc[c][n][2 + e] * f);
+              } else {
+                rec[e * REC + c * 16 + gr] = oacc[c][n][e];
+                rec[e * REC + c * 16 + 8 + gr] = oacc[c][n][2 + e];
+              }
+            }
+          if (gr == 0) {
+            *reinterpret_cast<float2*>(rec + D) = make_float2(m[n][0], l[n][0]);
+            *reinterpret_cast<float2*>(rec + REC + D) = make_float2(m[n][1], l[n][1]);
           }
         }
-        if (tq == 0) *reinterpret_cast<float2*>(rec + D) = half ? make_float2(m[R - 1], l[R - 1]) : make_float2(m[0], l[0]);
       }
       __syncthreads();
       for (int i = tid; i < min(8, rows - half * 8) * (D / 4); i += kThreads) {

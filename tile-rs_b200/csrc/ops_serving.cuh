@@ -226,9 +226,9 @@ inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& 
 }
 
 // The tiles of all sequences' caches dealt out evenly over the SMs, and what several of them have a part of merged (attention_paged.cuh).
-template <typename T, bool kI8, int D, bool kRows8>
+template <typename T, bool kI8, int D, bool kWide>
 inline int32_t attention_paged_few_launch(std::string* err, paged::Params p, const void* q, void* o, cudaStream_t s) {
-  using L = paged::Tile<kI8, D, kRows8>;
+  using L = paged::Tile<kI8, D, kWide>;
   int sms = 0;
   int32_t st = sm_count(err, &sms);
   if (st != TSM100_OK) return st;
@@ -266,7 +266,7 @@ inline int32_t attention_paged_few_launch(std::string* err, paged::Params p, con
     st = make_tmap(err, &map[i], key, kI8 ? 1 : 2);
   }
   if (st == TSM100_OK) {
-    auto kern = boxes ? paged::attention_paged_kernel<T, kI8, D, true, kRows8> : paged::attention_paged_kernel<T, kI8, D, false, kRows8>;
+    auto kern = boxes ? paged::attention_paged_kernel<T, kI8, D, true, kWide> : paged::attention_paged_kernel<T, kI8, D, false, kWide>;
     cudaError_t e = set_dyn_smem_once(kern, L::kSmem);
     if (e == cudaSuccess) e = launch_chained(kern, ctas, L::kThreads, L::kSmem, s, 0, map[0], map[1], static_cast<const T*>(q), static_cast<T*>(o), p);
     if (e == cudaSuccess) e = launch_chained(paged::attention_paged_merge_kernel<T, D, L::kHeld>, dim3(ctas, static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, 0, static_cast<T*>(o), p);
@@ -283,7 +283,7 @@ inline int32_t attention_paged_launch(std::string* err, const paged::Params& p, 
   const int64_t rows = static_cast<int64_t>(p.step.max_new) * p.group;
   const int wide = page_run_log2(p.cache.page_size, 7);
   if (rows > paged::kRows && p.group <= paged::tc::kMaxGroup && (kI8 || wide >= 3)) return attention_paged_tc_launch<T, kI8, D>(err, p, wide, q, o, s);
-  return rows <= 8 ? attention_paged_few_launch<T, kI8, D, true>(err, p, q, o, s) : attention_paged_few_launch<T, kI8, D, false>(err, p, q, o, s);
+  return rows > 8 ? attention_paged_few_launch<T, kI8, D, true>(err, p, q, o, s) : attention_paged_few_launch<T, kI8, D, false>(err, p, q, o, s);
 }
 
 template <typename T>
