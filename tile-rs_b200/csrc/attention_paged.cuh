@@ -29,7 +29,7 @@ namespace mma = attn_decode::mma;
 
 constexpr int kRows = 16;     // of a pass, at most
 constexpr int kMaxCtas = 1024;
-constexpr int kUnitCost = 6;  // what beginning and ending a pair costs, in tiles: shares are as long in tiles and these
+constexpr int kUnitCost = 16;  // what beginning and ending a pair costs, in tiles: shares are as long in tiles and these
 template <bool kI8, int D, bool kWide>
 struct Tile {
   static constexpr int kWarps = kWide ? 8 : 12, kThreads = kWarps * 32;
@@ -242,13 +242,15 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   };
 
   // The warp's tiles, ahead of their use: K and V of a tile in turn.  Tiles are dealt to the warps in turn, across units.
-  int load_slot = 0, page = 0, tile_ahead = ahead.begin + warp, end_ahead = ahead.end, head_ahead = 0, turn_ahead = 0, b_ahead = 0, len_ahead = 0;
+  int load_slot = 0, tile_ahead = ahead.begin + warp, end_ahead = ahead.end, head_ahead = 0, turn_ahead = 0, b_ahead = 0, len_ahead = 0;
   bool load_v = false, more = ahead.there;
   auto look = [&]() {
     b_ahead = ahead.seq.b, len_ahead = ahead.seq.len, end_ahead = ahead.end;
     head_ahead = ahead.seq.passes == 1 ? ahead.unit : ahead.unit / ahead.seq.passes;
   };
   look();
+  int row_ahead = 0, at_ahead = 0;  // (lane i) the tile's i-th run: its row of pages times heads, and its first position there
+  const int page_bits = (ps & (ps - 1)) == 0 ? 31 - __clz(ps) : -1;
   auto settle = [&]() {  // on to the first unit that has tile_ahead for this warp, and (lane i) the page of the tile's i-th run
     while (more && tile_ahead >= end_ahead) {
       turn_ahead = (turn_ahead + end_ahead - ahead.begin) % kWarps;
@@ -262,8 +264,14 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     if (!more) return;
     if (kTma) {
       const int pos = tile_ahead * TP + (lane << lb);
-      page = 0;
-      if ((lane << lb) < TP && pos < len_ahead) page = max(0, pages::page_of(p.cache, p.step, b_ahead, pos, p.status, 144));
+      row_ahead = head_ahead, at_ahead = 0;
+      if ((lane << lb) < TP && pos < len_ahead) {
+        const int nth = page_bits >= 0 ? pos >> page_bits : pos / ps;
+        at_ahead = pos - nth * ps;
+        int page = p.step.table[static_cast<int64_t>(b_ahead) * p.step.pitch + nth];
+        if (page < 0 || page >= p.cache.pages) pages::report(p.status, 144), page = 0;
+        row_ahead += page * heads;
+      }
     }
   };
   auto issue = [&]() {
@@ -278,13 +286,12 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       if (lane == 0) ptx::mbar_arrive_expect_tx(&full[load_slot], runs * (run * (L::kRowBytes + (kI8 ? 4 : 0))));
       __syncwarp();
       if (lane < runs) {
-        const int in_page = (pos0 + (lane << lb)) % ps;
         const CUtensorMap* map = load_v ? &tmap_v : &tmap_k;
         const uint32_t to = dst + ((lane << lb) * L::kRowBytes);
-        const int row = page * heads + head_ahead;
-        if constexpr (L::kRowBytes == 256) tma_load_4d(to, map, &full[load_slot], in_page, row);
-        else tma_load_3d(to, map, &full[load_slot], in_page, row);
-        if constexpr (kI8) bulk_load(dst_steps + (lane << lb) * 4, p.cache.scales[load_v] + static_cast<int64_t>(row) * ps + in_page, run * 4, &full[load_slot]);
+        if constexpr (L::kRowBytes == 256) tma_load_4d(to, map, &full[load_slot], at_ahead, row_ahead);
+        else tma_load_3d(to, map, &full[load_slot], at_ahead, row_ahead);
+        if constexpr (kI8)
+          bulk_load(dst_steps + (lane << lb) * 4, (load_v ? p.cache.scales[1] : p.cache.scales[0]) + static_cast<int64_t>(row_ahead) * ps + at_ahead, run * 4, &full[load_slot]);
       }
     } else {
       for (int i = lane; i < TP * kChunks; i += 32) {
@@ -637,6 +644,19 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   }
 }
 
+// How many records a unit has that goes on behind the share of this CTA's column: that share's second, and the first of those behind it up to the one it ends in.  A warp
+// looks at 32 shares at once.
+__device__ __forceinline__ int records_of(const int4* info) {
+  const int lane = threadIdx.x & 31;
+  int n = 1;
+  for (int at = blockIdx.x + 1; at < static_cast<int>(gridDim.x); at += 32) {
+    const unsigned on = __ballot_sync(0xffffffffu, at + lane < static_cast<int>(gridDim.x) && __ldcg(&info[at + lane].x) == 2);
+    if (on != 0xffffffffu) return n + __ffs(~on);
+    n += 32;
+  }
+  return n;
+}
+
 // The records of a pair that several shares have a part of, in order; a warp per row, CTA (x, y) rows 4 y .. of the pair that goes on behind share x.
 template <typename T, int D, int kHeld>
 __global__ void __launch_bounds__(128)
@@ -647,12 +667,7 @@ attention_paged_merge_kernel(T* __restrict__ o, const __grid_constant__ Params p
   ptx::wait_prior_grid();
   const int4 mine = __ldcg(p.info + blockIdx.x);
   if (mine.y < 0) return;
-  int n = 1;  // records: this share's second, and the first of the shares behind it
-  while (blockIdx.x + n < gridDim.x) {
-    const int state = __ldcg(p.info + blockIdx.x + n).x;
-    ++n;
-    if (state != 2) break;
-  }
+  const int n = records_of(p.info);
   const int first = p.step.starts[mine.y], count = p.step.starts[mine.y + 1] - first;
   const int passes = static_cast<int>((static_cast<int64_t>(count) * p.group + kHeld - 1) / kHeld), head = mine.z / passes, row = mine.z % passes * kHeld + r;
   if (r >= kHeld || row >= count * p.group) return;

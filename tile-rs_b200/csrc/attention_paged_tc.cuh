@@ -15,6 +15,7 @@
 // Bound: the tensor core and the exponentials, as there.
 #pragma once
 
+#include "attention_paged.cuh"
 #include "attention_tc.cuh"
 #include "kv_pages.cuh"
 #include "ptx.cuh"
@@ -707,16 +708,11 @@ attention_paged_tc_merge_kernel(uint16_t* __restrict__ o, const __grid_constant_
   ptx::wait_prior_grid();
   const int4 mine = __ldcg(p.info + blockIdx.x);
   if (mine.y < 0) return;
+  const int n = records_of(p.info);
   const int first = p.step.starts[mine.y], count = p.step.starts[mine.y + 1] - first;
   const int g = threadIdx.x >> 7, r = threadIdx.x & 127, r_token = r / p.group;
   const int token = (mine.w * 2 + g) * p.tokens + r_token;
   if (r_token >= p.tokens || token >= count) return;
-  int n = 1;  // records: this share's second, and the first of the shares behind it
-  while (blockIdx.x + n < gridDim.x) {
-    const int state = __ldcg(p.info + blockIdx.x + n).x;
-    ++n;
-    if (state != 2) break;
-  }
   auto record = [&](int i) { return static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0); };
   float gm = -INFINITY;
   for (int i = 0; i < n; ++i) gm = fmaxf(gm, __ldcg(p.part_ml + record(i) * 256 + threadIdx.x).x);
