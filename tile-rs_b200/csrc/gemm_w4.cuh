@@ -4,11 +4,11 @@
 // of W on the M side, up to 128 rows of A on the N side.  A group's sum comes back from tensor memory, is multiplied by its scale and added in
 // f32, so C is rounded once and nothing else.
 //
-// Bound: with few rows of A reading the weights, 46 of them a clock and SM.  That rules mma.sync out, which gives 256 multiply-adds a clock and SM on
-// sm_100a (16 x 16384 x 4096 took 31 us that way), and weights in shared memory as well, which would write and read 184 bytes a clock of them.  So a thread, which has
-// a row of W, brings 64 k of it from the TMA's tile into registers, makes numbers of them with eleven instructions for eight (three shifts, four masks that also
-// set the exponent of 128 + q or 1024 + q, four subtractions) and stores them to tensor memory, from where the product takes them.  With many rows of A
-// the tensor core is the bound.
+// Bound: with few rows of A reading the weights, 46 of them a clock and SM.  Weights in shared memory would write and read 184 bytes a clock there for the tensor core, more
+// than it gives; mma.sync tiles with the weights in registers took 31 us for 16 x 16384 x 4096.  So a thread, which has a row of W, brings 64 k of it from the
+// TMA's tile into registers, makes numbers of them with eleven instructions for eight (three shifts, four masks that also set the exponent of 128 + q or 1024 + q, four
+// subtractions) and stores them to tensor memory, from where the product takes them.  What bounds it as it is: instructions, 200 a warp for 64 k of its 32
+// rows where 88 make the numbers.  With many rows of A the tensor core would be the bound, and the chain of steps of a chunk is.
 //
 // A CTA has 128 rows of W, up to 128 of A and a range of K, 128 k at a time: eight warps make the weights (four of them the first 64 k, four the others) and bring A's part to
 // shared memory in the order in which masks find the weights (of eight k 0 4 1 5 2 6 3 7, K-major, 128-byte swizzle); a warp fetches W by TMA, a warp issues the products.
@@ -203,41 +203,40 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
     }
   } else {
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    // A chunk's scales and zero points, and its part of A, are fetched two chunks ahead (many rows of A: one), into the registers that the chunk before has
-    // left.
-    constexpr int kAhead = S::kVecs <= 2 ? 2 : 1;
+    // A chunk's scales and zero points, and its part of A, are fetched two chunks ahead, into the registers that the chunk before has left.  (128 rows of A: one, 200 x 5003
+    // x 2048 21.5 us; two take too many registers, 42.)
+    constexpr int kAhead = S::kVecs <= 4 ? 2 : 1;
     const int64_t row_groups = static_cast<int64_t>(min(row_base + row, p.n - 1)) * p.groups + first * GC;
     const uint16_t* scale_at = static_cast<const uint16_t*>(p.scales) + row_groups;
     const uint8_t* zero_at = p.zeros ? p.zeros + row_groups : nullptr;
-    const int groups_left = row_base + row < p.n ? min(p.groups - first * GC, chunks * GC) : 0;
+    const int groups_left = min(p.groups - first * GC, chunks * GC);
     // a chunk's groups in one load where they never start inside one
     const bool together = GC > 1 && p.groups % GC == 0 && reinterpret_cast<uintptr_t>(p.scales) % (2 * GC) == 0 && reinterpret_cast<uintptr_t>(p.zeros) % GC == 0;
     uint16_t sc[2][GC];
     uint32_t zp[2];  // a byte a group
+    const int last_group = max(groups_left - 1, 0), last_chunk = max((groups_left - 1) / GC, 0);
+    // Behind the last group it is fetched again: A is zero there, and rows behind N are not stored.
     auto fetch_row = [&](int i, uint16_t (&to)[GC], uint32_t& zero) {
-#pragma unroll
-      for (int j = 0; j < GC; ++j) to[j] = 0;
-      if (zero_at) zero = 0x08080808u;
-      if (together) {
-        if (i * GC < groups_left) {
-          if constexpr (GC == 4) {
-            const uint2 x = *reinterpret_cast<const uint2*>(scale_at + i * GC);
-            to[0] = static_cast<uint16_t>(x.x), to[GC - 3] = static_cast<uint16_t>(x.x >> 16);
-            to[GC - 2] = static_cast<uint16_t>(x.y), to[GC - 1] = static_cast<uint16_t>(x.y >> 16);
-            if (zero_at) zero = *reinterpret_cast<const uint32_t*>(zero_at + i * GC);
-          } else {
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(scale_at + i * GC);
-            to[0] = static_cast<uint16_t>(x), to[GC - 1] = static_cast<uint16_t>(x >> 16);
-            if (zero_at) zero = *reinterpret_cast<const uint16_t*>(zero_at + i * GC);
-          }
+      if (GC > 1 && together) {
+        const int at = min(i, last_chunk) * GC;
+        if constexpr (GC == 4) {
+          const uint2 x = *reinterpret_cast<const uint2*>(scale_at + at);
+          to[0] = static_cast<uint16_t>(x.x), to[GC - 3] = static_cast<uint16_t>(x.x >> 16);
+          to[GC - 2] = static_cast<uint16_t>(x.y), to[GC - 1] = static_cast<uint16_t>(x.y >> 16);
+          if (zero_at) zero = *reinterpret_cast<const uint32_t*>(zero_at + at);
+        } else {
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(scale_at + at);
+          to[0] = static_cast<uint16_t>(x), to[GC - 1] = static_cast<uint16_t>(x >> 16);
+          if (zero_at) zero = *reinterpret_cast<const uint16_t*>(zero_at + at);
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < GC; ++j)
-          if (i * GC + j < groups_left) {
-            to[j] = scale_at[i * GC + j];
-            if (zero_at) zero = (zero & ~(0xffu << (8 * j))) | static_cast<uint32_t>(zero_at[i * GC + j]) << (8 * j);
-          }
+        for (int j = 0; j < GC; ++j) to[j] = scale_at[min(i * GC + j, last_group)];
+        if (zero_at) {
+          zero = 0;
+#pragma unroll
+          for (int j = 0; j < GC; ++j) zero |= static_cast<uint32_t>(zero_at[min(i * GC + j, last_group)]) << (8 * j);
+        }
       }
     };
     using Vec = typename std::conditional<kEight, uint2, uint4>::type;  // eight numbers of A
