@@ -10,8 +10,9 @@
 //     for a merging kernel.
 //   * K and V come by pages: boxes of a power of two of positions (8 and more), a lane each.  What a page holds behind the sequence's end is
 //     replaced by zeros in V (it has no weight, but may be NaN) and masked in S.
-//   * 8 bits (kI8): four warps write the tiles that TMA would have written.  K's whole numbers are exact in 16 bits and the scores are multiplied by the steps (rounded
-//     with them, f16 outputs were up to 1e-2 of a row's magnitude off); V is multiplied by its steps and rounded once.
+//   * 8 bits (kI8): four warps write the tiles that TMA would have written, whole numbers, which 16 bits hold exactly.  K's steps multiply the scores and V's the
+//     probabilities, so that nothing but the probabilities is rounded (with K and V times their steps rounded, errors were 1.6 times as large).  f16 probabilities times steps
+//     keep their bits by a power of two that follows the largest step and is taken out again with the sum.
 // Bound: the tensor core and the exponentials, as there.
 #pragma once
 
@@ -40,9 +41,8 @@ struct Shape {
   static constexpr int kTileBytes = kHalves * kHalfBytes;
   static constexpr int kPBytes = 2 * kHalfBytes;
   static constexpr int kRing = D == 128 ? 3 : 6;
-  // K's steps of the last key tiles: tile s is written when the softmax of s - 3 is over (ring of 3) or of s - 5 (of 6, by the order of the steps)
-  static constexpr int kStepTiles = kI8 ? (D == 128 ? 3 : 8) : 0;
-  static constexpr int kPOff = 2 * kTileBytes, kRingOff = kPOff + 2 * kPBytes, kStepsOff = kRingOff + kRing * kTileBytes, kBarsOff = kStepsOff + kStepTiles * 512;
+  static constexpr int kStepBytes = kI8 ? 2 * kKeys * 4 + 16 : 0;  // of a tile: K's, V's, and the largest of V's that each of the four warps saw; two tiles
+  static constexpr int kPOff = 2 * kTileBytes, kRingOff = kPOff + 2 * kPBytes, kStepsOff = kRingOff + kRing * kTileBytes, kBarsOff = kStepsOff + 2 * kStepBytes;
 };
 static_assert(256 * 184 + 128 * 48 + 128 * 96 <= 512 * 128 && 256 * 216 + 128 * 72 <= 384 * 168, "registers of a block at launch");
 
@@ -51,6 +51,7 @@ struct alignas(8) Barriers {
   uint64_t kv_full[6], kv_empty[6];
   uint64_t tail;              // the copies of a V tile that ends behind its sequence
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], o_free[2];
+  uint64_t steps_free[2][2];  // [query tile][place]
   int64_t scan[17];
   int64_t first_base;
   int32_t first_seq;
@@ -58,8 +59,9 @@ struct alignas(8) Barriers {
   uint32_t abort_flag;
   uint32_t pv_steps;          // steps whose P V has been issued (only grows)
 };
+// The shared memory of a kernel without variables of its own begins on a 1024-byte boundary (it is checked); there is no room for more.
 template <bool kI8, int D>
-constexpr int smem_bytes() { return Shape<kI8, D>::kBarsOff + static_cast<int>(sizeof(Barriers)) + 1024; }
+constexpr int smem_bytes() { return Shape<kI8, D>::kBarsOff + static_cast<int>(sizeof(Barriers)); }
 static_assert(smem_bytes<true, 128>() <= 227 * 1024 && smem_bytes<true, 64>() <= 227 * 1024, "shared memory of one CTA");
 
 struct Params {
@@ -148,8 +150,12 @@ __global__ void __launch_bounds__(Shape<kI8, D>::kThreads, 1)
 attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                           uint16_t* __restrict__ o, const __grid_constant__ Params p) {
   using S = Shape<kI8, D>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((ptx::smem_u32(smem) & 1023u) != 0u) {
+    ptx::wait_prior_grid();
+    if (threadIdx.x == 0) p.info[blockIdx.x] = make_int4(0, -1, 0, 0), atomicCAS(p.status, ptx::kStatusOk, ptx::kStatusWaitTimeout | 174u);
+    return;
+  }
   uint8_t* smem_q = smem;                  // two tiles
   uint8_t* smem_p = smem + S::kPOff;       // the probabilities of tile A and of tile B
   uint8_t* smem_kv = smem + S::kRingOff;
@@ -170,6 +176,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       ptx::mbar_init(&bars->p_ready[g], 128);
       ptx::mbar_init(&bars->pv_done[g], 1);
       ptx::mbar_init(&bars->o_free[g], 128);
+      for (int i = 0; i < 2; ++i) ptx::mbar_init(&bars->steps_free[g][i], 128);
     }
     bars->abort_flag = 0;
     bars->pv_steps = 0;
@@ -400,7 +407,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       // A warp has 32 rows of a tile, a lane finds one of them: row (lane / kOwn) * kRowsAt + cw * kOwn + lane % kOwn
       constexpr int kOwn = 32 / kVecs;
       const int my_row = lane / kOwn * kRowsAt + cw * kOwn + lane % kOwn;
-      int idx0 = 0;
+      int idx0 = 0, uses[2][2] = {{0, 0}, {0, 0}};  // how often a query tile has read a place's steps
       bool ok = true;
       while (ok && stream.next(p, w)) {
         // A tile's page is asked for three tiles ahead, its steps two and its rows one, so that none of these loads is waited for.
@@ -409,7 +416,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         auto pos_of = [&](int i) { return (w.begin + (i == 0 ? 0 : i == total - 1 ? w.n - 1 : (i & 1) == 0 ? (i >> 1) - 1 : (i + 1) >> 1)) * kKeys + my_row; };
         int32_t page = -1;        // of this lane's row of a tile
         int64_t row_at = -1;      // -1: behind the sequence's end
-        float step_at = 0.f, step_next = 0.f;
+        float k_step = 0.f, v_step = 0.f, k_next = 0.f, v_next = 0.f;  // with a tile of K come the steps of both
         uint4 next[kVecs];
         auto ask_page = [&](int i) {
           const int pos = pos_of(i);
@@ -418,18 +425,18 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         auto ask_step = [&](int i) {
           const int pos = pos_of(i);
           row_at = -1;
-          step_at = 0.f;
+          k_step = v_step = 0.f;
           if (i < total && pos < w.len) {
             if (page < 0 || page >= p.cache.pages) {
               pages::report(p.status, 146);
               page = 0;
             }
             row_at = (static_cast<int64_t>(page) * p.cache.heads + w.head) * ps + pos % ps;
-            step_at = (second(i) ? p.cache.scales[1] : p.cache.scales[0])[row_at];
+            if (!second(i)) k_step = p.cache.scales[0][row_at], v_step = p.cache.scales[1][row_at];
           }
         };
         auto ask_rows = [&](int i) {
-          step_next = step_at;
+          k_next = k_step, v_next = v_step;
           const uint8_t* from = static_cast<const uint8_t*>(second(i) ? p.cache.kv[1] : p.cache.kv[0]);
 #pragma unroll
           for (int v = 0; v < kVecs; ++v) {
@@ -448,31 +455,39 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           uint4 x[kVecs];
 #pragma unroll
           for (int v = 0; v < kVecs; ++v) x[v] = next[v];
-          const float step_now = step_next;
+          const float k_now = k_next, v_now = v_next;
           ask_rows(i + 1);
           ask_step(i + 2);
           ask_page(i + 3);
           const int slot = (idx0 + i) % S::kRing;
           if (!(ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->kv_empty[slot], (((idx0 + i) / S::kRing) & 1u) ^ 1u, abort_flag, p.status, 164)))) break;
           const uint32_t to = ptx::smem_u32(smem_kv + slot * S::kTileBytes);
-          const bool is_v = second(i);
-          const float mine = is_v ? step_now : 1.f;  // K stays whole numbers
 #pragma unroll
           for (int v = 0; v < kVecs; ++v) {
-            const float st = __shfl_sync(0xffffffffu, mine, v * kOwn + lane / kVecs);
             const int row = v * kRowsAt + cw * kOwn + lane / kVecs;
             const uint32_t in[4] = {x[v].x, x[v].y, x[v].z, x[v].w};
             uint32_t out[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              out[e] = attn::pack16x2<kIsBf16>(quant::number(in[e >> 1], 2 * (e & 1)) * st, quant::number(in[e >> 1], 2 * (e & 1) + 1) * st);
+            for (int e = 0; e < 8; ++e) out[e] = quant::pair_of<kIsBf16>(in[e >> 1], (e & 1) != 0);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int chunk = lane % kVecs * 2 + h;
               ptx::st_shared_v4(to + (chunk >> 3) * S::kHalfBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), out[4 * h], out[4 * h + 1], out[4 * h + 2], out[4 * h + 3]);
             }
           }
-          if (!is_v) reinterpret_cast<float*>(smem + S::kStepsOff)[(idx0 / 2 + (i + 1) / 2) % S::kStepTiles * kKeys + my_row] = step_now;
+          if (!second(i)) {
+            // the steps of this tile go where those of the tile before the last were, once the query tiles that took part in that have read them
+            const int j = (i + 1) / 2, place = (idx0 / 2 + j) & 1;
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+              if (ok && uses[g][place] > 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->steps_free[g][place], (uses[g][place] - 1) & 1u, abort_flag, p.status, 175));
+            if (!ok) break;
+            uses[0][place] += j < w.n_a ? 1 : 0, uses[1][place] += w.lone ? 0 : 1;
+            float* steps = reinterpret_cast<float*>(smem + S::kStepsOff + place * S::kStepBytes);
+            const float top = softmax::warp_max(v_now);
+            steps[my_row] = k_now, steps[kKeys + my_row] = v_now;
+            if (lane == 0) steps[2 * kKeys + cw] = top;
+          }
           ptx::fence_proxy_async_smem();
           ptx::mbar_arrive(&bars->kv_full[slot]);
         }
@@ -500,6 +515,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       const bool idle = __all_sync(0xffffffffu, !row_ok);           // no row of this warp exists
       const int limit = w.len - w.count + min(token, w.count - 1);  // last visible position
       float m_used = -INFINITY, l = 0.f;
+      int v_used = 0;  // probabilities and their sum are 2^-v_used of what they were
       for (int j = 0; j < n_g; ++j) {
         const int c = before + j;
         bool ready = ptx::mbar_wait(&bars->s_full[g], c & 1u, abort_flag, p.status, 165 + g);
@@ -511,6 +527,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         if (idle) {  // its probabilities may be anything, but it hands them over in step with the others
           ptx::tcgen05_fence_before_thread_sync();
           ptx::mbar_arrive(&bars->s_free[g]);
+          if constexpr (kI8) ptx::mbar_arrive(&bars->steps_free[g][(steps_before + j) & 1]);
           if (j > 0 && !__all_sync(0xffffffffu, ptx::mbar_wait(&bars->pv_done[g], (c - 1) & 1u, abort_flag, p.status, 169 + g))) {
             alive = false;
             break;
@@ -527,14 +544,22 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         // the scores are in registers: S_g goes back to the tensor core for the next step's Q K^T
         ptx::tcgen05_fence_before_thread_sync();
         ptx::mbar_arrive(&bars->s_free[g]);
+        const int place = (steps_before + j) & 1;
+        const uint32_t steps = ptx::smem_u32(smem + S::kStepsOff) + place * S::kStepBytes;
+        int v_new = 0;  // the exponent of the largest step of V: f16 probabilities times steps would run out of theirs
         if constexpr (kI8) {
-          const uint32_t steps = ptx::smem_u32(smem + S::kStepsOff) + (steps_before + j) % S::kStepTiles * (kKeys * 4);
 #pragma unroll
           for (int i = 0; i < 128; i += 4) {
             float f[4];
             asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]) : "r"(steps + i * 4));
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[i >> 5][(i & 31) + e] = __float_as_uint(__uint_as_float(v[i >> 5][(i & 31) + e]) * f[e]);
+          }
+          if constexpr (!kIsBf16) {
+            float f[4];
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]) : "r"(steps + 2 * kKeys * 4));
+            const float top = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+            v_new = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -60), 60);
           }
         }
 
@@ -558,8 +583,10 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         const float m_new = fmaxf(m_used, mx);
         if (j == 0) {
           m_used = m_new;
+          v_used = v_new;
         } else {
-          const bool need = (m_new - m_used) * sl2 > attn::kRescaleThreshold;
+          const bool grown = kI8 && !kIsBf16 && v_new > v_used + 3;  // alike in all threads of the tile
+          const bool need = (m_new - m_used) * sl2 > attn::kRescaleThreshold || grown;
           if (__any_sync(0xffffffffu, need)) {
             // O_g is rescaled in place once the P V of the step before has retired
             ready = ptx::mbar_wait(&bars->pv_done[g], (c - 1) & 1u, abort_flag, p.status, 167 + g);
@@ -568,8 +595,10 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
               break;
             }
             ptx::tcgen05_fence_after_thread_sync();
-            const float alpha = need ? ptx::ex2_approx((m_used - m_new) * sl2) : 1.0f;
+            // a row of no scores so far has nothing to lose
+            const float alpha = need ? ptx::ex2_approx((m_new == -INFINITY ? 0.f : (m_used - m_new) * sl2) + static_cast<float>(grown ? v_used - v_new : 0)) : 1.0f;
             if (need) m_used = m_new;
+            if (grown) v_used = v_new;
             l *= alpha;
 #pragma unroll 1
             for (int q = 0; q < D / 32; ++q) {
@@ -587,7 +616,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
 
         // probabilities: exp2, rounded to 16 bits, in the K-major layout of the P V product; of every 8 pairs attn::kPolyPairs avoid MUFU.  A row
         // whose scores so far are all -inf takes them against 0.
-        const float ms = m_used == -INFINITY ? 0.f : m_used * sl2;
+        const float ms = (m_used == -INFINITY ? 0.f : m_used * sl2) + static_cast<float>(v_used);
         const ptx::f32x2_t sl2x2 = ptx::pack_f32x2(sl2, sl2);
         const ptx::f32x2_t nmsx2 = ptx::pack_f32x2(-ms, -ms);
         ptx::f32x2_t lsum[2] = {0ull, 0ull};
@@ -607,8 +636,13 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
               p0 = ptx::ex2_approx(t0);
               p1 = ptx::ex2_approx(t1);
             }
-            pk[i] = attn::pack16x2<kIsBf16>(p0, p1);
             lsum[i & 1] = ptx::add_f32x2(lsum[i & 1], ptx::pack_f32x2(p0, p1));
+            if constexpr (kI8) {
+              float f0, f1;
+              asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f0), "=f"(f1) : "r"(steps + (kKeys + q * 32 + e0) * 4));
+              p0 *= f0, p1 *= f1;
+            }
+            pk[i] = attn::pack16x2<kIsBf16>(p0, p1);
           }
           if (h2 == 0 && j > 0) {  // P_g is free once the P V of the step before has read it
             ready = ptx::mbar_wait(&bars->pv_done[g], (c - 1) & 1u, abort_flag, p.status, 169 + g);
@@ -622,6 +656,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           for (int q = 0; q < 8; ++q) ptx::st_shared_v4(prow + ((q ^ (r & 7)) << 4), pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
         }
         if (!alive) break;
+        if constexpr (kI8) ptx::mbar_arrive(&bars->steps_free[g][place]);
         float l4[4];
         ptx::unpack_f32x2(lsum[0], l4[0], l4[1]);
         ptx::unpack_f32x2(lsum[1], l4[2], l4[3]);
@@ -672,7 +707,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
               part[i * 256] = make_float4(__uint_as_float(ov[4 * i]), __uint_as_float(ov[4 * i + 1]), __uint_as_float(ov[4 * i + 2]), __uint_as_float(ov[4 * i + 3]));
           }
         }
-        if (!whole) p.part_ml[rec * 256 + g * kTileRows + r] = make_float2(n_g > 0 ? m_used : -INFINITY, n_g > 0 ? l : 0.f);
+        if (!whole) p.part_ml[rec * 256 + g * kTileRows + r] = make_float2(n_g > 0 ? m_used + static_cast<float>(v_used) / sl2 : -INFINITY, n_g > 0 ? l : 0.f);
       }
       if (n_g > 0) {
         ptx::tcgen05_fence_before_thread_sync();

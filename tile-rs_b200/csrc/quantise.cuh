@@ -42,5 +42,23 @@ __device__ __forceinline__ float number(uint32_t x, int i) {
   return __uint_as_float(__byte_perm(x ^ 0x80808080u, 0x4b000000u, 0x7540 + i)) - 8388736.f;
 }
 
+// Two of the four whole numbers of x, bytes 0 and 1 (or 2 and 3: `upper`), as 16-bit numbers, exactly.  f16: a byte behind 0x64 is 1024 + byte.  bf16: 128 and the lower
+// seven bits, less 128, or 256 where the sign is set.
+template <bool kIsBf16>
+__device__ __forceinline__ uint32_t pair_of(uint32_t x, bool upper) {
+  uint32_t r;
+  if (kIsBf16) {
+    const uint32_t h = __byte_perm(x, 0u, upper ? 0x4342 : 0x4140);
+    uint32_t a, b;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(a) : "r"(h), "r"(0x007f007fu), "r"(0x43004300u));
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(b) : "r"(h), "r"(0x00800080u), "r"(0x43004300u));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  } else {
+    const uint32_t h = __byte_perm(x ^ 0x80808080u, 0x64646464u, upper ? 0x4342 : 0x4140);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));
+  }
+  return r;
+}
+
 }  // namespace quant
 }  // namespace tsm100
