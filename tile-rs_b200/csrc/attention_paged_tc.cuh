@@ -11,8 +11,8 @@
 //   * K and V come by pages: boxes of a power of two of positions (8 and more), a lane each.  What a page holds behind the sequence's end is
 //     replaced by zeros in V (it has no weight, but may be NaN) and masked in S.
 //   * 8 bits (kI8): four warps write the tiles that TMA would have written, whole numbers, which 16 bits hold exactly.  K's steps multiply the scores and V's the
-//     probabilities, so that nothing but the probabilities is rounded (with K and V times their steps rounded, errors were 1.6 times as large).  f16 probabilities times steps
-//     keep their bits by a power of two that follows the largest step and is taken out again with the sum.
+//     probabilities, so that nothing but the probabilities is rounded (with K and V times their steps rounded, errors were 1.6 times as large), and those to f16, whatever q's type
+//     is.  They keep their bits by a power of two that follows the largest step and is taken out again with the sum.
 // Bound: the tensor core and the exponentials, as there.
 #pragma once
 
@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(Shape<kI8, D>::kThreads, 1)
 attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                           uint16_t* __restrict__ o, const __grid_constant__ Params p) {
   using S = Shape<kI8, D>;
+  constexpr bool kPvBf16 = kIsBf16 && !kI8;  // of P and V
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((ptx::smem_u32(smem) & 1023u) != 0u) {
     ptx::wait_prior_grid();
@@ -300,7 +301,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
     // ------------------------------ MMA issuers --------------------------------
     ptx::setmaxnreg_dec<S::kRegsOther>();
     constexpr uint32_t idesc_qk = ptx::make_idesc_f16(kTileRows, kKeys, false, false, kIsBf16);
-    constexpr uint32_t idesc_pv = ptx::make_idesc_f16(kTileRows, D, false, true, kIsBf16);
+    constexpr uint32_t idesc_pv = ptx::make_idesc_f16(kTileRows, D, false, true, kPvBf16);
     constexpr uint64_t kmajor = ptx::make_smem_desc_base(16, 1024);
     constexpr uint64_t v_mnmajor = ptx::make_smem_desc_base(S::kHalfBytes, 1024);
     // everything per MMA is one add on the low word of a descriptor
@@ -462,20 +463,22 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           const int slot = (idx0 + i) % S::kRing;
           if (!(ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->kv_empty[slot], (((idx0 + i) / S::kRing) & 1u) ^ 1u, abort_flag, p.status, 164)))) break;
           const uint32_t to = ptx::smem_u32(smem_kv + slot * S::kTileBytes);
+          const bool is_v = second(i);
 #pragma unroll
           for (int v = 0; v < kVecs; ++v) {
             const int row = v * kRowsAt + cw * kOwn + lane / kVecs;
             const uint32_t in[4] = {x[v].x, x[v].y, x[v].z, x[v].w};
             uint32_t out[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) out[e] = quant::pair_of<kIsBf16>(in[e >> 1], (e & 1) != 0);
+            for (int e = 0; e < 8; ++e)
+              out[e] = kIsBf16 && !is_v ? quant::pair_of<true>(in[e >> 1], (e & 1) != 0) : quant::pair_of<false>(in[e >> 1], (e & 1) != 0);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int chunk = lane % kVecs * 2 + h;
               ptx::st_shared_v4(to + (chunk >> 3) * S::kHalfBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), out[4 * h], out[4 * h + 1], out[4 * h + 2], out[4 * h + 3]);
             }
           }
-          if (!second(i)) {
+          if (!is_v) {
             // the steps of this tile go where those of the tile before the last were, once the query tiles that took part in that have read them
             const int j = (i + 1) / 2, place = (idx0 / 2 + j) & 1;
 #pragma unroll
@@ -546,7 +549,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         ptx::mbar_arrive(&bars->s_free[g]);
         const int place = (steps_before + j) & 1;
         const uint32_t steps = ptx::smem_u32(smem + S::kStepsOff) + place * S::kStepBytes;
-        int v_new = 0;  // the exponent of the largest step of V: f16 probabilities times steps would run out of theirs
+        int v_new = 0;  // the exponent of the largest step of V
         if constexpr (kI8) {
 #pragma unroll
           for (int i = 0; i < 128; i += 4) {
@@ -555,12 +558,10 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[i >> 5][(i & 31) + e] = __float_as_uint(__uint_as_float(v[i >> 5][(i & 31) + e]) * f[e]);
           }
-          if constexpr (!kIsBf16) {
-            float f[4];
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]) : "r"(steps + 2 * kKeys * 4));
-            const float top = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
-            v_new = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -60), 60);
-          }
+          float f[4];
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]) : "r"(steps + 2 * kKeys * 4));
+          const float top = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+          v_new = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
         }
 
         float mx = -INFINITY;
@@ -585,7 +586,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           m_used = m_new;
           v_used = v_new;
         } else {
-          const bool grown = kI8 && !kIsBf16 && v_new > v_used + 3;  // alike in all threads of the tile
+          const bool grown = kI8 && v_new > v_used + 3;  // alike in all threads of the tile
           const bool need = (m_new - m_used) * sl2 > attn::kRescaleThreshold || grown;
           if (__any_sync(0xffffffffu, need)) {
             // O_g is rescaled in place once the P V of the step before has retired
@@ -642,7 +643,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
               asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f0), "=f"(f1) : "r"(steps + (kKeys + q * 32 + e0) * 4));
               p0 *= f0, p1 *= f1;
             }
-            pk[i] = attn::pack16x2<kIsBf16>(p0, p1);
+            pk[i] = attn::pack16x2<kPvBf16>(p0, p1);
           }
           if (h2 == 0 && j > 0) {  // P_g is free once the P V of the step before has read it
             ready = ptx::mbar_wait(&bars->pv_done[g], (c - 1) & 1u, abort_flag, p.status, 169 + g);
