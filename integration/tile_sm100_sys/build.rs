@@ -16,7 +16,7 @@ fn main() {
         "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC,-fopenmp",
     ];
     let mut objects = Vec::new();
-    for src in ["runtime.cu", "capi_ops.cu", "multi.cu", "inputs.cpp", "emit.cpp"] {
+    for src in ["runtime.cu", "capi_ops.cu", "serving_w4_bf16.cu", "serving_w4_f16.cu", "serving.cu", "multi.cu", "inputs.cpp", "emit.cpp"] {
         let obj = out.join(format!("{src}.o"));
         let mut cmd = Command::new(&nvcc);
         cmd.args(common).arg(format!("-I{}", include.display()));

@@ -17,6 +17,7 @@ pub const ERR_EMIT: i32 = 9;
 pub const F32: i32 = 0;
 pub const F16: i32 = 1;
 pub const BF16: i32 = 2;
+pub const I8: i32 = 3; // only where an operator says so
 pub const OP_SOFTMAX: i32 = 0;
 pub const OP_GEMM: i32 = 1;
 pub const OP_ATTENTION: i32 = 2;
@@ -44,6 +45,19 @@ pub struct KvCacheUpdateDesc { pub dtype: i32, pub batch: i32, pub seq_len: i32,
 pub struct AttentionPrefillDesc { pub dtype: i32, pub heads_q: i32, pub heads_kv: i32, pub seq_len: i32, pub start_pos: i32, pub max_seq: i32, pub head_dim: i32 }
 #[repr(C)] #[derive(Clone, Copy, Default)]
 pub struct AttentionDecodeDesc { pub dtype: i32, pub batch: i32, pub heads_q: i32, pub heads_kv: i32, pub seq_len: i32, pub max_seq: i32, pub head_dim: i32 }
+#[repr(C)] #[derive(Clone, Copy, Default)]
+pub struct AddRmsNormDesc { pub dtype: i32, pub out_dtype: i32, pub rows: i64, pub cols: i64, pub eps: f32 }
+#[repr(C)] #[derive(Clone, Copy, Default)]
+pub struct GemmW4Desc { pub dtype: i32, pub a_dtype: i32, pub group: i32, pub m: i64, pub n: i64, pub k: i64 }
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct PagedKv { pub dtype: i32, pub heads_kv: i32, pub head_dim: i32, pub page_size: i32, pub pages: i64, pub k: *mut c_void, pub v: *mut c_void,
+                     pub k_scales: *mut f32, pub v_scales: *mut f32 }
+/// table, lens, starts: device memory, read when the call's kernels run.
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct PagedBatch { pub batch: i32, pub tokens: i32, pub max_new: i32, pub max_len: i32, pub table_pitch: i32, pub table: *const i32,
+                        pub lens: *const i32, pub starts: *const i32 }
+#[repr(C)] #[derive(Clone, Copy, Default)]
+pub struct AttentionPagedDesc { pub dtype: i32, pub heads_q: i32 }
 #[repr(C)] #[derive(Clone, Copy)]
 pub struct MultiJob { pub op: i32, pub desc: *const c_void, pub inputs: [*const c_void; 3], pub out: *mut c_void, pub launches: i32, pub timeout_ms: i32 }
 #[repr(C)] #[derive(Clone, Copy)]
@@ -104,6 +118,17 @@ extern "C" {
                                     v_cache: *const c_void, o: *mut c_void, stream: RawStream) -> i32;
     pub fn tsm100_attention_decode(dev: Device, d: *const AttentionDecodeDesc, q: *const c_void, k_cache: *const c_void,
                                    v_cache: *const c_void, o: *mut c_void, stream: RawStream) -> i32;
+    // serving: residual norm, 4-bit weights, paged KV cache
+    pub fn tsm100_add_rms_norm(dev: Device, d: *const AddRmsNormDesc, x: *const c_void, residual: *const c_void, sum: *mut c_void,
+                               weight: *const c_void, y: *mut c_void, scales: *mut f32, stream: RawStream) -> i32;
+    pub fn tsm100_gemm_w4(dev: Device, d: *const GemmW4Desc, a: *const c_void, a_scales: *const f32, w: *const u8, w_scales: *const c_void,
+                          w_zeros: *const u8, c: *mut c_void, stream: RawStream) -> i32;
+    pub fn tsm100_kv_page_append(dev: Device, kv: *const PagedKv, batch: *const PagedBatch, dtype: i32, k: *const c_void, v: *const c_void,
+                                 stream: RawStream) -> i32;
+    pub fn tsm100_kv_page_read(dev: Device, kv: *const PagedKv, batch: *const PagedBatch, dtype: i32, k: *mut c_void, v: *mut c_void,
+                               stream: RawStream) -> i32;
+    pub fn tsm100_attention_paged(dev: Device, kv: *const PagedKv, batch: *const PagedBatch, d: *const AttentionPagedDesc, q: *const c_void,
+                                  o: *mut c_void, stream: RawStream) -> i32;
     // operators on host memory
     pub fn tsm100_softmax_host(dev: Device, d: *const SoftmaxDesc, x: *const c_void, y: *mut c_void) -> i32;
     pub fn tsm100_gemm_host(dev: Device, d: *const GemmDesc, a: *const c_void, b: *const c_void, c: *mut c_void) -> i32;
