@@ -32,7 +32,7 @@ constexpr int kBlockCost = 3 * kKeys;      // beginning and ending a block, as a
 constexpr int kMinShare = 4 * 3 * kKeys;   // a share's length at least: four steps of two tiles
 template <bool kI8, int D>
 struct Shape {
-  static constexpr int kThreads = kI8 ? 512 : 384;   // warps 0..3 softmax A, 4..7 softmax B, 8 TMA, 9 Q K^T, 10 P V, 11 idle, 12..15 conversion
+  static constexpr int kThreads = kI8 ? 512 : 384;   // warps 0..3 softmax A, 4..7 softmax B, 8 TMA, 9 Q K^T, 10 P V, 11 planning, 12..15 conversion
   // registers after setmaxnreg; the shares of a block add up to what it was launched with
   static constexpr int kRegsSoftmax = kI8 ? 184 : 216, kRegsOther = kI8 ? 48 : 72, kRegsConvert = 96;
   static constexpr int kLoneWeight = kI8 ? 3 : 2;     // a step of a block of one tile, against 3 of two: conversion takes as long for either
@@ -46,12 +46,24 @@ struct Shape {
 };
 static_assert(256 * 184 + 128 * 48 + 128 * 96 <= 512 * 128 && 256 * 216 + 128 * 72 <= 384 * 168, "registers of a block at launch");
 
+// A block, or a share's part of it.  One warp finds them, a few ahead, and the others read them here.
+struct Work {
+  int b, first, count, len;
+  int head, block, token0;   // first token, in the sequence's new ones
+  int steps, begin, n;       // of the block, and the part that is this share's
+  int n_a;                   // of that, what tile A takes part in (causality)
+  int lone, there;           // one tile; false behind the last part
+};
+constexpr int kPlans = 4;
+
 struct alignas(8) Barriers {
   uint64_t q_full, q_free;
   uint64_t kv_full[6], kv_empty[6];
   uint64_t tail;              // the copies of a V tile that ends behind its sequence
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], o_free[2];
   uint64_t steps_free[2][2];  // [query tile][place]
+  uint64_t plan_full[kPlans], plan_empty[kPlans];
+  Work plan[kPlans];
   int64_t scan[17];
   int64_t first_base;
   int32_t first_seq;
@@ -82,13 +94,6 @@ struct Params {
 struct Seq {
   int b, first, count, len, blocks;
   int64_t per_head, base, end;
-};
-struct Work {
-  int b, first, count, len;
-  int head, block, token0;   // first token, in the sequence's new ones
-  int steps, begin, n;       // of the block, and the part that is this share's
-  int n_a;                   // of that, what tile A takes part in (causality)
-  bool lone;
 };
 __device__ __forceinline__ int64_t full_blocks(const Params& p, const Seq& s, int64_t i) {  // the length of the first i blocks, which have two tiles
   const int64_t two = 2 * p.tokens;
@@ -179,6 +184,10 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       ptx::mbar_init(&bars->o_free[g], 128);
       for (int i = 0; i < 2; ++i) ptx::mbar_init(&bars->steps_free[g][i], 128);
     }
+    for (int i = 0; i < kPlans; ++i) {
+      ptx::mbar_init(&bars->plan_full[i], 1);
+      ptx::mbar_init(&bars->plan_empty[i], kI8 ? 15 : 11);  // the other warps
+    }
     bars->abort_flag = 0;
     bars->pv_steps = 0;
     bars->first_seq = p.step.batch;
@@ -232,11 +241,20 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       sum += here;
     }
     __syncthreads();
-    stream.open(p, bars->first_seq, bars->first_base);
   }
   const uint32_t tmem_s = tmem_base;        // S_A at +0, S_B at +128
   const uint32_t tmem_o = tmem_base + 256;  // O_A at +256, O_B at +384
-  Work w;
+  // The next part, for a whole warp; given back when the warp is through with it.
+  int part_no = -1;
+  auto take = [&]() -> bool {
+    ++part_no;
+    const bool ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->plan_full[part_no % kPlans], (part_no / kPlans) & 1u, abort_flag, p.status, 176));
+    return ok && bars->plan[part_no % kPlans].there;
+  };
+  auto give = [&]() {
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(&bars->plan_empty[part_no % kPlans]);
+  };
 
   if (warp == 8) {
     // ------------------------------ TMA producer ------------------------------
@@ -248,7 +266,8 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
     const int run = 1 << p.run_log2, ps = p.cache.page_size;
     int idx0 = 0, tails = 0;
     bool ok = true;
-    for (int seg = 0; ok && stream.next(p, w); ++seg) {
+    for (int seg = 0; ok && take(); ++seg) {
+      const Work w = bars->plan[part_no % kPlans];
       if (seg > 0 && !(ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->q_free, (seg - 1) & 1u, abort_flag, p.status, 151)))) break;
       if (lane == 0) {
         ptx::mbar_arrive_expect_tx(&bars->q_full, (w.lone ? 1 : 2) * (p.tokens * p.group * 128 * S::kHalves));
@@ -296,6 +315,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         }
         idx0 += total;
       }
+      give();
     }
   } else if (warp == 9 || warp == 10) {
     // ------------------------------ MMA issuers --------------------------------
@@ -319,7 +339,8 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
     int done[2] = {0, 0};       // steps of each tile in earlier segments
     int segs[2] = {0, 0};       // segments that each tile took part in
     bool ok = true;
-    for (int seg = 0; ok && stream.next(p, w); ++seg) {
+    for (int seg = 0; ok && take(); ++seg) {
+      const Work w = bars->plan[part_no % kPlans];
       auto k_pos = [&](int j) { return idx0 + (j == 0 ? 0 : 2 * j - 1); };
       auto v_pos = [&](int j) { return idx0 + (j == w.n - 1 ? 2 * w.n - 1 : 2 * j + 2); };
       const int n_of[2] = {w.n_a, w.lone ? 0 : w.n};
@@ -395,9 +416,26 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       steps_before += w.n;
 #pragma unroll
       for (int g = 0; g < 2; ++g) done[g] += n_of[g], segs[g] += n_of[g] > 0 ? 1 : 0;
+      give();
     }
   } else if (warp == 11) {
+    // ------------------------------ planning -----------------------------------
     ptx::setmaxnreg_dec<S::kRegsOther>();
+    if (lane == 0) {
+      int head_state = 0, tail_b = -1, tail_head = 0, tail_block = 0;
+      stream.open(p, bars->first_seq, bars->first_base);
+      for (int i = 0;; ++i) {
+        Work w = {};
+        w.there = stream.next(p, w) ? 1 : 0;
+        if (!ptx::mbar_wait(&bars->plan_empty[i % kPlans], ((i / kPlans) & 1u) ^ 1u, abort_flag, p.status, 177)) break;
+        bars->plan[i % kPlans] = w;
+        ptx::mbar_arrive(&bars->plan_full[i % kPlans]);
+        if (!w.there) break;
+        if (w.begin > 0) head_state = w.begin + w.n == w.steps ? 1 : 2;
+        else if (w.n < w.steps) tail_b = w.b, tail_head = w.head, tail_block = w.block;
+      }
+      p.info[blockIdx.x] = make_int4(head_state, tail_b, tail_head, tail_block);
+    }
   } else if (kI8 && warp >= 12) {
     // ------------------------------ conversion ---------------------------------
     if constexpr (kI8) {
@@ -410,7 +448,8 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       const int my_row = lane / kOwn * kRowsAt + cw * kOwn + lane % kOwn;
       int idx0 = 0, uses[2][2] = {{0, 0}, {0, 0}};  // how often a query tile has read a place's steps
       bool ok = true;
-      while (ok && stream.next(p, w)) {
+      while (ok && take()) {
+        const Work w = bars->plan[part_no % kPlans];
         // A tile's page is asked for three tiles ahead, its steps two and its rows one, so that none of these loads is waited for.
         const int total = 2 * w.n;
         auto second = [&](int i) { return i == total - 1 || (i >= 2 && (i & 1) == 0); };  // V
@@ -495,6 +534,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           ptx::mbar_arrive(&bars->kv_full[slot]);
         }
         idx0 += total;
+        give();
       }
     }
   } else {
@@ -509,9 +549,9 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
     const uint32_t p_row = ptx::smem_u32(smem_p) + g * S::kPBytes + r * 128;
     const int r_token = r / p.group, r_head = r - r_token * p.group;
     int before = 0, steps_before = 0;       // this tile's steps in earlier segments, and the block's
-    int head_state = 0, tail_b = -1, tail_head = 0, tail_block = 0;
     bool alive = true;
-    while (alive && stream.next(p, w)) {
+    while (alive && take()) {
+      const Work& w = bars->plan[part_no % kPlans];
       const int n_g = g == 0 ? w.n_a : w.lone ? 0 : w.n;
       const int token = w.token0 + g * p.tokens + r_token;
       const bool row_ok = r_token < p.tokens && token < w.count;
@@ -716,10 +756,8 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       }
       before += n_g;
       steps_before += w.n;
-      if (w.begin > 0) head_state = w.begin + w.n == w.steps ? 1 : 2;
-      else if (w.n < w.steps) tail_b = w.b, tail_head = w.head, tail_block = w.block;
+      give();
     }
-    if (tid == 0) p.info[blockIdx.x] = make_int4(head_state, tail_b, tail_head, tail_block);
   }
 
   // ------------------------------ teardown ------------------------------------
