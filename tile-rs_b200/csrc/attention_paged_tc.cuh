@@ -4,10 +4,10 @@
 // tensor memory, a thread per row, probabilities handed over through shared memory, one warp issuing Q K^T a step ahead and one P V.  What differs:
 //   * The rows of a tile are tokens times the heads of a group (row = token * group + head), so that a group's heads read K and V once and a chunk of a few tokens
 //     still fills a tile.  One TMA box brings them: 64 columns x group x tokens.
-//   * The work is one stream, dealt out evenly: blocks of up to two tiles are numbered through (sequence, KV head, block) with the keys they see as their length
-//     (times 3, or 2 where a block has one tile: 3240 and 2060 clocks a step in attention_tc.cuh), and every SM takes an equal, contiguous share of it, to the step.  Lengths are only
-//     known on the device, prompts and single tokens come in one call, and 64 blocks over 148 SMs would leave half of them idle.  A block that is cut leaves (maximum, sum, O)
-//     for a merging kernel.
+//   * The work is one stream, dealt out evenly: blocks of up to two tiles are numbered through (sequence, KV head, block) with the keys they see, and what beginning one
+//     costs, as their length, and every SM takes an equal, contiguous share of it, to the step.  Lengths are only known on the device, prompts and single tokens come in
+//     one call, and 64 blocks over 148 SMs would leave half of them idle.  A block that is cut leaves (maximum, sum, O) for a merging kernel.  (A block of one tile counts
+//     like one of two: two thirds of that cost 1 to 9 % in five mixes out of six, though its steps alone are shorter.  256 keys for beginning a block: 128 cost 1 to 13 %, 512 up to 7.)
 //   * K and V come by pages: boxes of a power of two of positions (8 and more), a lane each.  What a page holds behind the sequence's end is
 //     replaced by zeros in V (it has no weight, but may be NaN) and masked in S.
 //   * 8 bits (kI8): four warps write the tiles that TMA would have written, whole numbers, which 16 bits hold exactly.  K's steps multiply the scores and V's the
@@ -28,14 +28,13 @@ namespace tc {
 
 constexpr int kTileRows = 128, kKeys = 128;
 constexpr int kMaxGroup = 128;
-constexpr int kBlockCost = 3 * kKeys;      // beginning and ending a block, as a length: about a step of two tiles
-constexpr int kMinShare = 4 * 3 * kKeys;   // a share's length at least: four steps of two tiles
+constexpr int kBlockCost = 2 * kKeys;  // beginning and ending a block, as a length
+constexpr int kMinShare = 4 * kKeys;   // a share's length at least
 template <bool kI8, int D>
 struct Shape {
   static constexpr int kThreads = kI8 ? 512 : 384;   // warps 0..3 softmax A, 4..7 softmax B, 8 TMA, 9 Q K^T, 10 P V, 11 planning, 12..15 conversion
   // registers after setmaxnreg; the shares of a block add up to what it was launched with
   static constexpr int kRegsSoftmax = kI8 ? 184 : 216, kRegsOther = kI8 ? 48 : 72, kRegsConvert = 96;
-  static constexpr int kLoneWeight = kI8 ? 3 : 2;     // a step of a block of one tile, against 3 of two: conversion takes as long for either
   static constexpr int kHalves = D / 64;
   static constexpr int kHalfBytes = 128 * 128;        // 128 rows x 64 columns
   static constexpr int kTileBytes = kHalves * kHalfBytes;
@@ -81,7 +80,6 @@ struct Params {
   pages::Batch step;
   int32_t heads_q, group;
   int32_t tokens;      // of a tile: 128 / group
-  int32_t lone_weight; // Shape::kLoneWeight
   int32_t run_log2;    // positions of a page's box
   float scale_log2;
   float4* part;        // [CTA][2][D / 4][256 rows]: of a block that began in an earlier share, of one that goes on in the next
@@ -90,20 +88,19 @@ struct Params {
   uint32_t* status;
 };
 
-// The stream of blocks.  A block's length is the keys that its last token sees, times its weight, and kBlockCost.
+// The stream of blocks.  A block's length is the keys that its last token sees, and kBlockCost.
 struct Seq {
   int b, first, count, len, blocks;
   int64_t per_head, base, end;
 };
 __device__ __forceinline__ int64_t full_blocks(const Params& p, const Seq& s, int64_t i) {  // the length of the first i blocks, which have two tiles
   const int64_t two = 2 * p.tokens;
-  return 3 * (i * (s.len - s.count) + two * (i * (i + 1) / 2)) + i * kBlockCost;
+  return i * (s.len - s.count + kBlockCost) + two * (i * (i + 1) / 2);
 }
-__device__ __forceinline__ int last_weight(const Params& p, const Seq& s) { return s.count - (s.blocks - 1) * 2 * p.tokens <= p.tokens ? p.lone_weight : 3; }
 __device__ __forceinline__ int64_t sequence_length(const Params& p, int b, Seq& s, uint32_t* status) {
   if (!pages::sequence(p.step, p.cache.page_size, b, s.first, s.count, s.len, status, 145)) return 0;
   s.blocks = (s.count + 2 * p.tokens - 1) / (2 * p.tokens);
-  s.per_head = full_blocks(p, s, s.blocks - 1) + static_cast<int64_t>(s.len) * last_weight(p, s) + kBlockCost;
+  s.per_head = full_blocks(p, s, s.blocks - 1) + s.len + kBlockCost;
   return s.per_head * p.cache.heads;
 }
 struct Stream {
@@ -130,13 +127,11 @@ struct Stream {
       }
       const bool last = lo == seq.blocks - 1;
       const int64_t from = full_blocks(p, seq, lo), to = last ? seq.per_head : full_blocks(p, seq, lo + 1);
-      const int weight = last ? last_weight(p, seq) : 3;
       w.token0 = lo * 2 * p.tokens;
       const int keys = seq.len - seq.count + min(seq.count, w.token0 + 2 * p.tokens);
       w.steps = (keys + kKeys - 1) / kKeys;
-      const int step = weight * kKeys;  // a block's length fits 32 bits
       const int64_t stop = min(to, in_head + (end - at));
-      auto steps_to = [&](int64_t x) { return static_cast<int>((static_cast<uint32_t>(max(x - from - kBlockCost, static_cast<int64_t>(0))) + step - 1) / step); };
+      auto steps_to = [&](int64_t x) { return static_cast<int>((static_cast<uint32_t>(max(x - from - kBlockCost, static_cast<int64_t>(0))) + kKeys - 1) / kKeys); };
       w.begin = steps_to(in_head);
       w.n = steps_to(stop) - w.begin;
       w.b = seq.b, w.first = seq.first, w.count = seq.count, w.len = seq.len, w.block = lo;

@@ -186,7 +186,6 @@ inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& 
   p.cache = base.cache, p.step = base.step;
   p.heads_q = base.heads_q, p.group = base.group;
   p.tokens = tc::kTileRows / base.group;
-  p.lone_weight = S::kLoneWeight;
   p.run_log2 = run_log2;
   p.scale_log2 = base.scale_log2;
   p.status = base.status;
