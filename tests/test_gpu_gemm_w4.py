@@ -93,6 +93,36 @@ def test_what_is_not_finite_stays_in_its_row(dev, pkg, m):
     assert torch.isnan(c[1]).all() and torch.isfinite(c[0]).all() and torch.isfinite(c[2:]).all()
 
 
+@pytest.mark.parametrize("m,n,k,group", [(513, 264, 8192, 32), (520, 2049, 1024, 64), (641, 4001, 544, 32), (300, 8200, 512, 128), (385, 4801, 640, 64), (1030, 1028, 2048, 128)])
+@pytest.mark.parametrize("dtype,a_dtype,zeros", [("bf16", "bf16", True), ("f16", "i8", True), ("bf16", "i8", False), ("f16", "f16", False)])
+def test_rows_enough_to_make_the_weights_first(dev, pkg, dtype, a_dtype, zeros, m, n, k, group):
+    a, a_scales, w, scales, z = problem(m + n, dtype, a_dtype, m, n, k, group, zeros)
+    raw = torch.full((m * n + 16,), 77.0, dtype=u.TORCH[dtype], device=u.GPU)
+    ref, mag = reference(a, a_scales, w, scales, z, group)
+    for start in (0, 1):  # C on a vector's boundary and off it
+        c = raw[start:start + m * n].view(m, n)
+        call(pkg, dev, dtype, a_dtype, group, a, a_scales, w, scales, z, c)
+        check(c, ref, mag, dtype, m)
+        assert (raw[m * n + start:] == 77).all()
+    assert dev.status() == 0
+
+
+def test_rows_enough_to_make_the_weights_first_exact_and_not_finite(dev, pkg):
+    g = u.gen(5)
+    a = torch.randint(-3, 4, (530, 1024), generator=g, device=u.GPU).bfloat16()
+    w = torch.randint(0, 256, (2100, 512), generator=g, device=u.GPU, dtype=torch.uint8)
+    scales = torch.full((2100, 8), 0.5, dtype=torch.bfloat16, device=u.GPU)
+    c = torch.empty((530, 2100), dtype=torch.bfloat16, device=u.GPU)
+    call(pkg, dev, "bf16", "bf16", 128, a, None, w, scales, None, c)
+    ref = reference(a, None, w, scales, None, 128)[0].bfloat16()
+    assert torch.equal(c, ref)
+    a[129, 7] = float("nan")
+    call(pkg, dev, "bf16", "bf16", 128, a, None, w, scales, None, c)
+    assert torch.isnan(c[129]).all()
+    c[129] = ref[129]
+    assert torch.equal(c, ref)
+
+
 def test_no_terms(dev, pkg):
     capi = pkg.capi
     c = torch.full((3, 5), 9.0, dtype=torch.bfloat16, device=u.GPU)

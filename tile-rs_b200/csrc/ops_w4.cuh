@@ -5,6 +5,7 @@
 
 #include "gemm_w4.cuh"
 #include "launch.cuh"
+#include "w4_dense.cuh"
 
 namespace tsm100 {
 namespace ops {
@@ -57,8 +58,62 @@ int32_t gemm_w4_typed(std::string* err, const tsm100_gemm_w4_desc* d, const uint
 extern template int32_t gemm_w4_typed<__nv_bfloat16>(std::string*, const tsm100_gemm_w4_desc*, const uint8_t*, const w4::Params&, cudaStream_t);
 extern template int32_t gemm_w4_typed<__half>(std::string*, const tsm100_gemm_w4_desc*, const uint8_t*, const w4::Params&, cudaStream_t);
 
+// Whether the weights are made 16-bit ones first.  The kernel of gemm_w4.cuh makes each of them for every 128 rows, in waves of a tile of 128 x 128
+// per SM; made once they are written and read again, by three launches or more.  bf16, rows in 16 bits | 8 bits, us with the weights made in the
+// kernel, made first:
+//   256 rows, N = 16384, K = 4096: 62, 65 | 73, 75      300 rows: 91, 84 | 107, 92      400: 122, 86 | 142, 95      1000: 225, 135 | 263, 181
+//   N = K = 4096, 400 rows, one wave: 31, 33 | 37, 38   513 rows: 58, 35 | 68, 40       1000: 61, 34 | 72, 43       4000: 237, 107 | 251, 153
+//   N = 16384, K = 512, 300 rows: 25, 21 | 29, 28       K = 128, 640 rows, where the f32 result of 8-bit rows is most of it: 29, 22 | 34, 41
+//   N = 1024, 640 rows, K = 4096: 24, 19 | 28, 22       K = 1024: 14.1, 14.5 | 16.3, 17.0
+inline bool gemm_w4_dense_pays(int64_t m, int64_t n, int64_t k, int sms) {
+  const int64_t blocks = (m + 127) / 128;
+  return k >= 512 && n * k >= (1 << 21) && (blocks > 4 || (blocks > 2 && blocks * ((n + w4::kRows - 1) / w4::kRows) > sms));
+}
+
+// `gemm` is the library's own 16-bit product, (desc, a, b, c) on this stream.  kNoScratch: no memory for the weights.
+template <typename T, typename Gemm>
+inline int32_t gemm_w4_dense(std::string* err, const tsm100_gemm_w4_desc* d, const uint8_t* w, const w4::Params& p, cudaStream_t s, Gemm gemm) {
+  const int64_t n8 = (d->n + 7) / 8 * 8;  // rows of C, and of W's last tiles, as the tensor cores' product takes them
+  const bool eight = p.a_scales != nullptr, apart = eight || n8 != d->n || !aligned16(p.c);
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t w_bytes = up(static_cast<size_t>(n8) * d->k * 2), a_bytes = eight ? up(static_cast<size_t>(d->m) * d->k * 2) : 0,
+               f_bytes = apart ? static_cast<size_t>(d->m) * n8 * (eight ? 4 : 2) : 0;
+  uint8_t* ws = nullptr;
+  int32_t st = take_scratch(err, reinterpret_cast<void**>(&ws), w_bytes + a_bytes + f_bytes, s);
+  if (st != TSM100_OK) return st;
+  uint8_t *wide = ws + w_bytes, *f = wide + a_bytes;
+  const int group_log2 = d->group == 32 ? 5 : d->group == 64 ? 6 : 7;
+  cudaError_t e = launch_chained(w4::w4_expand_kernel<T>, static_cast<unsigned>(n8), w4::kDenseThreads, 0, s, 0, w, static_cast<const uint16_t*>(p.scales),
+                                 p.zeros, reinterpret_cast<uint16_t*>(ws), p.n, p.k, static_cast<int32_t>(group_log2));
+  st = cuda_ok(err, e, "w4_expand_kernel launch");
+  if (st == TSM100_OK && eight) {
+    const int64_t vecs = d->m * d->k / 8;
+    e = launch_chained(w4::w4_widen_kernel<T>, static_cast<unsigned>((vecs + w4::kDenseThreads - 1) / w4::kDenseThreads), w4::kDenseThreads, 0, s, 0,
+                       static_cast<const uint2*>(p.a), reinterpret_cast<uint4*>(wide), vecs);
+    st = cuda_ok(err, e, "w4_widen_kernel launch");
+  }
+  if (st == TSM100_OK) {
+    tsm100_gemm_desc g = {};
+    g.dtype = d->dtype, g.out_dtype = eight ? TSM100_F32 : d->dtype;
+    g.b_transposed = 1, g.batch = 1;
+    g.m = d->m, g.n = n8, g.k = d->k;
+    st = gemm(&g, eight ? static_cast<const void*>(wide) : p.a, static_cast<const void*>(ws), apart ? static_cast<void*>(f) : p.c);
+  }
+  if (st == TSM100_OK && apart) {
+    const dim3 grid(static_cast<unsigned>(d->m), static_cast<unsigned>(std::min<int64_t>((d->n + 2047) / 2048, 64)));
+    const int32_t pitch = static_cast<int32_t>(n8);
+    e = eight ? launch_chained(w4::w4_rows_kernel<T, float>, grid, w4::kDenseThreads, 0, s, 0, reinterpret_cast<const float*>(f), p.a_scales, static_cast<T*>(p.c), p.n, pitch)
+              : launch_chained(w4::w4_rows_kernel<T, T>, grid, w4::kDenseThreads, 0, s, 0, reinterpret_cast<const T*>(f), p.a_scales, static_cast<T*>(p.c), p.n, pitch);
+    st = cuda_ok(err, e, "w4_rows_kernel launch");
+  }
+  e = cudaFreeAsync(ws, s);
+  if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
+  return st;
+}
+
+template <typename Gemm>
 inline int32_t gemm_w4(std::string* err, const tsm100_gemm_w4_desc* d, const void* a, const float* a_scales, const uint8_t* w, const void* w_scales,
-                       const uint8_t* w_zeros, void* c, uint32_t* status, void* stream) {
+                       const uint8_t* w_zeros, void* c, uint32_t* status, void* stream, Gemm gemm) {
   if (!d) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: null descriptor");
   if (!dtype_16bit(d->dtype)) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: dtype must be TSM100_F16 or TSM100_BF16");
   if (d->a_dtype != d->dtype && d->a_dtype != TSM100_I8) return op_fail(err, TSM100_ERR_INVALID, "gemm_w4: a_dtype must be dtype or TSM100_I8");
@@ -83,6 +138,13 @@ inline int32_t gemm_w4(std::string* err, const tsm100_gemm_w4_desc* d, const voi
   p.groups = static_cast<int32_t>(d->k / d->group);
   p.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int sms = 0;
+  int32_t st = sm_count(err, &sms);
+  if (st != TSM100_OK) return st;
+  if (gemm_w4_dense_pays(d->m, d->n, d->k, sms)) {
+    st = d->dtype == TSM100_BF16 ? gemm_w4_dense<__nv_bfloat16>(err, d, w, p, s, gemm) : gemm_w4_dense<__half>(err, d, w, p, s, gemm);
+    if (st != kNoScratch) return st;
+  }
   return d->dtype == TSM100_BF16 ? gemm_w4_typed<__nv_bfloat16>(err, d, w, p, s) : gemm_w4_typed<__half>(err, d, w, p, s);
 }
 

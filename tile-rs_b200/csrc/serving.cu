@@ -15,7 +15,7 @@ int32_t on_device(tsm100_device_t dev, F op) {
   try {
     std::string err;
     const int32_t r = op(&err);
-    if (r != TSM100_OK) last_error_ref() = err;
+    if (r != TSM100_OK && !err.empty()) last_error_ref() = err;  // an operator called on the way has left its own
     return r;
   } catch (...) {
     return TSM100_ERR_RUNTIME;
@@ -33,7 +33,10 @@ int32_t tsm100_add_rms_norm(tsm100_device_t dev, const tsm100_add_rms_norm_desc*
 
 int32_t tsm100_gemm_w4(tsm100_device_t dev, const tsm100_gemm_w4_desc* desc, const void* a, const float* a_scales, const uint8_t* w, const void* w_scales,
                        const uint8_t* w_zeros, void* c, void* stream) {
-  return on_device(dev, [&](std::string* err) { return ops::gemm_w4(err, desc, a, a_scales, w, w_scales, w_zeros, c, dev->status, stream); });
+  return on_device(dev, [&](std::string* err) {
+    return ops::gemm_w4(err, desc, a, a_scales, w, w_scales, w_zeros, c, dev->status, stream,
+                        [&](const tsm100_gemm_desc* g, const void* x, const void* y, void* z) { return tsm100_gemm(dev, g, x, y, z, stream); });
+  });
 }
 
 int32_t tsm100_kv_page_append(tsm100_device_t dev, const tsm100_paged_kv* kv, const tsm100_paged_batch* batch, int32_t dtype, const void* k, const void* v,
