@@ -7,7 +7,7 @@
 //   * The work is one stream, dealt out evenly: blocks of up to two tiles are numbered through (sequence, KV head, block) with the keys they see, and what beginning one
 //     costs, as their length, and every SM takes an equal, contiguous share of it, to the step.  Lengths are only known on the device, prompts and single tokens come in
 //     one call, and 64 blocks over 148 SMs would leave half of them idle.  A block that is cut leaves (maximum, sum, O) for a merging kernel.  (A block of one tile counts
-//     like one of two: two thirds of that cost 1 to 9 % in five mixes out of six, though its steps alone are shorter.  256 keys for beginning a block: 128 cost 1 to 13 %, 512 up to 7.)
+//     like one of two: two thirds of that cost 2 to 9 % in four mixes of six and gained nothing in the others.  256 keys for beginning a block: 128 cost up to 13 %, 512 up to 7.)
 //   * K and V come by pages: boxes of a power of two of positions (8 and more), a lane each.  What a page holds behind the sequence's end is
 //     replaced by zeros in V (it has no weight, but may be NaN) and masked in S.
 //   * 8 bits (kI8): four warps write the tiles that TMA would have written, whole numbers, which 16 bits hold exactly.  K's steps multiply the scores and V's the
