@@ -51,24 +51,26 @@ struct Params {
 struct alignas(8) Barriers {
   uint64_t full[8], empty[8];  // W's slots
   uint64_t ready[2], done[2];  // a chunk's operands are there; its products are
+  uint64_t a_full[kBuffers], a_empty[kBuffers];  // kTmaA: the places of A's chunks
   uint32_t tmem_base;
   uint32_t abort_flag;
 };
 
 // Up to N rows of A; GC groups in a chunk
-template <int N, int GC, bool kScaled>
+template <int N, int GC, bool kScaled, bool kTmaA = false>
 struct Shape {
   static constexpr int kSumsOff = kBuffers * 64;         // columns of tensor memory: weights, then sums
   static constexpr int kTmemUsed = kSumsOff + (kScaled ? N : 2 * GC * N);
   static constexpr int kTmem = kTmemUsed <= 256 ? 256 : 512;
   static constexpr bool kTwo = kTmem == 256 && N <= 32;  // CTAs to an SM
   static constexpr int kSlots = kTwo ? 5 : 6;
+  static constexpr int kPlaces = N == 256 ? 2 : kBuffers;  // of A's chunks: what fits
   static constexpr int kActBytes = N * kChunkK * 2;
-  static constexpr int kActOff = kSlots * kSlotBytes, kBarsOff = kActOff + kBuffers * kActBytes;
+  static constexpr int kActOff = kSlots * kSlotBytes, kBarsOff = kActOff + kPlaces * kActBytes;
   static constexpr int kSmem = kBarsOff + static_cast<int>(sizeof(Barriers)) + 1024;
-  static constexpr int kVecs = N * kChunkK / 8 / kWorkers;  // eights of A's numbers a worker brings for a chunk
+  static constexpr int kVecs = kTmaA ? 1 : N * kChunkK / 8 / kWorkers;  // eights of A's numbers a worker brings for a chunk
   static_assert(kTmemUsed <= 512 && kSmem <= (kTwo ? 113 : 227) * 1024 && kVecs >= 1, "what an SM has");
-  static_assert(N * kRows * 4 <= kBarsOff, "partial sums lie over the slots");
+  static_assert(N * kRows * 4 <= kBarsOff && kPlaces <= kBuffers, "partial sums lie over the slots");
 };
 
 template <bool kBf16>
@@ -133,8 +135,9 @@ __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[X]) {
 
 template <typename T, int N, int GC, bool kScaled, bool kEight>
 __global__ void __launch_bounds__(kThreads, Shape<N, GC, kScaled>::kTwo ? 2 : 1)
-gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
-  using S = Shape<N, GC, kScaled>;
+gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a, const Params p) {
+  constexpr bool kTmaA = kScaled && !kEight;
+  using S = Shape<N, GC, kScaled, kTmaA>;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -149,6 +152,8 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
   if (tid == 0) {
     for (int i = 0; i < S::kSlots; ++i) ptx::mbar_init(&bars->full[i], 1), ptx::mbar_init(&bars->empty[i], kWorkers);
     for (int i = 0; i < 2; ++i) ptx::mbar_init(&bars->ready[i], kWorkers), ptx::mbar_init(&bars->done[i], 1);
+    if constexpr (kTmaA)
+      for (int i = 0; i < S::kPlaces; ++i) ptx::mbar_init(&bars->a_full[i], 1), ptx::mbar_init(&bars->a_empty[i], 1);
     bars->abort_flag = 0;
     ptx::fence_mbar_init();
   }
@@ -173,23 +178,45 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
   for (int i = 0; i < NH; ++i) acc[i] = 0.f;
   const int wg = warp >> 2, row = (warp & 3) * 32 + lane;
   if (warp == 8) {
-    if (lane == 0)
-      for (int s = s0; s < s1; ++s) {
+    if (lane == 0) {
+      auto fetch_w = [&](int s) {
         const int i = s - s0, slot = i % S::kSlots;
-        if (!ptx::mbar_wait(&bars->empty[slot], ((i / S::kSlots) & 1u) ^ 1u, abort_flag, p.status, 135)) break;
+        if (!ptx::mbar_wait(&bars->empty[slot], ((i / S::kSlots) & 1u) ^ 1u, abort_flag, p.status, 135)) return false;
         ptx::mbar_arrive_expect_tx(&bars->full[slot], kSlotBytes);
         ptx::tma_load_3d(smem + slot * kSlotBytes, &tmap_w, &bars->full[slot], s * (kStepK / 2), row_base, 0);
+        return true;
+      };
+      if constexpr (kTmaA) {
+        // W keeps kAheadW steps before A: a step's place is free when the products that A's next chunk waits for are about to be
+        constexpr int kAheadW = S::kSlots - 2;
+        bool more = true;
+        for (int s = s0; more && s < min(s0 + kAheadW, s1); ++s) more = fetch_w(s);
+        for (int i = 0; more && i < chunks; ++i) {
+          if (i % 2 == 0 && s0 + i / 2 + kAheadW < s1) more = fetch_w(s0 + i / 2 + kAheadW);
+          const int b = i % S::kPlaces;
+          if (!more || !ptx::mbar_wait(&bars->a_empty[b], ((i / S::kPlaces) & 1u) ^ 1u, abort_flag, p.status, 139)) break;
+          ptx::mbar_arrive_expect_tx(&bars->a_full[b], static_cast<uint32_t>(p.tokens) * kChunkK * 2);
+#pragma unroll
+          for (int h = 0; h < kChunkK / 64; ++h)
+            ptx::tma_load_3d(smem + S::kActOff + b * S::kActBytes + h * (N * 128), &tmap_a, &bars->a_full[b], (first + i) * kChunkK + h * 64, token0, 0);
+        }
+      } else {
+        for (int s = s0; s < s1; ++s)
+          if (!fetch_w(s)) break;
       }
+    }
   } else if (warp == 9) {
     const uint32_t idesc = ptx::make_idesc_f16(kRows, static_cast<uint32_t>(p.tokens), false, false, kBf16);
     constexpr uint64_t kmajor = ptx::make_smem_desc_base(16, 1024);
-    int b = 0;
+    int b = 0, place = 0;
+    uint32_t place_phase = 0;
     for (int i = 0; i < chunks; ++i) {
       const int d = i & 1;
       if (!warp_wait(&bars->ready[d], (i >> 1) & 1u, abort_flag, p.status, 136)) break;
+      if (kTmaA && !warp_wait(&bars->a_full[place], place_phase, abort_flag, p.status, 140)) break;
       ptx::tcgen05_fence_after_thread_sync();
       if (ptx::elect_one_sync()) {
-        const uint32_t act = ptx::smem_u32(smem + S::kActOff + b * S::kActBytes);
+        const uint32_t act = ptx::smem_u32(smem + S::kActOff + place * S::kActBytes);
 #pragma unroll
         for (int kk = 0; kk < kChunkK / 16; ++kk) {
           constexpr int kPer = kChunkK / 16 / GC;  // of a group
@@ -197,9 +224,11 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
                                   ptx::smem_desc(kmajor, act + (kk >> 2) * (N * 128) + (kk & 3) * 32), idesc, (kScaled ? i + kk : kk % kPer) != 0 ? 1u : 0u);
         }
         ptx::tcgen05_commit(&bars->done[d]);
+        if (kTmaA && i + S::kPlaces < chunks) ptx::tcgen05_commit(&bars->a_empty[place]);  // only where it is waited for: none outlives the CTA
       }
       __syncwarp();
       b = b + 1 == kBuffers ? 0 : b + 1;
+      if (++place == S::kPlaces) place = 0, place_phase ^= 1u;
     }
   } else {
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -248,6 +277,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
     const int act_chunks = rows_left > 0 ? min(chunks, (p.k - first * kChunkK - e8 + kChunkK - 1) / kChunkK) : 0;
     Vec act[kAhead][S::kVecs];
     auto fetch_act = [&](int i, Vec (&to)[S::kVecs]) {
+      if constexpr (kTmaA) return;
 #pragma unroll
       for (int v = 0; v < S::kVecs; ++v) {
         to[v] = Vec{};
@@ -299,7 +329,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
     auto hand_over = [&](int i) {  // chunk i's operands to the tensor core
       ptx::tmem_st_wait();
       ptx::tcgen05_fence_before_thread_sync();
-      ptx::fence_proxy_async_smem();
+      if constexpr (!kTmaA) ptx::fence_proxy_async_smem();
       ptx::mbar_arrive(&bars->ready[i & 1]);
     };
     const uint32_t w_at = ptx::smem_u32(smem) + row * 128;
@@ -331,13 +361,21 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const Params p) {
           f *= 0x10001u;
 #pragma unroll
           for (int j = 0; j < 16; ++j) w[j] = mul2<kBf16>(w[j], f);
+          if constexpr (kTmaA) {  // as A is: 0 1, 2 3, 4 5, 6 7
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+              const uint32_t y[4] = {w[j], w[j + 1], w[j + 2], w[j + 3]};
+              w[j] = __byte_perm(y[0], y[1], 0x5410), w[j + 1] = __byte_perm(y[2], y[3], 0x5410);
+              w[j + 2] = __byte_perm(y[0], y[1], 0x7632), w[j + 3] = __byte_perm(y[2], y[3], 0x7632);
+            }
+          }
         }
         if (h == 0 && i > 0) hand_over(i - 1);  // its stores have had this time to end
         ptx::tmem_st_32x32b_x16(tmem + b * 64 + wg * 32 + h * 16 + lanes, w);
       }
       if (d == 1 || i == chunks - 1) ptx::mbar_arrive(&bars->empty[slot]);
 #pragma unroll
-      for (int v = 0; v < S::kVecs; ++v) {
+      for (int v = 0; v < (kTmaA ? 0 : S::kVecs); ++v) {
         const Vec x = act[from][v];
         uint4 y;
         if constexpr (kEight) y = make_uint4(i8_to_16<T>(x.x, x.y, 0), i8_to_16<T>(x.x, x.y, 1), i8_to_16<T>(x.x, x.y, 2), i8_to_16<T>(x.x, x.y, 3));

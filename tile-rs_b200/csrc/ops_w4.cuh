@@ -24,10 +24,16 @@ inline int32_t gemm_w4_launch(std::string* err, const CUtensorMap& map, w4::Para
   const int blocks = (p.m + N - 1) / N;
   p.tokens = ((p.m + blocks - 1) / blocks + 15) / 16 * 16;
   p.splits = gemm_w4_splits(p.n, p.k, blocks, S::kTwo ? 2ll * sms : sms);
+  CUtensorMap map_a{};
+  if (kScaled && !p.a_scales) {
+    const int32_t st = make_tmap_16bit_3d(err, &map_a, p.a, p.k, p.m, 1, p.k, static_cast<uint64_t>(p.m) * p.k, 64, static_cast<uint32_t>(p.tokens),
+                                          std::is_same<T, __nv_bfloat16>::value);
+    if (st != TSM100_OK) return st;
+  }
   auto kern = p.a_scales ? w4::gemm_w4_kernel<T, N, GC, kScaled, true> : w4::gemm_w4_kernel<T, N, GC, kScaled, false>;
   cudaError_t e = set_dyn_smem_once(kern, S::kSmem);
   const dim3 grid(static_cast<unsigned>((p.n + w4::kRows - 1) / w4::kRows * p.splits), static_cast<unsigned>((p.m + p.tokens - 1) / p.tokens));
-  if (e == cudaSuccess) e = launch_chained(kern, grid, w4::kThreads, S::kSmem, s, p.splits > 1 ? p.splits : 0, map, p);
+  if (e == cudaSuccess) e = launch_chained(kern, grid, w4::kThreads, S::kSmem, s, p.splits > 1 ? p.splits : 0, map, map_a, p);
   return cuda_ok(err, e, "gemm_w4_kernel launch");
 }
 template <typename T, int GC>
