@@ -16,7 +16,8 @@
 // K may be split over a cluster; partial sums are added through distributed shared memory in rank order.
 //
 // More than 64 rows of A (kScaled): a weight is multiplied by its scale and rounded to 16 bits, as a weight of a 16-bit product would have been, and the sums stay
-// in tensor memory over all of K: bringing a group's 128 sums a row back cost as much as its products.
+// in tensor memory over all of K: bringing a group's 128 sums a row back cost as much as its products.  A comes in 16 bits (rows in 8 are made such first, w4_dense.cuh),
+// by TMA, as it is: the weights' pairs are exchanged instead, four instructions for eight (200 x 5003 x 2048 21.5 us with A through registers, 14.8 this way).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -51,13 +52,13 @@ struct Params {
 struct alignas(8) Barriers {
   uint64_t full[8], empty[8];  // W's slots
   uint64_t ready[2], done[2];  // a chunk's operands are there; its products are
-  uint64_t a_full[kBuffers], a_empty[kBuffers];  // kTmaA: the places of A's chunks
+  uint64_t a_full[kBuffers], a_empty[kBuffers];  // kScaled: the places of A's chunks
   uint32_t tmem_base;
   uint32_t abort_flag;
 };
 
 // Up to N rows of A; GC groups in a chunk
-template <int N, int GC, bool kScaled, bool kTmaA = false>
+template <int N, int GC, bool kScaled>
 struct Shape {
   static constexpr int kSumsOff = kBuffers * 64;         // columns of tensor memory: weights, then sums
   static constexpr int kTmemUsed = kSumsOff + (kScaled ? N : 2 * GC * N);
@@ -68,7 +69,7 @@ struct Shape {
   static constexpr int kActBytes = N * kChunkK * 2;
   static constexpr int kActOff = kSlots * kSlotBytes, kBarsOff = kActOff + kPlaces * kActBytes;
   static constexpr int kSmem = kBarsOff + static_cast<int>(sizeof(Barriers)) + 1024;
-  static constexpr int kVecs = kTmaA ? 1 : N * kChunkK / 8 / kWorkers;  // eights of A's numbers a worker brings for a chunk
+  static constexpr int kVecs = kScaled ? 1 : N * kChunkK / 8 / kWorkers;  // eights of A's numbers a worker brings for a chunk
   static_assert(kTmemUsed <= 512 && kSmem <= (kTwo ? 113 : 227) * 1024 && kVecs >= 1, "what an SM has");
   static_assert(N * kRows * 4 <= kBarsOff && kPlaces <= kBuffers, "partial sums lie over the slots");
 };
@@ -136,8 +137,8 @@ __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[X]) {
 template <typename T, int N, int GC, bool kScaled, bool kEight>
 __global__ void __launch_bounds__(kThreads, Shape<N, GC, kScaled>::kTwo ? 2 : 1)
 gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a, const Params p) {
-  constexpr bool kTmaA = kScaled && !kEight;
-  using S = Shape<N, GC, kScaled, kTmaA>;
+  static_assert(!kScaled || !kEight, "more than 64 rows come in 16 bits");
+  using S = Shape<N, GC, kScaled>;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -152,7 +153,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
   if (tid == 0) {
     for (int i = 0; i < S::kSlots; ++i) ptx::mbar_init(&bars->full[i], 1), ptx::mbar_init(&bars->empty[i], kWorkers);
     for (int i = 0; i < 2; ++i) ptx::mbar_init(&bars->ready[i], kWorkers), ptx::mbar_init(&bars->done[i], 1);
-    if constexpr (kTmaA)
+    if constexpr (kScaled)
       for (int i = 0; i < S::kPlaces; ++i) ptx::mbar_init(&bars->a_full[i], 1), ptx::mbar_init(&bars->a_empty[i], 1);
     bars->abort_flag = 0;
     ptx::fence_mbar_init();
@@ -186,7 +187,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
         ptx::tma_load_3d(smem + slot * kSlotBytes, &tmap_w, &bars->full[slot], s * (kStepK / 2), row_base, 0);
         return true;
       };
-      if constexpr (kTmaA) {
+      if constexpr (kScaled) {
         // W keeps kAheadW steps before A: a step's place is free when the products that A's next chunk waits for are about to be
         constexpr int kAheadW = S::kSlots - 2;
         bool more = true;
@@ -213,7 +214,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     for (int i = 0; i < chunks; ++i) {
       const int d = i & 1;
       if (!warp_wait(&bars->ready[d], (i >> 1) & 1u, abort_flag, p.status, 136)) break;
-      if (kTmaA && !warp_wait(&bars->a_full[place], place_phase, abort_flag, p.status, 140)) break;
+      if (kScaled && !warp_wait(&bars->a_full[place], place_phase, abort_flag, p.status, 140)) break;
       ptx::tcgen05_fence_after_thread_sync();
       if (ptx::elect_one_sync()) {
         const uint32_t act = ptx::smem_u32(smem + S::kActOff + place * S::kActBytes);
@@ -224,7 +225,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
                                   ptx::smem_desc(kmajor, act + (kk >> 2) * (N * 128) + (kk & 3) * 32), idesc, (kScaled ? i + kk : kk % kPer) != 0 ? 1u : 0u);
         }
         ptx::tcgen05_commit(&bars->done[d]);
-        if (kTmaA && i + S::kPlaces < chunks) ptx::tcgen05_commit(&bars->a_empty[place]);  // only where it is waited for: none outlives the CTA
+        if (kScaled && i + S::kPlaces < chunks) ptx::tcgen05_commit(&bars->a_empty[place]);  // only where it is waited for: none outlives the CTA
       }
       __syncwarp();
       b = b + 1 == kBuffers ? 0 : b + 1;
@@ -232,9 +233,8 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     }
   } else {
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    // A chunk's scales and zero points, and its part of A, are fetched two chunks ahead, into the registers that the chunk before has left.  (128 rows of A: one, 200 x 5003
-    // x 2048 21.5 us; two take too many registers, 42.)
-    constexpr int kAhead = S::kVecs <= 4 ? 2 : 1;
+    // A chunk's scales and zero points, and its part of A, are fetched two chunks ahead, into the registers that the chunk before has left.
+    constexpr int kAhead = 2;
     const int64_t row_groups = static_cast<int64_t>(min(row_base + row, p.n - 1)) * p.groups + first * GC;
     const uint16_t* scale_at = static_cast<const uint16_t*>(p.scales) + row_groups;
     const uint8_t* zero_at = p.zeros ? p.zeros + row_groups : nullptr;
@@ -277,7 +277,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     const int act_chunks = rows_left > 0 ? min(chunks, (p.k - first * kChunkK - e8 + kChunkK - 1) / kChunkK) : 0;
     Vec act[kAhead][S::kVecs];
     auto fetch_act = [&](int i, Vec (&to)[S::kVecs]) {
-      if constexpr (kTmaA) return;
+      if constexpr (kScaled) return;
 #pragma unroll
       for (int v = 0; v < S::kVecs; ++v) {
         to[v] = Vec{};
@@ -288,7 +288,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     for (int b = 0; b < 2; ++b) {
       zp[b] = 0x08080808u;
       fetch_row(b, sc[b], zp[b]);
-      if (b < kAhead) fetch_act(b, act[b]);
+      fetch_act(b, act[b]);
     }
     uint16_t sc_of[2][GC];  // of the two chunks whose sums are still out
     bool ok = true;
@@ -329,7 +329,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     auto hand_over = [&](int i) {  // chunk i's operands to the tensor core
       ptx::tmem_st_wait();
       ptx::tcgen05_fence_before_thread_sync();
-      if constexpr (!kTmaA) ptx::fence_proxy_async_smem();
+      if constexpr (!kScaled) ptx::fence_proxy_async_smem();
       ptx::mbar_arrive(&bars->ready[i & 1]);
     };
     const uint32_t w_at = ptx::smem_u32(smem) + row * 128;
@@ -342,7 +342,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     int slot = 0, b = 0;
     uint32_t full_phase = 0;
     auto chunk = [&](int i, auto which) {
-      constexpr int d = decltype(which)::value, from = d % kAhead;
+      constexpr int d = decltype(which)::value;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         // 32 k of this row, as numbers
@@ -361,13 +361,11 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
           f *= 0x10001u;
 #pragma unroll
           for (int j = 0; j < 16; ++j) w[j] = mul2<kBf16>(w[j], f);
-          if constexpr (kTmaA) {  // as A is: 0 1, 2 3, 4 5, 6 7
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const uint32_t y[4] = {w[j], w[j + 1], w[j + 2], w[j + 3]};
-              w[j] = __byte_perm(y[0], y[1], 0x5410), w[j + 1] = __byte_perm(y[2], y[3], 0x5410);
-              w[j + 2] = __byte_perm(y[0], y[1], 0x7632), w[j + 3] = __byte_perm(y[2], y[3], 0x7632);
-            }
+          for (int j = 0; j < 16; j += 4) {  // as A is: 0 1, 2 3, 4 5, 6 7
+            const uint32_t y[4] = {w[j], w[j + 1], w[j + 2], w[j + 3]};
+            w[j] = __byte_perm(y[0], y[1], 0x5410), w[j + 1] = __byte_perm(y[2], y[3], 0x5410);
+            w[j + 2] = __byte_perm(y[0], y[1], 0x7632), w[j + 3] = __byte_perm(y[2], y[3], 0x7632);
           }
         }
         if (h == 0 && i > 0) hand_over(i - 1);  // its stores have had this time to end
@@ -375,14 +373,14 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
       }
       if (d == 1 || i == chunks - 1) ptx::mbar_arrive(&bars->empty[slot]);
 #pragma unroll
-      for (int v = 0; v < (kTmaA ? 0 : S::kVecs); ++v) {
-        const Vec x = act[from][v];
+      for (int v = 0; v < (kScaled ? 0 : S::kVecs); ++v) {
+        const Vec x = act[d][v];
         uint4 y;
         if constexpr (kEight) y = make_uint4(i8_to_16<T>(x.x, x.y, 0), i8_to_16<T>(x.x, x.y, 1), i8_to_16<T>(x.x, x.y, 2), i8_to_16<T>(x.x, x.y, 3));
         else y = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
         *reinterpret_cast<uint4*>(act_to + b * S::kActBytes + v * 2048) = y;
       }
-      fetch_act(i + kAhead, act[from]);
+      fetch_act(i + kAhead, act[d]);
       if (i >= 2) collect(i - 2, which);  // frees its sums for this chunk, and its operands for the next
 #pragma unroll
       for (int j = 0; j < GC; ++j) sc_of[d][j] = sc[d][j];
@@ -440,7 +438,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
       for (int i = 0; i < NH; ++i) {
         const int t = wg * NH + i;
         if (t < here)
-          softmax::Elem<T>::store1(out + static_cast<int64_t>(token0 + t) * p.n + row_base + row, kEight ? acc[i] * p.a_scales[token0 + t] : acc[i]);
+          softmax::Elem<T>::store1(out + static_cast<int64_t>(token0 + t) * p.n + row_base + row, kEight || (kScaled && p.a_scales) ? acc[i] * p.a_scales[token0 + t] : acc[i]);
       }
     }
     return;
@@ -459,7 +457,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     float sum = 0.f;
 #pragma unroll 4
     for (int q = 0; q < p.splits; ++q) sum += ptx::ld_shared_cluster_f32(ptx::mapa_shared(ptx::smem_u32(red + i), q));
-    softmax::Elem<T>::store1(out + static_cast<int64_t>(t) * p.n + r, kEight ? sum * p.a_scales[t] : sum);
+    softmax::Elem<T>::store1(out + static_cast<int64_t>(t) * p.n + r, kEight || (kScaled && p.a_scales) ? sum * p.a_scales[t] : sum);
   }
   ptx::cluster_sync_all();  // the others have read this CTA's sums
 }

@@ -25,12 +25,14 @@ inline int32_t gemm_w4_launch(std::string* err, const CUtensorMap& map, w4::Para
   p.tokens = ((p.m + blocks - 1) / blocks + 15) / 16 * 16;
   p.splits = gemm_w4_splits(p.n, p.k, blocks, S::kTwo ? 2ll * sms : sms);
   CUtensorMap map_a{};
-  if (kScaled && !p.a_scales) {
+  if (kScaled) {
     const int32_t st = make_tmap_16bit_3d(err, &map_a, p.a, p.k, p.m, 1, p.k, static_cast<uint64_t>(p.m) * p.k, 64, static_cast<uint32_t>(p.tokens),
                                           std::is_same<T, __nv_bfloat16>::value);
     if (st != TSM100_OK) return st;
   }
-  auto kern = p.a_scales ? w4::gemm_w4_kernel<T, N, GC, kScaled, true> : w4::gemm_w4_kernel<T, N, GC, kScaled, false>;
+  auto kern = w4::gemm_w4_kernel<T, N, GC, kScaled, false>;
+  if constexpr (!kScaled)
+    if (p.a_scales) kern = w4::gemm_w4_kernel<T, N, GC, kScaled, true>;
   cudaError_t e = set_dyn_smem_once(kern, S::kSmem);
   const dim3 grid(static_cast<unsigned>((p.n + w4::kRows - 1) / w4::kRows * p.splits), static_cast<unsigned>((p.m + p.tokens - 1) / p.tokens));
   if (e == cudaSuccess) e = launch_chained(kern, grid, w4::kThreads, S::kSmem, s, p.splits > 1 ? p.splits : 0, map, map_a, p);
@@ -64,46 +66,35 @@ int32_t gemm_w4_typed(std::string* err, const tsm100_gemm_w4_desc* d, const uint
 extern template int32_t gemm_w4_typed<__nv_bfloat16>(std::string*, const tsm100_gemm_w4_desc*, const uint8_t*, const w4::Params&, cudaStream_t);
 extern template int32_t gemm_w4_typed<__half>(std::string*, const tsm100_gemm_w4_desc*, const uint8_t*, const w4::Params&, cudaStream_t);
 
-// Whether the weights are made 16-bit ones first.  The kernel of gemm_w4.cuh makes each of them for every 128 rows, in waves of a tile of 128 x 128
-// per SM; made once they are written and read again, by three launches or more.  bf16, rows in 16 bits | 8 bits, us with the weights made in the
-// kernel, made first:
-//   256 rows, N = 16384, K = 4096: 62, 65 | 73, 75      300 rows: 91, 84 | 107, 92      400: 122, 86 | 142, 95      1000: 225, 135 | 263, 181
-//   N = K = 4096, 400 rows, one wave: 31, 33 | 37, 38   513 rows: 58, 35 | 68, 40       1000: 61, 34 | 72, 43       4000: 237, 107 | 251, 153
-//   N = 16384, K = 512, 300 rows: 25, 21 | 29, 28       K = 128, 640 rows, where the f32 result of 8-bit rows is most of it: 29, 22 | 34, 41
-//   N = 1024, 640 rows, K = 4096: 24, 19 | 28, 22       K = 1024: 14.1, 14.5 | 16.3, 17.0
-inline bool gemm_w4_dense_pays(int64_t m, int64_t n, int64_t k, int sms) {
-  const int64_t blocks = (m + 127) / 128;
-  return k >= 512 && n * k >= (1 << 21) && (blocks > 4 || (blocks > 2 && blocks * ((n + w4::kRows - 1) / w4::kRows) > sms));
-}
+// Whether the weights are made 16-bit ones first.  The kernel of gemm_w4.cuh makes each of them for every 128 rows; made once they are written and
+// read again, by two launches more.  bf16, rows in 16 bits | 8 bits, us with the weights made in the kernel, made first:
+//   N = K = 4096, 400 rows: 22, 33 | 28, 38     520: 43, 34 | 49, 40     1000: 44, 35 | 52, 43     3000: 131, 84 | 148, 110
+//   N = 16384, K = 4096, 400 rows: 88, 85 | 97, 101     520: 109, 109 | 120, 126     1000: 158, 136 | 175, 175     3000: 481, 321 | 524, 416
+//   N = 16384, K = 512, 520 rows: 38, 26 | 46, 37       N = 1024, K = 4096, 520 rows: 19, 19 | 24, 22     1500: 24, 30 | 29, 36     3000: 44, 38 | 54, 53
+//   N = 1024, K = 1024, 640 rows: 14, 14 | 16, 17       N = 16384, K = 128, 640 rows, where the f32 result of 8-bit rows is most of it: 29, 22 | 34, 41
+inline bool gemm_w4_dense_pays(int64_t m, int64_t n, int64_t k) { return k >= 512 && n * k >= (1 << 21) && m > 4 * w4::kRows; }
 
-// `gemm` is the library's own 16-bit product, (desc, a, b, c) on this stream.  kNoScratch: no memory for the weights.
+// A is in 16 bits (p.a_scales: from 8); `gemm` is the library's own 16-bit product, (desc, a, b, c) on this stream.  kNoScratch: no memory for the weights.
 template <typename T, typename Gemm>
 inline int32_t gemm_w4_dense(std::string* err, const tsm100_gemm_w4_desc* d, const uint8_t* w, const w4::Params& p, cudaStream_t s, Gemm gemm) {
   const int64_t n8 = (d->n + 7) / 8 * 8;  // rows of C, and of W's last tiles, as the tensor cores' product takes them
   const bool eight = p.a_scales != nullptr, apart = eight || n8 != d->n || !aligned16(p.c);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  const size_t w_bytes = up(static_cast<size_t>(n8) * d->k * 2), a_bytes = eight ? up(static_cast<size_t>(d->m) * d->k * 2) : 0,
-               f_bytes = apart ? static_cast<size_t>(d->m) * n8 * (eight ? 4 : 2) : 0;
+  const size_t w_bytes = up(static_cast<size_t>(n8) * d->k * 2), f_bytes = apart ? static_cast<size_t>(d->m) * n8 * (eight ? 4 : 2) : 0;
   uint8_t* ws = nullptr;
-  int32_t st = take_scratch(err, reinterpret_cast<void**>(&ws), w_bytes + a_bytes + f_bytes, s);
+  int32_t st = take_scratch(err, reinterpret_cast<void**>(&ws), w_bytes + f_bytes, s);
   if (st != TSM100_OK) return st;
-  uint8_t *wide = ws + w_bytes, *f = wide + a_bytes;
+  uint8_t* f = ws + w_bytes;
   const int group_log2 = d->group == 32 ? 5 : d->group == 64 ? 6 : 7;
   cudaError_t e = launch_chained(w4::w4_expand_kernel<T>, static_cast<unsigned>(n8), w4::kDenseThreads, 0, s, 0, w, static_cast<const uint16_t*>(p.scales),
                                  p.zeros, reinterpret_cast<uint16_t*>(ws), p.n, p.k, static_cast<int32_t>(group_log2));
   st = cuda_ok(err, e, "w4_expand_kernel launch");
-  if (st == TSM100_OK && eight) {
-    const int64_t vecs = d->m * d->k / 8;
-    e = launch_chained(w4::w4_widen_kernel<T>, static_cast<unsigned>((vecs + w4::kDenseThreads - 1) / w4::kDenseThreads), w4::kDenseThreads, 0, s, 0,
-                       static_cast<const uint2*>(p.a), reinterpret_cast<uint4*>(wide), vecs);
-    st = cuda_ok(err, e, "w4_widen_kernel launch");
-  }
   if (st == TSM100_OK) {
     tsm100_gemm_desc g = {};
     g.dtype = d->dtype, g.out_dtype = eight ? TSM100_F32 : d->dtype;
     g.b_transposed = 1, g.batch = 1;
     g.m = d->m, g.n = n8, g.k = d->k;
-    st = gemm(&g, eight ? static_cast<const void*>(wide) : p.a, static_cast<const void*>(ws), apart ? static_cast<void*>(f) : p.c);
+    st = gemm(&g, p.a, static_cast<const void*>(ws), apart ? static_cast<void*>(f) : p.c);
   }
   if (st == TSM100_OK && apart) {
     const dim3 grid(static_cast<unsigned>(d->m), static_cast<unsigned>(std::min<int64_t>((d->n + 2047) / 2048, 64)));
@@ -115,6 +106,18 @@ inline int32_t gemm_w4_dense(std::string* err, const tsm100_gemm_w4_desc* d, con
   e = cudaFreeAsync(ws, s);
   if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
   return st;
+}
+
+// Rows in 8 bits as rows of T, in scratch; without memory for them the product is refused.
+template <typename T>
+inline int32_t gemm_w4_widen(std::string* err, const tsm100_gemm_w4_desc* d, const void* a, void** wide, cudaStream_t s) {
+  const int32_t st = take_scratch(err, wide, static_cast<size_t>(d->m) * d->k * 2, s);
+  if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "gemm_w4: no device memory for the rows in 16 bits");
+  if (st != TSM100_OK) return st;
+  const int64_t vecs = d->m * d->k / 8;
+  return cuda_ok(err, launch_chained(w4::w4_widen_kernel<T>, static_cast<unsigned>((vecs + w4::kDenseThreads - 1) / w4::kDenseThreads), w4::kDenseThreads, 0, s, 0,
+                                     static_cast<const uint2*>(a), static_cast<uint4*>(*wide), vecs),
+                 "w4_widen_kernel launch");
 }
 
 template <typename Gemm>
@@ -144,14 +147,23 @@ inline int32_t gemm_w4(std::string* err, const tsm100_gemm_w4_desc* d, const voi
   p.groups = static_cast<int32_t>(d->k / d->group);
   p.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int sms = 0;
-  int32_t st = sm_count(err, &sms);
-  if (st != TSM100_OK) return st;
-  if (gemm_w4_dense_pays(d->m, d->n, d->k, sms)) {
-    st = d->dtype == TSM100_BF16 ? gemm_w4_dense<__nv_bfloat16>(err, d, w, p, s, gemm) : gemm_w4_dense<__half>(err, d, w, p, s, gemm);
-    if (st != kNoScratch) return st;
+  int32_t st = TSM100_OK;
+  void* wide = nullptr;
+  if (p.a_scales && d->m > w4::kExactTokens && d->k > 0) {
+    st = d->dtype == TSM100_BF16 ? gemm_w4_widen<__nv_bfloat16>(err, d, p.a, &wide, s) : gemm_w4_widen<__half>(err, d, p.a, &wide, s);
+    p.a = wide;
   }
-  return d->dtype == TSM100_BF16 ? gemm_w4_typed<__nv_bfloat16>(err, d, w, p, s) : gemm_w4_typed<__half>(err, d, w, p, s);
+  if (st == TSM100_OK) {
+    st = kNoScratch;
+    if (gemm_w4_dense_pays(d->m, d->n, d->k))
+      st = d->dtype == TSM100_BF16 ? gemm_w4_dense<__nv_bfloat16>(err, d, w, p, s, gemm) : gemm_w4_dense<__half>(err, d, w, p, s, gemm);
+    if (st == kNoScratch) st = d->dtype == TSM100_BF16 ? gemm_w4_typed<__nv_bfloat16>(err, d, w, p, s) : gemm_w4_typed<__half>(err, d, w, p, s);
+  }
+  if (wide) {
+    const cudaError_t e = cudaFreeAsync(wide, s);
+    if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
+  }
+  return st;
 }
 
 }  // namespace ops
