@@ -396,7 +396,8 @@ int32_t tsm100_add_rms_norm(tsm100_device_t dev, const tsm100_add_rms_norm_desc*
  * NULL for 8 everywhere.  A is of type dtype, or TSM100_I8 with the steps of its rows in a_scales[M] (what
  * tsm100_add_rms_norm leaves).  C is of type dtype.  Sums are f32 and C is rounded once.  Up to
  * 64 rows products are exact and scales multiply sums; with more, a weight times its scale is rounded to dtype first.  Rows in 8 bits, more than
- * 64, take 2 M K bytes of scratch (TSM100_ERR_MEMORY without), and more than 512 rows may take 2 N K, and 4 M N, more.  a and w 16-byte aligned. */
+ * 64, take 2 M K bytes of scratch (TSM100_ERR_MEMORY without), and
+ * more than 1024 rows in 16 bits may take 2 N K + 2 M N.  a and w 16-byte aligned. */
 typedef struct {
   int32_t dtype;   /* of w_scales, C, and A unless a_dtype says otherwise: TSM100_F16 | TSM100_BF16 */
   int32_t a_dtype; /* dtype | TSM100_I8 */

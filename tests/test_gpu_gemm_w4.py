@@ -107,6 +107,29 @@ def test_rows_enough_to_make_the_weights_first(dev, pkg, dtype, a_dtype, zeros, 
     assert dev.status() == 0
 
 
+@pytest.mark.parametrize("m,n,k,group", [(200, 16400, 256, 32), (130, 16384, 384, 64), (1030, 2056, 512, 128), (1100, 2049, 1024, 64), (1025, 2048, 544, 32)])
+@pytest.mark.parametrize("dtype,a_dtype,zeros", [("bf16", "bf16", True), ("f16", "i8", True), ("bf16", "i8", False), ("f16", "f16", False)])
+def test_many_tiles_and_many_rows(dev, pkg, dtype, a_dtype, zeros, m, n, k, group):
+    """Tiles of 256 rows; weights made 16-bit ones first."""
+    test_rows_enough_to_make_the_weights_first(dev, pkg, dtype, a_dtype, zeros, m, n, k, group)
+
+
+def test_many_rows_exact_and_not_finite(dev, pkg):
+    g = u.gen(6)
+    a = torch.randint(-3, 4, (1040, 1024), generator=g, device=u.GPU).half()
+    w = torch.randint(0, 256, (2100, 512), generator=g, device=u.GPU, dtype=torch.uint8)
+    scales = torch.full((2100, 8), 0.5, dtype=torch.float16, device=u.GPU)
+    c = torch.empty((1040, 2100), dtype=torch.float16, device=u.GPU)
+    ref = reference(a, None, w, scales, None, 128)[0].half()
+    call(pkg, dev, "f16", "f16", 128, a, None, w, scales, None, c)
+    assert torch.equal(c, ref)
+    a[129, 7] = float("nan")
+    call(pkg, dev, "f16", "f16", 128, a, None, w, scales, None, c)
+    assert torch.isnan(c[129]).all()
+    c[129] = ref[129]
+    assert torch.equal(c, ref)
+
+
 def test_rows_enough_to_make_the_weights_first_exact_and_not_finite(dev, pkg):
     g = u.gen(5)
     a = torch.randint(-3, 4, (530, 1024), generator=g, device=u.GPU).bfloat16()

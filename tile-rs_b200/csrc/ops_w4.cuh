@@ -41,6 +41,10 @@ inline int32_t gemm_w4_launch(std::string* err, const CUtensorMap& map, w4::Para
 template <typename T, int GC>
 inline int32_t gemm_w4_grouped(std::string* err, const CUtensorMap& map, const w4::Params& p, int sms, cudaStream_t s) {
   if (p.m <= 16) return gemm_w4_launch<T, 16, GC>(err, map, p, sms, s);
+  // Tiles of 256 rows make half the weights but have more to a CTA: where those of 128 are more than a wave.  bf16, us with 128, 256: 200 x 16384 x 4096 44, 30;
+  // 400 x 8192 x 4096 43, 29; 400 x 4096 x 4096 (128 tiles of 128) 22, 28; 200 x 8192 x 4096 (128) 22, 28; 200 x 4096 x 16384 (64, split in two) 39, 32.
+  const int64_t tiles = static_cast<int64_t>((p.m + 127) / 128) * ((p.n + w4::kRows - 1) / w4::kRows);
+  if (p.m > 128 && tiles > sms) return gemm_w4_launch<T, 256, GC, true>(err, map, p, sms, s);
   if (p.m > w4::kExactTokens) return gemm_w4_launch<T, 128, GC, true>(err, map, p, sms, s);
   if constexpr (GC <= 2)
     if (p.m > 32) return gemm_w4_launch<T, 64, GC>(err, map, p, sms, s);
@@ -66,41 +70,38 @@ int32_t gemm_w4_typed(std::string* err, const tsm100_gemm_w4_desc* d, const uint
 extern template int32_t gemm_w4_typed<__nv_bfloat16>(std::string*, const tsm100_gemm_w4_desc*, const uint8_t*, const w4::Params&, cudaStream_t);
 extern template int32_t gemm_w4_typed<__half>(std::string*, const tsm100_gemm_w4_desc*, const uint8_t*, const w4::Params&, cudaStream_t);
 
-// Whether the weights are made 16-bit ones first.  The kernel of gemm_w4.cuh makes each of them for every 128 rows; made once they are written and
-// read again, by two launches more.  bf16, rows in 16 bits | 8 bits, us with the weights made in the kernel, made first:
-//   N = K = 4096, 400 rows: 22, 33 | 28, 38     520: 43, 34 | 49, 40     1000: 44, 35 | 52, 43     3000: 131, 84 | 148, 110
-//   N = 16384, K = 4096, 400 rows: 88, 85 | 97, 101     520: 109, 109 | 120, 126     1000: 158, 136 | 175, 175     3000: 481, 321 | 524, 416
-//   N = 16384, K = 512, 520 rows: 38, 26 | 46, 37       N = 1024, K = 4096, 520 rows: 19, 19 | 24, 22     1500: 24, 30 | 29, 36     3000: 44, 38 | 54, 53
-//   N = 1024, K = 1024, 640 rows: 14, 14 | 16, 17       N = 16384, K = 128, 640 rows, where the f32 result of 8-bit rows is most of it: 29, 22 | 34, 41
-inline bool gemm_w4_dense_pays(int64_t m, int64_t n, int64_t k) { return k >= 512 && n * k >= (1 << 21) && m > 4 * w4::kRows; }
+// Whether the weights are made 16-bit ones first.  The kernel of gemm_w4.cuh makes each of them for every 128 or 256 rows; made once they are written
+// and read again, by a launch more.  bf16, us with the weights made in the kernel, made first:
+//   N = K = 4096, 640 rows: 30, 35     1000: 32, 37     1500: 61, 55     3000: 97, 81         N = 16384, K = 4096: 94, 106     130, 132     193, 187     353, 313
+//   N = 16384, K = 512: 34, 28     48, 32     71, 44     130, 79                              N = 1024, K = 4096: 15, 20     15, 24     23, 31     32, 42
+//   N = 672, K = 864, 3000 rows: 10, 15
+// Rows that came in 8 bits have the steps to multiply besides, in another pass over an f32 result: 3000 x 16384 x 4096 took 416 so, 95 more than with 16 bits.
+inline bool gemm_w4_dense_pays(const tsm100_gemm_w4_desc* d) { return d->a_dtype == d->dtype && d->m > 1024 && d->n >= 2048 && d->k >= 512; }
 
-// A is in 16 bits (p.a_scales: from 8); `gemm` is the library's own 16-bit product, (desc, a, b, c) on this stream.  kNoScratch: no memory for the weights.
+// `gemm` is the library's own 16-bit product, (desc, a, b, c) on this stream.  kNoScratch: no memory for the weights.
 template <typename T, typename Gemm>
 inline int32_t gemm_w4_dense(std::string* err, const tsm100_gemm_w4_desc* d, const uint8_t* w, const w4::Params& p, cudaStream_t s, Gemm gemm) {
   const int64_t n8 = (d->n + 7) / 8 * 8;  // rows of C, and of W's last tiles, as the tensor cores' product takes them
-  const bool eight = p.a_scales != nullptr, apart = eight || n8 != d->n || !aligned16(p.c);
-  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  const size_t w_bytes = up(static_cast<size_t>(n8) * d->k * 2), f_bytes = apart ? static_cast<size_t>(d->m) * n8 * (eight ? 4 : 2) : 0;
+  const bool apart = n8 != d->n || !aligned16(p.c);
+  const size_t w_bytes = (static_cast<size_t>(n8) * d->k * 2 + 255) / 256 * 256, c_bytes = apart ? static_cast<size_t>(d->m) * n8 * 2 : 0;
   uint8_t* ws = nullptr;
-  int32_t st = take_scratch(err, reinterpret_cast<void**>(&ws), w_bytes + f_bytes, s);
+  int32_t st = take_scratch(err, reinterpret_cast<void**>(&ws), w_bytes + c_bytes, s);
   if (st != TSM100_OK) return st;
-  uint8_t* f = ws + w_bytes;
+  T* rows = reinterpret_cast<T*>(ws + w_bytes);
   const int group_log2 = d->group == 32 ? 5 : d->group == 64 ? 6 : 7;
   cudaError_t e = launch_chained(w4::w4_expand_kernel<T>, static_cast<unsigned>(n8), w4::kDenseThreads, 0, s, 0, w, static_cast<const uint16_t*>(p.scales),
                                  p.zeros, reinterpret_cast<uint16_t*>(ws), p.n, p.k, static_cast<int32_t>(group_log2));
   st = cuda_ok(err, e, "w4_expand_kernel launch");
   if (st == TSM100_OK) {
     tsm100_gemm_desc g = {};
-    g.dtype = d->dtype, g.out_dtype = eight ? TSM100_F32 : d->dtype;
+    g.dtype = d->dtype, g.out_dtype = d->dtype;
     g.b_transposed = 1, g.batch = 1;
     g.m = d->m, g.n = n8, g.k = d->k;
-    st = gemm(&g, p.a, static_cast<const void*>(ws), apart ? static_cast<void*>(f) : p.c);
+    st = gemm(&g, p.a, static_cast<const void*>(ws), apart ? static_cast<void*>(rows) : p.c);
   }
   if (st == TSM100_OK && apart) {
     const dim3 grid(static_cast<unsigned>(d->m), static_cast<unsigned>(std::min<int64_t>((d->n + 2047) / 2048, 64)));
-    const int32_t pitch = static_cast<int32_t>(n8);
-    e = eight ? launch_chained(w4::w4_rows_kernel<T, float>, grid, w4::kDenseThreads, 0, s, 0, reinterpret_cast<const float*>(f), p.a_scales, static_cast<T*>(p.c), p.n, pitch)
-              : launch_chained(w4::w4_rows_kernel<T, T>, grid, w4::kDenseThreads, 0, s, 0, reinterpret_cast<const T*>(f), p.a_scales, static_cast<T*>(p.c), p.n, pitch);
+    e = launch_chained(w4::w4_rows_kernel<T>, grid, w4::kDenseThreads, 0, s, 0, static_cast<const T*>(rows), static_cast<T*>(p.c), p.n, static_cast<int32_t>(n8));
     st = cuda_ok(err, e, "w4_rows_kernel launch");
   }
   e = cudaFreeAsync(ws, s);
@@ -155,7 +156,7 @@ inline int32_t gemm_w4(std::string* err, const tsm100_gemm_w4_desc* d, const voi
   }
   if (st == TSM100_OK) {
     st = kNoScratch;
-    if (gemm_w4_dense_pays(d->m, d->n, d->k))
+    if (gemm_w4_dense_pays(d))
       st = d->dtype == TSM100_BF16 ? gemm_w4_dense<__nv_bfloat16>(err, d, w, p, s, gemm) : gemm_w4_dense<__half>(err, d, w, p, s, gemm);
     if (st == kNoScratch) st = d->dtype == TSM100_BF16 ? gemm_w4_typed<__nv_bfloat16>(err, d, w, p, s) : gemm_w4_typed<__half>(err, d, w, p, s);
   }

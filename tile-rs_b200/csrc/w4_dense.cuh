@@ -1,6 +1,6 @@
 // 4-bit weights as 16-bit ones, for products with so many rows of A that making the weights once and multiplying them as a 16-bit matrix takes
-// less time than making them for every 128 rows (gemm_w4.cuh): each weight times its scale, rounded once, as there.  Rows of A in 8 bits become
-// 16-bit numbers, exactly; their steps multiply an f32 result.  A C with rows off 16-byte boundaries is copied from one with rows on them.
+// less time than making them for every 128 or 256 rows (gemm_w4.cuh): each weight times its scale, rounded once, as there.  A C with rows off 16-byte
+// boundaries is copied from one with rows on them.  And rows of A in 8 bits as 16-bit numbers, exactly.
 // Bound: memory, writing the weights (16 bytes a thread and access); the product after it is bound as the 16-bit one.
 #pragma once
 
@@ -58,26 +58,18 @@ w4_widen_kernel(const uint2* __restrict__ a, uint4* __restrict__ out, int64_t ve
   };
   out[i] = make_uint4(two(x.x, 0), two(x.x, 2), two(x.y, 0), two(x.y, 2));
 }
-// Rows of 8-element pitch to C's rows, four elements a thread and access: f32 ones times a_scales[m], rounded once, or 16-bit ones as they are.
-template <typename T, typename F>
+// Rows of `pitch` elements, a multiple of eight, to rows of n: four elements a thread and access.
+template <typename T>
 __global__ void __launch_bounds__(kDenseThreads)
-w4_rows_kernel(const F* __restrict__ f, const float* __restrict__ a_scales, T* __restrict__ c, int32_t n, int32_t f_pitch) {
+w4_rows_kernel(const T* __restrict__ from, T* __restrict__ c, int32_t n, int32_t pitch) {
   ptx::launch_dependents_if_few();
-  f = ptx::wait_prior_grid(f);
-  f += static_cast<int64_t>(blockIdx.x) * f_pitch;
+  from = ptx::wait_prior_grid(from);
+  from += static_cast<int64_t>(blockIdx.x) * pitch;
   c += static_cast<int64_t>(blockIdx.x) * n;
   const bool vectors = reinterpret_cast<uintptr_t>(c) % 8 == 0;
-  float s = 1.f;
-  if constexpr (sizeof(F) == 4) s = ptx::wait_prior_grid(a_scales)[blockIdx.x];
   for (int i = 4 * (blockIdx.y * kDenseThreads + threadIdx.x); i < n; i += 4 * gridDim.y * kDenseThreads) {
     alignas(8) T y[4];
-    if constexpr (sizeof(F) == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(f + i);
-      softmax::Elem<T>::store1(y, x.x * s), softmax::Elem<T>::store1(y + 1, x.y * s), softmax::Elem<T>::store1(y + 2, x.z * s);
-      softmax::Elem<T>::store1(y + 3, x.w * s);
-    } else {
-      *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(f + i);
-    }
+    *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(from + i);
     if (vectors && i + 4 <= n) {
       *reinterpret_cast<uint2*>(c + i) = *reinterpret_cast<const uint2*>(y);
     } else {
