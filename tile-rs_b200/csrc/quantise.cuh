@@ -1,4 +1,5 @@
-// Rows of f32 as whole numbers of steps of their largest magnitude: step = max|x| * (1/127), q = x / step rounded to nearest even (the quotient in f32).
+// Rows of f32 as whole numbers of steps of their largest magnitude: step = max|x| * (1/127), q = x / step rounded to nearest even (the quotient in f32).  Where the
+// largest is taken with max_nan, a row with a NaN has a step of NaN, one with an infinity and no NaN an infinite one, and every number is 0: q * step is NaN all along.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -7,13 +8,20 @@
 namespace tsm100 {
 namespace quant {
 
+// The larger of two, NaN if either is: fmaxf would drop it, and a row would lose its NaN with that.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 struct Step {
   float step, inv;
 };
 __device__ __forceinline__ Step step_of(float top) {
   Step s;
   s.step = top * static_cast<float>(1.0 / 127.0);
-  // NaN where the reciprocal is no use (zero, far from 1, not finite): every number then takes the division
+  // NaN where the reciprocal is no use (zero, far from 1, not finite): every number then takes the division, or is 0
   s.inv = s.step >= 0x1p-120f && s.step <= 0x1p120f ? 1.f / s.step : __uint_as_float(0x7fffffffu);
   return s;
 }
@@ -32,7 +40,7 @@ __device__ __forceinline__ uint32_t quantise4(const float* x, const Step& s) {
   }
   if (divide) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = (s.step > 0.f ? x[i] / s.step : 0.f) + kMagic;
+    for (int i = 0; i < 4; ++i) u[i] = (s.step > 0.f && s.step < INFINITY ? x[i] / s.step : 0.f) + kMagic;
   }
   const uint32_t lo = __byte_perm(__float_as_uint(u[0]), __float_as_uint(u[1]), 0x0040), hi = __byte_perm(__float_as_uint(u[2]), __float_as_uint(u[3]), 0x0040);
   return __byte_perm(lo, hi, 0x5410);
