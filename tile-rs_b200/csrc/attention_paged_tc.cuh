@@ -606,15 +606,15 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               if (col0 + q * 32 + i > limit) v[q][i] = 0xff800000u;  // -inf
-              mx = fmaxf(mx, __uint_as_float(v[q][i]));
+              mx = ptx::fmax_nan(mx, __uint_as_float(v[q][i]));
             }
         } else {
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) mx4[(i >> 1) & 3] = ptx::fmax3(mx4[(i >> 1) & 3], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
-          mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            for (int i = 0; i < 32; i += 2) mx4[(i >> 1) & 3] = ptx::fmax3_nan(mx4[(i >> 1) & 3], __uint_as_float(v[q][i]), __uint_as_float(v[q][i + 1]));
+          mx = ptx::fmax_nan(ptx::fmax_nan(mx4[0], mx4[1]), ptx::fmax_nan(mx4[2], mx4[3]));
         }
         const float m_new = fmaxf(m_used, mx);
         if (j == 0) {
@@ -651,8 +651,8 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         }
 
         // probabilities: exp2, rounded to 16 bits, in the K-major layout of the P V product; of every 8 pairs attn::kPolyPairs avoid MUFU.  A row
-        // whose scores so far are all -inf takes them against 0.
-        const float ms = (m_used == -INFINITY ? 0.f : m_used * sl2) + static_cast<float>(v_used);
+        // whose scores so far are all -inf takes them against 0, one with a NaN or +inf among them against NaN (attention_tc.cuh).
+        const float ms = (mx != mx || m_used == INFINITY ? NAN : m_used == -INFINITY ? 0.f : m_used * sl2) + static_cast<float>(v_used);
         const ptx::f32x2_t sl2x2 = ptx::pack_f32x2(sl2, sl2);
         const ptx::f32x2_t nmsx2 = ptx::pack_f32x2(-ms, -ms);
         ptx::f32x2_t lsum[2] = {0ull, 0ull};

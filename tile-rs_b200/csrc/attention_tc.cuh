@@ -412,7 +412,7 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             if (col0 + c * 32 + i > limit) v[c][i] = 0xff800000u;  // -inf
-            mx = fmaxf(mx, __uint_as_float(v[c][i]));
+            mx = ptx::fmax_nan(mx, __uint_as_float(v[c][i]));
           }
       } else {
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -420,8 +420,8 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 32; i += 2)  // three-input max: 64 instructions for 128 values
-            mx4[(i >> 1) & 3] = ptx::fmax3(mx4[(i >> 1) & 3], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
-        mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            mx4[(i >> 1) & 3] = ptx::fmax3_nan(mx4[(i >> 1) & 3], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+        mx = ptx::fmax_nan(ptx::fmax_nan(mx4[0], mx4[1]), ptx::fmax_nan(mx4[2], mx4[3]));
       }
       const float m_new = fmaxf(m_used, mx);
       if (j == 0) {
@@ -462,7 +462,8 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       // f32 probabilities before they are rounded (packed adds, two per instruction).
       // A row whose scores so far are all -inf (a step, or in kSplit a whole range, may lie behind the row's last visible key):
       // taking them against 0 gives them no weight, against their maximum of -inf NaN.
-      const float ms = m_used == -INFINITY ? 0.f : m_used * sl2;
+      // A NaN among the scores, which the maximum keeps (m_used drops it), or a score of +inf makes NaN of all of the row's probabilities: those that avoid MUFU lose it.
+      const float ms = mx != mx || m_used == INFINITY ? NAN : m_used == -INFINITY ? 0.f : m_used * sl2;
       const ptx::f32x2_t sl2x2 = ptx::pack_f32x2(sl2, sl2);
       const ptx::f32x2_t nmsx2 = ptx::pack_f32x2(-ms, -ms);
       ptx::f32x2_t lsum[2] = {0ull, 0ull};  // (+0.0f, +0.0f)

@@ -143,9 +143,9 @@ kv_page_rows_kernel(const Cache c, const Batch s, T* k, T* v, int32_t per_cta, u
         float f[8], top = 0.f;
         Elem<T>::unpack(x[i], f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = quant::max_nan(top, fabsf(f[j]));
+        for (int j = 0; j < 8; ++j) top = ptx::fmax_nan(top, fabsf(f[j]));
 #pragma unroll
-        for (int off = LANES / 2; off > 0; off >>= 1) top = quant::max_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
+        for (int off = LANES / 2; off > 0; off >>= 1) top = ptx::fmax_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
         if (at[i] < 0 || !inside) continue;
         const quant::Step step = quant::step_of(top);
         *reinterpret_cast<uint2*>(held(i)) = make_uint2(quant::quantise4(f, step), quant::quantise4(f + 4, step));

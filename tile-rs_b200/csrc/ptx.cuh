@@ -576,7 +576,7 @@ __device__ __forceinline__ f32x2_t add_f32x2(f32x2_t a, f32x2_t b) {
 // 2^t for a pair of t <= 0 on the FMA pipe (no MUFU): round t to the nearest integer n
 // with the 1.5*2^23 trick, evaluate a cubic for 2^(t-n) on [-0.5, 0.5] (relative error
 // 7.5e-5, far below the 16-bit rounding that follows) and add n to the exponent field.
-// t is clamped at -125 so the exponent cannot wrap; 2^-125 stands in for zero.
+// t is clamped at -125 so the exponent cannot wrap; 2^-125 stands in for zero, and for a NaN: who may have one looks for it elsewhere.
 __device__ __forceinline__ void exp2_poly_x2(f32x2_t t2, float& out_lo, float& out_hi) {
   float lo, hi;
   unpack_f32x2(t2, lo, hi);
@@ -601,6 +601,17 @@ __device__ __forceinline__ void exp2_poly_x2(f32x2_t t2, float& out_lo, float& o
   out_hi = __uint_as_float(__float_as_uint(ph) + (__float_as_uint(rh) << 23));
 }
 
+// The largest, NaN if any of them is.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));

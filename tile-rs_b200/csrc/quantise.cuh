@@ -1,5 +1,5 @@
 // Rows of f32 as whole numbers of steps of their largest magnitude: step = max|x| * (1/127), q = x / step rounded to nearest even (the quotient in f32).  Where the
-// largest is taken with max_nan, a row with a NaN has a step of NaN, one with an infinity and no NaN an infinite one, and every number is 0: q * step is NaN all along.
+// largest is taken with fmax_nan, a row with a NaN has a step of NaN, one with an infinity and no NaN an infinite one, and every number is 0: q * step is NaN all along.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -7,13 +7,6 @@
 
 namespace tsm100 {
 namespace quant {
-
-// The larger of two, NaN if either is: fmaxf would drop it, and a row would lose its NaN with that.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
 
 struct Step {
   float step, inv;
