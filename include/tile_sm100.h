@@ -396,7 +396,8 @@ int32_t tsm100_add_rms_norm(tsm100_device_t dev, const tsm100_add_rms_norm_desc*
  * w is [N][K/2] bytes, the even k in the low half; w_scales [N][K/group] of type dtype; w_zeros [N][K/group] bytes (0 .. 15), or
  * NULL for 8 everywhere.  A is of type dtype, or TSM100_I8 with the steps of its rows in a_scales[M] (what
  * tsm100_add_rms_norm leaves).  C is of type dtype.  Sums are f32 and C is rounded once.  Up to
- * 64 rows products are exact and scales multiply sums; with more, a weight times its scale is rounded to dtype first.  Rows in 8 bits, more than
+ * 64 rows products are exact and scales multiply sums; with more, a weight times its scale is rounded to dtype first (f16: up to 65504, so scales
+ * below 4368, or 8192 without zero points).  Rows in 8 bits, more than
  * 64, take 2 M K bytes of scratch (TSM100_ERR_MEMORY without), and
  * more than 1024 rows in 16 bits may take 2 N K + 2 M N.  a and w 16-byte aligned. */
 typedef struct {

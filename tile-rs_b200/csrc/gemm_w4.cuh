@@ -220,6 +220,8 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
         const uint32_t act = ptx::smem_u32(smem + S::kActOff + place * S::kActBytes);
 #pragma unroll
         for (int kk = 0; kk < kChunkK / 16; ++kk) {
+          // nothing behind K: A is zero there, but a weight as far from its zero point as 15, times the last group's scale, may be infinite in 16 bits
+          if (kScaled && GC > 1 && (first + i) * kChunkK + kk * 16 >= p.k) break;
           constexpr int kPer = kChunkK / 16 / GC;  // of a group
           ptx::tcgen05_mma_f16_ts(kScaled ? sums_at : sums_at + (d * GC + kk / kPer) * N, tmem + b * 64 + kk * 8,
                                   ptx::smem_desc(kmajor, act + (kk >> 2) * (N * 128) + (kk & 3) * 32), idesc, (kScaled ? i + kk : kk % kPer) != 0 ? 1u : 0u);
@@ -244,7 +246,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant
     uint16_t sc[2][GC];
     uint32_t zp[2];  // a byte a group
     const int last_group = max(groups_left - 1, 0), last_chunk = max((groups_left - 1) / GC, 0);
-    // Behind the last group it is fetched again: A is zero there, and rows behind N are not stored.
+    // Behind the last group it is fetched again: no product or one with zeros follows, and rows behind N are not stored.
     auto fetch_row = [&](int i, uint16_t (&to)[GC], uint32_t& zero) {
       if (GC > 1 && together) {
         const int at = min(i, last_chunk) * GC;
