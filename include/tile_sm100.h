@@ -372,7 +372,7 @@ int32_t tsm100_attention_decode(tsm100_device_t dev, const tsm100_attention_deco
  * reference, whose norm, matmul and KV cache (tile.rs:2063, :192-193, :2113-2136) these go beside.
  *
  * Values in 8 bits are whole numbers q in -127 .. 127 with an f32 step per row, x ~ q * step: step =
- * max|x| / 127, q = x / step rounded to nearest even; a row of zeros has step 0, and one that is not finite a step that is not, so that q * step is
+ * max|x| / 127 (rounded up where the nearest f32 would make q more than 127, below 2^-140), q = x / step rounded to nearest even; a row of zeros has step 0, and one that is not finite a step that is not, so that q * step is
  * NaN in all of it. */
 
 /* RMS normalisation with the residual's addition, a weight, and an output in storage type or 8 bits:

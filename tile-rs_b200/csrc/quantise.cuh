@@ -1,5 +1,5 @@
-// Rows of f32 as whole numbers of steps of their largest magnitude: step = max|x| * (1/127), q = x / step rounded to nearest even (the quotient in f32).  Where the
-// largest is taken with fmax_nan, a row with a NaN has a step of NaN, one with an infinity and no NaN an infinite one, and every number is 0: q * step is NaN all along.
+// Rows of f32 as whole numbers of steps of their largest magnitude: step = max|x| * (1/127), q = x / step rounded to nearest even (the quotient in f32).  A row with an
+// infinity, or with a NaN if the largest is taken with fmax_nan, has a step of NaN, and so has q * step all along.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -14,8 +14,11 @@ struct Step {
 __device__ __forceinline__ Step step_of(float top) {
   Step s;
   s.step = top * static_cast<float>(1.0 / 127.0);
-  // NaN where the reciprocal is no use (zero, far from 1, not finite): every number then takes the division, or is 0
-  s.inv = s.step >= 0x1p-120f && s.step <= 0x1p120f ? 1.f / s.step : __uint_as_float(0x7fffffffu);
+  // among the smallest numbers, where a step is a few times 2^-149, the nearest one may be too short for the largest x (190 over 1) or be 0: the next one then
+  if (s.step < 0x1p-120f && 255.f * s.step <= 2.f * top && top > 0.f) s.step = __uint_as_float(__float_as_uint(s.step) + 1u);
+  if (top == INFINITY) s.step = __uint_as_float(0x7fffffffu);
+  // 0 for a row of zeros; NaN where the reciprocal is no use (far from 1, not finite): every number then takes the division
+  s.inv = top == 0.f ? 0.f : s.step >= 0x1p-120f && s.step <= 0x1p120f ? 1.f / s.step : __uint_as_float(0x7fffffffu);
   return s;
 }
 // Four numbers as bytes.  A product with the reciprocal is within 4e-5 of the quotient, so both round alike unless that ends near a half; only then is it divided
@@ -33,7 +36,7 @@ __device__ __forceinline__ uint32_t quantise4(const float* x, const Step& s) {
   }
   if (divide) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = (s.step > 0.f && s.step < INFINITY ? x[i] / s.step : 0.f) + kMagic;
+    for (int i = 0; i < 4; ++i) u[i] = x[i] / s.step + kMagic;
   }
   const uint32_t lo = __byte_perm(__float_as_uint(u[0]), __float_as_uint(u[1]), 0x0040), hi = __byte_perm(__float_as_uint(u[2]), __float_as_uint(u[3]), 0x0040);
   return __byte_perm(lo, hi, 0x5410);
