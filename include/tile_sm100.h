@@ -427,7 +427,7 @@ typedef struct {
  * lens[b] positions with them; position p of it lies in page table[b][p / page_size].  The arrays are in device memory and are read when the call's
  * kernels run.  A sequence with more positions than its row of the table has room for, more than max_new tokens, or more tokens than
  * positions, is left out; what a table entry outside 0 .. pages-1 stands for is not written, and a result that reads it means nothing.  Nothing
- * outside the buffers is touched, other sequences are served, and the next tsm100_stream_synchronize answers TSM100_ERR_INVALID (status
+ * outside the buffers is touched, other sequences are served, and the next tsm100_stream_synchronize, or operator on host memory, answers TSM100_ERR_INVALID (status
  * 0x2000|site).  Tokens from starts[batch] on belong to no sequence and are left alone. */
 typedef struct {
   int32_t batch;

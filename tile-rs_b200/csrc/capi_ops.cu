@@ -47,8 +47,7 @@ int32_t sync_pipe(tsm100_device_t dev) {
   uint32_t v = 0;
   int32_t st = read_status(dev, p.stream[0], &v);
   if (st != TSM100_OK) return st;
-  if (v != 0) return fail(TSM100_ERR_TIMEOUT, "a kernel gave up a bounded device-side wait (status 0x%x)", v);
-  return TSM100_OK;
+  return status_result(v);
 }
 
 inline size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }

@@ -60,5 +60,7 @@ int32_t use_device(tsm100_device_t dev);
 
 // Reads and clears the device status word (synchronises `stream`).
 int32_t read_status(tsm100_device_t dev, cudaStream_t stream, uint32_t* value);
+// What a status word that was read means: TSM100_OK for 0, else an error with its message.
+int32_t status_result(uint32_t value);
 
 }  // namespace tsm100

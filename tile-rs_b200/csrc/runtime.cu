@@ -54,6 +54,13 @@ int32_t read_status(tsm100_device_t dev, cudaStream_t stream, uint32_t* value) {
   return TSM100_OK;
 }
 
+int32_t status_result(uint32_t v) {
+  if (v == 0) return TSM100_OK;
+  if ((v & 0xf000u) == 0x2000u)
+    return fail(TSM100_ERR_INVALID, "a kernel met a page, a position or a sequence outside what its call described, and left it out (status 0x%x)", v);
+  return fail(TSM100_ERR_TIMEOUT, "a kernel gave up a bounded device-side wait (status 0x%x)", v);
+}
+
 namespace {
 // Open handles of a device, after adding `change`.
 int open_handles(int ordinal, int change) {
@@ -201,10 +208,7 @@ int32_t tsm100_stream_synchronize(tsm100_device_t dev, void* stream) {
   uint32_t v = 0;
   st = read_status(dev, static_cast<cudaStream_t>(stream), &v);
   if (st != TSM100_OK) return st;
-  if ((v & 0xf000u) == 0x2000u)
-    return fail(TSM100_ERR_INVALID, "a kernel met a page, a position or a sequence outside what its call described, and left it out (status 0x%x)", v);
-  if (v != 0) return fail(TSM100_ERR_TIMEOUT, "a kernel gave up a bounded device-side wait (status 0x%x)", v);
-  return TSM100_OK;
+  return status_result(v);
 }
 
 int32_t tsm100_stream_query(tsm100_device_t dev, void* stream, int32_t* done) {
