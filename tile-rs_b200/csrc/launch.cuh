@@ -58,7 +58,9 @@ struct KernelFacts {
   std::mutex mu;
   std::map<std::tuple<const void*, int, int>, int> value;  // (kernel, device, what) -> answer
 };
-inline KernelFacts& kernel_facts() {
+// Hidden, so that the library and every kernel module built from these headers have one each: a module's kernels lie at addresses that another may have after it is
+// unloaded, and what a module is first to construct is destroyed with it.
+__attribute__((visibility("hidden"))) inline KernelFacts& kernel_facts() {
   static KernelFacts f;
   return f;
 }

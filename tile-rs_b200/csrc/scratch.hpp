@@ -20,9 +20,11 @@ struct Pools {
   std::mutex mu;
   std::map<int, cudaMemPool_t> of_device;
 };
+// One for the library and all kernel modules of a process, so that closing a device gives back what a module took; never destroyed, since a module may be the first to
+// construct it and is unloaded before the others.
 inline Pools& pools() {
-  static Pools p;
-  return p;
+  static Pools* all = new Pools;
+  return *all;
 }
 
 inline cudaError_t current_pool(cudaMemPool_t* out) {
