@@ -30,6 +30,15 @@ constexpr int kTileRows = 128, kKeys = 128;
 constexpr int kMaxGroup = 128;
 constexpr int kBlockCost = 2 * kKeys;  // beginning and ending a block, as a length
 constexpr int kMinShare = 4 * kKeys;   // a share's length at least
+// How far the maximum that probabilities are taken against may lag, in log2 units.  8 bits: little, for the sake of what follows (the mixed step
+// of 12 sequences 203 us, 202 with 8 and three more for the step of V).
+template <bool kI8>
+constexpr float kLag = kI8 ? 2.f : attn::kRescaleThreshold;
+// f16 has numbers to 2^-14 in full: there probabilities and their sum are taken so many powers of two larger that the largest (2^kLag; 8 bits: times a step of less than
+// twice 2^v_used) stay within 2^15, and those of keys far behind the first, or beside a large V, keep their bits (attention_paged.cuh).
+template <bool kI8, bool kPvBf16>
+constexpr float kRaised = kPvBf16 ? 0.f : kI8 ? 14.f - kLag<true> : 15.f - kLag<false>;
+
 template <bool kI8, int D>
 struct Shape {
   static constexpr int kThreads = kI8 ? 512 : 384;   // warps 0..3 softmax A, 4..7 softmax B, 8 TMA, 9 Q K^T, 10 P V, 11 planning, 12..15 conversion
@@ -596,7 +605,8 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           float f[4];
           asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]) : "r"(steps + 2 * kKeys * 4));
           const float top = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
-          v_new = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
+          // from -80 on: l, which 2^-v_used multiplies, stays finite over 2^31 keys whose V is 0
+          v_new = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -80), 100);
         }
 
         float mx = -INFINITY;
@@ -621,8 +631,8 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           m_used = m_new;
           v_used = v_new;
         } else {
-          const bool grown = kI8 && v_new > v_used + 3;  // alike in all threads of the tile
-          const bool need = (m_new - m_used) * sl2 > attn::kRescaleThreshold || grown;
+          const bool grown = kI8 && v_new > v_used;  // alike in all threads of the tile
+          const bool need = (m_new - m_used) * sl2 > kLag<kI8> || grown;
           if (__any_sync(0xffffffffu, need)) {
             // O_g is rescaled in place once the P V of the step before has retired
             ready = ptx::mbar_wait(&bars->pv_done[g], (c - 1) & 1u, abort_flag, p.status, 167 + g);
@@ -652,7 +662,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
 
         // probabilities: exp2, rounded to 16 bits, in the K-major layout of the P V product; of every 8 pairs attn::kPolyPairs avoid MUFU.  A row
         // whose scores so far are all -inf takes them against 0, one with a NaN or +inf among them against NaN (attention_tc.cuh).
-        const float ms = (mx != mx || m_used == INFINITY ? NAN : m_used == -INFINITY ? 0.f : m_used * sl2) + static_cast<float>(v_used);
+        const float ms = (mx != mx || m_used == INFINITY ? NAN : m_used == -INFINITY ? 0.f : m_used * sl2) + (static_cast<float>(v_used) - kRaised<kI8, kPvBf16>);
         const ptx::f32x2_t sl2x2 = ptx::pack_f32x2(sl2, sl2);
         const ptx::f32x2_t nmsx2 = ptx::pack_f32x2(-ms, -ms);
         ptx::f32x2_t lsum[2] = {0ull, 0ull};
