@@ -391,8 +391,9 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           for (int i = 0; i < 2; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(qb[n][kk][i] << 16)), fabsf(__uint_as_float(qb[n][kk][i] & 0xffff0000u))));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the power of two below the largest magnitude: what lies 2^24 under that is lost, which f32 sums would lose too
-        const int ex = min(max(static_cast<int>(__float_as_uint(top) >> 23), 20), 250) - 127;
+        // the largest magnitude to 2^14 and more: f16 has all eight bits of what lies 2^28 below it, and some down to 2^38.  Over whole numbers that are 0 where the largest
+        // is, that is what makes the scores
+        const int ex = min(max(static_cast<int>(__float_as_uint(top) >> 23), 20), 254) - 127 - 14;
         factor = __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
         const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
 #pragma unroll

@@ -13,6 +13,7 @@
 //   * 8 bits (kI8): four warps write the tiles that TMA would have written, whole numbers, which 16 bits hold exactly.  K's steps multiply the scores and V's the
 //     probabilities, so that nothing but the probabilities is rounded (with K and V times their steps rounded, errors were 1.6 times as large), and those to f16, whatever q's type
 //     is.  They keep their bits by a power of two that follows the largest step and is taken out again with the sum.
+//     (Sums of queries times whole numbers are f32 before K's step comes to them: queries end at 2^114.)
 // Bound: the tensor core and the exponentials, as there.
 #pragma once
 
