@@ -144,11 +144,15 @@ int32_t tsm100_launch(tsm100_module_t mod, const char* name, uint32_t blocks, vo
  *   bytes of K and V;
  *   the same in 16 bit, 4096 keys or more and query blocks for at most half of the SMs: up to 20 MB;
  *   tsm100_attention_decode, 16 bit, few caches of 1024 positions or more, or 50 MB of caches with up to eight query heads to
- *   each: up to 1.3 MB.
+ *   each: up to 1.3 MB;
+ *   tsm100_attention_paged, whatever the lengths (with 148 SMs): 39 MB for heads of 128 and 20 MB for heads of 64 where max_new times the query heads to a KV head is
+ *   more than 16, else up to 2.5 MB;
+ *   tsm100_gemm_w4, more than 64 rows in 8 bits: 2 bytes per element of A; more than 1024 rows in 16 bits, N >= 2048 and K >= 512: 2 per element of W,
+ *   and of C where its rows do not start on 16-byte boundaries.
  * It is taken and returned on the caller's stream, from a pool of the library's own on each device (the device's default
  * memory pool is neither used nor changed).  The pool keeps up to 1/16 of the device's memory for later calls and gives it
  * back when the device's last handle is closed.  When the device has no memory left, such a call takes a form without
- * scratch: slower, and with its sums in another order.
+ * scratch: slower, and with its sums in another order.  tsm100_attention_paged, and tsm100_gemm_w4 for rows in 8 bits, have none and answer TSM100_ERR_MEMORY.
  * While a stream is captured, taking and returning become allocation nodes of the graph.  The graph can be replayed any
  * number of times; as CUDA has it for graphs with such nodes, it has one executable instance at a time and cannot be a
  * child graph or be cloned. */
@@ -397,9 +401,8 @@ int32_t tsm100_add_rms_norm(tsm100_device_t dev, const tsm100_add_rms_norm_desc*
  * NULL for 8 everywhere.  A is of type dtype, or TSM100_I8 with the steps of its rows in a_scales[M] (what
  * tsm100_add_rms_norm leaves).  C is of type dtype.  Sums are f32 and C is rounded once.  Up to
  * 64 rows products are exact and scales multiply sums; with more, a weight times its scale is rounded to dtype first (f16: up to 65504, so scales
- * below 4368, or 8192 without zero points).  Rows in 8 bits, more than
- * 64, take 2 M K bytes of scratch (TSM100_ERR_MEMORY without), and
- * more than 1024 rows in 16 bits may take 2 N K + 2 M N.  a and w 16-byte aligned. */
+ * below 4368, or 8192 without zero points).  More than 64 rows in 8 bits, and
+ * more than 1024 in 16, take scratch (above).  a and w 16-byte aligned. */
 typedef struct {
   int32_t dtype;   /* of w_scales, C, and A unless a_dtype says otherwise: TSM100_F16 | TSM100_BF16 */
   int32_t a_dtype; /* dtype | TSM100_I8 */
