@@ -436,7 +436,7 @@ typedef struct {
   int32_t batch;
   int32_t tokens;      /* of the call: rows of its token-major arrays, starts[batch] or more */
   int32_t max_new;     /* no sequence has more tokens in this call */
-  int32_t max_len;     /* how long sequences get, for planning; 0: as long as the table's rows allow */
+  int32_t max_len;     /* reserved for planning: 0, or a bound on lens; not read, except that it must not be negative */
   int32_t table_pitch; /* entries of a row of the table */
   const int32_t* table;
   const int32_t* lens;

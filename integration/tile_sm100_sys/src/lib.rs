@@ -52,7 +52,7 @@ pub struct GemmW4Desc { pub dtype: i32, pub a_dtype: i32, pub group: i32, pub m:
 #[repr(C)] #[derive(Clone, Copy)]
 pub struct PagedKv { pub dtype: i32, pub heads_kv: i32, pub head_dim: i32, pub page_size: i32, pub pages: i64, pub k: *mut c_void, pub v: *mut c_void,
                      pub k_scales: *mut f32, pub v_scales: *mut f32 }
-/// table, lens, starts: device memory, read when the call's kernels run.
+/// table, lens, starts: device memory, read when the call's kernels run.  max_len: reserved, 0 or a bound on lens.
 #[repr(C)] #[derive(Clone, Copy)]
 pub struct PagedBatch { pub batch: i32, pub tokens: i32, pub max_new: i32, pub max_len: i32, pub table_pitch: i32, pub table: *const i32,
                         pub lens: *const i32, pub starts: *const i32 }

@@ -331,7 +331,8 @@ class PagedKv:
 
 class PagedBatch:
     """The sequences of a call (tsm100_paged_batch): table [batch, table_pitch], lens [batch] and starts [batch + 1] are int32 arrays in device
-    memory.  No sequence has more than max_new tokens in the call; max_len is for planning (0: unknown)."""
+    memory.  No sequence has more than max_new tokens in the call; max_len is reserved
+    for planning and not read (0, or a bound on lens)."""
 
     def __init__(self, batch: int, tokens: int, max_new: int, max_len: int, table_pitch: int, table: int, lens: int, starts: int):
         self.desc = capi.PagedBatch(batch, tokens, max_new, max_len, table_pitch, table or None, lens or None, starts or None)
