@@ -30,7 +30,7 @@ namespace mma = attn_decode::mma;
 constexpr int kRows = 16;     // of a pass, at most
 constexpr int kMaxCtas = 1024;
 // What beginning and ending a pair costs, in tiles: shares are as long in tiles and these.  64 sequences of up to 6000 positions in 8 bits, costs of 4, 8, 12, 16, 24, 32 tiles:
-// 109, 100, 94, 94, 97, 100 us.
+// 109, 100, 94, 94, 97, 100 us.  (Heads of 128; taken for 16-bit caches, heads of 64 and wide rows too, unmeasured.)
 constexpr int kUnitCost = 16;
 template <bool kI8, int D, bool kWide>
 struct Tile {

@@ -17,7 +17,7 @@
 //
 // More than 64 rows of A (kScaled): a weight is multiplied by its scale and rounded to 16 bits, as a weight of a 16-bit product would have been, and the sums stay
 // in tensor memory over all of K: bringing a group's 128 sums a row back cost as much as its products.  A comes in 16 bits (rows in 8 are made such first, w4_dense.cuh),
-// by TMA, as it is: the weights' pairs are exchanged instead, four instructions for eight (200 x 5003 x 2048 21.5 us with A through registers, 14.8 this way).
+// by TMA, as it is: the weights' pairs are exchanged instead, four instructions for eight (200 x 5003 x 2048 21.5 us with A through registers, 15.4 this way).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -42,7 +42,8 @@ template <typename T, int GC>
 inline int32_t gemm_w4_grouped(std::string* err, const CUtensorMap& map, const w4::Params& p, int sms, cudaStream_t s) {
   if (p.m <= 16) return gemm_w4_launch<T, 16, GC>(err, map, p, sms, s);
   // Tiles of 256 rows make half the weights but have more to a CTA: where those of 128 are more than a wave.  bf16, us with 128, 256: 200 x 16384 x 4096 44, 30;
-  // 400 x 8192 x 4096 43, 29; 400 x 4096 x 4096 (128 tiles of 128) 22, 28; 200 x 8192 x 4096 (128) 22, 28; 200 x 4096 x 16384 (64, split in two) 39, 32.
+  // 400 x 8192 x 4096 43, 29; 400 x 4096 x 4096 (128 tiles of 128) 22, 28; 200 x 8192 x 4096 (128) 22, 28.  Left out: fewer tiles whose K
+  // is split, 200 x 4096 x 16384 (64, in two) 39, 32.
   const int64_t tiles = static_cast<int64_t>((p.m + 127) / 128) * ((p.n + w4::kRows - 1) / w4::kRows);
   if (p.m > 128 && tiles > sms) return gemm_w4_launch<T, 256, GC, true>(err, map, p, sms, s);
   if (p.m > w4::kExactTokens) return gemm_w4_launch<T, 128, GC, true>(err, map, p, sms, s);
@@ -75,7 +76,11 @@ extern template int32_t gemm_w4_typed<__half>(std::string*, const tsm100_gemm_w4
 //   N = K = 4096, 640 rows: 30, 35     1000: 32, 37     1500: 61, 55     3000: 97, 81         N = 16384, K = 4096: 94, 106     130, 132     193, 187     353, 313
 //   N = 16384, K = 512: 34, 28     48, 32     71, 44     130, 79                              N = 1024, K = 4096: 15, 20     15, 24     23, 31     32, 42
 //   N = 672, K = 864, 3000 rows: 10, 15
-// Rows that came in 8 bits have the steps to multiply besides, in another pass over an f32 result: 3000 x 16384 x 4096 took 416 so, 95 more than with 16 bits.
+// The rule is one bound for all, and not the better of both everywhere.  1024 rows in the kernel and 1025 made first: N = 2048, K = 2048 15, 19,
+// K = 4096 22, 30; 3000 x 2048 21, 21; 4096 x 4096 31, 54 (1025 rows are a second wave of tiles in the kernel too); 5003 x 2048 56, 38; 8192 x 512 23, 20; 16384 x 512 47, 32;
+// 16384 x 4096 130, 154.  So short K and N off vectors would gain from fewer rows on, and N of 2048 from more.
+// Rows that came in 8 bits have the steps to multiply besides, in another pass over an f32 result: 3000 x 16384 x 4096 took 416 so, 95 more than with 16 bits,
+// and 410 in the kernel.  (With K = 512 the kernel takes 165, three times the 16-bit form.)
 inline bool gemm_w4_dense_pays(const tsm100_gemm_w4_desc* d) { return d->a_dtype == d->dtype && d->m > 1024 && d->n >= 2048 && d->k >= 512; }
 
 // `gemm` is the library's own 16-bit product, (desc, a, b, c) on this stream.  kNoScratch: no memory for the weights.

