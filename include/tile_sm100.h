@@ -148,11 +148,12 @@ int32_t tsm100_launch(tsm100_module_t mod, const char* name, uint32_t blocks, vo
  *   tsm100_attention_paged, whatever the lengths (with 148 SMs): 39 MB for heads of 128 and 20 MB for heads of 64 where max_new times the query heads to a KV head is
  *   more than 16, else up to 2.5 MB;
  *   tsm100_gemm_w4, more than 64 rows in 8 bits: 2 bytes per element of A; more than 1024 rows in 16 bits, N >= 2048 and K >= 512: 2 per element of W,
- *   and of C where its rows do not start on 16-byte boundaries.
+ *   and of C where its rows do not start on 16-byte boundaries;
+ *   tsm100_gemm_i8, rows of a or w that do not start on 16-byte boundaries: a copy of a, of w, or of both.
  * It is taken and returned on the caller's stream, from a pool of the library's own on each device (the device's default
  * memory pool is neither used nor changed).  The pool keeps up to 1/16 of the device's memory for later calls and gives it
  * back when the device's last handle is closed.  When the device has no memory left, such a call takes a form without
- * scratch: slower, and with its sums in another order.  tsm100_attention_paged, and tsm100_gemm_w4 for rows in 8 bits, have none and answer TSM100_ERR_MEMORY.
+ * scratch: slower, and with its sums in another order.  tsm100_attention_paged, tsm100_gemm_i8, and tsm100_gemm_w4 for rows in 8 bits, have none and answer TSM100_ERR_MEMORY.
  * While a stream is captured, taking and returning become allocation nodes of the graph.  The graph can be replayed any
  * number of times; as CUDA has it for graphs with such nodes, it has one executable instance at a time and cannot be a
  * child graph or be cloned. */
@@ -411,6 +412,30 @@ typedef struct {
 } tsm100_gemm_w4_desc;
 int32_t tsm100_gemm_w4(tsm100_device_t dev, const tsm100_gemm_w4_desc* desc, const void* a, const float* a_scales, const uint8_t* w,
                        const void* w_scales, const uint8_t* w_zeros, void* c, void* stream);
+
+/* Rows as whole numbers and steps, where no norm before a product leaves them: v = x, or with `up` v = silu(x) * up, silu(x) = x / (1 + exp(-x)), in f32;
+ * y[rows][cols] = the whole numbers of v, scales[rows] their steps.  x and up have `pitch` elements from row to row (0: cols), so that gate and up may
+ * lie side by side in the rows of one product; y is packed.  No overlap of y with x or up.  Rows may start anywhere. */
+typedef struct {
+  int32_t dtype; /* of x and up: TSM100_F32 | TSM100_F16 | TSM100_BF16 */
+  int64_t rows;
+  int64_t cols;
+  int64_t pitch;
+} tsm100_quantise_rows_desc;
+int32_t tsm100_quantise_rows(tsm100_device_t dev, const tsm100_quantise_rows_desc* desc, const void* x, const void* up, void* y, float* scales,
+                             void* stream);
+
+/* Product in 8 bits, C[m,n] = (sum_k a[m,k] w[n,k]) * a_scales[m] * w_scales[n]: a [M][K] and w [N][K] are whole numbers (any int8), with a
+ * step for every row of each (what tsm100_add_rms_norm and tsm100_quantise_rows leave).  The sums are exact (32-bit whole numbers, K < 131072), their
+ * scaling is f32 and C is rounded once to dtype, so results do not depend on how the work is dealt out.  A row whose step is NaN is NaN.  lda / ldw / ldc
+ * are row pitches in elements, 0 = packed.  Operands whose rows do not start on 16-byte boundaries are copied to scratch (above). */
+typedef struct {
+  int32_t dtype; /* of C: TSM100_F32 | TSM100_F16 | TSM100_BF16 */
+  int64_t m, n, k;
+  int64_t lda, ldw, ldc;
+} tsm100_gemm_i8_desc;
+int32_t tsm100_gemm_i8(tsm100_device_t dev, const tsm100_gemm_i8_desc* desc, const void* a, const float* a_scales, const void* w, const float* w_scales,
+                       void* c, void* stream);
 
 /* A KV cache in pages: k, v are [pages][heads_kv][page_size][head_dim], with dtype TSM100_I8 the steps of the rows in
  * k_scales, v_scales [pages][heads_kv][page_size] (else NULL). */

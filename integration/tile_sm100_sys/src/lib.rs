@@ -59,6 +59,10 @@ pub struct PagedBatch { pub batch: i32, pub tokens: i32, pub max_new: i32, pub m
 #[repr(C)] #[derive(Clone, Copy, Default)]
 pub struct AttentionPagedDesc { pub dtype: i32, pub heads_q: i32 }
 #[repr(C)] #[derive(Clone, Copy)]
+pub struct QuantiseRowsDesc { pub dtype: i32, pub rows: i64, pub cols: i64, pub pitch: i64 }
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct GemmI8Desc { pub dtype: i32, pub m: i64, pub n: i64, pub k: i64, pub lda: i64, pub ldw: i64, pub ldc: i64 }
+#[repr(C)] #[derive(Clone, Copy)]
 pub struct MultiJob { pub op: i32, pub desc: *const c_void, pub inputs: [*const c_void; 3], pub out: *mut c_void, pub launches: i32, pub timeout_ms: i32 }
 #[repr(C)] #[derive(Clone, Copy)]
 pub struct MultiReport { pub ordinal: i32, pub status: i32, pub first: i64, pub count: i64, pub upload_ms: f32, pub kernel_ms: f32,
@@ -129,6 +133,11 @@ extern "C" {
                                stream: RawStream) -> i32;
     pub fn tsm100_attention_paged(dev: Device, kv: *const PagedKv, batch: *const PagedBatch, d: *const AttentionPagedDesc, q: *const c_void,
                                   o: *mut c_void, stream: RawStream) -> i32;
+    // serving: rows and products in 8 bits
+    pub fn tsm100_quantise_rows(dev: Device, d: *const QuantiseRowsDesc, x: *const c_void, up: *const c_void, y: *mut c_void, scales: *mut f32,
+                                stream: RawStream) -> i32;
+    pub fn tsm100_gemm_i8(dev: Device, d: *const GemmI8Desc, a: *const c_void, a_scales: *const f32, w: *const c_void, w_scales: *const f32,
+                          c: *mut c_void, stream: RawStream) -> i32;
     // operators on host memory
     pub fn tsm100_softmax_host(dev: Device, d: *const SoftmaxDesc, x: *const c_void, y: *mut c_void) -> i32;
     pub fn tsm100_gemm_host(dev: Device, d: *const GemmDesc, a: *const c_void, b: *const c_void, c: *mut c_void) -> i32;

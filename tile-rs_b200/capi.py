@@ -78,6 +78,14 @@ class GemmW4Desc(C.Structure):
     _fields_ = [("dtype", c_i32), ("a_dtype", c_i32), ("group", c_i32), ("m", c_i64), ("n", c_i64), ("k", c_i64)]
 
 
+class QuantiseRowsDesc(C.Structure):
+    _fields_ = [("dtype", c_i32), ("rows", c_i64), ("cols", c_i64), ("pitch", c_i64)]
+
+
+class GemmI8Desc(C.Structure):
+    _fields_ = [("dtype", c_i32), ("m", c_i64), ("n", c_i64), ("k", c_i64), ("lda", c_i64), ("ldw", c_i64), ("ldc", c_i64)]
+
+
 class PagedKv(C.Structure):
     _fields_ = [("dtype", c_i32), ("heads_kv", c_i32), ("head_dim", c_i32), ("page_size", c_i32), ("pages", c_i64), ("k", c_vp), ("v", c_vp),
                 ("k_scales", c_vp), ("v_scales", c_vp)]
@@ -153,6 +161,8 @@ PROTOTYPES = {
     "tsm100_attention_decode": (c_i32, [c_vp, P(AttentionDecodeDesc), c_vp, c_vp, c_vp, c_vp, c_vp]),
     "tsm100_add_rms_norm": (c_i32, [c_vp, P(AddRmsNormDesc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "tsm100_gemm_w4": (c_i32, [c_vp, P(GemmW4Desc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "tsm100_quantise_rows": (c_i32, [c_vp, P(QuantiseRowsDesc), c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "tsm100_gemm_i8": (c_i32, [c_vp, P(GemmI8Desc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "tsm100_kv_page_append": (c_i32, [c_vp, P(PagedKv), P(PagedBatch), c_i32, c_vp, c_vp, c_vp]),
     "tsm100_kv_page_read": (c_i32, [c_vp, P(PagedKv), P(PagedBatch), c_i32, c_vp, c_vp, c_vp]),
     "tsm100_attention_paged": (c_i32, [c_vp, P(PagedKv), P(PagedBatch), P(AttentionPagedDesc), c_vp, c_vp, c_vp]),
@@ -203,7 +213,7 @@ class _ThroughCtypes:
 
 _FAST = None
 FAST_ENTRIES = ("softmax", "rms_norm", "silu_mul", "gemm", "attention", "rope", "kv_cache_update", "attention_prefill", "attention_decode",
-                "add_rms_norm", "gemm_w4", "kv_page_append", "kv_page_read", "attention_paged")
+                "add_rms_norm", "gemm_w4", "kv_page_append", "kv_page_read", "attention_paged", "quantise_rows", "gemm_i8")
 
 
 def fast():

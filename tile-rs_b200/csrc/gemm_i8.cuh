@@ -1,0 +1,287 @@
+// Products of 8-bit whole numbers on tcgen05 (kind::i8), with a step for every row of A and every row of W:
+//
+//   C[m,n] = f(sum_k a[m,k] w[n,k]) * a_scales[m] * w_scales[n]
+//
+// The sums are 32-bit whole numbers and exact (K below 2^17 keeps them in range), f is their one rounding to f32, and C is rounded once from the
+// f32 product.  So a result does not depend on tiles, on how K is split, or on the order of anything.
+//
+// Few output tiles: as gemm_skinny.cuh, with 128 of K where that has 64 (the same bytes).  Bound for a few rows: HBM, W is read once.  W fills the 128-row side of the
+// tensor core and the rows of A its N side, NT = 16 .. 128 wide; K is split over a cluster of up to 8 CTAs where tiles are fewer than the SMs can
+// take, and the partial sums are added through distributed shared memory.
+#pragma once
+
+#include <type_traits>
+
+#include "gemm_skinny.cuh"
+#include "ptx.cuh"
+
+namespace tsm100 {
+namespace gemm_i8 {
+
+constexpr int kBN = 128;                 // rows of W (columns of C) per tile: the tensor core's M side
+constexpr int kBK = 128;                 // 128 bytes: one swizzle row
+constexpr int kThreads = 128;
+constexpr int kMaxSplit = 8;
+constexpr int kWBytes = kBN * kBK;       // 16 KiB of W per stage
+constexpr int kMaxStages = 6;
+constexpr int kAhead = 8;                // tiles of W that a CTA fetches into the L2 before the kernel before it has ended
+
+template <int NT>
+struct Shape {
+  static constexpr int kXBytes = NT * kBK;  // rows of A per stage
+  static constexpr int kStageBytes = kWBytes + kXBytes;
+  static constexpr int kStages = NT <= 16 ? 6 : NT <= 32 ? 5 : NT <= 64 ? 4 : 3;
+  static constexpr int kTmemCols = NT < 32 ? 32 : NT;
+};
+
+struct alignas(8) Barriers {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t acc_full;
+  uint32_t tmem_base;
+  uint32_t abort_flag;
+};
+
+template <int NT>
+constexpr int smem_bytes() {
+  return Shape<NT>::kStages * Shape<NT>::kStageBytes + static_cast<int>(sizeof(Barriers)) + 1024;
+}
+// the partial tile of a split (NT rows x 128 columns, 32 bits) takes the place of the stages
+static_assert(Shape<128>::kStages * Shape<128>::kStageBytes >= 128 * kBN * 4 && Shape<16>::kStages * Shape<16>::kStageBytes >= 16 * kBN * 4,
+              "the partial tile fits the stages");
+static_assert(2 * (smem_bytes<128>() + 1024) <= 227 * 1024 && 2 * (smem_bytes<16>() + 1024) <= 227 * 1024 &&
+              2 * (smem_bytes<64>() + 1024) <= 227 * 1024 && 2 * (smem_bytes<32>() + 1024) <= 227 * 1024, "two CTAs per SM");
+
+struct Params {
+  const float* a_scales;    // [m]
+  const float* w_scales;    // [n]
+  int32_t m, n, k;
+  int32_t m_blocks, n_blocks;
+  int32_t kb_per_cta;       // blocks of 128 of K per CTA of the cluster (every CTA has at least one)
+  int32_t vectors;          // rows of C start on 16-byte boundaries, N is a multiple of 4
+  int64_t ldc;
+  uint32_t* status;
+};
+
+__device__ __forceinline__ float scaled(uint32_t sum, float a_scale, float w_scale) { return __int2float_rn(static_cast<int32_t>(sum)) * a_scale * w_scale; }
+
+// grid: (nb * m_blocks + mb) * cluster size + rank; CTAs that share a tile of W are neighbours.
+template <typename OutT, int NT>
+__global__ void __launch_bounds__(kThreads)
+gemm_i8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w, OutT* c, const Params p) {
+  using S = Shape<NT>;
+  using gemm_skinny::narrow;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Barriers* bars = reinterpret_cast<Barriers*>(smem + S::kStages * S::kStageBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile uint32_t* abort_flag = &bars->abort_flag;
+
+  const uint32_t splits = ptx::cluster_nctarank(), rank = ptx::cluster_ctarank();
+  const int t = static_cast<int>(blockIdx.x / splits);
+  const int mb = t % p.m_blocks, nb = t / p.m_blocks;
+  const int kb_all = (p.k + kBK - 1) / kBK;
+  const int kb0 = static_cast<int>(rank) * p.kb_per_cta;
+  const int num_kb = min(kb_all - kb0, p.kb_per_cta);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      ptx::mbar_init(&bars->full[s], 1);
+      ptx::mbar_init(&bars->empty[s], 1);
+    }
+    ptx::mbar_init(&bars->acc_full, 1);
+    bars->abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(&bars->tmem_base, S::kTmemCols);
+    ptx::tmem_relinquish_alloc_permit();
+  }
+  ptx::tcgen05_fence_before_thread_sync();
+  __syncthreads();
+  ptx::tcgen05_fence_after_thread_sync();
+  const uint32_t tmem_base = bars->tmem_base;
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tensormap(&tmap_a);
+    ptx::prefetch_tensormap(&tmap_w);
+    // while the kernel before this one runs: its first tiles of W
+    for (int i = 0; i < min(num_kb, kAhead); ++i) ptx::prefetch_l2_3d(&tmap_w, (kb0 + i) * kBK, nb * kBN, 0);
+  }
+  ptx::wait_prior_grid();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int i = 0; i < num_kb; ++i) {
+        if (!ptx::mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, 181)) break;
+        uint8_t* w = smem + stage * S::kStageBytes;
+        const int k0 = (kb0 + i) * kBK;
+        ptx::mbar_arrive_expect_tx(&bars->full[stage], S::kStageBytes);
+        ptx::tma_load_3d(w, &tmap_w, &bars->full[stage], k0, nb * kBN, 0);
+        ptx::tma_load_3d(w + kWBytes, &tmap_a, &bars->full[stage], k0, mb * NT, 0);
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = ptx::make_idesc_i8(kBN, NT);
+      constexpr uint64_t kmajor = ptx::make_smem_desc_base(16, 1024);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = 0; i < num_kb; ++i) {
+        if (!(ok = ptx::mbar_wait_relaxed(&bars->full[stage], phase, abort_flag, p.status, 182))) break;
+        ptx::tcgen05_fence_after_thread_sync();
+        const uint32_t w = ptx::smem_u32(smem + stage * S::kStageBytes), x = w + kWBytes;
+#pragma unroll
+        for (int kk = 0; kk < kBK / 32; ++kk)
+          ptx::tcgen05_mma_i8_ss(tmem_base, ptx::smem_desc(kmajor, w + kk * 32), ptx::smem_desc(kmajor, x + kk * 32), idesc, (i | kk) != 0 ? 1u : 0u);
+        ptx::tcgen05_commit(&bars->empty[stage]);
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (ok) ptx::tcgen05_commit(&bars->acc_full);
+    }
+  }
+  __syncwarp();
+
+  // ------------------------------ sums -> C ------------------------------
+  const bool ready = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->acc_full, 0, abort_flag, p.status, 183));
+  ptx::tcgen05_fence_after_thread_sync();
+  ptx::launch_dependents();  // not before: gemm_skinny.cuh
+  const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+  constexpr int kStep = NT < 32 ? 16 : 32;  // rows of C (TMEM columns) per read
+  const int rows = min(NT, p.m - mb * NT);
+  const float* a_scales = p.a_scales + mb * NT;
+  auto read = [&](int r0, uint32_t (&v)[kStep]) {
+    if constexpr (kStep == 16) ptx::tmem_ld_32x32b_x16(lane_addr + r0, v);
+    else ptx::tmem_ld_32x32b_x32(lane_addr + r0, v);
+    ptx::tmem_ld_wait();
+  };
+  if (splits == 1) {
+    const int col = nb * kBN + warp * 32 + lane;
+    if (ready) {
+      const float ws = col < p.n ? p.w_scales[col] : 0.f;
+#pragma unroll
+      for (int r0 = 0; r0 < NT; r0 += kStep) {
+        if (r0 >= rows) break;
+        uint32_t v[kStep];
+        read(r0, v);
+        OutT* dst = c + static_cast<int64_t>(mb * NT + r0) * p.ldc + col;
+        if (col < p.n) {
+#pragma unroll
+          for (int i = 0; i < kStep; ++i)
+            if (r0 + i < rows) dst[i * p.ldc] = narrow<OutT>(scaled(v[i], a_scales[r0 + i], ws));
+        }
+      }
+    }
+  } else {
+    // every CTA leaves its partial tile in its stages (all copies into them and products from them have retired) ...
+    uint32_t* part = reinterpret_cast<uint32_t*>(smem);
+    if (ready) {
+#pragma unroll
+      for (int r0 = 0; r0 < NT; r0 += kStep) {
+        if (r0 >= rows) break;
+        uint32_t v[kStep];
+        read(r0, v);
+#pragma unroll
+        for (int i = 0; i < kStep; ++i) part[(r0 + i) * kBN + warp * 32 + lane] = v[i];
+      }
+    }
+    ptx::cluster_sync_all();
+    // ... and sums its share of the rows over all of them
+    const uint32_t part_addr = ptx::smem_u32(part);
+    const int items = rows * (kBN / 4);  // four columns each
+    for (int i = static_cast<int>(rank) * kThreads + threadIdx.x; i < items; i += static_cast<int>(splits) * kThreads) {
+      uint32_t s[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int q = 0; q < kMaxSplit; ++q)
+        if (q < static_cast<int>(splits)) {
+          const float4 v = ptx::ld_shared_cluster_f32x4(ptx::mapa_shared(part_addr + i * 16, q));
+          s[0] += __float_as_uint(v.x), s[1] += __float_as_uint(v.y), s[2] += __float_as_uint(v.z), s[3] += __float_as_uint(v.w);
+        }
+      const int row = i / (kBN / 4), col = nb * kBN + (i % (kBN / 4)) * 4;
+      if (col >= p.n) continue;
+      const float as = a_scales[row];
+      OutT* dst = c + static_cast<int64_t>(mb * NT + row) * p.ldc + col;
+      OutT x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = narrow<OutT>(scaled(s[j], as, col + j < p.n ? p.w_scales[col + j] : 0.f));
+      if (p.vectors) {
+        if constexpr (sizeof(OutT) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(x);
+        else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < p.n) dst[j] = x[j];
+      }
+    }
+    ptx::cluster_sync_all();  // nobody's partial tile goes while a peer reads it
+  }
+
+  // ------------------------------ teardown ------------------------------------
+  if (*abort_flag != 0u) {
+    // A wait gave up: give copies and products already in flight time to land before shared and tensor memory are released.
+    const unsigned long long t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 1000000ull) {
+    }
+  }
+  ptx::tcgen05_fence_before_thread_sync();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tcgen05_fence_after_thread_sync();
+    ptx::tmem_dealloc(tmem_base, S::kTmemCols);
+  }
+}
+
+// Operands whose rows do not start on 16-byte boundaries, as rows that do: src [rows][cols], pitch ld -> dst [rows][pitch], zeros beyond cols.
+// A thread has 16 bytes of dst; words of src that hold them, shifted into place, a byte at a time where those reach past the matrix.
+struct Operand {
+  const uint8_t* src;
+  uint4* dst;
+  int64_t ld;
+  int32_t rows, cols, pitch;
+  int32_t blocks;   // of the launch that work on it, 0: it is not copied
+};
+constexpr int kPadThreads = 256;
+__device__ __forceinline__ uint4 load16(const uint8_t* src, int64_t at, int64_t size, int valid) {
+  const uintptr_t address = reinterpret_cast<uintptr_t>(src + at), from = address & ~uintptr_t(3);
+  const uint32_t bits = static_cast<uint32_t>(address & 3) * 8;
+  uint32_t w[5];
+  if (valid >= 16 && from >= reinterpret_cast<uintptr_t>(src) && from + 20 <= reinterpret_cast<uintptr_t>(src + size)) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = reinterpret_cast<const uint32_t*>(from)[i];
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = 0u;
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (j < valid) w[j >> 2] |= static_cast<uint32_t>(src[at + j]) << ((j & 3) * 8);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__global__ void __launch_bounds__(kPadThreads) gemm_i8_pad_kernel(const Operand a, const Operand b) {
+  ptx::launch_dependents_if_few();
+  ptx::wait_prior_grid();
+  const bool first = static_cast<int32_t>(blockIdx.x) < a.blocks;
+  const Operand& p = first ? a : b;
+  const int32_t block = first ? blockIdx.x : blockIdx.x - a.blocks;
+  const uint32_t per_row = static_cast<uint32_t>(p.pitch) / 16;
+  const int64_t total = static_cast<int64_t>(p.rows) * per_row, step = static_cast<int64_t>(p.blocks) * kPadThreads;
+  const int64_t size = static_cast<int64_t>(p.rows - 1) * p.ld + p.cols;
+#pragma unroll 2
+  for (int64_t i = static_cast<int64_t>(block) * kPadThreads + threadIdx.x; i < total; i += step) {
+    const int64_t r = total <= 0xffffffffll ? static_cast<int64_t>(static_cast<uint32_t>(i) / per_row) : i / per_row;
+    const int32_t c = static_cast<int32_t>(i - r * per_row) * 16;
+    p.dst[i] = load16(p.src, r * p.ld + c, size, p.cols - c);
+  }
+}
+
+}  // namespace gemm_i8
+}  // namespace tsm100

@@ -13,7 +13,7 @@
 
 namespace {
 
-enum Entry { kSoftmax, kRmsNorm, kSiluMul, kGemm, kAttention, kRope, kKvCacheUpdate, kPrefill, kDecode, kAddRmsNorm, kGemmW4, kPageAppend, kPageRead, kPaged, kEntries };
+enum Entry { kSoftmax, kRmsNorm, kSiluMul, kGemm, kAttention, kRope, kKvCacheUpdate, kPrefill, kDecode, kAddRmsNorm, kGemmW4, kPageAppend, kPageRead, kPaged, kQuantiseRows, kGemmI8, kEntries };
 void* g_entry[kEntries] = {};
 
 // Walks through the arguments; `ok` turns false at the first that does not fit.
@@ -223,10 +223,35 @@ PyObject* attention_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return call<decltype(&tsm100_attention_paged)>(a, kPaged, dev, kv, batch, &d, q, o, s);
 }
 
+// (device, dtype, rows, cols, pitch, x, up, y, scales, stream)
+PyObject* quantise_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 10, kQuantiseRows);
+  auto* dev = a.ptr<tsm100_device_s>();
+  tsm100_quantise_rows_desc d = {};
+  d.dtype = a.i32(), d.rows = a.i64(), d.cols = a.i64(), d.pitch = a.i64();
+  void *x = a.ptr(), *up = a.ptr(), *y = a.ptr();
+  float* scales = a.ptr<float>();
+  void* s = a.ptr();
+  return call<decltype(&tsm100_quantise_rows)>(a, kQuantiseRows, dev, &d, x, up, y, scales, s);
+}
+// (device, dtype, m, n, k, lda, ldw, ldc, a, a_scales, w, w_scales, c, stream)
+PyObject* gemm_i8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 14, kGemmI8);
+  auto* dev = a.ptr<tsm100_device_s>();
+  tsm100_gemm_i8_desc d = {};
+  d.dtype = a.i32(), d.m = a.i64(), d.n = a.i64(), d.k = a.i64(), d.lda = a.i64(), d.ldw = a.i64(), d.ldc = a.i64();
+  void* x = a.ptr();
+  const float* x_scales = a.ptr<float>();
+  void* w = a.ptr();
+  const float* w_scales = a.ptr<float>();
+  void *c = a.ptr(), *s = a.ptr();
+  return call<decltype(&tsm100_gemm_i8)>(a, kGemmI8, dev, &d, x, x_scales, w, w_scales, c, s);
+}
+
 #define TSM_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {TSM_METHOD(bind), TSM_METHOD(softmax), TSM_METHOD(rms_norm), TSM_METHOD(silu_mul), TSM_METHOD(gemm), TSM_METHOD(attention),
                            TSM_METHOD(rope), TSM_METHOD(kv_cache_update), TSM_METHOD(attention_prefill), TSM_METHOD(attention_decode),
-                           TSM_METHOD(add_rms_norm), TSM_METHOD(gemm_w4), TSM_METHOD(kv_page_append), TSM_METHOD(kv_page_read), TSM_METHOD(attention_paged),
+                           TSM_METHOD(add_rms_norm), TSM_METHOD(gemm_w4), TSM_METHOD(kv_page_append), TSM_METHOD(kv_page_read), TSM_METHOD(attention_paged), TSM_METHOD(quantise_rows), TSM_METHOD(gemm_i8),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_tile_sm100", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

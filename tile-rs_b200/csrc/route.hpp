@@ -107,6 +107,25 @@ inline Gemm16 gemm16(int64_t m, int64_t n, int64_t k, int64_t batch, int sms) {
   return r;
 }
 
+// 8-bit product (gemm_i8.cuh): 128 columns x `rows` rows of C per CTA, K over `splits` CTAs of a cluster.
+struct GemmI8 {
+  int rows;
+  int splits;
+  int64_t k_blocks_per_cta;  // 128 of K each
+};
+inline GemmI8 gemm_i8(int64_t m, int64_t n, int64_t k, int sms) {
+  GemmI8 r{m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, 1, 0};
+  const int64_t tiles = div_up(m, r.rows) * div_up(n, 128), kb = div_up(k, 128);
+  while (r.splits < kMaxGemmSplit) {
+    const int to = 2 * r.splits;
+    const int64_t room = to == 2 || kb >= 128 ? 2 * sms : to == 4 ? sms * 15 / 8 : sms * 8 / 5;
+    if (tiles * to > room || kb / to < 4) break;
+    r.splits = to;
+  }
+  r.k_blocks_per_cta = div_up(kb > 0 ? kb : 1, r.splits);
+  return r;
+}
+
 // CTA pairs: does C leave through shared memory, in whole boxes, or from the lanes that hold its rows?  The boxes are out in a sixth of the time, which
 // counts where a tile's products take no longer than its end (K below 2048) or where the last wave's end is a part of the whole; in a
 // long row of long tiles the board's power decides, and the slower way is 1 to 5 % cheaper.  Rows / boxes: 4096 x 4096 x 512 of a batch of 2 39.6 / 30.0 us, x

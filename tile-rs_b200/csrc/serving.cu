@@ -1,28 +1,10 @@
 // C-ABI operators around the intrinsics in a serving step: tsm100_add_rms_norm / _gemm_w4 / _kv_page_append / _kv_page_read / _attention_paged.
 #include "common.hpp"
+#include "on_device.hpp"
 #include "ops_serving.cuh"
 #include "ops_w4.cuh"
 
 using namespace tsm100;
-
-namespace {
-
-// Runs `op` with dev's CUDA device current; an exception (memory for a message) ends here.
-template <typename F>
-int32_t on_device(tsm100_device_t dev, F op) {
-  const int32_t st = use_device(dev);
-  if (st != TSM100_OK) return st;
-  try {
-    std::string err;
-    const int32_t r = op(&err);
-    if (r != TSM100_OK && !err.empty()) last_error_ref() = err;  // an operator called on the way has left its own
-    return r;
-  } catch (...) {
-    return TSM100_ERR_RUNTIME;
-  }
-}
-
-}  // namespace
 
 extern "C" {
 

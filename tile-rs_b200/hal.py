@@ -515,6 +515,25 @@ class CudaSm100Device:
         elif st:
             check(st)
 
+    def quantise_rows(self, dtype: int, rows: int, cols: int, x: int, y: int, scales: int, *, up: int = 0, pitch: int = 0, stream: int = 0) -> None:
+        """y[rows, cols] int8 and scales[rows] f32 of x, or with up of silu(x) * up; pitch elements from row to row of x and up (0: cols)."""
+        st = self._fast.quantise_rows(self._raw, dtype, rows, cols, pitch, x, up or 0, y, scales, stream)
+        if st is None:
+            d = capi.QuantiseRowsDesc(dtype, rows, cols, pitch)
+            check(capi.lib().tsm100_quantise_rows(self._h, C.byref(d), x, up or None, y, scales, stream or None))
+        elif st:
+            check(st)
+
+    def gemm_i8(self, dtype: int, m: int, n: int, k: int, a: int, a_scales: int, w: int, w_scales: int, c: int, *, lda: int = 0, ldw: int = 0,
+                ldc: int = 0, stream: int = 0) -> None:
+        """C[m, n] of type dtype = (a [m, k] times w [n, k], int8, exact sums) * a_scales[m] * w_scales[n]; pitches in elements, 0 = packed."""
+        st = self._fast.gemm_i8(self._raw, dtype, m, n, k, lda, ldw, ldc, a, a_scales, w, w_scales, c, stream)
+        if st is None:
+            d = capi.GemmI8Desc(dtype, m, n, k, lda, ldw, ldc)
+            check(capi.lib().tsm100_gemm_i8(self._h, C.byref(d), a, a_scales, w, w_scales, c, stream or None))
+        elif st:
+            check(st)
+
     def kv_page_append(self, kv: PagedKv, batch: PagedBatch, dtype: int, k: int, v: int, stream: int = 0) -> None:
         """Writes the call's tokens k, v [tokens, heads_kv, d] into their sequences' pages, quantised on the way if the cache holds 8 bits."""
         st = self._fast.kv_page_append(self._raw, kv.address, batch.address, dtype, k, v, stream)
