@@ -488,6 +488,26 @@ typedef struct {
 int32_t tsm100_attention_paged(tsm100_device_t dev, const tsm100_paged_kv* kv, const tsm100_paged_batch* batch,
                                const tsm100_attention_paged_desc* desc, const void* q, void* o, void* stream);
 
+/* Cross attention of the call's tokens over their sequences' pages: a token sees all lens[b] positions of its sequence (an encoder's states, say), however many
+ * tokens it has in the call, and where there are none o is zero.  As tsm100_attention_paged otherwise: a sequence with more positions than
+ * its row of the table has room for, or more than max_new tokens, is left out. */
+int32_t tsm100_attention_paged_cross(tsm100_device_t dev, const tsm100_paged_kv* kv, const tsm100_paged_batch* batch,
+                                     const tsm100_attention_paged_desc* desc, const void* q, void* o, void* stream);
+
+/* tsm100_attention_paged for sequences that begin with the same pages: their first prefix_len positions lie in pages prefix[0], prefix[1], ... (in device
+ * memory, prefix_len / page_size of them), which are read once for all, and of a row of the table only what comes behind them.  lens, and the places in a
+ * row, count from the sequence's beginning, so that one description serves this call and tsm100_kv_page_append.  The same result as
+ * tsm100_attention_paged on rows that begin with those pages, up to the rounding of f32 sums in another order.  A sequence with tokens whose new ones do not all
+ * lie behind the prefix is left out too. */
+typedef struct {
+  int32_t dtype; /* TSM100_F16 | TSM100_BF16 */
+  int32_t heads_q;
+  int32_t prefix_len; /* a multiple of page_size; 0: tsm100_attention_paged */
+  const int32_t* prefix;
+} tsm100_attention_paged_prefix_desc;
+int32_t tsm100_attention_paged_prefix(tsm100_device_t dev, const tsm100_paged_kv* kv, const tsm100_paged_batch* batch,
+                                      const tsm100_attention_paged_prefix_desc* desc, const void* q, void* o, void* stream);
+
 /* The path a tile_hal host program takes per kernel: alloc_from_slice ->
  * launch -> copy_to_host (crates/tile_hal/src/cuda.rs:348-371, :245-288,
  * :190-199), here chunked through page-locked staging so that copies in both

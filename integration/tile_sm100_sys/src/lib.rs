@@ -59,6 +59,8 @@ pub struct PagedBatch { pub batch: i32, pub tokens: i32, pub max_new: i32, pub m
 #[repr(C)] #[derive(Clone, Copy, Default)]
 pub struct AttentionPagedDesc { pub dtype: i32, pub heads_q: i32 }
 #[repr(C)] #[derive(Clone, Copy)]
+pub struct AttentionPagedPrefixDesc { pub dtype: i32, pub heads_q: i32, pub prefix_len: i32, pub prefix: *const i32 }
+#[repr(C)] #[derive(Clone, Copy)]
 pub struct QuantiseRowsDesc { pub dtype: i32, pub rows: i64, pub cols: i64, pub pitch: i64 }
 #[repr(C)] #[derive(Clone, Copy)]
 pub struct GemmI8Desc { pub dtype: i32, pub m: i64, pub n: i64, pub k: i64, pub lda: i64, pub ldw: i64, pub ldc: i64 }
@@ -133,6 +135,10 @@ extern "C" {
                                stream: RawStream) -> i32;
     pub fn tsm100_attention_paged(dev: Device, kv: *const PagedKv, batch: *const PagedBatch, d: *const AttentionPagedDesc, q: *const c_void,
                                   o: *mut c_void, stream: RawStream) -> i32;
+    pub fn tsm100_attention_paged_cross(dev: Device, kv: *const PagedKv, batch: *const PagedBatch, d: *const AttentionPagedDesc, q: *const c_void,
+                                        o: *mut c_void, stream: RawStream) -> i32;
+    pub fn tsm100_attention_paged_prefix(dev: Device, kv: *const PagedKv, batch: *const PagedBatch, d: *const AttentionPagedPrefixDesc,
+                                         q: *const c_void, o: *mut c_void, stream: RawStream) -> i32;
     // serving: rows and products in 8 bits
     pub fn tsm100_quantise_rows(dev: Device, d: *const QuantiseRowsDesc, x: *const c_void, up: *const c_void, y: *mut c_void, scales: *mut f32,
                                 stream: RawStream) -> i32;

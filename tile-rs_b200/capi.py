@@ -100,6 +100,10 @@ class AttentionPagedDesc(C.Structure):
     _fields_ = [("dtype", c_i32), ("heads_q", c_i32)]
 
 
+class AttentionPagedPrefixDesc(C.Structure):
+    _fields_ = [("dtype", c_i32), ("heads_q", c_i32), ("prefix_len", c_i32), ("prefix", c_vp)]
+
+
 OP_SOFTMAX, OP_GEMM, OP_ATTENTION = 0, 1, 2
 
 
@@ -166,6 +170,8 @@ PROTOTYPES = {
     "tsm100_kv_page_append": (c_i32, [c_vp, P(PagedKv), P(PagedBatch), c_i32, c_vp, c_vp, c_vp]),
     "tsm100_kv_page_read": (c_i32, [c_vp, P(PagedKv), P(PagedBatch), c_i32, c_vp, c_vp, c_vp]),
     "tsm100_attention_paged": (c_i32, [c_vp, P(PagedKv), P(PagedBatch), P(AttentionPagedDesc), c_vp, c_vp, c_vp]),
+    "tsm100_attention_paged_cross": (c_i32, [c_vp, P(PagedKv), P(PagedBatch), P(AttentionPagedDesc), c_vp, c_vp, c_vp]),
+    "tsm100_attention_paged_prefix": (c_i32, [c_vp, P(PagedKv), P(PagedBatch), P(AttentionPagedPrefixDesc), c_vp, c_vp, c_vp]),
     "tsm100_softmax_host": (c_i32, [c_vp, P(SoftmaxDesc), c_vp, c_vp]),
     "tsm100_gemm_host": (c_i32, [c_vp, P(GemmDesc), c_vp, c_vp, c_vp]),
     "tsm100_attention_host": (c_i32, [c_vp, P(AttentionDesc), c_vp, c_vp, c_vp, c_vp]),
@@ -213,7 +219,8 @@ class _ThroughCtypes:
 
 _FAST = None
 FAST_ENTRIES = ("softmax", "rms_norm", "silu_mul", "gemm", "attention", "rope", "kv_cache_update", "attention_prefill", "attention_decode",
-                "add_rms_norm", "gemm_w4", "kv_page_append", "kv_page_read", "attention_paged", "quantise_rows", "gemm_i8")
+                "add_rms_norm", "gemm_w4", "kv_page_append", "kv_page_read", "attention_paged", "quantise_rows", "gemm_i8",
+                "attention_paged_cross", "attention_paged_prefix")
 
 
 def fast():

@@ -27,6 +27,13 @@ namespace paged {
 
 namespace mma = attn_decode::mma;
 
+// Which keys a token sees, and what becomes of its result.
+//   kPast  positions 0 .. its own of its sequence; o
+//   kAll   all positions of its sequence, however many tokens that has (attention to an encoder's states; none: zeros); o, or records where p.records is not null.  With
+//          p.sequences not 0 all tokens of that many sequences are the ones of a single sequence, p.prefix positions of which they see (a prefix that they share)
+//   kRest  positions p.prefix .. its own; o, joined with the record of what it sees before them
+enum Keys { kPast, kAll, kRest };
+
 constexpr int kRows = 16;     // of a pass, at most
 constexpr int kMaxCtas = 1024;
 // What beginning and ending a pair costs, in tiles: shares are as long in tiles and these.  64 sequences of up to 6000 positions in 8 bits, costs of 4, 8, 12, 16, 24, 32 tiles:
@@ -52,6 +59,9 @@ struct Params {
   int32_t heads_q, group;
   int32_t run_log2;   // positions a copy brings: a power of two that divides the page (kTma), else the whole tile
   float scale_log2;   // log2(e) / sqrt(d)
+  int32_t prefix;     // Keys
+  int32_t sequences;
+  float* records;     // [tokens][heads_q][D + 4]: O and, behind it, the logarithm to base 2 of the sum of weights
   float* part;        // [CTA][2][kHeld][kRec]: of a pair that began in an earlier share, of one that goes on in the next
   int4* info;         // [CTA]: 1 if a pair of earlier shares ends in this one, 2 if it goes on; sequence and unit of the pair that goes on in the next, or -1
   uint32_t* status;
@@ -72,9 +82,46 @@ struct Part {
   int64_t start;         // where the unit begins
   bool there;
 };
-template <int kPos, int kHeld>
+// The tokens of sequence b and the keys that they see; false, and reported, if they contradict each other or the call.  kRest counts positions from the
+// prefix on, and so does its table.
+template <Keys kKeys, typename P>
+__device__ __forceinline__ bool sequence(const P& p, int b, int& first, int& count, int& len, uint32_t* status, uint32_t site) {
+  if constexpr (kKeys == kPast) {
+    return pages::sequence(p.step, p.cache.page_size, b, first, count, len, status, site);
+  } else if constexpr (kKeys == kAll) {
+    if (p.sequences > 0) {
+      first = 0, count = min(max(p.step.starts[p.sequences], 0), p.step.tokens), len = p.prefix;
+      return count > 0;
+    }
+    return pages::sequence<false>(p.step, p.cache.page_size, b, first, count, len, status, site) && len > 0;
+  } else {
+    if (!pages::sequence(p.step, p.cache.page_size, b, first, count, len, status, site)) return false;
+    len -= p.prefix;
+    if (len >= count) return true;
+    pages::report(status, site);
+    return false;
+  }
+}
+// Its tokens alone, of a sequence that is known to have some.
+template <Keys kKeys, typename P>
+__device__ __forceinline__ void tokens_of(const P& p, int b, int& first, int& count) {
+  if (kKeys == kAll && p.sequences > 0) {
+    first = 0, count = min(max(p.step.starts[p.sequences], 0), p.step.tokens);
+  } else {
+    first = p.step.starts[b], count = p.step.starts[b + 1] - first;
+  }
+}
+// Four numbers of a row's O, normalised, and the logarithm of its sum of weights.  A part whose scores are all -inf weighs nothing beside another.
+__device__ __forceinline__ float log_sum(float m_log2, float l) { return m_log2 == -INFINITY && l == 0.f ? -INFINITY : m_log2 + log2f(l); }
+__device__ __forceinline__ float2 join_weights(float a, float b) {  // of two parts, by their logarithms; the sum is 1.  Both -inf: NaN
+  const float m = fmaxf(a, b), wa = a == -INFINITY ? 0.f : exp2f(a - m), wb = b == -INFINITY ? 0.f : exp2f(b - m), inv = 1.f / (wa + wb);
+  return make_float2(wa * inv, wb * inv);
+}
+__device__ __forceinline__ float weighed(float w, float x) { return w == 0.f ? 0.f : w * x; }
+
+template <Keys kKeys, int kPos, int kHeld>
 __device__ __forceinline__ int64_t sequence_tiles(const Params& p, int b, Seq& s, uint32_t* status) {
-  if (!pages::sequence(p.step, p.cache.page_size, b, s.first, s.count, s.len, status, 143)) return 0;
+  if (!sequence<kKeys>(p, b, s.first, s.count, s.len, status, 143)) return 0;
   s.tiles = (s.len + kPos - 1) / kPos;
   s.passes = static_cast<int>((static_cast<int64_t>(s.count) * p.group + kHeld - 1) / kHeld);
   s.units = s.passes * p.cache.heads;
@@ -123,7 +170,45 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {  // an 8 x 8 tile o
   return r;
 }
 
-template <typename T, bool kI8, int D, bool kTma, bool kWide>
+// Four numbers of a row's result, not yet normalised, where they belong (Keys).  `m`: the logarithm of what its weights were taken against.
+template <typename T, int D, Keys kKeys>
+__device__ __forceinline__ void put(T* o, const Params& p, int64_t row, int at, float4 x, float m, float l) {
+  constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
+  if (kKeys == kAll && p.records) {
+    float* rec = p.records + row * (D + 4);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<float4*>(rec + at) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    if (at == 0) rec[D] = log_sum(m, l);
+    return;
+  }
+  const float inv = 1.f / l;
+  if constexpr (kKeys == kRest) {
+    const float* rec = p.records + row * (D + 4);
+    const float4 y = __ldcg(reinterpret_cast<const float4*>(rec + at));
+    const float2 w = join_weights(log_sum(m, l), __ldcg(rec + D));
+    const float f = w.x == 0.f ? 0.f : w.x * inv;
+    x.x = weighed(f, x.x) + weighed(w.y, y.x), x.y = weighed(f, x.y) + weighed(w.y, y.y), x.z = weighed(f, x.z) + weighed(w.y, y.z), x.w = weighed(f, x.w) + weighed(w.y, y.w);
+    *reinterpret_cast<uint2*>(o + row * D + at) = make_uint2(mma::pack2<kIsBf16>(x.x, x.y), mma::pack2<kIsBf16>(x.z, x.w));
+  } else {
+    *reinterpret_cast<uint2*>(o + row * D + at) = make_uint2(mma::pack2<kIsBf16>(x.x * inv, x.y * inv), mma::pack2<kIsBf16>(x.z * inv, x.w * inv));
+  }
+}
+// kAll: a sequence without positions has zeros for results.  Of all threads of a grid's first column.
+template <int D, Keys kKeys, typename T, typename P>
+__device__ __forceinline__ void put_zeros(T* o, const P& p) {
+  if constexpr (kKeys == kAll) {
+    if (blockIdx.y != 0 || p.sequences > 0) return;
+    for (int b = blockIdx.x; b < p.step.batch; b += gridDim.x) {
+      int first, count, len;
+      if (!pages::sequence<false>(p.step, p.cache.page_size, b, first, count, len, nullptr, 0) || len > 0) continue;
+      uint4* to = reinterpret_cast<uint4*>(o + static_cast<int64_t>(first) * p.heads_q * D);
+      const int64_t n = static_cast<int64_t>(count) * p.heads_q * (D / 8);
+      for (int64_t i = threadIdx.x; i < n; i += blockDim.x) to[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+}
+
+template <typename T, bool kI8, int D, bool kTma, bool kWide, Keys kKeys = kPast>
 __global__ void __launch_bounds__((Tile<kI8, D, kWide>::kThreads), 1)
 attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const T* __restrict__ q, T* __restrict__ o,
                        const __grid_constant__ Params p) {
@@ -177,7 +262,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   int64_t total = 0, before = 0, own = 0;
   for (int base = 0; base < batch; base += kThreads) {
     Seq s;
-    own = base + tid < batch ? sequence_tiles<TP, kHeld>(p, base + tid, s, p.status) : 0;
+    own = base + tid < batch ? sequence_tiles<kKeys, TP, kHeld>(p, base + tid, s, p.status) : 0;
     total += block_scan(own, before);
   }
   const int64_t per = (total + gridDim.x - 1) / gridDim.x;
@@ -189,7 +274,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       int64_t sum = 0;
       for (int base = 0; base < batch; base += kThreads) {
         Seq s;
-        own = base + tid < batch ? sequence_tiles<TP, kHeld>(p, base + tid, s, nullptr) : 0;
+        own = base + tid < batch ? sequence_tiles<kKeys, TP, kHeld>(p, base + tid, s, nullptr) : 0;
         const int64_t here = block_scan(own, before);
         if (sum + before <= t0 && t0 < sum + before + own) first_seq = base + tid, scan[kWarps] = sum + before;
         sum += here;
@@ -208,7 +293,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   };
   auto open = [&](Part& x, int b, int64_t base) {  // the first sequence from b on that has units
     for (; b < batch; ++b)
-      if (sequence_tiles<TP, kHeld>(p, b, x.seq, nullptr) > 0) break;
+      if (sequence_tiles<kKeys, TP, kHeld>(p, b, x.seq, nullptr) > 0) break;
     x.seq.b = b, x.seq.base = base;
     x.unit = 0, x.start = base;
   };
@@ -408,10 +493,10 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       for (int e = 0; e < 2; ++e) {
         q_factor[n][e] = __shfl_sync(0xffffffffu, factor, (2 * tq + e) * 4) * p.scale_log2;
         const int mine = row0 + min(n * 8 + 2 * tq + e, rows - 1);
-        limit[n][e] = seq.len - seq.count + mine / p.group;
+        limit[n][e] = kKeys == kAll ? seq.len - 1 : seq.len - seq.count + mine / p.group;
       }
     }
-    const int least = seq.len - seq.count + row0 / p.group;  // the first row's last position: tiles up to it need no masks
+    const int least = kKeys == kAll ? seq.len - 1 : seq.len - seq.count + row0 / p.group;  // the first row's last position: tiles up to it need no masks
     float oacc[KSTEPS][NB][4];
 #pragma unroll
     for (int c = 0; c < KSTEPS; ++c)
@@ -628,9 +713,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const int r = half * 8 + rr;
         if (whole) {
           const int token = (row0 + r) / p.group, h = head * p.group + (row0 + r) % p.group;
-          const float inv = 1.f / ll;
-          *reinterpret_cast<uint2*>(o + (static_cast<int64_t>(seq.first + token) * p.heads_q + h) * D + dd) =
-              make_uint2(mma::pack2<kIsBf16>(oo.x * inv, oo.y * inv), mma::pack2<kIsBf16>(oo.z * inv, oo.w * inv));
+          put<T, D, kKeys>(o, p, static_cast<int64_t>(seq.first + token) * p.heads_q + h, dd, oo, mm - kRaised<kMmaBf16>, ll);
         } else {
           float* out = p.part + ((static_cast<int64_t>(blockIdx.x) * 2 + (begin == 0 ? 1 : 0)) * kHeld + r) * REC;
           *reinterpret_cast<float4*>(out + dd) = oo;
@@ -667,17 +750,19 @@ __device__ __forceinline__ int records_of(const int4* info) {
 }
 
 // The records of a pair that several shares have a part of, in order; a warp per row, CTA (x, y) rows 4 y .. of the pair that goes on behind share x.
-template <typename T, int D, int kHeld>
+template <typename T, int D, int kHeld, bool kMmaBf16, Keys kKeys = kPast>
 __global__ void __launch_bounds__(128)
 attention_paged_merge_kernel(T* __restrict__ o, const __grid_constant__ Params p) {
   constexpr int REC = D + 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 4 + warp;
   ptx::launch_dependents();
   ptx::wait_prior_grid();
+  put_zeros<D, kKeys>(o, p);
   const int4 mine = __ldcg(p.info + blockIdx.x);
   if (mine.y < 0) return;
   const int n = records_of(p.info);
-  const int first = p.step.starts[mine.y], count = p.step.starts[mine.y + 1] - first;
+  int first, count;
+  tokens_of<kKeys>(p, mine.y, first, count);
   const int passes = static_cast<int>((static_cast<int64_t>(count) * p.group + kHeld - 1) / kHeld), head = mine.z / passes, row = mine.z % passes * kHeld + r;
   if (r >= kHeld || row >= count * p.group) return;
   auto record = [&](int i) { return p.part + ((static_cast<int64_t>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kHeld + r) * REC; };
@@ -706,12 +791,8 @@ attention_paged_merge_kernel(T* __restrict__ o, const __grid_constant__ Params p
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
-  if (lane < D / 4) {
-    const float inv = 1.f / ll;
-    constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
-    *reinterpret_cast<uint2*>(o + (static_cast<int64_t>(first + row / p.group) * p.heads_q + head * p.group + row % p.group) * D + lane * 4) =
-        make_uint2(mma::pack2<kIsBf16>(oo.x * inv, oo.y * inv), mma::pack2<kIsBf16>(oo.z * inv, oo.w * inv));
-  }
+  if (lane < D / 4)
+    put<T, D, kKeys>(o, p, static_cast<int64_t>(first + row / p.group) * p.heads_q + head * p.group + row % p.group, lane * 4, oo, mm - kRaised<kMmaBf16>, ll);
 }
 
 }  // namespace paged

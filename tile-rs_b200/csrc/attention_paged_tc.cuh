@@ -92,6 +92,9 @@ struct Params {
   int32_t tokens;      // of a tile: 128 / group
   int32_t run_log2;    // positions of a page's box
   float scale_log2;
+  int32_t prefix;      // attention_paged.cuh: Keys
+  int32_t sequences;
+  float* records;
   float4* part;        // [CTA][2][D / 4][256 rows]: of a block that began in an earlier share, of one that goes on in the next
   float2* part_ml;     // [CTA][2][256]
   int4* info;          // [CTA]: as attention_paged.cuh, with the block's sequence, KV head and number
@@ -103,23 +106,27 @@ struct Seq {
   int b, first, count, len, blocks;
   int64_t per_head, base, end;
 };
+template <Keys kKeysSeen>
 __device__ __forceinline__ int64_t full_blocks(const Params& p, const Seq& s, int64_t i) {  // the length of the first i blocks, which have two tiles
+  if (kKeysSeen == kAll) return i * (s.len + kBlockCost);
   const int64_t two = 2 * p.tokens;
   return i * (s.len - s.count + kBlockCost) + two * (i * (i + 1) / 2);
 }
+template <Keys kKeysSeen>
 __device__ __forceinline__ int64_t sequence_length(const Params& p, int b, Seq& s, uint32_t* status) {
-  if (!pages::sequence(p.step, p.cache.page_size, b, s.first, s.count, s.len, status, 145)) return 0;
+  if (!sequence<kKeysSeen>(p, b, s.first, s.count, s.len, status, 145)) return 0;
   s.blocks = (s.count + 2 * p.tokens - 1) / (2 * p.tokens);
-  s.per_head = full_blocks(p, s, s.blocks - 1) + s.len + kBlockCost;
+  s.per_head = full_blocks<kKeysSeen>(p, s, s.blocks - 1) + s.len + kBlockCost;
   return s.per_head * p.cache.heads;
 }
+template <Keys kKeysSeen>
 struct Stream {
   Seq seq;
   int64_t at, end;
   __device__ __forceinline__ void open(const Params& p, int b, int64_t base) {  // the first sequence from b on that has blocks
     int64_t n = 0;
     for (; b < p.step.batch; ++b)
-      if ((n = sequence_length(p, b, seq, nullptr)) > 0) break;
+      if ((n = sequence_length<kKeysSeen>(p, b, seq, nullptr)) > 0) break;
     seq.b = b, seq.base = base, seq.end = base + n;
   }
   __device__ __forceinline__ bool next(const Params& p, Work& w) {
@@ -132,13 +139,13 @@ struct Stream {
       int lo = 0, hi = seq.blocks - 1;  // the last block that begins at in_head or before
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (full_blocks(p, seq, mid) <= in_head) lo = mid;
+        if (full_blocks<kKeysSeen>(p, seq, mid) <= in_head) lo = mid;
         else hi = mid - 1;
       }
       const bool last = lo == seq.blocks - 1;
-      const int64_t from = full_blocks(p, seq, lo), to = last ? seq.per_head : full_blocks(p, seq, lo + 1);
+      const int64_t from = full_blocks<kKeysSeen>(p, seq, lo), to = last ? seq.per_head : full_blocks<kKeysSeen>(p, seq, lo + 1);
       w.token0 = lo * 2 * p.tokens;
-      const int keys = seq.len - seq.count + min(seq.count, w.token0 + 2 * p.tokens);
+      const int keys = kKeysSeen == kAll ? seq.len : seq.len - seq.count + min(seq.count, w.token0 + 2 * p.tokens);
       w.steps = (keys + kKeys - 1) / kKeys;
       const int64_t stop = min(to, in_head + (end - at));
       auto steps_to = [&](int64_t x) { return static_cast<int>((static_cast<uint32_t>(max(x - from - kBlockCost, static_cast<int64_t>(0))) + kKeys - 1) / kKeys); };
@@ -146,7 +153,7 @@ struct Stream {
       w.n = steps_to(stop) - w.begin;
       w.b = seq.b, w.first = seq.first, w.count = seq.count, w.len = seq.len, w.block = lo;
       w.lone = last && seq.count - w.token0 <= p.tokens;
-      const int keys_a = seq.len - seq.count + min(seq.count, w.token0 + p.tokens);
+      const int keys_a = kKeysSeen == kAll ? seq.len : seq.len - seq.count + min(seq.count, w.token0 + p.tokens);
       w.n_a = max(0, min(w.n, (keys_a + kKeys - 1) / kKeys - w.begin));
       at += stop - in_head;
       if (w.n > 0) return true;
@@ -155,7 +162,7 @@ struct Stream {
   }
 };
 
-template <bool kIsBf16, bool kI8, int D>
+template <bool kIsBf16, bool kI8, int D, Keys kKeysSeen = kPast>
 __global__ void __launch_bounds__(Shape<kI8, D>::kThreads, 1)
 attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                           uint16_t* __restrict__ o, const __grid_constant__ Params p) {
@@ -211,7 +218,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
   ptx::wait_prior_grid();
 
   // The stream: how long it is, and where this CTA's share begins.
-  Stream stream;
+  Stream<kKeysSeen> stream;
   {
     constexpr int kThreads = S::kThreads;
     const int batch = p.step.batch;
@@ -235,12 +242,12 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
     };
     int64_t total = 0, before = 0;
     Seq s;
-    for (int base = 0; base < batch; base += kThreads) total += block_scan(base + tid < batch ? sequence_length(p, base + tid, s, p.status) : 0, before);
+    for (int base = 0; base < batch; base += kThreads) total += block_scan(base + tid < batch ? sequence_length<kKeysSeen>(p, base + tid, s, p.status) : 0, before);
     const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kMinShare));
     stream.at = min(total, blockIdx.x * per), stream.end = min(total, stream.at + per);
     int64_t sum = 0;
     for (int base = 0; base < batch; base += kThreads) {
-      const int64_t own = base + tid < batch ? sequence_length(p, base + tid, s, nullptr) : 0;
+      const int64_t own = base + tid < batch ? sequence_length<kKeysSeen>(p, base + tid, s, nullptr) : 0;
       const int64_t here = block_scan(own, before);
       if (sum + before <= stream.at && stream.at < sum + before + own) bars->first_seq = base + tid, bars->first_base = sum + before;
       sum += here;
@@ -561,7 +568,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       const int token = w.token0 + g * p.tokens + r_token;
       const bool row_ok = r_token < p.tokens && token < w.count;
       const bool idle = __all_sync(0xffffffffu, !row_ok);           // no row of this warp exists
-      const int limit = w.len - w.count + min(token, w.count - 1);  // last visible position
+      const int limit = kKeysSeen == kAll ? w.len - 1 : w.len - w.count + min(token, w.count - 1);  // last visible position
       float m_used = -INFINITY, l = 0.f;
       int v_used = 0;  // probabilities and their sum are 2^-v_used of what they were
       for (int j = 0; j < n_g; ++j) {
@@ -724,7 +731,16 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       if (!idle) {
         const int64_t rec = static_cast<int64_t>(blockIdx.x) * 2 + (w.begin == 0 ? 1 : 0);
         const float inv = m_used == -INFINITY ? NAN : 1.0f / l;  // all scores -inf (or NaN): softmax is NaN there
-        uint16_t* orow = o + (static_cast<int64_t>(w.first + token) * p.heads_q + w.head * p.group + r_head) * D;
+        const int64_t row = static_cast<int64_t>(w.first + token) * p.heads_q + w.head * p.group + r_head;
+        uint16_t* orow = o + row * D;
+        [[maybe_unused]] float lse = 0.f, f_own = 0.f;
+        [[maybe_unused]] float2 joined = make_float2(0.f, 0.f);
+        if constexpr (kKeysSeen != kPast) {
+          if (whole && row_ok) {
+            lse = log_sum(m_used * sl2 + static_cast<float>(v_used) - kRaised<kI8, kPvBf16>, l);
+            if (kKeysSeen == kRest) joined = join_weights(lse, __ldcg(p.records + row * (D + 4) + D)), f_own = joined.x == 0.f ? 0.f : joined.x / l;
+          }
+        }
 #pragma unroll 1
         for (int q = 0; q < D / 32; ++q) {
           uint32_t ov[32];
@@ -736,7 +752,27 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
             for (int i = 0; i < 32; ++i) ov[i] = 0u;
           }
           if (whole) {
-            if (row_ok) {
+            if (row_ok && kKeysSeen == kAll && p.records) {
+              float* rec = p.records + row * (D + 4) + q * 32;
+              const float f = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+              for (int t = 0; t < 8; ++t)
+                reinterpret_cast<float4*>(rec)[t] = make_float4(__uint_as_float(ov[4 * t]) * f, __uint_as_float(ov[4 * t + 1]) * f, __uint_as_float(ov[4 * t + 2]) * f,
+                                                                __uint_as_float(ov[4 * t + 3]) * f);
+            } else if (row_ok) {
+              if constexpr (kKeysSeen == kRest) {
+                const float4* rec = reinterpret_cast<const float4*>(p.records + row * (D + 4) + q * 32);
+#pragma unroll
+                for (int t = 0; t < 8; ++t) {
+                  const float4 y = __ldcg(rec + t);
+                  const float prior[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    ov[4 * t + e] = __float_as_uint(weighed(f_own, __uint_as_float(ov[4 * t + e])) + weighed(joined.y, prior[e]));
+                }
+              }
+              [[maybe_unused]] const float inv_own = inv;
+              const float inv = kKeysSeen == kRest ? 1.f : inv_own;
 #pragma unroll
               for (int t = 0; t < 4; ++t) {
                 uint4 x;
@@ -754,6 +790,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
               part[i * 256] = make_float4(__uint_as_float(ov[4 * i]), __uint_as_float(ov[4 * i + 1]), __uint_as_float(ov[4 * i + 2]), __uint_as_float(ov[4 * i + 3]));
           }
         }
+        if (kKeysSeen == kAll && whole && row_ok && p.records) p.records[row * (D + 4) + D] = lse;
         if (!whole) p.part_ml[rec * 256 + g * kTileRows + r] = make_float2(n_g > 0 ? m_used + static_cast<float>(v_used) / sl2 : -INFINITY, n_g > 0 ? l : 0.f);
       }
       if (n_g > 0) {
@@ -781,15 +818,17 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
 }
 
 // The records of a block that several shares have a part of, in order: CTA (x, y) has the block that goes on behind share x and 16 of its columns, a thread a row.
-template <bool kIsBf16, int D>
+template <bool kIsBf16, bool kI8, int D, Keys kKeysSeen = kPast>
 __global__ void __launch_bounds__(256)
 attention_paged_tc_merge_kernel(uint16_t* __restrict__ o, const __grid_constant__ Params p) {
   ptx::launch_dependents();
   ptx::wait_prior_grid();
+  put_zeros<D, kKeysSeen>(o, p);
   const int4 mine = __ldcg(p.info + blockIdx.x);
   if (mine.y < 0) return;
   const int n = records_of(p.info);
-  const int first = p.step.starts[mine.y], count = p.step.starts[mine.y + 1] - first;
+  int first, count;
+  tokens_of<kKeysSeen>(p, mine.y, first, count);
   const int g = threadIdx.x >> 7, r = threadIdx.x & 127, r_token = r / p.group;
   const int token = (mine.w * 2 + g) * p.tokens + r_token;
   if (r_token >= p.tokens || token >= count) return;
@@ -813,8 +852,31 @@ attention_paged_tc_merge_kernel(uint16_t* __restrict__ o, const __grid_constant_
       acc[4 * q + 2] = fmaf(f, x.z, acc[4 * q + 2]), acc[4 * q + 3] = fmaf(f, x.w, acc[4 * q + 3]);
     }
   }
-  const float inv = 1.0f / gl;
-  uint16_t* orow = o + (static_cast<int64_t>(first + token) * p.heads_q + mine.z * p.group + (r - r_token * p.group)) * D + blockIdx.y * 16;
+  const int64_t row = static_cast<int64_t>(first + token) * p.heads_q + mine.z * p.group + (r - r_token * p.group);
+  [[maybe_unused]] const float lse = kKeysSeen == kPast ? 0.f : log_sum(gm * p.scale_log2 - kRaised<kI8, kIsBf16 && !kI8>, gl);
+  if (kKeysSeen == kAll && p.records) {
+    float* rec = p.records + row * (D + 4);
+    const float f = gl == 0.f ? 0.f : 1.f / gl;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(rec)[blockIdx.y * 4 + i] = make_float4(acc[4 * i] * f, acc[4 * i + 1] * f, acc[4 * i + 2] * f, acc[4 * i + 3] * f);
+    if (blockIdx.y == 0) rec[D] = lse;
+    return;
+  }
+  float inv = 1.0f / gl;
+  if constexpr (kKeysSeen == kRest) {
+    const float* rec = p.records + row * (D + 4);
+    const float2 w = join_weights(lse, __ldcg(rec + D));
+    const float f = w.x == 0.f ? 0.f : w.x * inv;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(rec) + blockIdx.y * 4 + i);
+      const float prior[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[4 * i + e] = weighed(f, acc[4 * i + e]) + weighed(w.y, prior[e]);
+    }
+    inv = 1.f;
+  }
+  uint16_t* orow = o + row * D + blockIdx.y * 16;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint4 x;

@@ -31,13 +31,14 @@ __device__ __forceinline__ void report(uint32_t* status, uint32_t site) {
   if (status) atomicCAS(status, 0u, kStatusOutside | site);
 }
 
-// The tokens and positions of sequence b; false, and reported, if they contradict each other or the call.
+// The tokens and positions of sequence b; false, and reported, if they contradict each other or the call.  kOwn: its tokens are the last of its positions.
+template <bool kOwn = true>
 __device__ __forceinline__ bool sequence(const Batch& s, int64_t page_size, int b, int& first, int& count, int& len, uint32_t* status, uint32_t site) {
   first = s.starts[b];
   count = s.starts[b + 1] - first;
   len = s.lens[b];
   if (count == 0) return false;
-  if (first < 0 || count < 0 || count > s.max_new || first > s.tokens - count || len < count || len > page_size * s.pitch) {
+  if (first < 0 || count < 0 || count > s.max_new || first > s.tokens - count || len < (kOwn ? count : 0) || len > page_size * s.pitch) {
     report(status, site);
     return false;
   }

@@ -174,7 +174,7 @@ inline int32_t page_tmap(std::string* err, CUtensorMap* map, const pages::Cache&
 }
 
 // Chunks of tokens: tcgen05 (attention_paged_tc.cuh).
-template <typename T, bool kI8, int D>
+template <typename T, bool kI8, int D, paged::Keys kKeys>
 inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& base, int run_log2, const void* q, void* o, cudaStream_t s) {
   namespace tc = paged::tc;
   constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
@@ -190,6 +190,7 @@ inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& 
   p.run_log2 = run_log2;
   p.scale_log2 = base.scale_log2;
   p.status = base.status;
+  p.prefix = base.prefix, p.sequences = base.sequences, p.records = base.records;
   CUtensorMap tq, tk, tv;
   TmapKey key;
   std::memset(&key, 0, sizeof key);
@@ -214,11 +215,11 @@ inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& 
   p.part = reinterpret_cast<float4*>(ws);
   p.part_ml = reinterpret_cast<float2*>(ws + part);
   p.info = reinterpret_cast<int4*>(ws + part + ml);
-  auto kern = tc::attention_paged_tc_kernel<kIsBf16, kI8, D>;
+  auto kern = tc::attention_paged_tc_kernel<kIsBf16, kI8, D, kKeys>;
   constexpr int smem = tc::smem_bytes<kI8, D>();
   cudaError_t e = set_dyn_smem_once(kern, smem);
   if (e == cudaSuccess) e = launch_chained(kern, ctas, S::kThreads, smem, s, 0, tq, tk, tv, static_cast<uint16_t*>(o), p);
-  if (e == cudaSuccess) e = launch_chained(tc::attention_paged_tc_merge_kernel<kIsBf16, D>, dim3(ctas, D / 16), 256, 0, s, 0, static_cast<uint16_t*>(o), p);
+  if (e == cudaSuccess) e = launch_chained(tc::attention_paged_tc_merge_kernel<kIsBf16, kI8, D, kKeys>, dim3(ctas, D / 16), 256, 0, s, 0, static_cast<uint16_t*>(o), p);
   st = cuda_ok(err, e, "attention_paged_tc_kernel launch");
   e = cudaFreeAsync(ws, s);
   if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
@@ -226,7 +227,7 @@ inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& 
 }
 
 // The tiles of all sequences' caches dealt out evenly over the SMs, and what several of them have a part of merged (attention_paged.cuh).
-template <typename T, bool kI8, int D, bool kWide>
+template <typename T, bool kI8, int D, bool kWide, paged::Keys kKeys>
 inline int32_t attention_paged_few_launch(std::string* err, paged::Params p, const void* q, void* o, cudaStream_t s) {
   using L = paged::Tile<kI8, D, kWide>;
   int sms = 0;
@@ -266,10 +267,10 @@ inline int32_t attention_paged_few_launch(std::string* err, paged::Params p, con
     st = make_tmap(err, &map[i], key, kI8 ? 1 : 2);
   }
   if (st == TSM100_OK) {
-    auto kern = boxes ? paged::attention_paged_kernel<T, kI8, D, true, kWide> : paged::attention_paged_kernel<T, kI8, D, false, kWide>;
+    auto kern = boxes ? paged::attention_paged_kernel<T, kI8, D, true, kWide, kKeys> : paged::attention_paged_kernel<T, kI8, D, false, kWide, kKeys>;
     cudaError_t e = set_dyn_smem_once(kern, L::kSmem);
     if (e == cudaSuccess) e = launch_chained(kern, ctas, L::kThreads, L::kSmem, s, 0, map[0], map[1], static_cast<const T*>(q), static_cast<T*>(o), p);
-    if (e == cudaSuccess) e = launch_chained(paged::attention_paged_merge_kernel<T, D, L::kHeld>, dim3(ctas, static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, 0, static_cast<T*>(o), p);
+    if (e == cudaSuccess) e = launch_chained(paged::attention_paged_merge_kernel<T, D, L::kHeld, !std::is_same<T, __half>::value && !kI8, kKeys>, dim3(ctas, static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, 0, static_cast<T*>(o), p);
     st = cuda_ok(err, e, "attention_paged_kernel launch");
   }
   const cudaError_t e = cudaFreeAsync(p.part, s);
@@ -278,18 +279,46 @@ inline int32_t attention_paged_few_launch(std::string* err, paged::Params p, con
 }
 
 // More rows than a tile of mma.sync has would go over their keys again: those take tcgen05, as long as a group's heads fit a tile and boxes of eight positions a page.
-template <typename T, bool kI8, int D>
+template <typename T, bool kI8, int D, paged::Keys kKeys>
 inline int32_t attention_paged_launch(std::string* err, const paged::Params& p, const void* q, void* o, cudaStream_t s) {
   const int64_t rows = static_cast<int64_t>(p.step.max_new) * p.group;
   const int wide = page_run_log2(p.cache.page_size, 7);
-  if (rows > paged::kRows && p.group <= paged::tc::kMaxGroup && (kI8 || wide >= 3)) return attention_paged_tc_launch<T, kI8, D>(err, p, wide, q, o, s);
-  return rows > 8 ? attention_paged_few_launch<T, kI8, D, true>(err, p, q, o, s) : attention_paged_few_launch<T, kI8, D, false>(err, p, q, o, s);
+  if (rows > paged::kRows && p.group <= paged::tc::kMaxGroup && (kI8 || wide >= 3)) return attention_paged_tc_launch<T, kI8, D, kKeys>(err, p, wide, q, o, s);
+  return rows > 8 ? attention_paged_few_launch<T, kI8, D, true, kKeys>(err, p, q, o, s) : attention_paged_few_launch<T, kI8, D, false, kKeys>(err, p, q, o, s);
 }
 
-template <typename T>
+template <typename T, paged::Keys kKeys>
 inline int32_t attention_paged_typed(std::string* err, const paged::Params& p, bool i8, const void* q, void* o, cudaStream_t s) {
-  if (p.cache.d == 128) return i8 ? attention_paged_launch<T, true, 128>(err, p, q, o, s) : attention_paged_launch<T, false, 128>(err, p, q, o, s);
-  return i8 ? attention_paged_launch<T, true, 64>(err, p, q, o, s) : attention_paged_launch<T, false, 64>(err, p, q, o, s);
+  if (p.cache.d == 128) return i8 ? attention_paged_launch<T, true, 128, kKeys>(err, p, q, o, s) : attention_paged_launch<T, false, 128, kKeys>(err, p, q, o, s);
+  return i8 ? attention_paged_launch<T, true, 64, kKeys>(err, p, q, o, s) : attention_paged_launch<T, false, 64, kKeys>(err, p, q, o, s);
+}
+// One translation unit for each kind of keys (serving.cu, serving_cross.cu, serving_prefix.cu).
+template <paged::Keys kKeys>
+int32_t attention_paged_keys(std::string* err, const paged::Params& p, bool bf16, bool i8, const void* q, void* o, cudaStream_t s) {
+  return bf16 ? attention_paged_typed<__nv_bfloat16, kKeys>(err, p, i8, q, o, s) : attention_paged_typed<__half, kKeys>(err, p, i8, q, o, s);
+}
+extern template int32_t attention_paged_keys<paged::kPast>(std::string*, const paged::Params&, bool, bool, const void*, void*, cudaStream_t);
+extern template int32_t attention_paged_keys<paged::kAll>(std::string*, const paged::Params&, bool, bool, const void*, void*, cudaStream_t);
+extern template int32_t attention_paged_keys<paged::kRest>(std::string*, const paged::Params&, bool, bool, const void*, void*, cudaStream_t);
+
+// What the attentions over pages ask of their arguments.  *nothing: there are no tokens.
+inline int32_t attention_paged_args(std::string* err, const char* op, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, int32_t dtype, int32_t heads_q, const void* q,
+                                    const void* o, uint32_t* status, paged::Params* p, bool* nothing) {
+  auto no = [&](const char* what) { return op_fail(err, TSM100_ERR_INVALID, std::string(op) + ": " + what); };
+  const int32_t st = paged_args(err, op, kv, b, dtype, &p->cache, &p->step, nothing);
+  if (st != TSM100_OK) return st;
+  if (kv->head_dim != 64 && kv->head_dim != 128) return no("head_dim must be 64 or 128");
+  if (heads_q <= 0 || heads_q % kv->heads_kv != 0) return no("heads_q must be a positive multiple of heads_kv");
+  if (*nothing) return TSM100_OK;
+  if (!q || !o) return no("null buffer");
+  if (!aligned16(q) || !aligned16(o)) return no("q and o must be 16-byte aligned");
+  if (static_cast<int64_t>(b->tokens) * heads_q > 0x7fffffff) return no("too many tokens times heads");
+  p->heads_q = heads_q;
+  p->group = heads_q / kv->heads_kv;
+  p->scale_log2 = static_cast<float>((1.0 / std::sqrt(static_cast<double>(kv->head_dim))) * 1.4426950408889634);
+  p->prefix = 0, p->sequences = 0, p->records = nullptr;
+  p->status = status;
+  return TSM100_OK;
 }
 
 inline int32_t attention_paged(std::string* err, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, const tsm100_attention_paged_desc* d, const void* q,
@@ -297,22 +326,57 @@ inline int32_t attention_paged(std::string* err, const tsm100_paged_kv* kv, cons
   if (!d) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: null descriptor");
   paged::Params p;
   bool nothing;
-  const int32_t st = paged_args(err, "attention_paged", kv, b, d->dtype, &p.cache, &p.step, &nothing);
+  const int32_t st = attention_paged_args(err, "attention_paged", kv, b, d->dtype, d->heads_q, q, o, status, &p, &nothing);
+  if (st != TSM100_OK || nothing) return st;
+  return attention_paged_keys<paged::kPast>(err, p, d->dtype == TSM100_BF16, kv->dtype == TSM100_I8, q, o, static_cast<cudaStream_t>(stream));
+}
+
+// Every token against all positions of its sequence.
+inline int32_t attention_paged_cross(std::string* err, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, const tsm100_attention_paged_desc* d, const void* q,
+                                     void* o, uint32_t* status, void* stream) {
+  if (!d) return op_fail(err, TSM100_ERR_INVALID, "attention_paged_cross: null descriptor");
+  paged::Params p;
+  bool nothing;
+  const int32_t st = attention_paged_args(err, "attention_paged_cross", kv, b, d->dtype, d->heads_q, q, o, status, &p, &nothing);
+  if (st != TSM100_OK || nothing) return st;
+  return attention_paged_keys<paged::kAll>(err, p, d->dtype == TSM100_BF16, kv->dtype == TSM100_I8, q, o, static_cast<cudaStream_t>(stream));
+}
+
+// All tokens against the prefix, once, as records; then each against its own positions, joined with its record.
+inline int32_t attention_paged_prefix(std::string* err, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, const tsm100_attention_paged_prefix_desc* d, const void* q,
+                                      void* o, uint32_t* status, void* stream) {
+  auto no = [&](const char* what) { return op_fail(err, TSM100_ERR_INVALID, std::string("attention_paged_prefix: ") + what); };
+  if (!d) return no("null descriptor");
+  paged::Params p;
+  bool nothing;
+  int32_t st = attention_paged_args(err, "attention_paged_prefix", kv, b, d->dtype, d->heads_q, q, o, status, &p, &nothing);
   if (st != TSM100_OK) return st;
-  if (kv->head_dim != 64 && kv->head_dim != 128) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: head_dim must be 64 or 128");
-  if (d->heads_q <= 0 || d->heads_q % kv->heads_kv != 0)
-    return op_fail(err, TSM100_ERR_INVALID, "attention_paged: heads_q must be a positive multiple of heads_kv");
+  if (d->prefix_len < 0 || d->prefix_len % kv->page_size != 0) return no("prefix_len must be a multiple of page_size");
+  if (d->prefix_len > static_cast<int64_t>(b->table_pitch) * kv->page_size) return no("prefix_len is more than a row of the table covers");
   if (nothing) return TSM100_OK;
-  if (!q || !o) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: null buffer");
-  if (!aligned16(q) || !aligned16(o)) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: q and o must be 16-byte aligned");
-  if (static_cast<int64_t>(b->tokens) * d->heads_q > 0x7fffffff) return op_fail(err, TSM100_ERR_INVALID, "attention_paged: too many tokens times heads");
-  p.heads_q = d->heads_q;
-  p.group = d->heads_q / kv->heads_kv;
-  p.scale_log2 = static_cast<float>((1.0 / std::sqrt(static_cast<double>(kv->head_dim))) * 1.4426950408889634);
-  p.status = status;
+  if (d->prefix_len > 0 && !d->prefix) return no("null prefix");
+  if (reinterpret_cast<uintptr_t>(d->prefix) & 3u) return no("prefix does not start on an element boundary");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool i8 = kv->dtype == TSM100_I8;
-  return d->dtype == TSM100_BF16 ? attention_paged_typed<__nv_bfloat16>(err, p, i8, q, o, s) : attention_paged_typed<__half>(err, p, i8, q, o, s);
+  const bool bf16 = d->dtype == TSM100_BF16, i8 = kv->dtype == TSM100_I8;
+  if (d->prefix_len == 0) return attention_paged_keys<paged::kPast>(err, p, bf16, i8, q, o, s);
+  void* records = nullptr;
+  st = take_scratch(err, &records, static_cast<size_t>(b->tokens) * d->heads_q * (kv->head_dim + 4) * sizeof(float), s);
+  if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged_prefix: no device memory for partial results");
+  if (st != TSM100_OK) return st;
+  p.records = static_cast<float*>(records);
+  p.prefix = d->prefix_len;
+  paged::Params shared = p;
+  shared.sequences = b->batch;
+  shared.step.batch = 1, shared.step.max_new = b->tokens;
+  shared.step.table = d->prefix, shared.step.pitch = d->prefix_len / kv->page_size;
+  st = attention_paged_keys<paged::kAll>(err, shared, bf16, i8, q, o, s);
+  if (st == TSM100_OK) {
+    p.step.table += d->prefix_len / kv->page_size;
+    st = attention_paged_keys<paged::kRest>(err, p, bf16, i8, q, o, s);
+  }
+  const cudaError_t e = cudaFreeAsync(records, s);
+  if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
+  return st;
 }
 
 }  // namespace ops

@@ -13,7 +13,8 @@
 
 namespace {
 
-enum Entry { kSoftmax, kRmsNorm, kSiluMul, kGemm, kAttention, kRope, kKvCacheUpdate, kPrefill, kDecode, kAddRmsNorm, kGemmW4, kPageAppend, kPageRead, kPaged, kQuantiseRows, kGemmI8, kEntries };
+enum Entry { kSoftmax, kRmsNorm, kSiluMul, kGemm, kAttention, kRope, kKvCacheUpdate, kPrefill, kDecode, kAddRmsNorm, kGemmW4, kPageAppend, kPageRead, kPaged, kQuantiseRows, kGemmI8,
+             kPagedCross, kPagedPrefix, kEntries };
 void* g_entry[kEntries] = {};
 
 // Walks through the arguments; `ok` turns false at the first that does not fit.
@@ -248,10 +249,34 @@ PyObject* gemm_i8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return call<decltype(&tsm100_gemm_i8)>(a, kGemmI8, dev, &d, x, x_scales, w, w_scales, c, s);
 }
 
+// (device, cache, batch, dtype, heads_q, q, o, stream)
+PyObject* attention_paged_cross(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 8, kPagedCross);
+  auto* dev = a.ptr<tsm100_device_s>();
+  auto* kv = a.ptr<tsm100_paged_kv>();
+  auto* batch = a.ptr<tsm100_paged_batch>();
+  tsm100_attention_paged_desc d = {};
+  d.dtype = a.i32(), d.heads_q = a.i32();
+  void *q = a.ptr(), *o = a.ptr(), *s = a.ptr();
+  return call<decltype(&tsm100_attention_paged_cross)>(a, kPagedCross, dev, kv, batch, &d, q, o, s);
+}
+// (device, cache, batch, dtype, heads_q, prefix_len, prefix, q, o, stream)
+PyObject* attention_paged_prefix(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Args a(args, n, 10, kPagedPrefix);
+  auto* dev = a.ptr<tsm100_device_s>();
+  auto* kv = a.ptr<tsm100_paged_kv>();
+  auto* batch = a.ptr<tsm100_paged_batch>();
+  tsm100_attention_paged_prefix_desc d = {};
+  d.dtype = a.i32(), d.heads_q = a.i32(), d.prefix_len = a.i32(), d.prefix = a.ptr<int32_t>();
+  void *q = a.ptr(), *o = a.ptr(), *s = a.ptr();
+  return call<decltype(&tsm100_attention_paged_prefix)>(a, kPagedPrefix, dev, kv, batch, &d, q, o, s);
+}
+
 #define TSM_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {TSM_METHOD(bind), TSM_METHOD(softmax), TSM_METHOD(rms_norm), TSM_METHOD(silu_mul), TSM_METHOD(gemm), TSM_METHOD(attention),
                            TSM_METHOD(rope), TSM_METHOD(kv_cache_update), TSM_METHOD(attention_prefill), TSM_METHOD(attention_decode),
                            TSM_METHOD(add_rms_norm), TSM_METHOD(gemm_w4), TSM_METHOD(kv_page_append), TSM_METHOD(kv_page_read), TSM_METHOD(attention_paged), TSM_METHOD(quantise_rows), TSM_METHOD(gemm_i8),
+                           TSM_METHOD(attention_paged_cross), TSM_METHOD(attention_paged_prefix),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_tile_sm100", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

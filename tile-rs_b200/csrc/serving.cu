@@ -1,10 +1,13 @@
-// C-ABI operators around the intrinsics in a serving step: tsm100_add_rms_norm / _gemm_w4 / _kv_page_append / _kv_page_read / _attention_paged.
+// C-ABI operators around the intrinsics in a serving step: tsm100_add_rms_norm / _gemm_w4 / _kv_page_append / _kv_page_read / _attention_paged /
+// _attention_paged_cross / _attention_paged_prefix.
 #include "common.hpp"
 #include "on_device.hpp"
 #include "ops_serving.cuh"
 #include "ops_w4.cuh"
 
 using namespace tsm100;
+
+template int32_t tsm100::ops::attention_paged_keys<paged::kPast>(std::string*, const paged::Params&, bool, bool, const void*, void*, cudaStream_t);
 
 extern "C" {
 
@@ -35,6 +38,16 @@ int32_t tsm100_kv_page_read(tsm100_device_t dev, const tsm100_paged_kv* kv, cons
 int32_t tsm100_attention_paged(tsm100_device_t dev, const tsm100_paged_kv* kv, const tsm100_paged_batch* batch, const tsm100_attention_paged_desc* desc,
                                const void* q, void* o, void* stream) {
   return on_device(dev, [&](std::string* err) { return ops::attention_paged(err, kv, batch, desc, q, o, dev->status, stream); });
+}
+
+int32_t tsm100_attention_paged_cross(tsm100_device_t dev, const tsm100_paged_kv* kv, const tsm100_paged_batch* batch, const tsm100_attention_paged_desc* desc,
+                                     const void* q, void* o, void* stream) {
+  return on_device(dev, [&](std::string* err) { return ops::attention_paged_cross(err, kv, batch, desc, q, o, dev->status, stream); });
+}
+
+int32_t tsm100_attention_paged_prefix(tsm100_device_t dev, const tsm100_paged_kv* kv, const tsm100_paged_batch* batch,
+                                      const tsm100_attention_paged_prefix_desc* desc, const void* q, void* o, void* stream) {
+  return on_device(dev, [&](std::string* err) { return ops::attention_paged_prefix(err, kv, batch, desc, q, o, dev->status, stream); });
 }
 
 }  // extern "C"

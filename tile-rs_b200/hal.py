@@ -559,6 +559,26 @@ class CudaSm100Device:
         elif st:
             check(st)
 
+    def attention_paged_cross(self, kv: PagedKv, batch: PagedBatch, dtype: int, heads_q: int, q: int, o: int, stream: int = 0) -> None:
+        """Attention of the call's tokens q [tokens, heads_q, d] to all positions of their sequences; zeros where a sequence has none."""
+        st = self._fast.attention_paged_cross(self._raw, kv.address, batch.address, dtype, heads_q, q, o, stream)
+        if st is None:
+            d = capi.AttentionPagedDesc(dtype, heads_q)
+            check(capi.lib().tsm100_attention_paged_cross(self._h, C.byref(kv.desc), C.byref(batch.desc), C.byref(d), q, o, stream or None))
+        elif st:
+            check(st)
+
+    def attention_paged_prefix(self, kv: PagedKv, batch: PagedBatch, dtype: int, heads_q: int, prefix_len: int, prefix: int, q: int, o: int,
+                               stream: int = 0) -> None:
+        """attention_paged of sequences whose first prefix_len positions lie in the same pages, prefix [prefix_len / page_size] int32 in device
+        memory: those are read once for all."""
+        st = self._fast.attention_paged_prefix(self._raw, kv.address, batch.address, dtype, heads_q, prefix_len, prefix or 0, q, o, stream)
+        if st is None:
+            d = capi.AttentionPagedPrefixDesc(dtype, heads_q, prefix_len, prefix or None)
+            check(capi.lib().tsm100_attention_paged_prefix(self._h, C.byref(kv.desc), C.byref(batch.desc), C.byref(d), q, o, stream or None))
+        elif st:
+            check(st)
+
     # -- operators on host buffers (upload + compute + download) --
     def softmax_host(self, dtype: int, rows: int, cols: int, x: int, y: int) -> None:
         d = capi.SoftmaxDesc(dtype, rows, cols)
