@@ -240,6 +240,259 @@ gemm_i8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many output tiles: CTA pairs (gemm_tc2.cuh), 256 rows of A by `bn` rows of W a tile
+// ---------------------------------------------------------------------------
+// Per CTA: warp 0 TMA producer (128 rows of A and half of the tile's rows of W, 128 of K a stage), warp 1 tensor memory and, in the leader, the products
+// (M = 256 over the pair, N = bn, K = 32), warps 2..5 this CTA's 128 rows of the sums, of which two sets alternate, scaled and stored as boxes.
+// Bound: the tensor pipe, 2 M N K.  Widths from 128 to 256 so that the last wave of tiles is a full one (route.hpp: gemm_i8_pair_width).
+namespace pairs {
+
+constexpr int kPairM = 256, kCtaM = 128, kMaxBN = 256;
+constexpr int kStages = 6;
+constexpr int kThreads = 192;
+constexpr int kABytes = kCtaM * kBK;              // 16 KiB
+constexpr int kStageBytes = kABytes + kMaxBN / 2 * kBK;
+constexpr int kTmemCols = 512;
+constexpr int kGroupM = 16;                       // pair tiles per band (gemm_tc2.cuh)
+constexpr int kBoxBytes = 32 * 128;
+
+struct alignas(8) Barriers {
+  uint64_t full[kStages];      // used in the leader: both CTAs' bytes of a stage have landed
+  uint64_t empty[kStages];     // in each CTA: the products reading the stage have retired
+  uint64_t acc_full[2];        // in each CTA: sums complete
+  uint64_t acc_empty[2];       // used in the leader: 8 epilogue warps of the pair have drained them
+  uint32_t tmem_base;
+  uint32_t abort_flag;
+};
+constexpr int kBarsOff = kStages * kStageBytes + 4 * 2 * kBoxBytes;
+constexpr int kSmemBytes = kBarsOff + sizeof(Barriers) + 1024;
+static_assert(kSmemBytes <= 227 * 1024, "shared memory budget of one CTA");
+
+struct Params {
+  const float* a_scales;
+  const float* w_scales;
+  int32_t m, n, k;
+  int32_t bn;                // a multiple of 32, and of a box's columns where C leaves in boxes
+  int32_t m_blocks, n_blocks;
+  int64_t ldc;
+  uint32_t* status;
+};
+
+__device__ __forceinline__ void tile_coords(const Params& p, int tile, int& mb, int& nb) {
+  const int band_tiles = kGroupM * p.n_blocks, band = tile / band_tiles, first_m = band * kGroupM;
+  const int rows_in_band = min(kGroupM, p.m_blocks - first_m), t = tile - band * band_tiles;
+  mb = first_m + t % rows_in_band;
+  nb = t / rows_in_band;
+}
+
+// One warp's 32 rows of a tile's sums (`tmem`: its lanes, first column), scaled, to C from (row0, col0) up to column `end`: as gemm_tc.cuh's store_rows.
+// kLoose: rows of C start anywhere.
+template <typename OutT, bool kLoose>
+__device__ __forceinline__ void store_rows(const CUtensorMap* tmap_c, OutT* c, const Params& p, uint32_t tmem, uint8_t* staging, uint32_t& boxes, int row0, int col0, int end, int lane) {
+  constexpr int kCols = gemm_tc::kBoxCols<OutT>, kHalves = kCols / 32;
+  if (row0 >= p.m) return;
+  const float as = p.a_scales[min(row0 + lane, p.m - 1)];
+  float ws[kHalves], next[kHalves];  // of this lane's columns in a box
+  auto ask = [&](int c0) {
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) next[h] = p.w_scales[min(c0 + h * 32 + lane, p.n - 1)];
+  };
+  ask(col0);
+#pragma unroll 1
+  for (int c0 = col0; c0 < end; c0 += kCols) {
+    uint32_t v[kHalves][32];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) ptx::tmem_ld_32x32b_x32(tmem + (c0 - col0) + h * 32, v[h]);
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) ws[h] = next[h];
+    if (c0 + kCols < end) ask(c0 + kCols);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[h][i] = __float_as_uint(scaled(v[h][i], as, __shfl_sync(0xffffffffu, ws[h], i)));
+    uint8_t* box = staging + (boxes++ & 1) * kBoxBytes;
+    if (!kLoose && lane == 0) ptx::tma_store_wait_read<1>();  // the store before last has read its buffer
+    __syncwarp();
+    const uint32_t row = ptx::smem_u32(box) + lane * 128;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t at = row + ((u ^ (lane & 7)) << 4);
+      if constexpr (sizeof(OutT) == 4) {
+        ptx::st_shared_v4(at, v[0][4 * u], v[0][4 * u + 1], v[0][4 * u + 2], v[0][4 * u + 3]);
+      } else {
+        using gemm_tc::narrow2;
+        const uint32_t(&w)[32] = v[u >> 2];
+        const int i = (u & 3) * 8;
+        ptx::st_shared_v4(at, narrow2<OutT>(w[i], w[i + 1]), narrow2<OutT>(w[i + 2], w[i + 3]), narrow2<OutT>(w[i + 4], w[i + 5]), narrow2<OutT>(w[i + 6], w[i + 7]));
+      }
+    }
+    if constexpr (kLoose) {
+      __syncwarp();
+      const int rows = min(32, p.m - row0);
+      OutT* dst = c + row0 * p.ldc + c0;
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r, dst += p.ldc)
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          const int x = h * 32 + lane;
+          const OutT value = *reinterpret_cast<const OutT*>(box + r * 128 + (((x * static_cast<int>(sizeof(OutT)) >> 4) ^ (r & 7)) << 4) + (x * static_cast<int>(sizeof(OutT)) & 15));
+          if (c0 + x < end) dst[x] = value;
+        }
+      continue;
+    }
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      ptx::tma_store_3d(tmap_c, box, c0, row0, 0);
+      ptx::tma_store_commit();
+    }
+  }
+}
+
+template <typename OutT, bool kLoose>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_i8_pairs_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_c, OutT* c,
+                     const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Barriers* bars = reinterpret_cast<Barriers*>(smem + kBarsOff);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();  // 0 = leader
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const int num_tiles = p.m_blocks * p.n_blocks;
+  const int num_kb = (p.k + kBK - 1) / kBK;
+  volatile uint32_t* abort_flag = &bars->abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(&bars->full[s], 1);
+      ptx::mbar_init(&bars->empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(&bars->acc_full[a], 1);
+      ptx::mbar_init(&bars->acc_empty[a], 8);
+    }
+    bars->abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(&bars->tmem_base, kTmemCols);
+    ptx::tmem_relinquish_alloc_permit_pair();
+  }
+  ptx::tcgen05_fence_before_thread_sync();
+  ptx::cluster_sync_all();  // the peer's barriers are initialised before anything signals them
+  ptx::tcgen05_fence_after_thread_sync();
+  const uint32_t tmem_base = bars->tmem_base;
+  ptx::launch_dependents();
+  ptx::wait_prior_grid();
+
+  if (warp == 0) {
+    // ------------------------------ TMA producer (both CTAs) ------------------
+    if (lane == 0) {
+      ptx::prefetch_tensormap(&tmap_a);
+      ptx::prefetch_tensormap(&tmap_w);
+      const uint32_t bytes = 2 * (kABytes + p.bn / 2 * kBK);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = pair; tile < num_tiles && ok; tile += num_pairs) {
+        int mb, nb;
+        tile_coords(p, tile, mb, nb);
+        const int row0 = mb * kPairM + static_cast<int>(rank) * kCtaM, col0 = nb * p.bn + static_cast<int>(rank) * (p.bn / 2);
+        const bool backward = ((tile / num_pairs) & 1) != 0;  // every other wave walks K backwards, to find in the L2 what the one before it read last
+        for (int kq = 0; kq < num_kb; ++kq) {
+          const int k0 = (backward ? num_kb - 1 - kq : kq) * kBK;
+          if (!ptx::mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag, p.status, 184)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full_leader = ptx::mapa_shared(ptx::smem_u32(&bars->full[stage]), 0);
+          if (rank == 0) ptx::mbar_arrive_expect_tx(&bars->full[stage], bytes);
+          uint8_t* to = smem + stage * kStageBytes;
+          ptx::tma_load_3d_pair(to, &tmap_a, full_leader, k0, row0, 0);
+          ptx::tma_load_3d_pair(to + kABytes, &tmap_w, full_leader, k0, col0, 0);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------ products (leader CTA only) ----------------
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = ptx::make_idesc_i8(kPairM, p.bn);
+      constexpr uint64_t kmajor = ptx::make_smem_desc_base(16, 1024);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      int local = 0;
+      for (int tile = pair; tile < num_tiles && ok; tile += num_pairs, ++local) {
+        const int acc = local & 1;
+        if (!ptx::mbar_wait(&bars->acc_empty[acc], ((local >> 1) & 1u) ^ 1u, abort_flag, p.status, 185)) break;
+        ptx::tcgen05_fence_after_thread_sync();
+        const uint32_t d_tmem = tmem_base + acc * kMaxBN;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!ptx::mbar_wait_relaxed(&bars->full[stage], phase, abort_flag, p.status, 186)) {  // relaxed: the data goes straight to the async proxy
+            ok = false;
+            break;
+          }
+          ptx::tcgen05_fence_after_thread_sync();
+          const uint32_t a = ptx::smem_u32(smem + stage * kStageBytes), w = a + kABytes;
+#pragma unroll
+          for (int kk = 0; kk < kBK / 32; ++kk)
+            ptx::tcgen05_mma_i8_ss_pair(d_tmem, ptx::smem_desc(kmajor, a + kk * 32), ptx::smem_desc(kmajor, w + kk * 32), idesc, (kb | kk) != 0 ? 1u : 0u);
+          ptx::tcgen05_commit_pair(&bars->empty[stage], 3);  // frees the stage in both CTAs
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) ptx::tcgen05_commit_pair(&bars->acc_full[acc], 3);
+      }
+    }
+  } else {
+    // ------------------------------ sums -> C (both CTAs) ---------------------
+    const int quad = warp & 3;
+    uint8_t* staging = smem + kStages * kStageBytes + (warp - 2) * 2 * kBoxBytes;
+    uint32_t boxes = 0;
+    int local = 0;
+    for (int tile = pair; tile < num_tiles; tile += num_pairs, ++local) {
+      const int acc = local & 1;
+      int mb, nb;
+      tile_coords(p, tile, mb, nb);
+      const bool ready = ptx::mbar_wait(&bars->acc_full[acc], (local >> 1) & 1u, abort_flag, p.status, 187);
+      if (!__all_sync(0xffffffffu, ready)) break;
+      ptx::tcgen05_fence_after_thread_sync();
+      const uint32_t from = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * kMaxBN;
+      const int row0 = mb * kPairM + static_cast<int>(rank) * kCtaM + quad * 32, col0 = nb * p.bn;
+      store_rows<OutT, kLoose>(&tmap_c, c, p, from, staging, boxes, row0, col0, min(p.n, col0 + p.bn), lane);
+      ptx::tcgen05_fence_before_thread_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_u32(&bars->acc_empty[acc]), 0));
+    }
+    if (!kLoose && lane == 0) ptx::tma_store_wait_all<0>();
+  }
+
+  // ------------------------------ teardown ------------------------------------
+  if (*abort_flag != 0u) {
+    const unsigned long long t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 1000000ull) {
+    }
+  }
+  ptx::tcgen05_fence_before_thread_sync();
+  // Neither CTA may leave while the other can still read its shared memory or signal its barriers.
+  ptx::cluster_sync_all();
+  if (warp == 1) {
+    ptx::tcgen05_fence_after_thread_sync();
+    ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+}
+
+}  // namespace pairs
+
 // Operands whose rows do not start on 16-byte boundaries, as rows that do: src [rows][cols], pitch ld -> dst [rows][pitch], zeros beyond cols.
 // A thread has 16 bytes of dst; words of src that hold them, shifted into place, a byte at a time where those reach past the matrix.
 struct Operand {

@@ -100,10 +100,41 @@ inline int32_t gemm_i8_few_launch(std::string* err, const GemmI8& g, const route
   return cuda_ok(err, e, "gemm_i8_few_kernel launch");
 }
 
+template <typename OutT, bool kLoose>
+inline int32_t gemm_i8_pairs_launch(std::string* err, const GemmI8& g, int bn, OutT* c, int sms, cudaStream_t s) {
+  namespace k8 = gemm_i8::pairs;
+  CUtensorMap ta, tw, tc = {};
+  int32_t st = gemm_i8_tmap(err, &ta, g.a, g.k, g.m, g.lda, k8::kCtaM);
+  if (st == TSM100_OK) st = gemm_i8_tmap(err, &tw, g.w, g.k, g.n, g.ldw, static_cast<uint32_t>(bn / 2));
+  if (st == TSM100_OK && !kLoose)
+    st = make_tmap_3d(err, &tc, c, g.n, g.m, 1, g.ldc, static_cast<uint64_t>(g.m) * g.ldc, gemm_tc::kBoxCols<OutT>, 32,
+                      sizeof(OutT) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                        : std::is_same<OutT, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, sizeof(OutT));
+  if (st != TSM100_OK) return st;
+  k8::Params p;
+  p.a_scales = g.a_scales, p.w_scales = g.w_scales;
+  p.m = static_cast<int32_t>(g.m), p.n = static_cast<int32_t>(g.n), p.k = static_cast<int32_t>(g.k);
+  p.bn = bn;
+  p.m_blocks = static_cast<int32_t>(route::div_up(g.m, k8::kPairM)), p.n_blocks = static_cast<int32_t>(route::div_up(g.n, bn));
+  p.ldc = g.ldc;
+  p.status = g.status;
+  auto kern = k8::gemm_i8_pairs_kernel<OutT, kLoose>;
+  cudaError_t e = set_dyn_smem_once(kern, k8::kSmemBytes);
+  if (e != cudaSuccess) return cuda_ok(err, e, "cudaFuncSetAttribute(gemm_i8_pairs_kernel)");
+  const int max_clusters = resident_clusters(kern, k8::kThreads, k8::kSmemBytes, 2, static_cast<unsigned>(sms & ~1), sms / 2);
+  const int64_t pairs = std::min<int64_t>(static_cast<int64_t>(p.m_blocks) * p.n_blocks, std::min<int64_t>(max_clusters, sms / 2));
+  return cuda_ok(err, launch_chained(kern, static_cast<unsigned>(2 * pairs), k8::kThreads, k8::kSmemBytes, s, 2, ta, tw, tc, c, p), "gemm_i8_pairs_kernel launch");
+}
+
 template <typename OutT>
 inline int32_t gemm_i8_typed(std::string* err, const GemmI8& g, void* c, int sms, cudaStream_t s) {
   const route::GemmI8 plan = route::gemm_i8(g.m, g.n, g.k, sms);
   OutT* out = static_cast<OutT*>(c);
+  if (plan.pairs) {
+    const bool loose = !aligned16(c) || g.ldc * sizeof(OutT) % 16 != 0;
+    const int bn = route::gemm_i8_pair_width(g.m, g.n, loose || sizeof(OutT) == 4 ? 32 : 64, sms);
+    return loose ? gemm_i8_pairs_launch<OutT, true>(err, g, bn, out, sms, s) : gemm_i8_pairs_launch<OutT, false>(err, g, bn, out, sms, s);
+  }
   switch (plan.rows) {
     case 16: return gemm_i8_few_launch<OutT, 16>(err, g, plan, out, s);
     case 32: return gemm_i8_few_launch<OutT, 32>(err, g, plan, out, s);

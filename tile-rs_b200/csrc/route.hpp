@@ -107,15 +107,17 @@ inline Gemm16 gemm16(int64_t m, int64_t n, int64_t k, int64_t batch, int sms) {
   return r;
 }
 
-// 8-bit product (gemm_i8.cuh): 128 columns x `rows` rows of C per CTA, K over `splits` CTAs of a cluster.
+// 8-bit product (gemm_i8.cuh): CTA pairs, or 128 columns x `rows` rows of C per CTA and K over `splits` CTAs of a cluster.
 struct GemmI8 {
+  bool pairs;
   int rows;
   int splits;
   int64_t k_blocks_per_cta;  // 128 of K each
 };
 inline GemmI8 gemm_i8(int64_t m, int64_t n, int64_t k, int sms) {
-  GemmI8 r{m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, 1, 0};
+  GemmI8 r{false, m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, 1, 0};
   const int64_t tiles = div_up(m, r.rows) * div_up(n, 128), kb = div_up(k, 128);
+  r.pairs = m > 128 && n > 128 && tiles > sms;
   while (r.splits < kMaxGemmSplit) {
     const int to = 2 * r.splits;
     const int64_t room = to == 2 || kb >= 128 ? 2 * sms : to == 4 ? sms * 15 / 8 : sms * 8 / 5;
@@ -124,6 +126,16 @@ inline GemmI8 gemm_i8(int64_t m, int64_t n, int64_t k, int sms) {
   }
   r.k_blocks_per_cta = div_up(kb > 0 ? kb : 1, r.splits);
   return r;
+}
+// Rows of W in a pair's tile, a multiple of `step`: what makes all waves together the shortest; the wider of two that do.
+inline int gemm_i8_pair_width(int64_t m, int64_t n, int step, int sms) {
+  int best = 256;
+  int64_t best_cost = INT64_MAX;
+  for (int bn = 256; bn >= 128; bn -= step) {
+    const int64_t cost = div_up(div_up(m, 256) * div_up(n, bn), sms / 2) * (bn + 16);
+    if (cost < best_cost) best_cost = cost, best = bn;
+  }
+  return best;
 }
 
 // CTA pairs: does C leave through shared memory, in whole boxes, or from the lanes that hold its rows?  The boxes are out in a sixth of the time, which
