@@ -395,7 +395,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       } else {
         const uint32_t p_lo = k_lo_base | (ptx::smem_u32(smem_p) >> 4), ring_lo = v_lo_base | (ptx::smem_u32(smem_kv) >> 4);
         for (int j = 0; j < w.n && ok; ++j) {
-          if (!(ok = wait_kv(v_pos(j), (w.begin + j + 1) * kKeys > w.len))) break;
+          bool landed = false;
           for (int g = 0; g < 2 && ok; ++g) {
             if (j >= n_of[g]) continue;
             if (j == 0 && segs[g] > 0) {  // the segment before has left tensor memory
@@ -403,6 +403,9 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
               if (!ok) break;
             }
             ok = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->p_ready[g], (done[g] + j) & 1u, abort_flag, p.status, 162 + g));
+            // V_j after P_j, never before: in a ring of three its slot had K_j, and while that has not landed a wait for V_j's phase, of which the parity is the one before K_j's,
+            // would pass at once.  Probabilities say that K_j was read.
+            if (ok && !landed) ok = landed = wait_kv(v_pos(j), (w.begin + j + 1) * kKeys > w.len);
             ptx::tcgen05_fence_after_thread_sync();
             if (!ok) break;
             const uint32_t a_lo = p_lo + g * (S::kPBytes >> 4), b_lo = ring_lo + v_pos(j) % S::kRing * (S::kTileBytes >> 4), d = tmem_o + g * 128;

@@ -349,13 +349,14 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         };
         bool ok = true;
         for (int j = 0; j < n_b && ok; ++j) {
-          if (!(ok = wait_kv(v_pos(j)))) break;
+          // V_j after P_j, never before: its slot of the ring of three had K_j, and while that has not landed a wait for V_j's phase, of which the parity is the one before
+          // K_j's, would pass at once.  Probabilities say that K_j was read.
           if (j < n_a) {
-            if (!(ok = wait_p(0, j))) break;
+            if (!(ok = wait_p(0, j) && wait_kv(v_pos(j)))) break;
             issue_pv(0, v_pos(j), j > 0);
           }
           if (!lone) {
-            if (!(ok = wait_p(1, j))) break;
+            if (!(ok = wait_p(1, j) && (j < n_a || wait_kv(v_pos(j))))) break;
             issue_pv(1, v_pos(j), j > 0);
           }
           // the last reader of V_j has been issued
