@@ -13,10 +13,16 @@ class Sharing(u.Paged):
     """seqs = [(new tokens, own positions with them)], behind `shared` pages that are the same for all."""
 
     def __init__(self, pkg, seed, seqs, heads, d, page, dtype, cache, shared, **more):
-        self.shared = shared
-        super().__init__(pkg, seed, [(new, shared * page + n) for new, n in seqs], heads, d, page, dtype, cache, **more)
-        self.prefix = self.table[0, :shared].clone()
-        self.table[:, :shared] = self.prefix
+        gap = more.pop("gap", 0)
+        super().__init__(pkg, seed, list(seqs) + [(0, shared * page)], heads, d, page, dtype, cache, **more)
+        own, self.shared = self.table[:-1], shared
+        self.prefix = self.table[-1, :shared].clone()
+        need = max([-(-n // page) for _, n in seqs] + [0]) + more.get("slack", 0)
+        self.table = torch.cat((self.prefix.expand(len(seqs), shared), own[:, :need]), 1).contiguous()
+        self.pitch = shared + need
+        self.seqs = [(new, shared * page + n) for new, n in seqs]
+        self.starts_h, self.starts, self.lens = self.starts_h[:-1], self.starts[:-1].contiguous(), self.lens[:-1] + shared * page
+        self.tokens = self.starts_h[-1] + gap
 
 
 def run(pkg, dev, cache, q, o=None):
@@ -95,6 +101,25 @@ def test_page_sizes(dev, pkg, page, shared, held, new):
 def test_long(dev, pkg, held, batch):
     """Every sequence has pages of its own below the prefix as well, so the batch is held small."""
     one(pkg, dev, 15, [(1, 1 + 29 * i % 97) for i in range(batch)], 8, 2, 64 if held == "i8" else 128, 64, "bf16", held, 200)
+
+
+@pytest.mark.parametrize("dtype,held", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("page", [8, 16, 24, 128])
+def test_prefix_of_many_rows(dev, pkg, dtype, held, d, page):
+    """The prefix on tcgen05 in blocks of 256 rows, the last ones in part, its end inside a tile; single tokens, some, and a chunk behind it."""
+    one(pkg, dev, 26, [(1, 1 + 29 * i % 97) for i in range(60)] + [(7, 50), (100, 130), (1, 700)], 28, 4, d, page, dtype, held, 7800 // page)
+
+
+@pytest.mark.parametrize("held", ["bf16", "i8"])
+def test_prefix_of_one_tile_and_many_rows(dev, pkg, held):
+    """So many rows that even a short prefix is tcgen05's, and blocks are whole."""
+    one(pkg, dev, 27, [(20, 60)] * 80, 32, 2, 128, 64, "bf16", held, 2)
+
+
+@pytest.mark.parametrize("page", [3, 20])
+def test_many_rows_on_pages_that_boxes_do_not_fit(dev, pkg, page):
+    one(pkg, dev, 28, [(1, 30)] * 50 + [(30, 60)], 16, 2, 64, page, "f16", "f16", 1500 // page)
 
 
 @pytest.mark.parametrize("batch", [150, 600])

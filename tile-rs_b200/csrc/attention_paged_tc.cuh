@@ -93,8 +93,9 @@ struct Params {
   int32_t run_log2;    // positions of a page's box
   float scale_log2;
   int32_t prefix;      // attention_paged.cuh: Keys
-  int32_t sequences;
-  float* records;
+  int32_t large;
+  const int32_t* prefix_table;
+  Records records;
   float4* part;        // [CTA][2][D / 4][256 rows]: of a block that began in an earlier share, of one that goes on in the next
   float2* part_ml;     // [CTA][2][256]
   int4* info;          // [CTA]: as attention_paged.cuh, with the block's sequence, KV head and number
@@ -108,31 +109,34 @@ struct Seq {
 };
 template <Keys kKeysSeen>
 __device__ __forceinline__ int64_t full_blocks(const Params& p, const Seq& s, int64_t i) {  // the length of the first i blocks, which have two tiles
-  if (kKeysSeen == kAll) return i * (s.len + kBlockCost);
+  if (kKeysSeen == kAll || kKeysSeen == kShared) return i * (s.len + kBlockCost);
   const int64_t two = 2 * p.tokens;
   return i * (s.len - s.count + kBlockCost) + two * (i * (i + 1) / 2);
 }
 template <Keys kKeysSeen>
 __device__ __forceinline__ int64_t sequence_length(const Params& p, int b, Seq& s, uint32_t* status) {
-  if (!sequence<kKeysSeen>(p, b, s.first, s.count, s.len, status, 145)) return 0;
+  if (!sequence<kKeysSeen>(p, kKeysSeen == kShared ? -1 : b, s.first, s.count, s.len, status, 145)) return 0;
+  if (kKeysSeen == kRest && !is_large(p, s.count)) return 0;
   s.blocks = (s.count + 2 * p.tokens - 1) / (2 * p.tokens);
   s.per_head = full_blocks<kKeysSeen>(p, s, s.blocks - 1) + s.len + kBlockCost;
   return s.per_head * p.cache.heads;
 }
 template <Keys kKeysSeen>
+__device__ __forceinline__ int sequences(const Params& p) { return kKeysSeen == kShared ? 1 : p.step.batch; }
+template <Keys kKeysSeen>
 struct Stream {
   Seq seq;
-  int64_t at, end;
+  int64_t at, end, per;
   __device__ __forceinline__ void open(const Params& p, int b, int64_t base) {  // the first sequence from b on that has blocks
     int64_t n = 0;
-    for (; b < p.step.batch; ++b)
+    for (; b < sequences<kKeysSeen>(p); ++b)
       if ((n = sequence_length<kKeysSeen>(p, b, seq, nullptr)) > 0) break;
     seq.b = b, seq.base = base, seq.end = base + n;
   }
   __device__ __forceinline__ bool next(const Params& p, Work& w) {
     while (at < end) {
-      while (at >= seq.end && seq.b < p.step.batch) open(p, seq.b + 1, seq.end);
-      if (seq.b >= p.step.batch) return false;
+      while (at >= seq.end && seq.b < sequences<kKeysSeen>(p)) open(p, seq.b + 1, seq.end);
+      if (seq.b >= sequences<kKeysSeen>(p)) return false;
       const int64_t in_seq = at - seq.base;
       w.head = static_cast<int>(in_seq / seq.per_head);
       const int64_t in_head = in_seq - w.head * seq.per_head;
@@ -145,7 +149,7 @@ struct Stream {
       const bool last = lo == seq.blocks - 1;
       const int64_t from = full_blocks<kKeysSeen>(p, seq, lo), to = last ? seq.per_head : full_blocks<kKeysSeen>(p, seq, lo + 1);
       w.token0 = lo * 2 * p.tokens;
-      const int keys = kKeysSeen == kAll ? seq.len : seq.len - seq.count + min(seq.count, w.token0 + 2 * p.tokens);
+      const int keys = kKeysSeen == kAll || kKeysSeen == kShared ? seq.len : seq.len - seq.count + min(seq.count, w.token0 + 2 * p.tokens);
       w.steps = (keys + kKeys - 1) / kKeys;
       const int64_t stop = min(to, in_head + (end - at));
       auto steps_to = [&](int64_t x) { return static_cast<int>((static_cast<uint32_t>(max(x - from - kBlockCost, static_cast<int64_t>(0))) + kKeys - 1) / kKeys); };
@@ -153,14 +157,34 @@ struct Stream {
       w.n = steps_to(stop) - w.begin;
       w.b = seq.b, w.first = seq.first, w.count = seq.count, w.len = seq.len, w.block = lo;
       w.lone = last && seq.count - w.token0 <= p.tokens;
-      const int keys_a = kKeysSeen == kAll ? seq.len : seq.len - seq.count + min(seq.count, w.token0 + p.tokens);
+      const int keys_a = kKeysSeen == kAll || kKeysSeen == kShared ? seq.len : seq.len - seq.count + min(seq.count, w.token0 + p.tokens);
       w.n_a = max(0, min(w.n, (keys_a + kKeys - 1) / kKeys - w.begin));
+      if constexpr (leaves_records(kKeysSeen)) {
+        if (w.n > 0 && w.begin == 0) {
+          const int64_t last = seq.base + w.head * seq.per_head + from + kBlockCost + static_cast<int64_t>(w.steps - 1) * kKeys;  // where the last step begins
+          p.records.cut[(kKeysSeen == kRest ? static_cast<int64_t>(seq.b) * p.cache.heads * p.records.units : 0) + static_cast<int64_t>(w.head) * p.records.units + lo] =
+              make_int2(static_cast<int>(blockIdx.x), w.n == w.steps ? 0 : static_cast<int>(last / per) - static_cast<int>(blockIdx.x) + 1);
+        }
+      }
       at += stop - in_head;
       if (w.n > 0) return true;
     }
     return false;
   }
 };
+
+// pages::page_of, of the prefix's pages for kShared.
+template <Keys kKeysSeen>
+__device__ __forceinline__ int page_at_position(const Params& p, int b, int pos) {
+  if constexpr (kKeysSeen == kShared) {
+    const int page = p.prefix_table[pos / p.cache.page_size];
+    if (page >= 0 && page < p.cache.pages) return page;
+    pages::report(p.status, 146);
+    return -1;
+  } else {
+    return pages::page_of(p.cache, p.step, b, pos, p.status, 146);
+  }
+}
 
 template <bool kIsBf16, bool kI8, int D, Keys kKeysSeen = kPast>
 __global__ void __launch_bounds__(Shape<kI8, D>::kThreads, 1)
@@ -171,7 +195,8 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((ptx::smem_u32(smem) & 1023u) != 0u) {
     ptx::wait_prior_grid();
-    if (threadIdx.x == 0) p.info[blockIdx.x] = make_int4(0, -1, 0, 0), atomicCAS(p.status, ptx::kStatusOk, ptx::kStatusWaitTimeout | 174u);
+    if (threadIdx.x == 0 && !leaves_records(kKeysSeen)) p.info[blockIdx.x] = make_int4(0, -1, 0, 0);
+    if (threadIdx.x == 0) atomicCAS(p.status, ptx::kStatusOk, ptx::kStatusWaitTimeout | 174u);
     return;
   }
   uint8_t* smem_q = smem;                  // two tiles
@@ -202,7 +227,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
     }
     bars->abort_flag = 0;
     bars->pv_steps = 0;
-    bars->first_seq = p.step.batch;
+    bars->first_seq = sequences<kKeysSeen>(p);
     bars->first_base = 0;
     ptx::fence_mbar_init();
   }
@@ -221,7 +246,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
   Stream<kKeysSeen> stream;
   {
     constexpr int kThreads = S::kThreads;
-    const int batch = p.step.batch;
+    const int batch = sequences<kKeysSeen>(p);
     auto block_scan = [&](int64_t v, int64_t& before) {  // answers the total
       int64_t x = v;
 #pragma unroll
@@ -244,7 +269,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
     Seq s;
     for (int base = 0; base < batch; base += kThreads) total += block_scan(base + tid < batch ? sequence_length<kKeysSeen>(p, base + tid, s, p.status) : 0, before);
     const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kMinShare));
-    stream.at = min(total, blockIdx.x * per), stream.end = min(total, stream.at + per);
+    stream.at = min(total, blockIdx.x * per), stream.end = min(total, stream.at + per), stream.per = per;
     int64_t sum = 0;
     for (int base = 0; base < batch; base += kThreads) {
       const int64_t own = base + tid < batch ? sequence_length<kKeysSeen>(p, base + tid, s, nullptr) : 0;
@@ -292,7 +317,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         const int my_run = S::kHalves == 2 ? lane >> 1 : lane, half = S::kHalves == 2 ? lane & 1 : 0;
         auto page_at = [&](int step) {  // of this lane's run; asked for a tile ahead
           const int pos = (w.begin + step) * kKeys + my_run * run;
-          return my_run * run < kKeys && step < w.n && pos < w.len ? max(0, pages::page_of(p.cache, p.step, w.b, pos, p.status, 146)) : 0;
+          return my_run * run < kKeys && step < w.n && pos < w.len ? max(0, page_at_position<kKeysSeen>(p, w.b, pos)) : 0;
         };
         const int total = 2 * w.n;
         int page_k = page_at(0), page_v = page_k;
@@ -449,7 +474,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         if (w.begin > 0) head_state = w.begin + w.n == w.steps ? 1 : 2;
         else if (w.n < w.steps) tail_b = w.b, tail_head = w.head, tail_block = w.block;
       }
-      p.info[blockIdx.x] = make_int4(head_state, tail_b, tail_head, tail_block);
+      if (!leaves_records(kKeysSeen)) p.info[blockIdx.x] = make_int4(head_state, tail_b, tail_head, tail_block);
     }
   } else if (kI8 && warp >= 12) {
     // ------------------------------ conversion ---------------------------------
@@ -475,7 +500,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         uint4 next[kVecs];
         auto ask_page = [&](int i) {
           const int pos = pos_of(i);
-          page = i < total && pos < w.len ? p.step.table[static_cast<int64_t>(w.b) * p.step.pitch + pos / ps] : 0;
+          page = i < total && pos < w.len ? (kKeysSeen == kShared ? p.prefix_table : p.step.table + static_cast<int64_t>(w.b) * p.step.pitch)[pos / ps] : 0;
         };
         auto ask_step = [&](int i) {
           const int pos = pos_of(i);
@@ -571,7 +596,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       const int token = w.token0 + g * p.tokens + r_token;
       const bool row_ok = r_token < p.tokens && token < w.count;
       const bool idle = __all_sync(0xffffffffu, !row_ok);           // no row of this warp exists
-      const int limit = kKeysSeen == kAll ? w.len - 1 : w.len - w.count + min(token, w.count - 1);  // last visible position
+      const int limit = kKeysSeen == kAll || kKeysSeen == kShared ? w.len - 1 : w.len - w.count + min(token, w.count - 1);  // last visible position
       float m_used = -INFINITY, l = 0.f;
       int v_used = 0;  // probabilities and their sum are 2^-v_used of what they were
       for (int j = 0; j < n_g; ++j) {
@@ -733,17 +758,12 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
       }
       if (!idle) {
         const int64_t rec = static_cast<int64_t>(blockIdx.x) * 2 + (w.begin == 0 ? 1 : 0);
-        const float inv = m_used == -INFINITY ? NAN : 1.0f / l;  // all scores -inf (or NaN): softmax is NaN there
+        [[maybe_unused]] const float inv = m_used == -INFINITY ? NAN : 1.0f / l;  // all scores -inf (or NaN): softmax is NaN there
         const int64_t row = static_cast<int64_t>(w.first + token) * p.heads_q + w.head * p.group + r_head;
-        uint16_t* orow = o + row * D;
-        [[maybe_unused]] float lse = 0.f, f_own = 0.f;
-        [[maybe_unused]] float2 joined = make_float2(0.f, 0.f);
-        if constexpr (kKeysSeen != kPast) {
-          if (whole && row_ok) {
-            lse = log_sum(m_used * sl2 + static_cast<float>(v_used) - kRaised<kI8, kPvBf16>, l);
-            if (kKeysSeen == kRest) joined = join_weights(lse, __ldcg(p.records + row * (D + 4) + D)), f_own = joined.x == 0.f ? 0.f : joined.x / l;
-          }
-        }
+        [[maybe_unused]] uint16_t* orow = o + row * D;
+        [[maybe_unused]] float* record = nullptr;
+        if constexpr (leaves_records(kKeysSeen))
+          record = whole ? p.records.whole + (row_ok ? row : 0) * (D + 4) : p.records.part + (rec * 256 + g * kTileRows + r) * (D + 4);
 #pragma unroll 1
         for (int q = 0; q < D / 32; ++q) {
           uint32_t ov[32];
@@ -754,28 +774,15 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
 #pragma unroll
             for (int i = 0; i < 32; ++i) ov[i] = 0u;
           }
-          if (whole) {
-            if (row_ok && kKeysSeen == kAll && p.records) {
-              float* rec = p.records + row * (D + 4) + q * 32;
-              const float f = l == 0.f ? 0.f : 1.f / l;
+          if constexpr (leaves_records(kKeysSeen)) {
+            if (row_ok) {
 #pragma unroll
-              for (int t = 0; t < 8; ++t)
-                reinterpret_cast<float4*>(rec)[t] = make_float4(__uint_as_float(ov[4 * t]) * f, __uint_as_float(ov[4 * t + 1]) * f, __uint_as_float(ov[4 * t + 2]) * f,
-                                                                __uint_as_float(ov[4 * t + 3]) * f);
-            } else if (row_ok) {
-              if constexpr (kKeysSeen == kRest) {
-                const float4* rec = reinterpret_cast<const float4*>(p.records + row * (D + 4) + q * 32);
-#pragma unroll
-                for (int t = 0; t < 8; ++t) {
-                  const float4 y = __ldcg(rec + t);
-                  const float prior[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    ov[4 * t + e] = __float_as_uint(weighed(f_own, __uint_as_float(ov[4 * t + e])) + weighed(joined.y, prior[e]));
-                }
-              }
-              [[maybe_unused]] const float inv_own = inv;
-              const float inv = kKeysSeen == kRest ? 1.f : inv_own;
+              for (int i = 0; i < 8; ++i)
+                reinterpret_cast<float4*>(record + q * 32)[i] =
+                    make_float4(__uint_as_float(ov[4 * i]), __uint_as_float(ov[4 * i + 1]), __uint_as_float(ov[4 * i + 2]), __uint_as_float(ov[4 * i + 3]));
+            }
+          } else if (whole) {
+            if (row_ok) {
 #pragma unroll
               for (int t = 0; t < 4; ++t) {
                 uint4 x;
@@ -793,8 +800,11 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
               part[i * 256] = make_float4(__uint_as_float(ov[4 * i]), __uint_as_float(ov[4 * i + 1]), __uint_as_float(ov[4 * i + 2]), __uint_as_float(ov[4 * i + 3]));
           }
         }
-        if (kKeysSeen == kAll && whole && row_ok && p.records) p.records[row * (D + 4) + D] = lse;
-        if (!whole) p.part_ml[rec * 256 + g * kTileRows + r] = make_float2(n_g > 0 ? m_used + static_cast<float>(v_used) / sl2 : -INFINITY, n_g > 0 ? l : 0.f);
+        if constexpr (leaves_records(kKeysSeen)) {
+          if (row_ok)
+            *reinterpret_cast<float2*>(record + D) =
+                make_float2(n_g > 0 ? m_used * sl2 + static_cast<float>(v_used) - kRaised<kI8, kPvBf16> : -INFINITY, n_g > 0 ? l : 0.f);
+        } else if (!whole) p.part_ml[rec * 256 + g * kTileRows + r] = make_float2(n_g > 0 ? m_used + static_cast<float>(v_used) / sl2 : -INFINITY, n_g > 0 ? l : 0.f);
       }
       if (n_g > 0) {
         ptx::tcgen05_fence_before_thread_sync();
@@ -821,7 +831,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
 }
 
 // The records of a block that several shares have a part of, in order: CTA (x, y) has the block that goes on behind share x and 16 of its columns, a thread a row.
-template <bool kIsBf16, bool kI8, int D, Keys kKeysSeen = kPast>
+template <bool kIsBf16, int D, Keys kKeysSeen = kPast>
 __global__ void __launch_bounds__(256)
 attention_paged_tc_merge_kernel(uint16_t* __restrict__ o, const __grid_constant__ Params p) {
   ptx::launch_dependents();
@@ -830,8 +840,7 @@ attention_paged_tc_merge_kernel(uint16_t* __restrict__ o, const __grid_constant_
   const int4 mine = __ldcg(p.info + blockIdx.x);
   if (mine.y < 0) return;
   const int n = records_of(p.info);
-  int first, count;
-  tokens_of<kKeysSeen>(p, mine.y, first, count);
+  const int first = p.step.starts[mine.y], count = p.step.starts[mine.y + 1] - first;
   const int g = threadIdx.x >> 7, r = threadIdx.x & 127, r_token = r / p.group;
   const int token = (mine.w * 2 + g) * p.tokens + r_token;
   if (r_token >= p.tokens || token >= count) return;
@@ -855,31 +864,8 @@ attention_paged_tc_merge_kernel(uint16_t* __restrict__ o, const __grid_constant_
       acc[4 * q + 2] = fmaf(f, x.z, acc[4 * q + 2]), acc[4 * q + 3] = fmaf(f, x.w, acc[4 * q + 3]);
     }
   }
-  const int64_t row = static_cast<int64_t>(first + token) * p.heads_q + mine.z * p.group + (r - r_token * p.group);
-  [[maybe_unused]] const float lse = kKeysSeen == kPast ? 0.f : log_sum(gm * p.scale_log2 - kRaised<kI8, kIsBf16 && !kI8>, gl);
-  if (kKeysSeen == kAll && p.records) {
-    float* rec = p.records + row * (D + 4);
-    const float f = gl == 0.f ? 0.f : 1.f / gl;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(rec)[blockIdx.y * 4 + i] = make_float4(acc[4 * i] * f, acc[4 * i + 1] * f, acc[4 * i + 2] * f, acc[4 * i + 3] * f);
-    if (blockIdx.y == 0) rec[D] = lse;
-    return;
-  }
-  float inv = 1.0f / gl;
-  if constexpr (kKeysSeen == kRest) {
-    const float* rec = p.records + row * (D + 4);
-    const float2 w = join_weights(lse, __ldcg(rec + D));
-    const float f = w.x == 0.f ? 0.f : w.x * inv;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(rec) + blockIdx.y * 4 + i);
-      const float prior[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[4 * i + e] = weighed(f, acc[4 * i + e]) + weighed(w.y, prior[e]);
-    }
-    inv = 1.f;
-  }
-  uint16_t* orow = o + row * D + blockIdx.y * 16;
+  const float inv = 1.0f / gl;
+  uint16_t* orow = o + (static_cast<int64_t>(first + token) * p.heads_q + mine.z * p.group + (r - r_token * p.group)) * D + blockIdx.y * 16;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint4 x;

@@ -4,12 +4,14 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 #include "add_rms_norm.cuh"
 #include "attention_paged.cuh"
 #include "attention_paged_tc.cuh"
 #include "kv_pages.cuh"
 #include "launch.cuh"
+#include "route.hpp"
 
 namespace tsm100 {
 namespace ops {
@@ -190,7 +192,8 @@ inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& 
   p.run_log2 = run_log2;
   p.scale_log2 = base.scale_log2;
   p.status = base.status;
-  p.prefix = base.prefix, p.sequences = base.sequences, p.records = base.records;
+  p.prefix = base.prefix, p.large = base.large, p.prefix_table = base.prefix_table;
+  p.records = kKeys == paged::kShared ? base.shared : base.rest;
   CUtensorMap tq, tk, tv;
   TmapKey key;
   std::memset(&key, 0, sizeof key);
@@ -207,23 +210,29 @@ inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& 
     if (st == TSM100_OK) st = page_tmap(err, &tv, p.cache, p.cache.kv[1], run_log2, kIsBf16);
   }
   if (st != TSM100_OK) return st;
-  const size_t rows = static_cast<size_t>(ctas) * 2 * 256, part = rows * D * sizeof(float), ml = rows * sizeof(float2);
-  uint8_t* ws = nullptr;
-  st = take_scratch(err, reinterpret_cast<void**>(&ws), part + ml + ctas * sizeof(int4), s);
-  if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged: no device memory for partial results");
-  if (st != TSM100_OK) return st;
-  p.part = reinterpret_cast<float4*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(ws + part);
-  p.info = reinterpret_cast<int4*>(ws + part + ml);
   auto kern = tc::attention_paged_tc_kernel<kIsBf16, kI8, D, kKeys>;
   constexpr int smem = tc::smem_bytes<kI8, D>();
   cudaError_t e = set_dyn_smem_once(kern, smem);
-  if (e == cudaSuccess) e = launch_chained(kern, ctas, S::kThreads, smem, s, 0, tq, tk, tv, static_cast<uint16_t*>(o), p);
-  if (e == cudaSuccess) e = launch_chained(tc::attention_paged_tc_merge_kernel<kIsBf16, kI8, D, kKeys>, dim3(ctas, D / 16), 256, 0, s, 0, static_cast<uint16_t*>(o), p);
-  st = cuda_ok(err, e, "attention_paged_tc_kernel launch");
-  e = cudaFreeAsync(ws, s);
-  if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
-  return st;
+  if constexpr (paged::leaves_records(kKeys)) {
+    p.part = nullptr, p.part_ml = nullptr, p.info = nullptr;
+    if (e == cudaSuccess) e = launch_chained(kern, ctas, S::kThreads, smem, s, 0, tq, tk, tv, static_cast<uint16_t*>(o), p);
+    return cuda_ok(err, e, "attention_paged_tc_kernel launch");
+  } else {
+    const size_t rows = static_cast<size_t>(ctas) * 2 * 256, part = rows * D * sizeof(float), ml = rows * sizeof(float2);
+    uint8_t* ws = nullptr;
+    st = take_scratch(err, reinterpret_cast<void**>(&ws), part + ml + ctas * sizeof(int4), s);
+    if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged: no device memory for partial results");
+    if (st != TSM100_OK) return st;
+    p.part = reinterpret_cast<float4*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(ws + part);
+    p.info = reinterpret_cast<int4*>(ws + part + ml);
+    if (e == cudaSuccess) e = launch_chained(kern, ctas, S::kThreads, smem, s, 0, tq, tk, tv, static_cast<uint16_t*>(o), p);
+    if (e == cudaSuccess) e = launch_chained(tc::attention_paged_tc_merge_kernel<kIsBf16, D, kKeys>, dim3(ctas, D / 16), 256, 0, s, 0, static_cast<uint16_t*>(o), p);
+    st = cuda_ok(err, e, "attention_paged_tc_kernel launch");
+    e = cudaFreeAsync(ws, s);
+    if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
+    return st;
+  }
 }
 
 // The tiles of all sequences' caches dealt out evenly over the SMs, and what several of them have a part of merged (attention_paged.cuh).
@@ -234,12 +243,15 @@ inline int32_t attention_paged_few_launch(std::string* err, paged::Params p, con
   int32_t st = sm_count(err, &sms);
   if (st != TSM100_OK) return st;
   const unsigned ctas = static_cast<unsigned>(std::min(sms, paged::kMaxCtas));
-  const int64_t rows = std::min<int64_t>(L::kHeld, static_cast<int64_t>(p.step.max_new) * p.group);
-  const size_t part = static_cast<size_t>(ctas) * 2 * L::kHeld * L::kRec * sizeof(float);
-  st = take_scratch(err, reinterpret_cast<void**>(&p.part), part + ctas * sizeof(int4), s);
-  if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged: no device memory for partial results");
-  if (st != TSM100_OK) return st;
-  p.info = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(p.part) + part);
+  if constexpr (paged::leaves_records(kKeys)) {
+    p.part = nullptr, p.info = nullptr;
+  } else {
+    const size_t part = static_cast<size_t>(ctas) * 2 * L::kHeld * L::kRec * sizeof(float);
+    st = take_scratch(err, reinterpret_cast<void**>(&p.part), part + ctas * sizeof(int4), s);
+    if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged: no device memory for partial results");
+    if (st != TSM100_OK) return st;
+    p.info = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(p.part) + part);
+  }
   // boxes of a power of two of positions that a page is a multiple of; 8-bit steps come by copies of 16 bytes and more
   constexpr int kTop = L::kPos == 16 ? 4 : L::kPos == 32 ? 5 : 6;
   const int run_log2 = page_run_log2(p.cache.page_size, kTop);
@@ -270,11 +282,17 @@ inline int32_t attention_paged_few_launch(std::string* err, paged::Params p, con
     auto kern = boxes ? paged::attention_paged_kernel<T, kI8, D, true, kWide, kKeys> : paged::attention_paged_kernel<T, kI8, D, false, kWide, kKeys>;
     cudaError_t e = set_dyn_smem_once(kern, L::kSmem);
     if (e == cudaSuccess) e = launch_chained(kern, ctas, L::kThreads, L::kSmem, s, 0, map[0], map[1], static_cast<const T*>(q), static_cast<T*>(o), p);
-    if (e == cudaSuccess) e = launch_chained(paged::attention_paged_merge_kernel<T, D, L::kHeld, !std::is_same<T, __half>::value && !kI8, kKeys>, dim3(ctas, static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, 0, static_cast<T*>(o), p);
+    if constexpr (!paged::leaves_records(kKeys)) {
+      const int64_t rows = std::min<int64_t>(L::kHeld, static_cast<int64_t>(p.step.max_new) * p.group);
+      if (e == cudaSuccess)
+        e = launch_chained(paged::attention_paged_merge_kernel<T, D, L::kHeld, kKeys>, dim3(ctas, static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, 0, static_cast<T*>(o), p);
+    }
     st = cuda_ok(err, e, "attention_paged_kernel launch");
   }
-  const cudaError_t e = cudaFreeAsync(p.part, s);
-  if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
+  if constexpr (!paged::leaves_records(kKeys)) {
+    const cudaError_t e = cudaFreeAsync(p.part, s);
+    if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
+  }
   return st;
 }
 
@@ -292,14 +310,13 @@ inline int32_t attention_paged_typed(std::string* err, const paged::Params& p, b
   if (p.cache.d == 128) return i8 ? attention_paged_launch<T, true, 128, kKeys>(err, p, q, o, s) : attention_paged_launch<T, false, 128, kKeys>(err, p, q, o, s);
   return i8 ? attention_paged_launch<T, true, 64, kKeys>(err, p, q, o, s) : attention_paged_launch<T, false, 64, kKeys>(err, p, q, o, s);
 }
-// One translation unit for each kind of keys (serving.cu, serving_cross.cu, serving_prefix.cu).
+// One translation unit for each kind of keys (serving.cu, serving_cross.cu).
 template <paged::Keys kKeys>
 int32_t attention_paged_keys(std::string* err, const paged::Params& p, bool bf16, bool i8, const void* q, void* o, cudaStream_t s) {
   return bf16 ? attention_paged_typed<__nv_bfloat16, kKeys>(err, p, i8, q, o, s) : attention_paged_typed<__half, kKeys>(err, p, i8, q, o, s);
 }
 extern template int32_t attention_paged_keys<paged::kPast>(std::string*, const paged::Params&, bool, bool, const void*, void*, cudaStream_t);
 extern template int32_t attention_paged_keys<paged::kAll>(std::string*, const paged::Params&, bool, bool, const void*, void*, cudaStream_t);
-extern template int32_t attention_paged_keys<paged::kRest>(std::string*, const paged::Params&, bool, bool, const void*, void*, cudaStream_t);
 
 // What the attentions over pages ask of their arguments.  *nothing: there are no tokens.
 inline int32_t attention_paged_args(std::string* err, const char* op, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, int32_t dtype, int32_t heads_q, const void* q,
@@ -316,7 +333,8 @@ inline int32_t attention_paged_args(std::string* err, const char* op, const tsm1
   p->heads_q = heads_q;
   p->group = heads_q / kv->heads_kv;
   p->scale_log2 = static_cast<float>((1.0 / std::sqrt(static_cast<double>(kv->head_dim))) * 1.4426950408889634);
-  p->prefix = 0, p->sequences = 0, p->records = nullptr;
+  p->prefix = 0, p->large = 0, p->prefix_table = nullptr;
+  std::memset(&p->shared, 0, sizeof p->shared), std::memset(&p->rest, 0, sizeof p->rest);
   p->status = status;
   return TSM100_OK;
 }
@@ -342,7 +360,76 @@ inline int32_t attention_paged_cross(std::string* err, const tsm100_paged_kv* kv
   return attention_paged_keys<paged::kAll>(err, p, d->dtype == TSM100_BF16, kv->dtype == TSM100_I8, q, o, static_cast<cudaStream_t>(stream));
 }
 
-// All tokens against the prefix, once, as records; then each against its own positions, joined with its record.
+// ---------------------------------------------------------------------------
+// sequences that begin with the same pages
+// ---------------------------------------------------------------------------
+// All tokens against the prefix and each against its own positions, both as records, and then those joined.  Translation units by cache and head size
+// (serving_prefix*.cu).
+struct PrefixPlan {
+  bool shared_tc;  // the prefix on tcgen05, else in one stream with the rest
+  bool rest_tc;    // so are sequences of many rows
+  int run_log2;    // boxes of pages for tcgen05
+};
+template <typename T, bool kI8, int D>
+inline int32_t attention_prefix_launch(std::string* err, paged::Params p, const PrefixPlan& plan, const void* q, void* o, cudaStream_t s) {
+  namespace pg = paged;
+  constexpr size_t REC = D + 4;
+  int sms = 0;
+  int32_t st = sm_count(err, &sms);
+  if (st != TSM100_OK) return st;
+  const int64_t ctas = std::min(sms, pg::kMaxCtas), rows = static_cast<int64_t>(p.step.tokens) * p.heads_q, heads = p.cache.heads;
+  const int32_t tile_tokens = pg::tc::kTileRows / p.group;
+  pg::Join join;
+  join.cache = p.cache, join.step = p.step;
+  join.heads_q = p.heads_q, join.group = p.group;
+  join.prefix = p.prefix, join.large = p.large;
+  join.shared_tokens = plan.shared_tc ? tile_tokens : 0, join.large_tokens = tile_tokens;
+  auto units = [&](bool tc, int64_t tokens) { return tc ? (tokens + 2 * tile_tokens - 1) / (2 * tile_tokens) : (tokens * p.group + pg::kRows - 1) / pg::kRows; };
+  const int64_t shared_units = units(plan.shared_tc, p.step.tokens), rest_units = units(false, plan.rest_tc ? p.large / p.group : p.step.max_new);
+  const int64_t large_units = plan.rest_tc ? units(true, p.step.max_new) : 0;
+  const size_t few_part = ctas * 2 * pg::kRows * REC * sizeof(float), tc_part = ctas * 2 * 256 * REC * sizeof(float), whole = rows * REC * sizeof(float);
+  const size_t cuts = heads * (shared_units + p.step.batch * (rest_units + large_units)) * sizeof(int2);
+  uint8_t* ws = nullptr;
+  st = take_scratch(err, reinterpret_cast<void**>(&ws), 2 * whole + few_part + (plan.shared_tc ? tc_part : 0) + (plan.rest_tc ? tc_part : 0) + cuts, s);
+  if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged_prefix: no device memory for partial results");
+  if (st != TSM100_OK) return st;
+  uint8_t* at = ws;
+  auto place = [&](size_t bytes) { return reinterpret_cast<float*>(std::exchange(at, at + bytes)); };
+  join.shared.whole = place(whole), join.rest.whole = place(whole);
+  join.rest.part = place(few_part);
+  join.shared.part = plan.shared_tc ? place(tc_part) : join.rest.part;  // a share's two places are for whatever it has cut
+  join.rest_large.part = plan.rest_tc ? place(tc_part) : nullptr, join.rest_large.whole = join.rest.whole;
+  join.shared.units = static_cast<int32_t>(shared_units), join.rest.units = static_cast<int32_t>(rest_units), join.rest_large.units = static_cast<int32_t>(large_units);
+  join.shared.cut = reinterpret_cast<int2*>(at), join.rest.cut = join.shared.cut + heads * shared_units, join.rest_large.cut = join.rest.cut + heads * p.step.batch * rest_units;
+  p.shared = join.shared, p.rest = join.rest;
+  if (plan.shared_tc) {
+    st = attention_paged_tc_launch<T, kI8, D, pg::kShared>(err, p, plan.run_log2, q, o, s);
+    if (st == TSM100_OK) st = attention_paged_few_launch<T, kI8, D, true, pg::kRest>(err, p, q, o, s);
+  } else {
+    st = attention_paged_few_launch<T, kI8, D, true, pg::kBoth>(err, p, q, o, s);
+  }
+  if (st == TSM100_OK && plan.rest_tc) {
+    p.rest = join.rest_large;
+    st = attention_paged_tc_launch<T, kI8, D, pg::kRest>(err, p, plan.run_log2, q, o, s);
+  }
+  if (st == TSM100_OK) {
+    const int64_t at_once = pg::kJoinThreads / (D / 4), ys = (static_cast<int64_t>(p.step.max_new) * p.heads_q + at_once - 1) / at_once;
+    const dim3 grid(static_cast<unsigned>(p.step.batch), static_cast<unsigned>(std::min<int64_t>(ys, 64)));
+    st = cuda_ok(err, launch_chained(pg::attention_paged_join_kernel<T, D>, grid, pg::kJoinThreads, 0, s, 0, static_cast<T*>(o), join), "attention_paged_join_kernel launch");
+  }
+  const cudaError_t e = cudaFreeAsync(ws, s);
+  if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
+  return st;
+}
+template <bool kI8, int D>
+int32_t attention_prefix_held(std::string* err, const paged::Params& p, bool bf16, const PrefixPlan& plan, const void* q, void* o, cudaStream_t s) {
+  return bf16 ? attention_prefix_launch<__nv_bfloat16, kI8, D>(err, p, plan, q, o, s) : attention_prefix_launch<__half, kI8, D>(err, p, plan, q, o, s);
+}
+extern template int32_t attention_prefix_held<false, 64>(std::string*, const paged::Params&, bool, const PrefixPlan&, const void*, void*, cudaStream_t);
+extern template int32_t attention_prefix_held<false, 128>(std::string*, const paged::Params&, bool, const PrefixPlan&, const void*, void*, cudaStream_t);
+extern template int32_t attention_prefix_held<true, 64>(std::string*, const paged::Params&, bool, const PrefixPlan&, const void*, void*, cudaStream_t);
+extern template int32_t attention_prefix_held<true, 128>(std::string*, const paged::Params&, bool, const PrefixPlan&, const void*, void*, cudaStream_t);
+
 inline int32_t attention_paged_prefix(std::string* err, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, const tsm100_attention_paged_prefix_desc* d, const void* q,
                                       void* o, uint32_t* status, void* stream) {
   auto no = [&](const char* what) { return op_fail(err, TSM100_ERR_INVALID, std::string("attention_paged_prefix: ") + what); };
@@ -359,24 +446,16 @@ inline int32_t attention_paged_prefix(std::string* err, const tsm100_paged_kv* k
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = d->dtype == TSM100_BF16, i8 = kv->dtype == TSM100_I8;
   if (d->prefix_len == 0) return attention_paged_keys<paged::kPast>(err, p, bf16, i8, q, o, s);
-  void* records = nullptr;
-  st = take_scratch(err, &records, static_cast<size_t>(b->tokens) * d->heads_q * (kv->head_dim + 4) * sizeof(float), s);
-  if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged_prefix: no device memory for partial results");
-  if (st != TSM100_OK) return st;
-  p.records = static_cast<float*>(records);
-  p.prefix = d->prefix_len;
-  paged::Params shared = p;
-  shared.sequences = b->batch;
-  shared.step.batch = 1, shared.step.max_new = b->tokens;
-  shared.step.table = d->prefix, shared.step.pitch = d->prefix_len / kv->page_size;
-  st = attention_paged_keys<paged::kAll>(err, shared, bf16, i8, q, o, s);
-  if (st == TSM100_OK) {
-    p.step.table += d->prefix_len / kv->page_size;
-    st = attention_paged_keys<paged::kRest>(err, p, bf16, i8, q, o, s);
-  }
-  const cudaError_t e = cudaFreeAsync(records, s);
-  if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
-  return st;
+  PrefixPlan plan;
+  plan.run_log2 = page_run_log2(kv->page_size, 7);
+  const bool tc = p.group <= paged::tc::kMaxGroup && (i8 || plan.run_log2 >= 3);
+  plan.shared_tc = tc && route::prefix_on_tcgen05(static_cast<int64_t>(b->tokens) * p.group, d->prefix_len, kv->heads_kv, kv->head_dim, i8);
+  plan.rest_tc = tc && static_cast<int64_t>(b->max_new) * p.group > route::kPrefixFewRows;
+  p.large = plan.rest_tc ? static_cast<int32_t>(route::kPrefixFewRows) : 0;
+  p.prefix = d->prefix_len, p.prefix_table = d->prefix;
+  p.step.table += d->prefix_len / kv->page_size;
+  if (kv->head_dim == 128) return i8 ? attention_prefix_held<true, 128>(err, p, bf16, plan, q, o, s) : attention_prefix_held<false, 128>(err, p, bf16, plan, q, o, s);
+  return i8 ? attention_prefix_held<true, 64>(err, p, bf16, plan, q, o, s) : attention_prefix_held<false, 64>(err, p, bf16, plan, q, o, s);
 }
 
 }  // namespace ops

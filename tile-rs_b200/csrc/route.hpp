@@ -327,6 +327,14 @@ inline bool softmax_twice_skip(int64_t vectors, int threads, int unroll) {
   return (div_up(vectors, step) * step - vectors) * 8 > vectors;
 }
 
+// Attention of sequences that begin with the same pages: are the prefix's rows (all tokens times the heads of a group) tcgen05's, 256 at a time, or the other kernel's, 16 at a time?
+inline bool prefix_on_tcgen05(int64_t rows, int64_t prefix, int heads_kv, int head_dim, bool i8) {
+  const int64_t passes = div_up(rows, 16), bytes = 2 * prefix * heads_kv * head_dim * (i8 ? 1 : 2);
+  return (passes - 1) * bytes > (i8 ? 64ll << 20 : 24ll << 20);
+}
+// Rows of a sequence's own tokens beyond which its own positions are tcgen05's.
+constexpr int64_t kPrefixFewRows = 64;
+
 // Rotary embedding: how many heads a thread walks through (`blocks` blocks of 256 threads for one head group).  Few tokens: groups of four
 // heads or more, as many as make two blocks per SM; the angles are computed once per group.  With a block for every second SM that
 // pays for any number of heads (128 tokens of 32 x 128 bf16 6.3 in one group, 3.1 in eight), with one for nearly every SM only for many (2048 of
