@@ -16,7 +16,7 @@ fn main() {
         "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC,-fopenmp",
     ];
     let mut objects = Vec::new();
-    for src in ["runtime.cu", "capi_ops.cu", "serving_w4_bf16.cu", "serving_w4_f16.cu", "serving.cu", "serving_cross.cu", "serving_prefix_16bit_64.cu", "serving_prefix_16bit_128.cu", "serving_prefix_i8_64.cu", "serving_prefix_i8_128.cu", "serving_i8.cu", "multi.cu", "inputs.cpp", "emit.cpp"] {
+    for src in ["runtime.cu", "capi_ops.cu", "serving_w4_bf16.cu", "serving_w4_f16.cu", "serving.cu", "serving_cross_16bit.cu", "serving_cross_i8.cu", "serving_prefix_16bit_64.cu", "serving_prefix_16bit_128.cu", "serving_prefix_i8_64.cu", "serving_prefix_i8_128.cu", "serving_i8.cu", "multi.cu", "inputs.cpp", "emit.cpp"] {
         let obj = out.join(format!("{src}.o"));
         let mut cmd = Command::new(&nvcc);
         cmd.args(common).arg(format!("-I{}", include.display()));

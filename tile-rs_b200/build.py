@@ -25,7 +25,7 @@ LIB_PATH = PKG_DIR / "libtile_sm100.so"
 # the operators for CPython without ctypes (csrc/python.cpp); absent where there are no CPython headers
 FAST_PATH = PKG_DIR / ("_tile_sm100" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
-CUDA_SOURCES = ["runtime.cu", "capi_ops.cu", "serving_w4_bf16.cu", "serving_w4_f16.cu", "serving.cu", "serving_cross.cu", "serving_prefix_16bit_64.cu", "serving_prefix_16bit_128.cu",
+CUDA_SOURCES = ["runtime.cu", "capi_ops.cu", "serving_w4_bf16.cu", "serving_w4_f16.cu", "serving.cu", "serving_cross_16bit.cu", "serving_cross_i8.cu", "serving_prefix_16bit_64.cu", "serving_prefix_16bit_128.cu",
                 "serving_prefix_i8_64.cu", "serving_prefix_i8_128.cu", "serving_i8.cu", "multi.cu"]
 CXX_SOURCES = ["inputs.cpp", "emit.cpp"]
 

@@ -27,16 +27,6 @@ namespace paged {
 
 namespace mma = attn_decode::mma;
 
-// Which keys a token sees.
-//   kPast    positions 0 .. its own of its sequence
-//   kAll     all positions of its sequence, however many tokens that has (attention to an encoder's states; none: zeros)
-//   kShared  the first p.prefix positions, which lie in the same pages for all sequences: all tokens of the call are the rows of one sequence, number -1
-//   kRest    positions p.prefix .. its own; a sequence with more than p.large rows is tcgen05's (attention_paged_tc.cuh), any other the other kernel's
-//   kBoth    as kShared and as kRest, as two results, in one stream
-// The last three leave records, which attention_paged_join_kernel puts together.
-enum Keys { kPast, kAll, kShared, kRest, kBoth };
-__host__ __device__ constexpr bool leaves_records(Keys k) { return k == kShared || k == kRest || k == kBoth; }
-
 constexpr int kRows = 16;     // of a pass, at most
 constexpr int kMaxCtas = 1024;
 // What beginning and ending a pair costs, in tiles: shares are as long in tiles and these.  64 sequences of up to 6000 positions in 8 bits, costs of 4, 8, 12, 16, 24, 32 tiles:
@@ -56,25 +46,12 @@ struct Tile {
   static_assert(kSmem + 224 + 72 * kWarps <= 227 * 1024, "shared memory of one CTA, with what is declared in the kernel");
 };
 
-// Records of rows: D numbers of O, not normalised, the logarithm to base 2 of what the weights were taken against, their sum, two unused.  A unit (or block) of rows that one
-// share has all of leaves them in `whole`, by token and head; one that is cut, in the shares' places, which `cut` tells by the unit.
-struct Records {
-  float* whole;       // [tokens][heads_q]
-  float* part;        // [CTA][2][held]
-  int2* cut;          // the share that the unit's keys begin in, and how many shares there are, 0 if one; [heads_kv][units], kRest: [batch][heads_kv][units]
-  int32_t units;      // of a KV head (of a sequence)
-};
-
 struct Params {
   pages::Cache cache;
   pages::Batch step;
   int32_t heads_q, group;
   int32_t run_log2;   // positions a copy brings: a power of two that divides the page (kTma), else the whole tile
   float scale_log2;   // log2(e) / sqrt(d)
-  int32_t prefix;     // Keys
-  int32_t large;      // 0: no sequence is
-  const int32_t* prefix_table;
-  Records shared, rest;  // (Keys with records: instead of part)
   float* part;        // [CTA][2][kHeld][kRec]: of a pair that began in an earlier share, of one that goes on in the next
   int4* info;         // [CTA]: 1 if a pair of earlier shares ends in this one, 2 if it goes on; sequence and unit of the pair that goes on in the next, or -1
   uint32_t* status;
@@ -95,29 +72,9 @@ struct Part {
   int64_t start;         // where the unit begins
   bool there;
 };
-// The tokens of sequence b and the keys that they see; false, and reported, if they contradict each other or the call.  kRest counts positions from the
-// prefix on, and so does its table.
-template <Keys kKeys, typename P>
-__device__ __forceinline__ bool sequence(const P& p, int b, int& first, int& count, int& len, uint32_t* status, uint32_t site) {
-  if (kKeys == kPast) return pages::sequence(p.step, p.cache.page_size, b, first, count, len, status, site);
-  if (kKeys == kAll) return pages::sequence<false>(p.step, p.cache.page_size, b, first, count, len, status, site) && len > 0;
-  if (b < 0) {
-    first = 0, count = min(max(p.step.starts[p.step.batch], 0), p.step.tokens), len = p.prefix;
-    return count > 0;
-  }
-  if (!pages::sequence(p.step, p.cache.page_size, b, first, count, len, status, site)) return false;
-  len -= p.prefix;
-  if (len >= count) return true;
-  pages::report(status, site);
-  return false;
-}
-template <typename P>
-__device__ __forceinline__ bool is_large(const P& p, int count) { return p.large > 0 && static_cast<int64_t>(count) * p.group > p.large; }
-
-template <Keys kKeys, int kPos, int kHeld>
+template <int kPos, int kHeld>
 __device__ __forceinline__ int64_t sequence_tiles(const Params& p, int b, Seq& s, uint32_t* status) {
-  if (!sequence<kKeys>(p, b, s.first, s.count, s.len, status, 143)) return 0;
-  if (leaves_records(kKeys) && b >= 0 && is_large(p, s.count)) return 0;
+  if (!pages::sequence(p.step, p.cache.page_size, b, s.first, s.count, s.len, status, 143)) return 0;
   s.tiles = (s.len + kPos - 1) / kPos;
   s.passes = static_cast<int>((static_cast<int64_t>(s.count) * p.group + kHeld - 1) / kHeld);
   s.units = s.passes * p.cache.heads;
@@ -166,27 +123,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {  // an 8 x 8 tile o
   return r;
 }
 
-// kAll: a sequence without positions has zeros for results.  Of all threads of a grid, which deal each such sequence's out.
-template <int D, Keys kKeys, typename T, typename P>
-__device__ __forceinline__ void put_zeros(T* o, const P& p) {
-  if constexpr (kKeys == kAll) {
-    const int64_t threads = static_cast<int64_t>(gridDim.x) * gridDim.y * blockDim.x;
-    const int64_t mine = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x;
-    for (int b0 = 0; b0 < p.step.batch; b0 += 32) {  // a warp looks at 32 sequences at once
-      const int b = b0 + static_cast<int>(threadIdx.x & 31);
-      unsigned empty = __ballot_sync(0xffffffffu, b < p.step.batch && p.step.lens[b] == 0);
-      for (; empty != 0u; empty &= empty - 1u) {
-        int first, count, len;
-        if (!pages::sequence<false>(p.step, p.cache.page_size, b0 + __ffs(empty) - 1, first, count, len, nullptr, 0)) continue;
-        uint4* to = reinterpret_cast<uint4*>(o + static_cast<int64_t>(first) * p.heads_q * D);
-        const int64_t n = static_cast<int64_t>(count) * p.heads_q * (D / 8);
-        for (int64_t i = mine; i < n; i += threads) to[i] = make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
-  }
-}
-
-template <typename T, bool kI8, int D, bool kTma, bool kWide, Keys kKeys = kPast>
+template <typename T, bool kI8, int D, bool kTma, bool kWide>
 __global__ void __launch_bounds__((Tile<kI8, D, kWide>::kThreads), 1)
 attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const T* __restrict__ q, T* __restrict__ o,
                        const __grid_constant__ Params p) {
@@ -218,7 +155,6 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 
   // The stream: how long it is, and the sequence in which this CTA's share begins.
   const int batch = p.step.batch;
-  constexpr int kFirst = kKeys == kBoth ? -1 : 0;  // the stream's first sequence
   auto block_scan = [&](int64_t v, int64_t& before) {  // of all threads; answers the total
     int64_t x = v;
 #pragma unroll
@@ -239,21 +175,21 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     return total;
   };
   int64_t total = 0, before = 0, own = 0;
-  for (int base = kFirst; base < batch; base += kThreads) {
+  for (int base = 0; base < batch; base += kThreads) {
     Seq s;
-    own = base + tid < batch ? sequence_tiles<kKeys, TP, kHeld>(p, base + tid, s, p.status) : 0;
+    own = base + tid < batch ? sequence_tiles<TP, kHeld>(p, base + tid, s, p.status) : 0;
     total += block_scan(own, before);
   }
   const int64_t per = (total + gridDim.x - 1) / gridDim.x;
   const int64_t t0 = min(total, blockIdx.x * per), t1 = min(total, t0 + per);
   if (t0 < t1) {
-    if (batch - kFirst <= kThreads) {
-      if (before <= t0 && t0 < before + own) first_seq = kFirst + tid, scan[kWarps] = before;
+    if (batch <= kThreads) {
+      if (before <= t0 && t0 < before + own) first_seq = tid, scan[kWarps] = before;
     } else {
       int64_t sum = 0;
-      for (int base = kFirst; base < batch; base += kThreads) {
+      for (int base = 0; base < batch; base += kThreads) {
         Seq s;
-        own = base + tid < batch ? sequence_tiles<kKeys, TP, kHeld>(p, base + tid, s, nullptr) : 0;
+        own = base + tid < batch ? sequence_tiles<TP, kHeld>(p, base + tid, s, nullptr) : 0;
         const int64_t here = block_scan(own, before);
         if (sum + before <= t0 && t0 < sum + before + own) first_seq = base + tid, scan[kWarps] = sum + before;
         sum += here;
@@ -262,7 +198,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   }
   __syncthreads();
   if (t0 >= t1) {
-    if (!leaves_records(kKeys) && tid == 0) p.info[blockIdx.x] = make_int4(0, -1, -1, 0);
+    if (tid == 0) p.info[blockIdx.x] = make_int4(0, -1, -1, 0);
     return;
   }
   auto cut = [&](Part& x) {  // what the share has of the unit, from its beginning on
@@ -272,7 +208,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   };
   auto open = [&](Part& x, int b, int64_t base) {  // the first sequence from b on that has units
     for (; b < batch; ++b)
-      if (sequence_tiles<kKeys, TP, kHeld>(p, b, x.seq, nullptr) > 0) break;
+      if (sequence_tiles<TP, kHeld>(p, b, x.seq, nullptr) > 0) break;
     x.seq.b = b, x.seq.base = base;
     x.unit = 0, x.start = base;
   };
@@ -339,7 +275,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       if ((lane << lb) < TP && pos < len_ahead) {
         const int nth = page_bits >= 0 ? pos >> page_bits : pos / ps;
         at_ahead = pos - nth * ps;
-        int page = kKeys == kBoth && b_ahead < 0 ? p.prefix_table[nth] : p.step.table[static_cast<int64_t>(b_ahead) * p.step.pitch + nth];
+        int page = p.step.table[static_cast<int64_t>(b_ahead) * p.step.pitch + nth];
         if (page < 0 || page >= p.cache.pages) pages::report(p.status, 144), page = 0;
         row_ahead += page * heads;
       }
@@ -368,12 +304,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       for (int i = lane; i < TP * kChunks; i += 32) {
         const int r = i / kChunks, c = i % kChunks, pos = pos0 + r;
         const bool ok = r < here;
-        int pg = 0;
-        if (kKeys == kBoth && b_ahead < 0) {
-          if (ok && ((pg = p.prefix_table[pos / ps]) < 0 || pg >= p.cache.pages)) pages::report(p.status, 144), pg = 0;
-        } else if (ok) {
-          pg = max(0, pages::page_of(p.cache, p.step, b_ahead, pos, p.status, 144));
-        }
+        const int pg = ok ? max(0, pages::page_of(p.cache, p.step, b_ahead, pos, p.status, 144)) : 0;
         const int64_t row = (static_cast<int64_t>(pg) * heads + head_ahead) * ps + (ok ? pos % ps : 0);
         mma::cp_async_16(dst + at(r, c), static_cast<const uint8_t*>(p.cache.kv[load_v]) + row * L::kRowBytes + c * 16, ok);
         if (kI8 && c == 0) ptx::cp_async_4(dst_steps + r * 4, p.cache.scales[load_v] + row, ok);
@@ -426,7 +357,6 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
   for (int which = 0; parts[which].there; which ^= 1) {
     const Part& now = parts[which];
     const int unit = now.unit, begin = now.begin, end = now.end;
-    [[maybe_unused]] const int64_t start = now.start;
     struct {
       int b, first, count, len, tiles, passes;
     } const seq = {now.seq.b, now.seq.first, now.seq.count, now.seq.len, now.seq.tiles, now.seq.passes};
@@ -478,10 +408,10 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
       for (int e = 0; e < 2; ++e) {
         q_factor[n][e] = __shfl_sync(0xffffffffu, factor, (2 * tq + e) * 4) * p.scale_log2;
         const int mine = row0 + min(n * 8 + 2 * tq + e, rows - 1);
-        limit[n][e] = kKeys == kAll || (kKeys == kBoth && seq.b < 0) ? seq.len - 1 : seq.len - seq.count + mine / p.group;
+        limit[n][e] = seq.len - seq.count + mine / p.group;
       }
     }
-    const int least = kKeys == kAll || (kKeys == kBoth && seq.b < 0) ? seq.len - 1 : seq.len - seq.count + row0 / p.group;  // the first row's last position: tiles up to it need no masks
+    const int least = seq.len - seq.count + row0 / p.group;  // the first row's last position: tiles up to it need no masks
     float oacc[KSTEPS][NB][4];
 #pragma unroll
     for (int c = 0; c < KSTEPS; ++c)
@@ -696,14 +626,7 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
           oo.x = fmaf(x.x, wgt, oo.x), oo.y = fmaf(x.y, wgt, oo.y), oo.z = fmaf(x.z, wgt, oo.z), oo.w = fmaf(x.w, wgt, oo.w);
         }
         const int r = half * 8 + rr;
-        if constexpr (leaves_records(kKeys)) {
-          const Records& to = kKeys == kBoth && seq.b < 0 ? p.shared : p.rest;
-          const int token = (row0 + r) / p.group, h = head * p.group + (row0 + r) % p.group;
-          float* out = whole ? to.whole + (static_cast<int64_t>(seq.first + token) * p.heads_q + h) * REC
-                             : to.part + ((static_cast<int64_t>(blockIdx.x) * 2 + (begin == 0 ? 1 : 0)) * kHeld + r) * REC;
-          *reinterpret_cast<float4*>(out + dd) = oo;
-          if (dd == 0) *reinterpret_cast<float2*>(out + D) = make_float2(mm - kRaised<kMmaBf16>, ll);
-        } else if (whole) {
+        if (whole) {
           const int token = (row0 + r) / p.group, h = head * p.group + (row0 + r) % p.group;
           const float inv = 1.f / ll;
           *reinterpret_cast<uint2*>(o + (static_cast<int64_t>(seq.first + token) * p.heads_q + h) * D + dd) =
@@ -715,20 +638,11 @@ attention_paged_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         }
       }
     }
-    if constexpr (leaves_records(kKeys)) {
-      if (tid == 0 && begin == 0) {
-        const int last = static_cast<int>((start + kUnitCost + seq.tiles - 1) / per);  // the share that has the unit's last tile
-        const Records& to = kKeys == kBoth && seq.b < 0 ? p.shared : p.rest;
-        to.cut[(seq.b < 0 ? 0 : static_cast<int64_t>(seq.b) * heads * to.units) + static_cast<int64_t>(head) * to.units + (unit - head * seq.passes)] =
-            make_int2(static_cast<int>(blockIdx.x), end == seq.tiles ? 0 : last - static_cast<int>(blockIdx.x) + 1);
-      }
-    } else {
-      if (begin > 0) head_state = end == seq.tiles ? 1 : 2;
-      else if (end < seq.tiles) tail_b = seq.b, tail_unit = unit;
-    }
+    if (begin > 0) head_state = end == seq.tiles ? 1 : 2;
+    else if (end < seq.tiles) tail_b = seq.b, tail_unit = unit;
     turn = (turn + end - begin) % kWarps;
   }
-  if (!leaves_records(kKeys) && tid == 0) p.info[blockIdx.x] = make_int4(head_state, tail_b, tail_unit, 0);
+  if (tid == 0) p.info[blockIdx.x] = make_int4(head_state, tail_b, tail_unit, 0);
   if constexpr (!kTma) mma::cp_async_wait<0>();
   if (*abort_flag != 0u) {
     // a wait gave up: copies in flight land before the shared memory is released
@@ -753,14 +667,13 @@ __device__ __forceinline__ int records_of(const int4* info) {
 }
 
 // The records of a pair that several shares have a part of, in order; a warp per row, CTA (x, y) rows 4 y .. of the pair that goes on behind share x.
-template <typename T, int D, int kHeld, Keys kKeys = kPast>
+template <typename T, int D, int kHeld>
 __global__ void __launch_bounds__(128)
 attention_paged_merge_kernel(T* __restrict__ o, const __grid_constant__ Params p) {
   constexpr int REC = D + 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 4 + warp;
   ptx::launch_dependents();
   ptx::wait_prior_grid();
-  put_zeros<D, kKeys>(o, p);
   const int4 mine = __ldcg(p.info + blockIdx.x);
   if (mine.y < 0) return;
   const int n = records_of(p.info);
@@ -798,97 +711,6 @@ attention_paged_merge_kernel(T* __restrict__ o, const __grid_constant__ Params p
     constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
     *reinterpret_cast<uint2*>(o + (static_cast<int64_t>(first + row / p.group) * p.heads_q + head * p.group + row % p.group) * D + lane * 4) =
         make_uint2(mma::pack2<kIsBf16>(oo.x * inv, oo.y * inv), mma::pack2<kIsBf16>(oo.z * inv, oo.w * inv));
-  }
-}
-
-// What a row sees of the prefix and of its sequence's own positions, put together.  CTA (b, y) has rows of sequence b, D / 4 threads a row; a row's records are in up to as many
-// places as there are shares, and all are asked for before the first is used.  A part whose scores are all -inf weighs nothing beside another.
-struct Join {
-  pages::Cache cache;
-  pages::Batch step;
-  int32_t heads_q, group;
-  int32_t prefix, large;
-  Records shared, rest, rest_large;
-  int32_t shared_tokens, large_tokens;  // of a tile, where the records are tcgen05's (256 rows a block); 0: 16 rows a unit
-};
-constexpr int kJoinThreads = 128;
-// A row's records: the first, and what lies between one share's and the next.
-template <int D>
-struct Pieces {
-  const float* first;
-  const float* next;
-  int64_t step;
-  int n;
-  __device__ __forceinline__ const float* at(int i) const { return i == 0 ? first : next + (i - 1) * step; }
-};
-template <int D>
-__device__ __forceinline__ Pieces<D> pieces(const Records& rec, int tile_tokens, int64_t cut0, int head, int group, int token, int h, int64_t row) {
-  constexpr int REC = D + 4;
-  int unit, r, held;
-  if (tile_tokens > 0) {
-    unit = token / (2 * tile_tokens);
-    const int t = token - unit * 2 * tile_tokens, g = t >= tile_tokens ? 1 : 0;
-    r = g * 128 + (t - g * tile_tokens) * group + h, held = 256;
-  } else {
-    const int64_t at = static_cast<int64_t>(token) * group + h;
-    unit = static_cast<int>(at / kRows), r = static_cast<int>(at % kRows), held = kRows;
-  }
-  const int2 cut = __ldcg(rec.cut + cut0 + static_cast<int64_t>(head) * rec.units + unit);
-  Pieces<D> x;
-  x.n = max(cut.y, 1);
-  x.step = static_cast<int64_t>(2) * held * REC;
-  x.first = cut.y == 0 ? rec.whole + row * REC : rec.part + ((static_cast<int64_t>(cut.x) * 2 + 1) * held + r) * REC;
-  x.next = rec.part + (static_cast<int64_t>(cut.x + 1) * 2 * held + r) * REC;
-  return x;
-}
-template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads)
-attention_paged_join_kernel(T* o, const __grid_constant__ Join p) {
-  constexpr int kLanes = D / 4, kRowsAt = kJoinThreads / kLanes;
-  constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
-  ptx::launch_dependents_if_few();
-  ptx::wait_prior_grid();
-  int first, count, len;
-  if (!sequence<kRest>(p, static_cast<int>(blockIdx.x), first, count, len, nullptr, 0)) return;
-  const bool large = is_large(p, count);
-  const Records& rest = large ? p.rest_large : p.rest;
-  const int rest_tokens = large ? p.large_tokens : 0, lane = threadIdx.x % kLanes;
-  for (int64_t i = static_cast<int64_t>(blockIdx.y) * kRowsAt + threadIdx.x / kLanes; i < static_cast<int64_t>(count) * p.heads_q; i += static_cast<int64_t>(gridDim.y) * kRowsAt) {
-    const int token = static_cast<int>(i / p.heads_q), hq = static_cast<int>(i - static_cast<int64_t>(token) * p.heads_q), head = hq / p.group, h = hq - head * p.group;
-    const int64_t row = static_cast<int64_t>(first + token) * p.heads_q + hq;
-    const Pieces<D> a = pieces<D>(p.shared, p.shared_tokens, 0, head, p.group, first + token, h, row);
-    const Pieces<D> b = pieces<D>(rest, rest_tokens, static_cast<int64_t>(blockIdx.x) * p.cache.heads * rest.units, head, p.group, token, h, row);
-    const int n = a.n + b.n;
-    float m = -INFINITY, l = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kAtOnce = 8;
-    for (int j0 = 0; j0 < n; j0 += kAtOnce) {
-      float2 ml[kAtOnce];
-      float4 y[kAtOnce];
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        ml[j] = make_float2(-INFINITY, 0.f), y[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (j0 + j < n) {
-          const float* rec = j0 + j < a.n ? a.at(j0 + j) : b.at(j0 + j - a.n);
-          ml[j] = __ldcg(reinterpret_cast<const float2*>(rec + D)), y[j] = __ldcg(reinterpret_cast<const float4*>(rec) + lane);
-        }
-      }
-      float top = m;
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) top = fmaxf(top, ml[j].x);
-      const float keep = m == -INFINITY ? 0.f : exp2f(m - top);
-      // a part that has no scores but -inf weighs nothing; it is added all the same, because one of NaN scores has that maximum too
-      l *= keep, x.x *= keep, x.y *= keep, x.z *= keep, x.w *= keep;
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        const float w = ml[j].x == -INFINITY ? 0.f : exp2f(ml[j].x - top);
-        l = fmaf(w, ml[j].y, l);
-        x.x = fmaf(w, y[j].x, x.x), x.y = fmaf(w, y[j].y, x.y), x.z = fmaf(w, y[j].z, x.z), x.w = fmaf(w, y[j].w, x.w);
-      }
-      m = top;
-    }
-    const float inv = 1.f / l;
-    *reinterpret_cast<uint2*>(o + row * D + lane * 4) = make_uint2(mma::pack2<kIsBf16>(x.x * inv, x.y * inv), mma::pack2<kIsBf16>(x.z * inv, x.w * inv));
   }
 }
 

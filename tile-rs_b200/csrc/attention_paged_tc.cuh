@@ -18,6 +18,7 @@
 #pragma once
 
 #include "attention_paged.cuh"
+#include "attention_paged_rows.cuh"
 #include "attention_tc.cuh"
 #include "kv_pages.cuh"
 #include "ptx.cuh"

@@ -8,6 +8,7 @@
 
 #include "add_rms_norm.cuh"
 #include "attention_paged.cuh"
+#include "attention_paged_rows.cuh"
 #include "attention_paged_tc.cuh"
 #include "kv_pages.cuh"
 #include "launch.cuh"
@@ -176,8 +177,13 @@ inline int32_t page_tmap(std::string* err, CUtensorMap* map, const pages::Cache&
 }
 
 // Chunks of tokens: tcgen05 (attention_paged_tc.cuh).
+struct PrefixArgs {  // of the attentions that leave records (attention_paged_rows.cuh)
+  int32_t prefix, large;
+  const int32_t* table;
+  paged::Records shared, rest;
+};
 template <typename T, bool kI8, int D, paged::Keys kKeys>
-inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& base, int run_log2, const void* q, void* o, cudaStream_t s) {
+inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& base, int run_log2, const void* q, void* o, cudaStream_t s, const PrefixArgs& more = PrefixArgs()) {
   namespace tc = paged::tc;
   constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
   using S = tc::Shape<kI8, D>;
@@ -192,8 +198,8 @@ inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& 
   p.run_log2 = run_log2;
   p.scale_log2 = base.scale_log2;
   p.status = base.status;
-  p.prefix = base.prefix, p.large = base.large, p.prefix_table = base.prefix_table;
-  p.records = kKeys == paged::kShared ? base.shared : base.rest;
+  p.prefix = more.prefix, p.large = more.large, p.prefix_table = more.table;
+  p.records = kKeys == paged::kShared ? more.shared : more.rest;
   CUtensorMap tq, tk, tv;
   TmapKey key;
   std::memset(&key, 0, sizeof key);
@@ -236,22 +242,19 @@ inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& 
 }
 
 // The tiles of all sequences' caches dealt out evenly over the SMs, and what several of them have a part of merged (attention_paged.cuh).
-template <typename T, bool kI8, int D, bool kWide, paged::Keys kKeys>
+template <typename T, bool kI8, int D, bool kWide>
 inline int32_t attention_paged_few_launch(std::string* err, paged::Params p, const void* q, void* o, cudaStream_t s) {
   using L = paged::Tile<kI8, D, kWide>;
   int sms = 0;
   int32_t st = sm_count(err, &sms);
   if (st != TSM100_OK) return st;
   const unsigned ctas = static_cast<unsigned>(std::min(sms, paged::kMaxCtas));
-  if constexpr (paged::leaves_records(kKeys)) {
-    p.part = nullptr, p.info = nullptr;
-  } else {
-    const size_t part = static_cast<size_t>(ctas) * 2 * L::kHeld * L::kRec * sizeof(float);
-    st = take_scratch(err, reinterpret_cast<void**>(&p.part), part + ctas * sizeof(int4), s);
-    if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged: no device memory for partial results");
-    if (st != TSM100_OK) return st;
-    p.info = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(p.part) + part);
-  }
+  const int64_t rows = std::min<int64_t>(L::kHeld, static_cast<int64_t>(p.step.max_new) * p.group);
+  const size_t part = static_cast<size_t>(ctas) * 2 * L::kHeld * L::kRec * sizeof(float);
+  st = take_scratch(err, reinterpret_cast<void**>(&p.part), part + ctas * sizeof(int4), s);
+  if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged: no device memory for partial results");
+  if (st != TSM100_OK) return st;
+  p.info = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(p.part) + part);
   // boxes of a power of two of positions that a page is a multiple of; 8-bit steps come by copies of 16 bytes and more
   constexpr int kTop = L::kPos == 16 ? 4 : L::kPos == 32 ? 5 : 6;
   const int run_log2 = page_run_log2(p.cache.page_size, kTop);
@@ -279,44 +282,32 @@ inline int32_t attention_paged_few_launch(std::string* err, paged::Params p, con
     st = make_tmap(err, &map[i], key, kI8 ? 1 : 2);
   }
   if (st == TSM100_OK) {
-    auto kern = boxes ? paged::attention_paged_kernel<T, kI8, D, true, kWide, kKeys> : paged::attention_paged_kernel<T, kI8, D, false, kWide, kKeys>;
+    auto kern = boxes ? paged::attention_paged_kernel<T, kI8, D, true, kWide> : paged::attention_paged_kernel<T, kI8, D, false, kWide>;
     cudaError_t e = set_dyn_smem_once(kern, L::kSmem);
     if (e == cudaSuccess) e = launch_chained(kern, ctas, L::kThreads, L::kSmem, s, 0, map[0], map[1], static_cast<const T*>(q), static_cast<T*>(o), p);
-    if constexpr (!paged::leaves_records(kKeys)) {
-      const int64_t rows = std::min<int64_t>(L::kHeld, static_cast<int64_t>(p.step.max_new) * p.group);
-      if (e == cudaSuccess)
-        e = launch_chained(paged::attention_paged_merge_kernel<T, D, L::kHeld, kKeys>, dim3(ctas, static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, 0, static_cast<T*>(o), p);
-    }
+    if (e == cudaSuccess) e = launch_chained(paged::attention_paged_merge_kernel<T, D, L::kHeld>, dim3(ctas, static_cast<unsigned>((rows + 3) / 4)), 128, 0, s, 0, static_cast<T*>(o), p);
     st = cuda_ok(err, e, "attention_paged_kernel launch");
   }
-  if constexpr (!paged::leaves_records(kKeys)) {
-    const cudaError_t e = cudaFreeAsync(p.part, s);
-    if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
-  }
+  const cudaError_t e = cudaFreeAsync(p.part, s);
+  if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
   return st;
 }
 
 // More rows than a tile of mma.sync has would go over their keys again: those take tcgen05, as long as a group's heads fit a tile and boxes of eight positions a page.
-template <typename T, bool kI8, int D, paged::Keys kKeys>
+inline bool paged_fits_tcgen05(int group, bool i8, int run_log2) { return group <= paged::tc::kMaxGroup && (i8 || run_log2 >= 3); }
+template <typename T, bool kI8, int D>
 inline int32_t attention_paged_launch(std::string* err, const paged::Params& p, const void* q, void* o, cudaStream_t s) {
   const int64_t rows = static_cast<int64_t>(p.step.max_new) * p.group;
   const int wide = page_run_log2(p.cache.page_size, 7);
-  if (rows > paged::kRows && p.group <= paged::tc::kMaxGroup && (kI8 || wide >= 3)) return attention_paged_tc_launch<T, kI8, D, kKeys>(err, p, wide, q, o, s);
-  return rows > 8 ? attention_paged_few_launch<T, kI8, D, true, kKeys>(err, p, q, o, s) : attention_paged_few_launch<T, kI8, D, false, kKeys>(err, p, q, o, s);
+  if (rows > paged::kRows && paged_fits_tcgen05(p.group, kI8, wide)) return attention_paged_tc_launch<T, kI8, D, paged::kPast>(err, p, wide, q, o, s);
+  return rows > 8 ? attention_paged_few_launch<T, kI8, D, true>(err, p, q, o, s) : attention_paged_few_launch<T, kI8, D, false>(err, p, q, o, s);
 }
 
-template <typename T, paged::Keys kKeys>
+template <typename T>
 inline int32_t attention_paged_typed(std::string* err, const paged::Params& p, bool i8, const void* q, void* o, cudaStream_t s) {
-  if (p.cache.d == 128) return i8 ? attention_paged_launch<T, true, 128, kKeys>(err, p, q, o, s) : attention_paged_launch<T, false, 128, kKeys>(err, p, q, o, s);
-  return i8 ? attention_paged_launch<T, true, 64, kKeys>(err, p, q, o, s) : attention_paged_launch<T, false, 64, kKeys>(err, p, q, o, s);
+  if (p.cache.d == 128) return i8 ? attention_paged_launch<T, true, 128>(err, p, q, o, s) : attention_paged_launch<T, false, 128>(err, p, q, o, s);
+  return i8 ? attention_paged_launch<T, true, 64>(err, p, q, o, s) : attention_paged_launch<T, false, 64>(err, p, q, o, s);
 }
-// One translation unit for each kind of keys (serving.cu, serving_cross.cu).
-template <paged::Keys kKeys>
-int32_t attention_paged_keys(std::string* err, const paged::Params& p, bool bf16, bool i8, const void* q, void* o, cudaStream_t s) {
-  return bf16 ? attention_paged_typed<__nv_bfloat16, kKeys>(err, p, i8, q, o, s) : attention_paged_typed<__half, kKeys>(err, p, i8, q, o, s);
-}
-extern template int32_t attention_paged_keys<paged::kPast>(std::string*, const paged::Params&, bool, bool, const void*, void*, cudaStream_t);
-extern template int32_t attention_paged_keys<paged::kAll>(std::string*, const paged::Params&, bool, bool, const void*, void*, cudaStream_t);
 
 // What the attentions over pages ask of their arguments.  *nothing: there are no tokens.
 inline int32_t attention_paged_args(std::string* err, const char* op, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, int32_t dtype, int32_t heads_q, const void* q,
@@ -333,10 +324,13 @@ inline int32_t attention_paged_args(std::string* err, const char* op, const tsm1
   p->heads_q = heads_q;
   p->group = heads_q / kv->heads_kv;
   p->scale_log2 = static_cast<float>((1.0 / std::sqrt(static_cast<double>(kv->head_dim))) * 1.4426950408889634);
-  p->prefix = 0, p->large = 0, p->prefix_table = nullptr;
-  std::memset(&p->shared, 0, sizeof p->shared), std::memset(&p->rest, 0, sizeof p->rest);
   p->status = status;
   return TSM100_OK;
+}
+
+// (serving.cu)
+inline int32_t attention_paged_any(std::string* err, const paged::Params& p, bool bf16, bool i8, const void* q, void* o, cudaStream_t s) {
+  return bf16 ? attention_paged_typed<__nv_bfloat16>(err, p, i8, q, o, s) : attention_paged_typed<__half>(err, p, i8, q, o, s);
 }
 
 inline int32_t attention_paged(std::string* err, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, const tsm100_attention_paged_desc* d, const void* q,
@@ -346,10 +340,131 @@ inline int32_t attention_paged(std::string* err, const tsm100_paged_kv* kv, cons
   bool nothing;
   const int32_t st = attention_paged_args(err, "attention_paged", kv, b, d->dtype, d->heads_q, q, o, status, &p, &nothing);
   if (st != TSM100_OK || nothing) return st;
-  return attention_paged_keys<paged::kPast>(err, p, d->dtype == TSM100_BF16, kv->dtype == TSM100_I8, q, o, static_cast<cudaStream_t>(stream));
+  return attention_paged_any(err, p, d->dtype == TSM100_BF16, kv->dtype == TSM100_I8, q, o, static_cast<cudaStream_t>(stream));
 }
 
-// Every token against all positions of its sequence.
+// ---------------------------------------------------------------------------
+// records of rows, joined: cross attention of few rows, and sequences that begin with the same pages
+// ---------------------------------------------------------------------------
+template <typename T, bool kI8, int D, bool kWide, paged::Keys kKeys>
+inline int32_t attention_rows_launch(std::string* err, const paged::Params& base, const PrefixArgs& more, const void* q, cudaStream_t s) {
+  using L = paged::RowsTile<kI8, D, kWide>;
+  int sms = 0;
+  int32_t st = sm_count(err, &sms);
+  if (st != TSM100_OK) return st;
+  paged::RowsParams p;
+  p.cache = base.cache, p.step = base.step;
+  p.heads_q = base.heads_q, p.group = base.group;
+  p.scale_log2 = base.scale_log2;
+  p.prefix = more.prefix, p.large = more.large, p.prefix_table = more.table;
+  p.shared = more.shared, p.rest = more.rest;
+  p.status = base.status;
+  // boxes of a power of two of positions that a page is a multiple of; 8-bit steps come by copies of 16 bytes and more
+  constexpr int kTop = L::kPos == 16 ? 4 : L::kPos == 32 ? 5 : 6;
+  const int run_log2 = page_run_log2(p.cache.page_size, kTop);
+  const bool boxes = run_log2 >= 3 && (!kI8 || (aligned16(p.cache.scales[0]) && aligned16(p.cache.scales[1])));
+  p.run_log2 = boxes ? run_log2 : kTop;
+  CUtensorMap map[2];
+  std::memset(map, 0, sizeof map);
+  for (int i = 0; i < 2 && boxes && st == TSM100_OK; ++i) {
+    TmapKey key;
+    std::memset(&key, 0, sizeof key);
+    constexpr bool kTwo = L::kRowBytes == 256;  // rows of two 128-byte groups
+    key.base = p.cache.kv[i];
+    const uint64_t rows = static_cast<uint64_t>(p.cache.page_size), units = static_cast<uint64_t>(p.cache.pages) * p.cache.heads;
+    if (kTwo) {
+      key.dim[0] = 64, key.dim[1] = rows, key.dim[2] = 2, key.dim[3] = units;
+      key.stride[0] = 256, key.stride[1] = 128, key.stride[2] = rows * 256;
+      key.box[0] = 64, key.box[1] = 1u << run_log2, key.box[2] = 2, key.box[3] = 1;
+    } else {
+      key.dim[0] = kI8 ? D : 64, key.dim[1] = rows, key.dim[2] = units;
+      key.stride[0] = L::kRowBytes, key.stride[1] = rows * L::kRowBytes;
+      key.box[0] = kI8 ? D : 64, key.box[1] = 1u << run_log2, key.box[2] = 1;
+    }
+    key.dtype = static_cast<int32_t>(kI8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+    key.rank = kTwo ? 4 : 3;
+    st = make_tmap(err, &map[i], key, kI8 ? 1 : 2);
+  }
+  if (st != TSM100_OK) return st;
+  auto kern = boxes ? paged::attention_paged_rows_kernel<T, kI8, D, true, kWide, kKeys> : paged::attention_paged_rows_kernel<T, kI8, D, false, kWide, kKeys>;
+  cudaError_t e = set_dyn_smem_once(kern, L::kSmem);
+  if (e == cudaSuccess)
+    e = launch_chained(kern, static_cast<unsigned>(std::min(sms, paged::kMaxCtas)), L::kThreads, L::kSmem, s, 0, map[0], map[1], static_cast<const T*>(q), p);
+  return cuda_ok(err, e, "attention_paged_rows_kernel launch");
+}
+template <typename T, int D>
+inline int32_t attention_join_launch(std::string* err, const paged::Join& join, void* o, cudaStream_t s) {
+  const int64_t at_once = paged::kJoinThreads / (D / 4) / paged::kJoinSplits, ys = (static_cast<int64_t>(join.step.max_new) * join.heads_q + at_once - 1) / at_once;
+  const dim3 grid(static_cast<unsigned>(join.step.batch), static_cast<unsigned>(std::min<int64_t>(ys, 64)));
+  return cuda_ok(err, launch_chained(paged::attention_paged_join_kernel<T, D>, grid, paged::kJoinThreads, 0, s, 0, static_cast<T*>(o), join), "attention_paged_join_kernel launch");
+}
+// What both need: scratch for `whole` arrays of records, `part` bytes of cut ones and `cuts` places.
+struct RecordSpace {
+  uint8_t *base = nullptr, *at = nullptr;
+  float* floats(size_t bytes) { return reinterpret_cast<float*>(std::exchange(at, at + bytes)); }
+  int2* places(size_t n) { return reinterpret_cast<int2*>(std::exchange(at, at + n * sizeof(int2))); }
+};
+inline int32_t take_records(std::string* err, const char* op, RecordSpace* x, size_t bytes, cudaStream_t s) {
+  const int32_t st = take_scratch(err, reinterpret_cast<void**>(&x->base), bytes, s);
+  if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, std::string(op) + ": no device memory for partial results");
+  x->at = x->base;
+  return st;
+}
+inline int32_t give_records(std::string* err, const RecordSpace& x, cudaStream_t s, int32_t st) {
+  const cudaError_t e = cudaFreeAsync(x.base, s);
+  return st == TSM100_OK && e != cudaSuccess ? cuda_ok(err, e, "cudaFreeAsync") : st;
+}
+// Bytes of the places that shares of the warps of all CTAs have for what they cut.
+template <bool kI8, int D, bool kWide>
+inline size_t rows_part_bytes(int64_t ctas) {
+  using L = paged::RowsTile<kI8, D, kWide>;
+  return static_cast<size_t>(ctas) * L::kWarps * 2 * L::kHeld * L::kRec * sizeof(float);
+}
+inline paged::Join join_of(const paged::Params& p) {
+  paged::Join x;
+  std::memset(&x, 0, sizeof x);
+  x.cache = p.cache, x.step = p.step;
+  x.heads_q = p.heads_q, x.group = p.group;
+  return x;
+}
+
+// Every token against all positions of its sequence (serving_cross.cu).
+template <typename T, bool kI8, int D, bool kWide>
+inline int32_t attention_cross_rows(std::string* err, const paged::Params& p, const void* q, void* o, cudaStream_t s) {
+  using L = paged::RowsTile<kI8, D, kWide>;
+  int sms = 0;
+  int32_t st = sm_count(err, &sms);
+  if (st != TSM100_OK) return st;
+  const int64_t ctas = std::min(sms, paged::kMaxCtas), units = (static_cast<int64_t>(p.step.max_new) * p.group + L::kHeld - 1) / L::kHeld;
+  const size_t whole = static_cast<size_t>(p.step.tokens) * p.heads_q * L::kRec * sizeof(float), part = rows_part_bytes<kI8, D, kWide>(ctas);
+  const size_t cuts = static_cast<size_t>(p.step.batch) * p.cache.heads * units;
+  RecordSpace space;
+  st = take_records(err, "attention_paged_cross", &space, whole + part + cuts * sizeof(int2), s);
+  if (st != TSM100_OK) return st;
+  PrefixArgs more = {};
+  more.rest.whole = space.floats(whole), more.rest.part = space.floats(part), more.rest.cut = space.places(cuts);
+  more.rest.units = static_cast<int32_t>(units);
+  paged::Join join = join_of(p);
+  join.all = 1, join.rest = more.rest, join.rest_held = L::kHeld;
+  st = attention_rows_launch<T, kI8, D, kWide, paged::kAll>(err, p, more, q, s);
+  if (st == TSM100_OK) st = attention_join_launch<T, D>(err, join, o, s);
+  return give_records(err, space, s, st);
+}
+template <typename T, bool kI8, int D>
+inline int32_t attention_cross_launch(std::string* err, const paged::Params& p, const void* q, void* o, cudaStream_t s) {
+  const int64_t rows = static_cast<int64_t>(p.step.max_new) * p.group;
+  const int wide = page_run_log2(p.cache.page_size, 7);
+  if (rows > paged::kRows && paged_fits_tcgen05(p.group, kI8, wide)) return attention_paged_tc_launch<T, kI8, D, paged::kAll>(err, p, wide, q, o, s);
+  return rows > 8 ? attention_cross_rows<T, kI8, D, true>(err, p, q, o, s) : attention_cross_rows<T, kI8, D, false>(err, p, q, o, s);
+}
+template <bool kI8>
+int32_t attention_cross_held(std::string* err, const paged::Params& p, bool bf16, const void* q, void* o, cudaStream_t s) {
+  if (p.cache.d == 128) return bf16 ? attention_cross_launch<__nv_bfloat16, kI8, 128>(err, p, q, o, s) : attention_cross_launch<__half, kI8, 128>(err, p, q, o, s);
+  return bf16 ? attention_cross_launch<__nv_bfloat16, kI8, 64>(err, p, q, o, s) : attention_cross_launch<__half, kI8, 64>(err, p, q, o, s);
+}
+extern template int32_t attention_cross_held<false>(std::string*, const paged::Params&, bool, const void*, void*, cudaStream_t);
+extern template int32_t attention_cross_held<true>(std::string*, const paged::Params&, bool, const void*, void*, cudaStream_t);
+
 inline int32_t attention_paged_cross(std::string* err, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, const tsm100_attention_paged_desc* d, const void* q,
                                      void* o, uint32_t* status, void* stream) {
   if (!d) return op_fail(err, TSM100_ERR_INVALID, "attention_paged_cross: null descriptor");
@@ -357,12 +472,11 @@ inline int32_t attention_paged_cross(std::string* err, const tsm100_paged_kv* kv
   bool nothing;
   const int32_t st = attention_paged_args(err, "attention_paged_cross", kv, b, d->dtype, d->heads_q, q, o, status, &p, &nothing);
   if (st != TSM100_OK || nothing) return st;
-  return attention_paged_keys<paged::kAll>(err, p, d->dtype == TSM100_BF16, kv->dtype == TSM100_I8, q, o, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf16 = d->dtype == TSM100_BF16;
+  return kv->dtype == TSM100_I8 ? attention_cross_held<true>(err, p, bf16, q, o, s) : attention_cross_held<false>(err, p, bf16, q, o, s);
 }
 
-// ---------------------------------------------------------------------------
-// sequences that begin with the same pages
-// ---------------------------------------------------------------------------
 // All tokens against the prefix and each against its own positions, both as records, and then those joined.  Translation units by cache and head size
 // (serving_prefix*.cu).
 struct PrefixPlan {
@@ -371,64 +485,58 @@ struct PrefixPlan {
   int run_log2;    // boxes of pages for tcgen05
 };
 template <typename T, bool kI8, int D>
-inline int32_t attention_prefix_launch(std::string* err, paged::Params p, const PrefixPlan& plan, const void* q, void* o, cudaStream_t s) {
+inline int32_t attention_prefix_launch(std::string* err, const paged::Params& p, const PrefixPlan& plan, PrefixArgs more, const void* q, void* o, cudaStream_t s) {
   namespace pg = paged;
   constexpr size_t REC = D + 4;
   int sms = 0;
   int32_t st = sm_count(err, &sms);
   if (st != TSM100_OK) return st;
-  const int64_t ctas = std::min(sms, pg::kMaxCtas), rows = static_cast<int64_t>(p.step.tokens) * p.heads_q, heads = p.cache.heads;
+  const int64_t ctas = std::min(sms, pg::kMaxCtas), heads = p.cache.heads;
   const int32_t tile_tokens = pg::tc::kTileRows / p.group;
-  pg::Join join;
-  join.cache = p.cache, join.step = p.step;
-  join.heads_q = p.heads_q, join.group = p.group;
-  join.prefix = p.prefix, join.large = p.large;
+  // the rows of a unit: what a sequence has, unless the prefix's, which are all tokens', are in the same stream
+  const bool wide = !plan.shared_tc || static_cast<int64_t>(p.step.max_new) * p.group > 8;
+  const int held = wide ? 16 : 8;
+  pg::Join join = join_of(p);
+  join.prefix = more.prefix, join.large = more.large;
   join.shared_tokens = plan.shared_tc ? tile_tokens : 0, join.large_tokens = tile_tokens;
-  auto units = [&](bool tc, int64_t tokens) { return tc ? (tokens + 2 * tile_tokens - 1) / (2 * tile_tokens) : (tokens * p.group + pg::kRows - 1) / pg::kRows; };
-  const int64_t shared_units = units(plan.shared_tc, p.step.tokens), rest_units = units(false, plan.rest_tc ? p.large / p.group : p.step.max_new);
+  join.shared_held = join.rest_held = held;
+  auto units = [&](bool tc, int64_t tokens) { return tc ? (tokens + 2 * tile_tokens - 1) / (2 * tile_tokens) : (tokens * p.group + held - 1) / held; };
+  const int64_t shared_units = units(plan.shared_tc, p.step.tokens), rest_units = units(false, plan.rest_tc ? more.large / p.group : p.step.max_new);
   const int64_t large_units = plan.rest_tc ? units(true, p.step.max_new) : 0;
-  const size_t few_part = ctas * 2 * pg::kRows * REC * sizeof(float), tc_part = ctas * 2 * 256 * REC * sizeof(float), whole = rows * REC * sizeof(float);
-  const size_t cuts = heads * (shared_units + p.step.batch * (rest_units + large_units)) * sizeof(int2);
-  uint8_t* ws = nullptr;
-  st = take_scratch(err, reinterpret_cast<void**>(&ws), 2 * whole + few_part + (plan.shared_tc ? tc_part : 0) + (plan.rest_tc ? tc_part : 0) + cuts, s);
-  if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged_prefix: no device memory for partial results");
+  const size_t rows_part = wide ? rows_part_bytes<kI8, D, true>(ctas) : rows_part_bytes<kI8, D, false>(ctas), tc_part = static_cast<size_t>(ctas) * 2 * 256 * REC * sizeof(float);
+  const size_t whole = static_cast<size_t>(p.step.tokens) * p.heads_q * REC * sizeof(float), cuts = heads * (shared_units + p.step.batch * (rest_units + large_units));
+  RecordSpace space;
+  st = take_records(err, "attention_paged_prefix", &space, 2 * whole + rows_part + (plan.shared_tc ? tc_part : 0) + (plan.rest_tc ? tc_part : 0) + cuts * sizeof(int2), s);
   if (st != TSM100_OK) return st;
-  uint8_t* at = ws;
-  auto place = [&](size_t bytes) { return reinterpret_cast<float*>(std::exchange(at, at + bytes)); };
-  join.shared.whole = place(whole), join.rest.whole = place(whole);
-  join.rest.part = place(few_part);
-  join.shared.part = plan.shared_tc ? place(tc_part) : join.rest.part;  // a share's two places are for whatever it has cut
-  join.rest_large.part = plan.rest_tc ? place(tc_part) : nullptr, join.rest_large.whole = join.rest.whole;
+  join.shared.whole = space.floats(whole), join.rest.whole = join.rest_large.whole = space.floats(whole);
+  join.rest.part = space.floats(rows_part);
+  join.shared.part = plan.shared_tc ? space.floats(tc_part) : join.rest.part;  // a share's two places are for whatever it has cut
+  join.rest_large.part = plan.rest_tc ? space.floats(tc_part) : nullptr;
+  join.shared.cut = space.places(heads * shared_units), join.rest.cut = space.places(heads * p.step.batch * rest_units);
+  join.rest_large.cut = space.places(heads * p.step.batch * large_units);
   join.shared.units = static_cast<int32_t>(shared_units), join.rest.units = static_cast<int32_t>(rest_units), join.rest_large.units = static_cast<int32_t>(large_units);
-  join.shared.cut = reinterpret_cast<int2*>(at), join.rest.cut = join.shared.cut + heads * shared_units, join.rest_large.cut = join.rest.cut + heads * p.step.batch * rest_units;
-  p.shared = join.shared, p.rest = join.rest;
+  more.shared = join.shared, more.rest = join.rest;
   if (plan.shared_tc) {
-    st = attention_paged_tc_launch<T, kI8, D, pg::kShared>(err, p, plan.run_log2, q, o, s);
-    if (st == TSM100_OK) st = attention_paged_few_launch<T, kI8, D, true, pg::kRest>(err, p, q, o, s);
+    st = attention_paged_tc_launch<T, kI8, D, pg::kShared>(err, p, plan.run_log2, q, o, s, more);
+    if (st == TSM100_OK) st = wide ? attention_rows_launch<T, kI8, D, true, pg::kRest>(err, p, more, q, s) : attention_rows_launch<T, kI8, D, false, pg::kRest>(err, p, more, q, s);
   } else {
-    st = attention_paged_few_launch<T, kI8, D, true, pg::kBoth>(err, p, q, o, s);
+    st = attention_rows_launch<T, kI8, D, true, pg::kBoth>(err, p, more, q, s);
   }
   if (st == TSM100_OK && plan.rest_tc) {
-    p.rest = join.rest_large;
-    st = attention_paged_tc_launch<T, kI8, D, pg::kRest>(err, p, plan.run_log2, q, o, s);
+    more.rest = join.rest_large;
+    st = attention_paged_tc_launch<T, kI8, D, pg::kRest>(err, p, plan.run_log2, q, o, s, more);
   }
-  if (st == TSM100_OK) {
-    const int64_t at_once = pg::kJoinThreads / (D / 4), ys = (static_cast<int64_t>(p.step.max_new) * p.heads_q + at_once - 1) / at_once;
-    const dim3 grid(static_cast<unsigned>(p.step.batch), static_cast<unsigned>(std::min<int64_t>(ys, 64)));
-    st = cuda_ok(err, launch_chained(pg::attention_paged_join_kernel<T, D>, grid, pg::kJoinThreads, 0, s, 0, static_cast<T*>(o), join), "attention_paged_join_kernel launch");
-  }
-  const cudaError_t e = cudaFreeAsync(ws, s);
-  if (st == TSM100_OK && e != cudaSuccess) st = cuda_ok(err, e, "cudaFreeAsync");
-  return st;
+  if (st == TSM100_OK) st = attention_join_launch<T, D>(err, join, o, s);
+  return give_records(err, space, s, st);
 }
 template <bool kI8, int D>
-int32_t attention_prefix_held(std::string* err, const paged::Params& p, bool bf16, const PrefixPlan& plan, const void* q, void* o, cudaStream_t s) {
-  return bf16 ? attention_prefix_launch<__nv_bfloat16, kI8, D>(err, p, plan, q, o, s) : attention_prefix_launch<__half, kI8, D>(err, p, plan, q, o, s);
+int32_t attention_prefix_held(std::string* err, const paged::Params& p, bool bf16, const PrefixPlan& plan, const PrefixArgs& more, const void* q, void* o, cudaStream_t s) {
+  return bf16 ? attention_prefix_launch<__nv_bfloat16, kI8, D>(err, p, plan, more, q, o, s) : attention_prefix_launch<__half, kI8, D>(err, p, plan, more, q, o, s);
 }
-extern template int32_t attention_prefix_held<false, 64>(std::string*, const paged::Params&, bool, const PrefixPlan&, const void*, void*, cudaStream_t);
-extern template int32_t attention_prefix_held<false, 128>(std::string*, const paged::Params&, bool, const PrefixPlan&, const void*, void*, cudaStream_t);
-extern template int32_t attention_prefix_held<true, 64>(std::string*, const paged::Params&, bool, const PrefixPlan&, const void*, void*, cudaStream_t);
-extern template int32_t attention_prefix_held<true, 128>(std::string*, const paged::Params&, bool, const PrefixPlan&, const void*, void*, cudaStream_t);
+extern template int32_t attention_prefix_held<false, 64>(std::string*, const paged::Params&, bool, const PrefixPlan&, const PrefixArgs&, const void*, void*, cudaStream_t);
+extern template int32_t attention_prefix_held<false, 128>(std::string*, const paged::Params&, bool, const PrefixPlan&, const PrefixArgs&, const void*, void*, cudaStream_t);
+extern template int32_t attention_prefix_held<true, 64>(std::string*, const paged::Params&, bool, const PrefixPlan&, const PrefixArgs&, const void*, void*, cudaStream_t);
+extern template int32_t attention_prefix_held<true, 128>(std::string*, const paged::Params&, bool, const PrefixPlan&, const PrefixArgs&, const void*, void*, cudaStream_t);
 
 inline int32_t attention_paged_prefix(std::string* err, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, const tsm100_attention_paged_prefix_desc* d, const void* q,
                                       void* o, uint32_t* status, void* stream) {
@@ -445,17 +553,18 @@ inline int32_t attention_paged_prefix(std::string* err, const tsm100_paged_kv* k
   if (reinterpret_cast<uintptr_t>(d->prefix) & 3u) return no("prefix does not start on an element boundary");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = d->dtype == TSM100_BF16, i8 = kv->dtype == TSM100_I8;
-  if (d->prefix_len == 0) return attention_paged_keys<paged::kPast>(err, p, bf16, i8, q, o, s);
+  if (d->prefix_len == 0) return attention_paged_any(err, p, bf16, i8, q, o, s);
   PrefixPlan plan;
   plan.run_log2 = page_run_log2(kv->page_size, 7);
-  const bool tc = p.group <= paged::tc::kMaxGroup && (i8 || plan.run_log2 >= 3);
+  const bool tc = paged_fits_tcgen05(p.group, i8, plan.run_log2);
   plan.shared_tc = tc && route::prefix_on_tcgen05(static_cast<int64_t>(b->tokens) * p.group, d->prefix_len, kv->heads_kv, kv->head_dim, i8);
   plan.rest_tc = tc && static_cast<int64_t>(b->max_new) * p.group > route::kPrefixFewRows;
-  p.large = plan.rest_tc ? static_cast<int32_t>(route::kPrefixFewRows) : 0;
-  p.prefix = d->prefix_len, p.prefix_table = d->prefix;
+  PrefixArgs more = {};
+  more.large = plan.rest_tc ? static_cast<int32_t>(route::kPrefixFewRows) : 0;
+  more.prefix = d->prefix_len, more.table = d->prefix;
   p.step.table += d->prefix_len / kv->page_size;
-  if (kv->head_dim == 128) return i8 ? attention_prefix_held<true, 128>(err, p, bf16, plan, q, o, s) : attention_prefix_held<false, 128>(err, p, bf16, plan, q, o, s);
-  return i8 ? attention_prefix_held<true, 64>(err, p, bf16, plan, q, o, s) : attention_prefix_held<false, 64>(err, p, bf16, plan, q, o, s);
+  if (kv->head_dim == 128) return i8 ? attention_prefix_held<true, 128>(err, p, bf16, plan, more, q, o, s) : attention_prefix_held<false, 128>(err, p, bf16, plan, more, q, o, s);
+  return i8 ? attention_prefix_held<true, 64>(err, p, bf16, plan, more, q, o, s) : attention_prefix_held<false, 64>(err, p, bf16, plan, more, q, o, s);
 }
 
 }  // namespace ops

@@ -7,8 +7,6 @@
 
 using namespace tsm100;
 
-template int32_t tsm100::ops::attention_paged_keys<paged::kPast>(std::string*, const paged::Params&, bool, bool, const void*, void*, cudaStream_t);
-
 extern "C" {
 
 int32_t tsm100_add_rms_norm(tsm100_device_t dev, const tsm100_add_rms_norm_desc* desc, const void* x, const void* residual, void* sum,
