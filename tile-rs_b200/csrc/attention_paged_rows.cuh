@@ -607,7 +607,7 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
   }
 }
 
-// What a row's records add up to.  CTA (b, y) has rows of sequence b: D / 4 threads a row, four times, which take every fourth record; eight are asked for before the first is used.
+// What a row's records add up to.  CTA (b, y) has rows of sequence b: D / 4 threads a row, four times, which take every fourth record; four are asked for before the first is used.
 // A part whose scores are all -inf weighs nothing beside another.
 struct Join {
   pages::Cache cache;
@@ -620,38 +620,39 @@ struct Join {
   int32_t shared_held, rest_held;
 };
 constexpr int kJoinThreads = 256, kJoinSplits = 4;
-// A row's records: the first, and what lies between one share's and the next.
+// A row's records: the first, and what lies between one share's and the next, in numbers.
 struct Pieces {
   const float* first;
   const float* next;
-  int64_t step;
+  uint32_t step;
   int n;
-  __device__ __forceinline__ const float* at(int i) const { return i == 0 ? first : next + (i - 1) * step; }
 };
+// (Tokens times heads fit 31 bits, so the rows of a KV head and all of them do.)
 template <int D>
-__device__ __forceinline__ Pieces pieces(const Records& rec, int tile_tokens, int held, int64_t cut0, int head, int group, int token, int h, int64_t row) {
-  constexpr int REC = D + 4;
-  int unit, r;
+__device__ __forceinline__ Pieces pieces(const Records& rec, int tile_tokens, uint32_t held, int64_t cut0, uint32_t head, uint32_t group, uint32_t token, uint32_t h, uint32_t row) {
+  constexpr uint32_t REC = D + 4;
+  uint32_t unit, r;
   if (tile_tokens > 0) {
     unit = token / (2 * tile_tokens);
-    const int t = token - unit * 2 * tile_tokens, g = t >= tile_tokens ? 1 : 0;
+    const uint32_t t = token - unit * 2 * tile_tokens, g = t >= static_cast<uint32_t>(tile_tokens) ? 1 : 0;
     r = g * 128 + (t - g * tile_tokens) * group + h, held = 256;
-  } else {
-    const int64_t at = static_cast<int64_t>(token) * group + h;
-    unit = static_cast<int>(at / held), r = static_cast<int>(at - static_cast<int64_t>(unit) * held);
+  } else {  // 8 or 16
+    const uint32_t at = token * group + h;
+    unit = held == 8 ? at >> 3 : at >> 4, r = at & (held - 1);
   }
   const int2 cut = __ldcg(rec.cut + cut0 + static_cast<int64_t>(head) * rec.units + unit);
   Pieces x;
   x.n = max(cut.y, 1);
-  x.step = static_cast<int64_t>(2) * held * REC;
-  x.first = cut.y == 0 ? rec.whole + row * REC : rec.part + ((static_cast<int64_t>(cut.x) * 2 + 1) * held + r) * REC;
-  x.next = rec.part + (static_cast<int64_t>(cut.x + 1) * 2 * held + r) * REC;
+  x.step = 2 * held * REC;
+  const float* place = rec.part + (static_cast<int64_t>(cut.x) * (2 * held) + r) * REC;
+  x.first = cut.y == 0 ? rec.whole + static_cast<int64_t>(row) * REC : place + held * REC;
+  x.next = place + x.step;
   return x;
 }
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(kJoinThreads, 4)
 attention_paged_join_kernel(T* o, const __grid_constant__ Join p) {
-  constexpr int kLanes = D / 4, kRowsAt = kJoinThreads / kLanes / kJoinSplits, kAtOnce = 8;
+  constexpr int kLanes = D / 4, kRowsAt = kJoinThreads / kLanes / kJoinSplits, kAtOnce = 4;
   constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
   __shared__ float4 part_x[kJoinSplits][kRowsAt][kLanes];
   __shared__ float2 part_ml[kJoinSplits][kRowsAt];
@@ -663,19 +664,23 @@ attention_paged_join_kernel(T* o, const __grid_constant__ Join p) {
   const bool large = is_large(p, count);
   const Records& rest = large ? p.rest_large : p.rest;
   const int rest_tokens = large ? p.large_tokens : 0, lane = threadIdx.x % kLanes, split = threadIdx.x / kLanes % kJoinSplits, mine = threadIdx.x / (kLanes * kJoinSplits);
-  const int64_t rows = static_cast<int64_t>(count) * p.heads_q;
-  for (int64_t i0 = static_cast<int64_t>(blockIdx.y) * kRowsAt; i0 < rows; i0 += static_cast<int64_t>(gridDim.y) * kRowsAt) {
-    const int64_t i = i0 + mine;
-    const bool ok = i < rows && len > 0;
-    const int64_t row = static_cast<int64_t>(first) * p.heads_q + i;
+  const uint32_t rows = static_cast<uint32_t>(count) * p.heads_q, group = p.group;
+  for (uint32_t i0 = blockIdx.y * kRowsAt; i0 < rows; i0 += gridDim.y * kRowsAt) {
+    const uint32_t i = i0 + mine, row = static_cast<uint32_t>(first) * p.heads_q + i;
     float m = -INFINITY, l = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (ok) {
-      const int token = static_cast<int>(i / p.heads_q), hq = static_cast<int>(i - static_cast<int64_t>(token) * p.heads_q), head = hq / p.group, h = hq - head * p.group;
+    if (i < rows && len > 0) {
+      const uint32_t token = i / static_cast<uint32_t>(p.heads_q), hq = i - token * p.heads_q, head = hq / group, h = hq - head * group;
       Pieces s = {};
-      if (!p.all) s = pieces<D>(p.shared, p.shared_tokens, p.shared_held, 0, head, p.group, first + token, h, row);
-      const Pieces r = pieces<D>(rest, rest_tokens, p.rest_held, static_cast<int64_t>(b) * p.cache.heads * rest.units, head, p.group, token, h, row);
+      if (!p.all) s = pieces<D>(p.shared, p.shared_tokens, p.shared_held, 0, head, group, first + token, h, row);
+      const Pieces r = pieces<D>(rest, rest_tokens, p.rest_held, static_cast<int64_t>(b) * p.cache.heads * rest.units, head, group, token, h, row);
       const int n = s.n + r.n;
+      auto record = [&](int at) {
+        const bool of_rest = at >= s.n;
+        at -= of_rest ? s.n : 0;
+        const float* next = of_rest ? r.next : s.next;
+        return at == 0 ? (of_rest ? r.first : s.first) : next + static_cast<int64_t>(at - 1) * (of_rest ? r.step : s.step);
+      };
       for (int j0 = split; j0 < n; j0 += kJoinSplits * kAtOnce) {
         float2 ml[kAtOnce];
         float4 y[kAtOnce];
@@ -684,19 +689,20 @@ attention_paged_join_kernel(T* o, const __grid_constant__ Join p) {
           const int at = j0 + j * kJoinSplits;
           ml[j] = make_float2(-INFINITY, 0.f), y[j] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (at < n) {
-            const float* rec = at < s.n ? s.at(at) : r.at(at - s.n);
+            const float* rec = record(at);
             ml[j] = __ldcg(reinterpret_cast<const float2*>(rec + D)), y[j] = __ldcg(reinterpret_cast<const float4*>(rec) + lane);
           }
         }
         float top = m;
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j) top = fmaxf(top, ml[j].x);
-        const float keep = m == -INFINITY ? 0.f : exp2f(m - top);
+        const float keep = m == -INFINITY ? 0.f : ptx::ex2_approx(m - top);
         l *= keep, x.x *= keep, x.y *= keep, x.z *= keep, x.w *= keep;
         // a part of no scores but -inf weighs nothing; it is added all the same, because one of NaN scores has that maximum too
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j) {
-          const float w = ml[j].x == -INFINITY ? 0.f : exp2f(ml[j].x - top);
+          if (j0 + j * kJoinSplits >= n) break;
+          const float w = ml[j].x == -INFINITY ? 0.f : ptx::ex2_approx(ml[j].x - top);
           l = fmaf(w, ml[j].y, l);
           x.x = fmaf(w, y[j].x, x.x), x.y = fmaf(w, y[j].y, x.y), x.z = fmaf(w, y[j].z, x.z), x.w = fmaf(w, y[j].w, x.w);
         }
@@ -716,12 +722,12 @@ attention_paged_join_kernel(T* o, const __grid_constant__ Join p) {
       for (int j = 0; j < kJoinSplits; ++j) {
         const float2 ml = part_ml[j][mine];
         const float4 y = part_x[j][mine][lane];
-        const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+        const float w = ml.x == -INFINITY ? 0.f : ptx::ex2_approx(ml.x - top);
         l = fmaf(w, ml.y, l);
         x.x = fmaf(w, y.x, x.x), x.y = fmaf(w, y.y, x.y), x.z = fmaf(w, y.z, x.z), x.w = fmaf(w, y.w, x.w);
       }
       const float inv = len > 0 ? 1.f / l : 0.f;
-      *reinterpret_cast<uint2*>(o + row * D + lane * 4) = make_uint2(mma::pack2<kIsBf16>(x.x * inv, x.y * inv), mma::pack2<kIsBf16>(x.z * inv, x.w * inv));
+      *reinterpret_cast<uint2*>(o + static_cast<int64_t>(row) * D + lane * 4) = make_uint2(mma::pack2<kIsBf16>(x.x * inv, x.y * inv), mma::pack2<kIsBf16>(x.z * inv, x.w * inv));
     }
   }
 }
