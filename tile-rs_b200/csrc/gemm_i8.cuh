@@ -152,13 +152,21 @@ gemm_i8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
   __syncwarp();
 
   // ------------------------------ sums -> C ------------------------------
+  // The scales, while the products run: lane i has those of rows i, 32 + i ... of A, and those of its own column, or four columns, of C.
+  const int rows = min(NT, p.m - mb * NT);
+  float as[(NT + 31) / 32], ws[4];
+#pragma unroll
+  for (int i = 0; i < (NT + 31) / 32; ++i) as[i] = i * 32 + lane < rows ? p.a_scales[mb * NT + i * 32 + lane] : 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int col = nb * kBN + (splits == 1 ? warp * 32 + lane : lane * 4 + j);
+    ws[j] = col < p.n ? p.w_scales[col] : 0.f;
+  }
   const bool ready = __all_sync(0xffffffffu, ptx::mbar_wait(&bars->acc_full, 0, abort_flag, p.status, 183));
   ptx::tcgen05_fence_after_thread_sync();
   ptx::launch_dependents();  // not before: gemm_skinny.cuh
   const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
   constexpr int kStep = NT < 32 ? 16 : 32;  // rows of C (TMEM columns) per read
-  const int rows = min(NT, p.m - mb * NT);
-  const float* a_scales = p.a_scales + mb * NT;
   auto read = [&](int r0, uint32_t (&v)[kStep]) {
     if constexpr (kStep == 16) ptx::tmem_ld_32x32b_x16(lane_addr + r0, v);
     else ptx::tmem_ld_32x32b_x32(lane_addr + r0, v);
@@ -167,17 +175,16 @@ gemm_i8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
   if (splits == 1) {
     const int col = nb * kBN + warp * 32 + lane;
     if (ready) {
-      const float ws = col < p.n ? p.w_scales[col] : 0.f;
 #pragma unroll
       for (int r0 = 0; r0 < NT; r0 += kStep) {
         if (r0 >= rows) break;
         uint32_t v[kStep];
         read(r0, v);
         OutT* dst = c + static_cast<int64_t>(mb * NT + r0) * p.ldc + col;
-        if (col < p.n) {
 #pragma unroll
-          for (int i = 0; i < kStep; ++i)
-            if (r0 + i < rows) dst[i * p.ldc] = narrow<OutT>(scaled(v[i], a_scales[r0 + i], ws));
+        for (int i = 0; i < kStep; ++i) {
+          const OutT x = narrow<OutT>(scaled(v[i], __shfl_sync(0xffffffffu, as[(r0 + i) / 32], (r0 + i) % 32), ws[0]));
+          if (col < p.n && r0 + i < rows) dst[i * p.ldc] = x;
         }
       }
     }
@@ -206,13 +213,13 @@ gemm_i8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
           const float4 v = ptx::ld_shared_cluster_f32x4(ptx::mapa_shared(part_addr + i * 16, q));
           s[0] += __float_as_uint(v.x), s[1] += __float_as_uint(v.y), s[2] += __float_as_uint(v.z), s[3] += __float_as_uint(v.w);
         }
-      const int row = i / (kBN / 4), col = nb * kBN + (i % (kBN / 4)) * 4;
+      const int row = i / (kBN / 4), col = nb * kBN + lane * 4;  // kBN / 4 is a warp's lanes
       if (col >= p.n) continue;
-      const float as = a_scales[row];
+      const float row_scale = p.a_scales[mb * NT + row];
       OutT* dst = c + static_cast<int64_t>(mb * NT + row) * p.ldc + col;
       OutT x[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = narrow<OutT>(scaled(s[j], as, col + j < p.n ? p.w_scales[col + j] : 0.f));
+      for (int j = 0; j < 4; ++j) x[j] = narrow<OutT>(scaled(s[j], row_scale, ws[j]));
       if (p.vectors) {
         if constexpr (sizeof(OutT) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(x);
         else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(x);
@@ -244,13 +251,14 @@ gemm_i8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
 // Many output tiles: CTA pairs (gemm_tc2.cuh), 256 rows of A by `bn` rows of W a tile
 // ---------------------------------------------------------------------------
 // Per CTA: warp 0 TMA producer (128 rows of A and half of the tile's rows of W, 128 of K a stage), warp 1 tensor memory and, in the leader, the products
-// (M = 256 over the pair, N = bn, K = 32), warps 2..5 this CTA's 128 rows of the sums, of which two sets alternate, scaled and stored as boxes.
+// (M = 256 over the pair, N = bn, K = 32), warps 2..9 this CTA's 128 rows of the sums, of which two sets alternate, scaled and stored as boxes
+// (four warps took 3.5 us for 128 x 256 in a row of tiles, longer than the products of K = 1280).
 // Bound: the tensor pipe, 2 M N K.  Widths from 128 to 256 so that the last wave of tiles is a full one (route.hpp: gemm_i8_pair_width).
 namespace pairs {
 
 constexpr int kPairM = 256, kCtaM = 128, kMaxBN = 256;
 constexpr int kStages = 6;
-constexpr int kThreads = 192;
+constexpr int kThreads = 320;
 constexpr int kABytes = kCtaM * kBK;              // 16 KiB
 constexpr int kStageBytes = kABytes + kMaxBN / 2 * kBK;
 constexpr int kTmemCols = 512;
@@ -261,11 +269,11 @@ struct alignas(8) Barriers {
   uint64_t full[kStages];      // used in the leader: both CTAs' bytes of a stage have landed
   uint64_t empty[kStages];     // in each CTA: the products reading the stage have retired
   uint64_t acc_full[2];        // in each CTA: sums complete
-  uint64_t acc_empty[2];       // used in the leader: 8 epilogue warps of the pair have drained them
+  uint64_t acc_empty[2];       // used in the leader: 16 epilogue warps of the pair have drained them
   uint32_t tmem_base;
   uint32_t abort_flag;
 };
-constexpr int kBarsOff = kStages * kStageBytes + 4 * 2 * kBoxBytes;
+constexpr int kBarsOff = kStages * kStageBytes + 8 * kBoxBytes;
 constexpr int kSmemBytes = kBarsOff + sizeof(Barriers) + 1024;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory budget of one CTA");
 
@@ -289,11 +297,12 @@ __device__ __forceinline__ void tile_coords(const Params& p, int tile, int& mb, 
 // One warp's 32 rows of a tile's sums (`tmem`: its lanes, first column), scaled, to C from (row0, col0) up to column `end`: as gemm_tc.cuh's store_rows.
 // kLoose: rows of C start anywhere.
 template <typename OutT, bool kLoose>
-__device__ __forceinline__ void store_rows(const CUtensorMap* tmap_c, OutT* c, const Params& p, uint32_t tmem, uint8_t* staging, uint32_t& boxes, int row0, int col0, int end, int lane) {
+__device__ __forceinline__ void store_rows(const CUtensorMap* tmap_c, OutT* c, const Params& p, uint32_t tmem, uint8_t* box, int row0, int col0, int end, int lane) {
   constexpr int kCols = gemm_tc::kBoxCols<OutT>, kHalves = kCols / 32;
   if (row0 >= p.m) return;
   const float as = p.a_scales[min(row0 + lane, p.m - 1)];
-  float ws[kHalves], next[kHalves];  // of this lane's columns in a box
+  const ptx::f32x2_t as2 = ptx::pack_f32x2(as, as);
+  float ws[kHalves], next[kHalves];  // of this lane's columns in a box, asked for a box ahead
   auto ask = [&](int c0) {
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) next[h] = p.w_scales[min(c0 + h * 32 + lane, p.n - 1)];
@@ -311,9 +320,14 @@ __device__ __forceinline__ void store_rows(const CUtensorMap* tmap_c, OutT* c, c
 #pragma unroll
     for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[h][i] = __float_as_uint(scaled(v[h][i], as, __shfl_sync(0xffffffffu, ws[h], i)));
-    uint8_t* box = staging + (boxes++ & 1) * kBoxBytes;
-    if (!kLoose && lane == 0) ptx::tma_store_wait_read<1>();  // the store before last has read its buffer
+      for (int i = 0; i < 32; i += 2) {  // as `scaled`, two at once
+        const ptx::f32x2_t x = ptx::pack_f32x2(__int2float_rn(static_cast<int32_t>(v[h][i])), __int2float_rn(static_cast<int32_t>(v[h][i + 1])));
+        const ptx::f32x2_t w = ptx::pack_f32x2(__shfl_sync(0xffffffffu, ws[h], i), __shfl_sync(0xffffffffu, ws[h], i + 1));
+        float lo, hi;
+        ptx::unpack_f32x2(ptx::mul_f32x2(ptx::mul_f32x2(x, as2), w), lo, hi);
+        v[h][i] = __float_as_uint(lo), v[h][i + 1] = __float_as_uint(hi);
+      }
+    if (!kLoose && lane == 0) ptx::tma_store_wait_read<0>();  // the store before has read the buffer
     __syncwarp();
     const uint32_t row = ptx::smem_u32(box) + lane * 128;
 #pragma unroll
@@ -372,7 +386,7 @@ gemm_i8_pairs_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     }
     for (int a = 0; a < 2; ++a) {
       ptx::mbar_init(&bars->acc_full[a], 1);
-      ptx::mbar_init(&bars->acc_empty[a], 8);
+      ptx::mbar_init(&bars->acc_empty[a], 16);
     }
     bars->abort_flag = 0;
     ptx::fence_mbar_init();
@@ -455,9 +469,9 @@ gemm_i8_pairs_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     }
   } else {
     // ------------------------------ sums -> C (both CTAs) ---------------------
-    const int quad = warp & 3;
-    uint8_t* staging = smem + kStages * kStageBytes + (warp - 2) * 2 * kBoxBytes;
-    uint32_t boxes = 0;
+    const int quad = warp & 3, side = (warp - 2) >> 2;  // two warps share rows: one the left half of the columns, in whole boxes, one the right
+    const int left = (p.bn / 2 + gemm_tc::kBoxCols<OutT> - 1) / gemm_tc::kBoxCols<OutT> * gemm_tc::kBoxCols<OutT>;
+    uint8_t* staging = smem + kStages * kStageBytes + (warp - 2) * kBoxBytes;
     int local = 0;
     for (int tile = pair; tile < num_tiles; tile += num_pairs, ++local) {
       const int acc = local & 1;
@@ -466,9 +480,9 @@ gemm_i8_pairs_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       const bool ready = ptx::mbar_wait(&bars->acc_full[acc], (local >> 1) & 1u, abort_flag, p.status, 187);
       if (!__all_sync(0xffffffffu, ready)) break;
       ptx::tcgen05_fence_after_thread_sync();
-      const uint32_t from = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * kMaxBN;
-      const int row0 = mb * kPairM + static_cast<int>(rank) * kCtaM + quad * 32, col0 = nb * p.bn;
-      store_rows<OutT, kLoose>(&tmap_c, c, p, from, staging, boxes, row0, col0, min(p.n, col0 + p.bn), lane);
+      const uint32_t from = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * kMaxBN + side * left;
+      const int row0 = mb * kPairM + static_cast<int>(rank) * kCtaM + quad * 32, col0 = nb * p.bn + side * left;
+      store_rows<OutT, kLoose>(&tmap_c, c, p, from, staging, row0, col0, min(p.n, nb * p.bn + (side ? p.bn : left)), lane);
       ptx::tcgen05_fence_before_thread_sync();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_u32(&bars->acc_empty[acc]), 0));

@@ -24,15 +24,14 @@ inline cudaError_t rows_i8_launch(const rows_i8::Params<T>& p, cudaStream_t s) {
   const bool vec = p.cols % PV == 0 && p.pitch % PV == 0 && aligned16(p.x) && (!kGated || aligned16(p.up)) && reinterpret_cast<uintptr_t>(p.y) % PV == 0;
   const unsigned rows = static_cast<unsigned>(p.rows);
   auto go = [&](auto kern, unsigned grid, int threads) { return launch_chained(kern, grid, threads, 0, s, 0, p); };
+  // a CTA of as many warps as leave no more than VPT vectors to a thread
+  const auto threads = [&](int vpt) { return static_cast<int>((vecs + 32 * vpt - 1) / (32 * vpt) * 32); };
   if (vec) {
     const unsigned warps = (rows + 7) / 8;
-    if (vecs <= 32) return go(r8::rows_i8_vec_kernel<T, kGated, 256, 32, 1>, warps, 256);
-    if (vecs <= 64) return go(r8::rows_i8_vec_kernel<T, kGated, 256, 32, 2>, warps, 256);
-    if (vecs <= 256) return go(r8::rows_i8_vec_kernel<T, kGated, 256, 256, 1>, rows, 256);
-    if (vecs <= 512) return go(r8::rows_i8_vec_kernel<T, kGated, 256, 256, 2>, rows, 256);
-    if (vecs <= 1024) return go(r8::rows_i8_vec_kernel<T, kGated, 256, 256, 4>, rows, 256);
-    if (vecs <= 2048) return go(r8::rows_i8_vec_kernel<T, kGated, 512, 512, 4>, rows, 512);
-    if (vecs <= 4096) return go(r8::rows_i8_vec_kernel<T, kGated, 1024, 1024, 4>, rows, 1024);
+    if (vecs <= 32) return go(r8::rows_i8_vec_kernel<T, kGated, true, 1>, warps, 256);
+    if (vecs <= 64) return go(r8::rows_i8_vec_kernel<T, kGated, true, 2>, warps, 256);
+    if (vecs <= 2 * 256) return go(r8::rows_i8_vec_kernel<T, kGated, false, 2>, rows, threads(2));
+    if (vecs <= 4 * r8::kMaxThreads) return go(r8::rows_i8_vec_kernel<T, kGated, false, 4>, rows, threads(4));
   }
   if (p.cols <= 4 * r8::kThreads) return go(r8::rows_i8_any_kernel<T, kGated, 4>, rows, r8::kThreads);
   if (p.cols <= 16 * r8::kThreads) return go(r8::rows_i8_any_kernel<T, kGated, 16>, rows, r8::kThreads);
@@ -128,13 +127,11 @@ inline int32_t gemm_i8_pairs_launch(std::string* err, const GemmI8& g, int bn, O
 
 template <typename OutT>
 inline int32_t gemm_i8_typed(std::string* err, const GemmI8& g, void* c, int sms, cudaStream_t s) {
-  const route::GemmI8 plan = route::gemm_i8(g.m, g.n, g.k, sms);
+  const bool loose = !aligned16(c) || g.ldc * sizeof(OutT) % 16 != 0;
+  const route::GemmI8 plan = route::gemm_i8(g.m, g.n, g.k, loose || sizeof(OutT) == 4 ? 32 : 64, sms);
   OutT* out = static_cast<OutT*>(c);
-  if (plan.pairs) {
-    const bool loose = !aligned16(c) || g.ldc * sizeof(OutT) % 16 != 0;
-    const int bn = route::gemm_i8_pair_width(g.m, g.n, loose || sizeof(OutT) == 4 ? 32 : 64, sms);
-    return loose ? gemm_i8_pairs_launch<OutT, true>(err, g, bn, out, sms, s) : gemm_i8_pairs_launch<OutT, false>(err, g, bn, out, sms, s);
-  }
+  if (plan.pairs)
+    return loose ? gemm_i8_pairs_launch<OutT, true>(err, g, plan.width, out, sms, s) : gemm_i8_pairs_launch<OutT, false>(err, g, plan.width, out, sms, s);
   switch (plan.rows) {
     case 16: return gemm_i8_few_launch<OutT, 16>(err, g, plan, out, s);
     case 32: return gemm_i8_few_launch<OutT, 32>(err, g, plan, out, s);

@@ -107,35 +107,44 @@ inline Gemm16 gemm16(int64_t m, int64_t n, int64_t k, int64_t batch, int sms) {
   return r;
 }
 
-// 8-bit product (gemm_i8.cuh): CTA pairs, or 128 columns x `rows` rows of C per CTA and K over `splits` CTAs of a cluster.
+// 8-bit product (gemm_i8.cuh): CTA pairs of 256 rows x `width` columns, or 128 columns x `rows` rows of C per CTA and K over `splits` CTAs of a cluster.
+// By the time they take in nanoseconds, fitted to 70 sizes: a wave of pairs costs 290 for 128 of K, whatever the width, and 10 for a column on its way out; the
+// other kernel's CTAs, two to an SM, what stands below, and no less than reading W takes.  us, pairs of 256 / 192 / 128 columns, best of few rows: 4096^3 56 / 60 / 75, 96 (64 rows);
+// 187 x 3712 x 768 7.3 / 7.0 / 6.4, 7.0; 80 x 6976 x 3264 14 / 14 / 13, 11.3 (128 rows, 4 CTAs); 187 x 64 x 1536 7.4 / 7.2 / 7.3, 6.1 (64, 4); 39 x 256 x 1920 in
+// units of 64 rows 5.7, of 32 5.1; 26 x 4672 x 384 of 32 4.6, of 16 3.8; 1 x 1088 x 12096 by 1, 2, 4, 8 CTAs 28.8, 16.6, 10.3, 7.7.
 struct GemmI8 {
   bool pairs;
+  int width;
   int rows;
   int splits;
   int64_t k_blocks_per_cta;  // 128 of K each
 };
-inline GemmI8 gemm_i8(int64_t m, int64_t n, int64_t k, int sms) {
-  GemmI8 r{false, m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128, 1, 0};
-  const int64_t tiles = div_up(m, r.rows) * div_up(n, 128), kb = div_up(k, 128);
-  r.pairs = m > 128 && n > 128 && tiles > sms;
-  while (r.splits < kMaxGemmSplit) {
-    const int to = 2 * r.splits;
-    const int64_t room = to == 2 || kb >= 128 ? 2 * sms : to == 4 ? sms * 15 / 8 : sms * 8 / 5;
-    if (tiles * to > room || kb / to < 4) break;
-    r.splits = to;
+// `step`: columns of a box that C leaves in.
+inline GemmI8 gemm_i8(int64_t m, int64_t n, int64_t k, int step, int sms) {
+  const int64_t kb = div_up(k, 128), read = 3500 + (m + n) * k / 6000;
+  GemmI8 r{false, 0, 16, 1, kb};
+  int64_t best = INT64_MAX;
+  // reading W hides what is shorter, but not all of it
+  auto consider = [&](int64_t ns, const GemmI8& x) {
+    ns = std::max(read, ns) + ns / 8;
+    if (ns < best) best = ns, r = x;
+  };
+  constexpr int kEnds[4] = {400, 1000, 2400, 5500}, kEndsSplit[4] = {1100, 1400, 2500, 4000}, kBlock[4] = {250, 270, 380, 400}, kBlockOfTwo[4] = {480, 500, 430, 750};
+  for (int i = 0; i < 4; ++i) {
+    const int rows = 16 << i;
+    for (int splits = 1; splits <= kMaxGemmSplit; splits *= 2) {
+      const int64_t per = div_up(kb, splits), ctas = div_up(m, rows) * div_up(n, 128) * splits;
+      const int64_t room = splits <= 2 ? 2 * sms : splits == 4 ? sms * 15 / 8 : sms * 8 / 5, waves = div_up(ctas, room);
+      if (splits > 1 && (per < 2 || div_up(kb, per) != splits || waves > 1)) continue;
+      consider(700 + waves * (1800 + (splits > 1 ? kEndsSplit : kEnds)[i] + per * (ctas > sms ? kBlockOfTwo : kBlock)[i]), GemmI8{false, 0, rows, splits, per});
+    }
   }
-  r.k_blocks_per_cta = div_up(kb > 0 ? kb : 1, r.splits);
+  if (m > 16)
+    for (int width = 256; width >= 128; width -= step) {
+      const int64_t tiles = div_up(m, 256) * div_up(n, width), waves = div_up(tiles, sms / 2);
+      consider(3600 + waves * (kb * 290 + width * 10) - (tiles < 8 ? 1000 : 0), GemmI8{true, width, 16, 1, kb});
+    }
   return r;
-}
-// Rows of W in a pair's tile, a multiple of `step`: what makes all waves together the shortest; the wider of two that do.
-inline int gemm_i8_pair_width(int64_t m, int64_t n, int step, int sms) {
-  int best = 256;
-  int64_t best_cost = INT64_MAX;
-  for (int bn = 256; bn >= 128; bn -= step) {
-    const int64_t cost = div_up(div_up(m, 256) * div_up(n, bn), sms / 2) * (bn + 16);
-    if (cost < best_cost) best_cost = cost, best = bn;
-  }
-  return best;
 }
 
 // CTA pairs: does C leave through shared memory, in whole boxes, or from the lanes that hold its rows?  The boxes are out in a sixth of the time, which

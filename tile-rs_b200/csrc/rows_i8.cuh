@@ -5,6 +5,7 @@
 // same way, an element at a time; wider ones are read twice, the second time from the caches.
 #pragma once
 
+#include "ptx.cuh"
 #include "quantise.cuh"
 #include "softmax.cuh"
 
@@ -26,46 +27,54 @@ struct Params {
 
 // |v| of which is the larger, NaN above all: as bits.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-// The largest magnitude over the LANES threads of a row (a warp or the CTA); each gets it.
-template <int LANES>
+// The largest magnitude over a row's threads (a warp or the CTA); each gets it.
+template <bool kWarp>
 __device__ __forceinline__ float row_max(uint32_t top, uint32_t* red) {
   top = __reduce_max_sync(0xffffffffu, top);
-  if (LANES == 32) return __uint_as_float(top);
+  if (kWarp) return __uint_as_float(top);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
   __syncthreads();
-  top = threadIdx.x % 32 < LANES / 32 ? red[threadIdx.x % 32] : 0u;
+  top = (threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0u;
   return __uint_as_float(__reduce_max_sync(0xffffffffu, top));
 }
-__device__ __forceinline__ float gated(float x, float up) { return x / (1.f + expf(-x)) * up; }
+// silu(x) * up, within 2^-20 of it where x is above -16 (and ten units more below the largest of any row that has an x above 0): the exponential and the reciprocal are the
+// approximate ones, 2^-22 and 2^-23 off, because exact ones are twenty more instructions and 8192 rows of 14336 bf16 took 170 us with them, XX so.
+__device__ __forceinline__ float gated(float x, float up) {
+  const float e = ptx::ex2_approx(x * -1.4426950408889634f);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return x * r * up;
+}
 
-// THREADS of a CTA, LANES of them a row; every row on 16-byte boundaries (y: on as many bytes as a vector has elements); VPT vectors a thread.
-template <typename T, bool kGated, int THREADS, int LANES, int VPT>
-__global__ void __launch_bounds__(THREADS)
+// Every row on 16-byte boundaries (y: on as many bytes as a vector has elements); VPT vectors a thread, a warp a row (kWarp) or a CTA of as many warps as the row fills.
+constexpr int kMaxThreads = 1024;
+template <typename T, bool kGated, bool kWarp, int VPT>
+__global__ void __launch_bounds__(kWarp ? 256 : kMaxThreads)
 rows_i8_vec_kernel(const Params<T> p) {
   constexpr int PV = Elem<T>::kPerVec;
   __shared__ uint32_t red[32];
   ptx::launch_dependents_if_few();
   ptx::wait_prior_grid();
-  const int lane = threadIdx.x % LANES;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (THREADS / LANES) + threadIdx.x / LANES;
-  if (row >= p.rows) return;  // rows of a CTA are all there, or each has a warp
+  const int lanes = kWarp ? 32 : blockDim.x, lane = kWarp ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t row = kWarp ? static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= p.rows) return;  // a warp's
   const int nvec = p.cols / PV;
   const Vec16* x = reinterpret_cast<const Vec16*>(p.x + row * p.pitch);
   const Vec16* up = reinterpret_cast<const Vec16*>(p.up + (kGated ? row * p.pitch : 0));
   Vec16 a[VPT], b[kGated ? VPT : 1];
 #pragma unroll
   for (int k = 0; k < VPT; ++k)
-    if (k * LANES + lane < nvec) a[k] = softmax::ld_stream(x + k * LANES + lane);
+    if (k * lanes + lane < nvec) a[k] = softmax::ld_stream(x + k * lanes + lane);
   if constexpr (kGated) {
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
-      if (k * LANES + lane < nvec) b[k] = softmax::ld_stream(up + k * LANES + lane);
+      if (k * lanes + lane < nvec) b[k] = softmax::ld_stream(up + k * lanes + lane);
   }
   float v[VPT][PV];
   uint32_t top = 0u;
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
-    if (k * LANES + lane >= nvec) continue;
+    if (k * lanes + lane >= nvec) continue;
     Elem<T>::unpack(a[k], v[k]);
     if constexpr (kGated) {
       float u[PV];
@@ -76,10 +85,10 @@ rows_i8_vec_kernel(const Params<T> p) {
 #pragma unroll
     for (int e = 0; e < PV; ++e) top = max(top, magnitude(v[k][e]));
   }
-  const quant::Step step = quant::step_of(row_max<LANES>(top, red));
+  const quant::Step step = quant::step_of(row_max<kWarp>(top, red));
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
-    const int i = k * LANES + lane;
+    const int i = k * lanes + lane;
     if (i >= nvec) continue;
     uint32_t q[PV / 4];
 #pragma unroll
@@ -117,7 +126,7 @@ rows_i8_any_kernel(const Params<T> p) {
   } else {
     for (int c = threadIdx.x; c < p.cols; c += kThreads) top = max(top, magnitude(value(c)));
   }
-  const quant::Step step = quant::step_of(row_max<kThreads>(top, red));
+  const quant::Step step = quant::step_of(row_max<false>(top, red));
   auto put = [&](int c, float x) { p.y[to + c] = static_cast<int8_t>(step.step > 0.f ? __float2int_rn(x / step.step) : 0); };
   if constexpr (EPT > 0) {
 #pragma unroll
