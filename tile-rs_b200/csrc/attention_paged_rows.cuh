@@ -44,7 +44,8 @@ __device__ __forceinline__ bool sequence(const P& p, int b, int& first, int& cou
   }
   if (!pages::sequence(p.step, p.cache.page_size, b, first, count, len, status, site)) return false;
   len -= p.prefix;
-  if (len >= count) return true;
+  // the prefix's rows are the tokens before starts[batch]: with starts in no order a sequence may have others
+  if (len >= count && first + count <= p.step.starts[p.step.batch]) return true;
   pages::report(status, site);
   return false;
 }
@@ -87,6 +88,8 @@ struct RowsTile {
 };
 // What beginning a unit costs a warp, in tiles.
 constexpr int kRowsUnitCost = 1;
+// A share's tiles at least: a row has as many records as its keys have shares.
+constexpr int kRowsMinShare = 3;
 
 struct RowsParams {
   pages::Cache cache;
@@ -166,7 +169,7 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
     own = base + tid < batch ? rows_sequence_tiles<kKeys, TP, kHeld>(p, base + tid, s, p.status) : 0;
     total += block_scan(own, before);
   }
-  const int64_t shares = static_cast<int64_t>(gridDim.x) * kWarps, per = (total + shares - 1) / shares;
+  const int64_t shares = static_cast<int64_t>(gridDim.x) * kWarps, per = max((total + shares - 1) / shares, static_cast<int64_t>(kRowsMinShare));
   const int64_t share0 = static_cast<int64_t>(blockIdx.x) * kWarps;
   auto find = [&](int b, int64_t from) {  // the warps whose shares begin in what this thread looked at
 #pragma unroll
@@ -607,7 +610,8 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
   }
 }
 
-// What a row's records add up to.  CTA (b, y) has rows of sequence b: D / 4 threads a row, four times, which take every fourth record; four are asked for before the first is used.
+// What a row's records add up to.  CTA (b, y) has rows of sequence b: D / 4 threads a row, kSplits times, which deal its records out; four are asked for before the first is used.
+// Four or sixteen: rows of 592 records (4 sequences on 16384, 2 KV heads) took the whole call from 30 to 50 us with four.
 // A part whose scores are all -inf weighs nothing beside another.
 struct Join {
   pages::Cache cache;
@@ -619,7 +623,8 @@ struct Join {
   int32_t shared_tokens, large_tokens;  // of a tile, where the records are tcgen05's (256 rows a block); 0: shared_held, rest_held rows a unit
   int32_t shared_held, rest_held;
 };
-constexpr int kJoinThreads = 256, kJoinSplits = 4;
+template <int kSplits>
+constexpr int kJoinThreads = kSplits == 4 ? 256 : 512;
 // A row's records: the first, and what lies between one share's and the next, in numbers.
 struct Pieces {
   const float* first;
@@ -649,13 +654,13 @@ __device__ __forceinline__ Pieces pieces(const Records& rec, int tile_tokens, ui
   x.next = place + x.step;
   return x;
 }
-template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads, 4)
+template <typename T, int D, int kSplits>
+__global__ void __launch_bounds__(kJoinThreads<kSplits>, 1024 / kJoinThreads<kSplits>)
 attention_paged_join_kernel(T* o, const __grid_constant__ Join p) {
-  constexpr int kLanes = D / 4, kRowsAt = kJoinThreads / kLanes / kJoinSplits, kAtOnce = 4;
+  constexpr int kLanes = D / 4, kRowsAt = kJoinThreads<kSplits> / kLanes / kSplits, kAtOnce = 4;
   constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
-  __shared__ float4 part_x[kJoinSplits][kRowsAt][kLanes];
-  __shared__ float2 part_ml[kJoinSplits][kRowsAt];
+  __shared__ float4 part_x[kSplits][kRowsAt][kLanes];
+  __shared__ float2 part_ml[kSplits][kRowsAt];
   ptx::launch_dependents_if_few();
   ptx::wait_prior_grid();
   const int b = static_cast<int>(blockIdx.x);
@@ -663,7 +668,7 @@ attention_paged_join_kernel(T* o, const __grid_constant__ Join p) {
   if (p.all ? !pages::sequence<false>(p.step, p.cache.page_size, b, first, count, len, nullptr, 0) : !sequence<kRest>(p, b, first, count, len, nullptr, 0)) return;
   const bool large = is_large(p, count);
   const Records& rest = large ? p.rest_large : p.rest;
-  const int rest_tokens = large ? p.large_tokens : 0, lane = threadIdx.x % kLanes, split = threadIdx.x / kLanes % kJoinSplits, mine = threadIdx.x / (kLanes * kJoinSplits);
+  const int rest_tokens = large ? p.large_tokens : 0, lane = threadIdx.x % kLanes, split = threadIdx.x / kLanes % kSplits, mine = threadIdx.x / (kLanes * kSplits);
   const uint32_t rows = static_cast<uint32_t>(count) * p.heads_q, group = p.group;
   for (uint32_t i0 = blockIdx.y * kRowsAt; i0 < rows; i0 += gridDim.y * kRowsAt) {
     const uint32_t i = i0 + mine, row = static_cast<uint32_t>(first) * p.heads_q + i;
@@ -681,12 +686,12 @@ attention_paged_join_kernel(T* o, const __grid_constant__ Join p) {
         const float* next = of_rest ? r.next : s.next;
         return at == 0 ? (of_rest ? r.first : s.first) : next + static_cast<int64_t>(at - 1) * (of_rest ? r.step : s.step);
       };
-      for (int j0 = split; j0 < n; j0 += kJoinSplits * kAtOnce) {
+      for (int j0 = split; j0 < n; j0 += kSplits * kAtOnce) {
         float2 ml[kAtOnce];
         float4 y[kAtOnce];
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j) {
-          const int at = j0 + j * kJoinSplits;
+          const int at = j0 + j * kSplits;
           ml[j] = make_float2(-INFINITY, 0.f), y[j] = make_float4(0.f, 0.f, 0.f, 0.f);
           if (at < n) {
             const float* rec = record(at);
@@ -701,7 +706,7 @@ attention_paged_join_kernel(T* o, const __grid_constant__ Join p) {
         // a part of no scores but -inf weighs nothing; it is added all the same, because one of NaN scores has that maximum too
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j) {
-          if (j0 + j * kJoinSplits >= n) break;
+          if (j0 + j * kSplits >= n) break;
           const float w = ml[j].x == -INFINITY ? 0.f : ptx::ex2_approx(ml[j].x - top);
           l = fmaf(w, ml[j].y, l);
           x.x = fmaf(w, y[j].x, x.x), x.y = fmaf(w, y[j].y, x.y), x.z = fmaf(w, y[j].z, x.z), x.w = fmaf(w, y[j].w, x.w);
@@ -716,10 +721,10 @@ attention_paged_join_kernel(T* o, const __grid_constant__ Join p) {
     if (split == 0 && i < rows) {
       float top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < kJoinSplits; ++j) top = fmaxf(top, part_ml[j][mine].x);
+      for (int j = 0; j < kSplits; ++j) top = fmaxf(top, part_ml[j][mine].x);
       l = 0.f, x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int j = 0; j < kJoinSplits; ++j) {
+      for (int j = 0; j < kSplits; ++j) {
         const float2 ml = part_ml[j][mine];
         const float4 y = part_x[j][mine][lane];
         const float w = ml.x == -INFINITY ? 0.f : ptx::ex2_approx(ml.x - top);

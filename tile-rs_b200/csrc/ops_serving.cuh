@@ -392,11 +392,15 @@ inline int32_t attention_rows_launch(std::string* err, const paged::Params& base
     e = launch_chained(kern, static_cast<unsigned>(std::min(sms, paged::kMaxCtas)), L::kThreads, L::kSmem, s, 0, map[0], map[1], static_cast<const T*>(q), p);
   return cuda_ok(err, e, "attention_paged_rows_kernel launch");
 }
+// `records`: about how many a row has.
 template <typename T, int D>
-inline int32_t attention_join_launch(std::string* err, const paged::Join& join, void* o, cudaStream_t s) {
-  const int64_t at_once = paged::kJoinThreads / (D / 4) / paged::kJoinSplits, ys = (static_cast<int64_t>(join.step.max_new) * join.heads_q + at_once - 1) / at_once;
-  const dim3 grid(static_cast<unsigned>(join.step.batch), static_cast<unsigned>(std::min<int64_t>(ys, 64)));
-  return cuda_ok(err, launch_chained(paged::attention_paged_join_kernel<T, D>, grid, paged::kJoinThreads, 0, s, 0, static_cast<T*>(o), join), "attention_paged_join_kernel launch");
+inline int32_t attention_join_launch(std::string* err, const paged::Join& join, int64_t records, void* o, cudaStream_t s) {
+  auto go = [&](auto kern, int splits, int threads) {
+    const int64_t at_once = threads / (D / 4) / splits, ys = (static_cast<int64_t>(join.step.max_new) * join.heads_q + at_once - 1) / at_once;
+    const dim3 grid(static_cast<unsigned>(join.step.batch), static_cast<unsigned>(std::min<int64_t>(ys, 64)));
+    return cuda_ok(err, launch_chained(kern, grid, threads, 0, s, 0, static_cast<T*>(o), join), "attention_paged_join_kernel launch");
+  };
+  return records > 40 ? go(paged::attention_paged_join_kernel<T, D, 16>, 16, paged::kJoinThreads<16>) : go(paged::attention_paged_join_kernel<T, D, 4>, 4, paged::kJoinThreads<4>);
 }
 // What both need: scratch for `whole` arrays of records, `part` bytes of cut ones and `cuts` places.
 struct RecordSpace {
@@ -447,7 +451,7 @@ inline int32_t attention_cross_rows(std::string* err, const paged::Params& p, co
   paged::Join join = join_of(p);
   join.all = 1, join.rest = more.rest, join.rest_held = L::kHeld;
   st = attention_rows_launch<T, kI8, D, kWide, paged::kAll>(err, p, more, q, s);
-  if (st == TSM100_OK) st = attention_join_launch<T, D>(err, join, o, s);
+  if (st == TSM100_OK) st = attention_join_launch<T, D>(err, join, ctas * L::kWarps / static_cast<int64_t>(cuts), o, s);
   return give_records(err, space, s, st);
 }
 template <typename T, bool kI8, int D>
@@ -526,7 +530,9 @@ inline int32_t attention_prefix_launch(std::string* err, const paged::Params& p,
     more.rest = join.rest_large;
     st = attention_paged_tc_launch<T, kI8, D, pg::kRest>(err, p, plan.run_log2, q, o, s, more);
   }
-  if (st == TSM100_OK) st = attention_join_launch<T, D>(err, join, o, s);
+  const int64_t tiles = more.prefix / pg::RowsTile<kI8, D, true>::kPos;
+  const int64_t records = plan.shared_tc ? ctas / (heads * shared_units) : std::min<int64_t>(ctas * 8 / (heads * shared_units), tiles / pg::kRowsMinShare);
+  if (st == TSM100_OK) st = attention_join_launch<T, D>(err, join, records, o, s);
   return give_records(err, space, s, st);
 }
 template <bool kI8, int D>

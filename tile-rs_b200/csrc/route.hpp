@@ -339,7 +339,7 @@ inline bool softmax_twice_skip(int64_t vectors, int threads, int unroll) {
 // Attention of sequences that begin with the same pages: are the prefix's rows (all tokens times the heads of a group) tcgen05's, 256 at a time, or the other kernel's, 16 at a time?
 inline bool prefix_on_tcgen05(int64_t rows, int64_t prefix, int heads_kv, int head_dim, bool i8) {
   const int64_t passes = div_up(rows, 16), bytes = 2 * prefix * heads_kv * head_dim * (i8 ? 1 : 2);
-  return (passes - 1) * bytes > (i8 ? 64ll << 20 : 24ll << 20);
+  return (passes - 1) * bytes > (i8 ? 200ll << 20 : 80ll << 20);
 }
 // Rows of a sequence's own tokens beyond which its own positions are tcgen05's.
 constexpr int64_t kPrefixFewRows = 64;
