@@ -149,11 +149,14 @@ int32_t tsm100_launch(tsm100_module_t mod, const char* name, uint32_t blocks, vo
  *   more than 16, else up to 2.5 MB;
  *   tsm100_gemm_w4, more than 64 rows in 8 bits: 2 bytes per element of A; more than 1024 rows in 16 bits, N >= 2048 and K >= 512: 2 per element of W,
  *   and of C where its rows do not start on 16-byte boundaries;
+ *   tsm100_attention_paged_cross: as tsm100_attention_paged for more than 16 rows, else 4 (d + 4) bytes for each token and query head, and up to 20 MB for heads of 128, 10 MB for 64;
+ *   tsm100_attention_paged_prefix: 8 (d + 4) bytes for each token and query head and 20 MB (10 for heads of 64), 40 (21) more where the prefix has many rows, and as many again
+ *   where a sequence has more than 64;
  *   tsm100_gemm_i8, rows of a or w that do not start on 16-byte boundaries: a copy of a, of w, or of both.
  * It is taken and returned on the caller's stream, from a pool of the library's own on each device (the device's default
  * memory pool is neither used nor changed).  The pool keeps up to 1/16 of the device's memory for later calls and gives it
  * back when the device's last handle is closed.  When the device has no memory left, such a call takes a form without
- * scratch: slower, and with its sums in another order.  tsm100_attention_paged, tsm100_gemm_i8, and tsm100_gemm_w4 for rows in 8 bits, have none and answer TSM100_ERR_MEMORY.
+ * scratch: slower, and with its sums in another order.  The attentions over pages, tsm100_gemm_i8, and tsm100_gemm_w4 for rows in 8 bits, have none and answer TSM100_ERR_MEMORY.
  * While a stream is captured, taking and returning become allocation nodes of the graph.  The graph can be replayed any
  * number of times; as CUDA has it for graphs with such nodes, it has one executable instance at a time and cannot be a
  * child graph or be cloned. */
@@ -497,8 +500,8 @@ int32_t tsm100_attention_paged_cross(tsm100_device_t dev, const tsm100_paged_kv*
 /* tsm100_attention_paged for sequences that begin with the same pages: their first prefix_len positions lie in pages prefix[0], prefix[1], ... (in device
  * memory, prefix_len / page_size of them), which are read once for all, and of a row of the table only what comes behind them.  lens, and the places in a
  * row, count from the sequence's beginning, so that one description serves this call and tsm100_kv_page_append.  The same result as
- * tsm100_attention_paged on rows that begin with those pages, up to the rounding of f32 sums in another order.  A sequence with tokens whose new ones do not all
- * lie behind the prefix is left out too. */
+ * tsm100_attention_paged on rows that begin with those pages, up to the rounding of f32 sums in another order.  A sequence whose new tokens do not all lie
+ * behind the prefix, or not all before starts[batch], is left out too. */
 typedef struct {
   int32_t dtype; /* TSM100_F16 | TSM100_BF16 */
   int32_t heads_q;

@@ -23,6 +23,11 @@ extern "C" void pair_tiles(long long m, long long n, long long k, long long batc
   const PairTiles r = gemm_f32_pair_tiles(m, n, k, batch, sms);
   out[0] = r.bn, out[1] = r.whole_tiles, out[2] = r.splits;
 }
+extern "C" void gemm_i8_plan(long long m, long long n, long long k, int step, int sms, long long* out) {
+  const GemmI8 r = gemm_i8(m, n, k, step, sms);
+  out[0] = r.pairs, out[1] = r.width, out[2] = r.rows, out[3] = r.splits, out[4] = r.k_blocks_per_cta;
+}
+extern "C" int prefix_tc(long long rows, long long prefix, int heads, int d, int i8) { return prefix_on_tcgen05(rows, prefix, heads, d, i8 != 0); }
 extern "C" int rope_is_few(long long blocks, int heads_per, int sms) { return rope_few(blocks, heads_per, sms); }
 extern "C" int decode_chained(long long ctas, long long bytes, int sms) { return decode_is_chained(ctas, bytes, sms); }
 extern "C" int early(long long b_bytes, long long ctas, int sms) { return skinny_places_early(b_bytes, ctas, sms); }
@@ -273,3 +278,39 @@ def test_f16_products_of_few_outputs(lib, m, n, k, batch, pays):
 @pytest.mark.parametrize("blocks,keys,ctas", [(1, 4095, 1), (1, 4096, 8), (8, 5361, 10), (64, 7512, 2), (74, 8191, 2), (75, 8191, 1), (30, 4100, 4), (1, 8191, 15), (1, 8192, 8), (64, 16384, 2)])
 def test_attention_steps_of_middling_caches(lib, blocks, keys, ctas):
     assert lib.split_ctas(C.c_longlong(blocks), C.c_longlong(keys), SMS) == ctas
+
+
+def gemm_i8(lib, m, n, k, step=64):
+    out = (C.c_longlong * 5)()
+    lib.gemm_i8_plan(*(C.c_longlong(x) for x in (m, n, k)), step, SMS, out)
+    return tuple(out)
+
+
+@pytest.mark.parametrize("m,n,k,plan", [
+    (1, 4096, 4096, ("few", 16, 4)), (1, 1088, 12096, ("few", 16, 8)), (48, 28672, 4096, ("few", 64, 1)), (187, 64, 1536, ("few", 16, 4)), (4096, 4096, 4096, ("pairs", 256)),
+    (8192, 28672, 4096, ("pairs", 256)), (346, 15552, 128, ("pairs", 256)), (1, 64, 64, ("few", 16, 1))])
+def test_8_bit_products(lib, m, n, k, plan):
+    """What measured best, or within a few percent of it."""
+    pairs, width, rows, splits, _ = gemm_i8(lib, m, n, k)
+    assert ("pairs", width) == plan if pairs else ("few", rows, splits) == plan
+
+
+def test_8_bit_products_cover_k_and_fit_a_launch(lib):
+    for m in (1, 7, 16, 17, 100, 300, 5000):
+        for n in (1, 100, 128, 5003, 30000):
+            for k in (1, 16, 128, 129, 1000, 4112, 16384, 131071):
+                for step in (32, 64):
+                    pairs, width, rows, splits, per = gemm_i8(lib, m, n, k, step)
+                    kb = -(-k // 128)
+                    if pairs:
+                        assert m > 16 and 128 <= width <= 256 and width % step == 0
+                    else:
+                        # every CTA of a cluster has a part of K, and all of it is somebody's
+                        assert rows in (16, 32, 64, 128) and 1 <= splits <= 8 and per * splits >= kb > per * (splits - 1)
+
+
+@pytest.mark.parametrize("rows,prefix,heads,d,i8,tcgen05", [
+    (16, 1 << 20, 8, 128, False, False), (32, 16384, 8, 128, False, False), (64, 16384, 8, 128, False, True), (64, 16384, 8, 64, False, True), (64, 4096, 8, 128, False, False),
+    (64, 16384, 8, 128, True, False), (256, 16384, 8, 128, True, True)])
+def test_rows_on_a_shared_prefix(lib, rows, prefix, heads, d, i8, tcgen05):
+    assert bool(lib.prefix_tc(C.c_longlong(rows), C.c_longlong(prefix), heads, d, int(i8))) == tcgen05

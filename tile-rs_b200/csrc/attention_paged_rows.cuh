@@ -3,7 +3,7 @@
 // The products, the running softmax and the tiles are those of attention_paged.cuh.  What differs is who works on what: a share of the stream is a WARP's, which goes from unit
 // to unit by itself and leaves a record (O, maximum, sum) of every unit that it has a part of; another kernel joins a row's records.  No barrier is
 // met after the stream has been measured, and beginning a unit costs the warp a load of its queries instead of costing the CTA two barriers and a merge of all warps' records:
-// 64 sequences of 750 positions in 8 bits, 8 KV heads, XX us by CTAs, XX so.
+// 64 sequences of 750 positions in the mean, 8 bits, 8 KV heads, 40 us by CTAs, 31 so (3.2 TB/s); 128 of 450 in bf16 62 and 45 (5.2 TB/s).
 //
 // Bound: HBM.
 #pragma once
@@ -122,6 +122,9 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
   constexpr int NB = kWide ? 2 : 1;  // eights of rows
   constexpr bool kIsBf16 = !std::is_same<T, __half>::value;
   constexpr bool kMmaBf16 = kIsBf16 && !kI8;
+  // f16 results from 8 bits: a probability times V's step takes two f16 numbers.  In one, even the weight of a row's first key was rounded, to as many bits as the result has, and
+  // results were 1.4 times as far from 64 bits as that alone makes them (2.9e-4, so 2.1e-4).
+  constexpr bool kTwoParts = kI8 && !kIsBf16;
   constexpr int TP = L::kPos, N16 = TP / 16, KSTEPS = D / 16, REC = L::kRec, kSlots = L::kSlots, kChunks = L::kRowBytes / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -521,13 +524,20 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
             for (int n = 0; n < NB; ++n) s[j][n][2 * h] *= x, s[j][n][2 * h + 1] *= x;
           }
       }
-      uint32_t pb[N16][NB][2];
+      uint32_t pb[N16][NB][2], rest[kTwoParts ? N16 : 1][NB][2];
 #pragma unroll
       for (int j = 0; j < N16; ++j)
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) pb[j][n][h] = transposed(mma::pack2<kMmaBf16>(s[j][n][2 * h], s[j][n][2 * h + 1]));
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t x = mma::pack2<kMmaBf16>(s[j][n][2 * h], s[j][n][2 * h + 1]);
+            pb[j][n][h] = transposed(x);
+            if constexpr (kTwoParts) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
+              rest[j][n][h] = transposed(mma::pack2<false>(s[j][n][2 * h] - f.x, s[j][n][2 * h + 1] - f.y));
+            }
+          }
 #pragma unroll
       for (int c = 0; c < KSTEPS; ++c)
 #pragma unroll
@@ -556,7 +566,10 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
               const uint32_t x = va[i] ^ 0x80808080u, y = va[2 + i] ^ 0x80808080u;
               const uint32_t a0 = i8_pair(x, 0x4240), a1 = i8_pair(x, 0x4341), a2 = i8_pair(y, 0x4240), a3 = i8_pair(y, 0x4341);
 #pragma unroll
-              for (int n = 0; n < NB; ++n) mma_tile<false>(oacc[c + i][n], a0, a1, a2, a3, pb[j][n][0], pb[j][n][1]);
+              for (int n = 0; n < NB; ++n) {
+                mma_tile<false>(oacc[c + i][n], a0, a1, a2, a3, pb[j][n][0], pb[j][n][1]);
+                if constexpr (kTwoParts) mma_tile<false>(oacc[c + i][n], a0, a1, a2, a3, rest[j][n][0], rest[j][n][1]);
+              }
             }
           }
         }

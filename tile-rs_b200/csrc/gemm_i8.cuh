@@ -252,8 +252,9 @@ gemm_i8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
 // ---------------------------------------------------------------------------
 // Per CTA: warp 0 TMA producer (128 rows of A and half of the tile's rows of W, 128 of K a stage), warp 1 tensor memory and, in the leader, the products
 // (M = 256 over the pair, N = bn, K = 32), warps 2..9 this CTA's 128 rows of the sums, of which two sets alternate, scaled and stored as boxes
-// (four warps took 3.5 us for 128 x 256 in a row of tiles, longer than the products of K = 1280).
-// Bound: the tensor pipe, 2 M N K.  Widths from 128 to 256 so that the last wave of tiles is a full one (route.hpp: gemm_i8_pair_width).
+// (by four warps 497 x 27968 x 192 took 17.6 us, by eight 14.0; K of thousands does not tell them apart).
+// Bound: the tensor pipe, 2 M N K: 8192^3 325 us (3.38 POP/s), 8192 x 28672 x 4096 600 (3.2), single CTAs of 128 x 128 1027.  Below that operands from the L2, 64 KB for 128 of K to
+// a pair, and what a tile takes to leave, 2.6 us, which the next tile's products do not hide: 4096^3 56 us (41 by the pipe).  Widths from 128 to 256 so that the last wave of tiles is a full one (route.hpp: gemm_i8).
 namespace pairs {
 
 constexpr int kPairM = 256, kCtaM = 128, kMaxBN = 256;
