@@ -20,7 +20,7 @@ namespace paged {
 //   kRest    positions p.prefix .. its own; a sequence with more than p.large rows is tcgen05's (attention_paged_tc.cuh), any other the other kernel's
 //   kBoth    as kShared and as kRest, as two results, in one stream
 enum Keys { kPast, kAll, kShared, kRest, kBoth };
-// On tcgen05 the last three leave records, which attention_paged_join_kernel puts together; so do all here.
+// kAll, kRest and kBoth here, kAll, kShared and kRest on tcgen05.  The last three leave records, which attention_paged_join_kernel puts together; here kAll does too.
 __host__ __device__ constexpr bool leaves_records(Keys k) { return k == kShared || k == kRest || k == kBoth; }
 
 // Records of rows: D numbers of O, not normalised, the logarithm to base 2 of what the weights were taken against, their sum, two unused.  A unit (or block) of rows that one
@@ -30,6 +30,7 @@ struct Records {
   float* part;        // [share][2][held], of a unit that began in an earlier share, of one that goes on in the next
   int2* cut;          // the share that the unit's keys begin in, and how many shares there are, 0 if one; [heads_kv][units], kRest: [batch][heads_kv][units]
   int32_t units;      // of a KV head (of a sequence)
+  int32_t shares;     // places in part
 };
 
 // The tokens of sequence b and the keys that they see; false, and reported, if they contradict each other or the call.  kRest counts positions from the
@@ -129,9 +130,10 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kWarps * kSlots * (L::kBytes + L::kScales));
-  __shared__ int64_t scan[kWarps], first_base[kWarps];
+  __shared__ int64_t scan[kWarps];
   __shared__ uint32_t abort_word;
-  __shared__ int first_seq[kWarps];
+  // Parts of units: the one that a warp works on (its sequence is found by whichever thread looked at it), and the one that its loads have come to.
+  __shared__ Part parts[kWarps], parts_ahead[kWarps];
   volatile uint32_t* abort_flag = &abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, tq = lane & 3;
   if (tid == 0) {
@@ -167,9 +169,9 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
     return total;
   };
   int64_t total = 0, before = 0, own = 0;
+  Seq mine;
   for (int base = kFirst; base < batch; base += kThreads) {
-    Seq s;
-    own = base + tid < batch ? rows_sequence_tiles<kKeys, TP, kHeld>(p, base + tid, s, p.status) : 0;
+    own = base + tid < batch ? rows_sequence_tiles<kKeys, TP, kHeld>(p, base + tid, mine, p.status) : 0;
     total += block_scan(own, before);
   }
   const int64_t shares = static_cast<int64_t>(gridDim.x) * kWarps, per = max((total + shares - 1) / shares, static_cast<int64_t>(kRowsMinShare));
@@ -178,7 +180,7 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const int64_t t = (share0 + w) * per;
-      if (from <= t && t < from + own) first_seq[w] = b, first_base[w] = from;
+      if (from <= t && t < from + own) parts[w].seq = mine, parts[w].seq.b = b, parts[w].seq.base = from;
     }
   };
   if (batch - kFirst <= kThreads) {
@@ -186,8 +188,7 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
   } else {
     int64_t sum = 0;
     for (int base = kFirst; base < batch; base += kThreads) {
-      Seq s;
-      own = base + tid < batch ? rows_sequence_tiles<kKeys, TP, kHeld>(p, base + tid, s, nullptr) : 0;
+      own = base + tid < batch ? rows_sequence_tiles<kKeys, TP, kHeld>(p, base + tid, mine, nullptr) : 0;
       const int64_t here = block_scan(own, before);
       find(base + tid, sum + before);
       sum += here;
@@ -214,12 +215,11 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
     if (x.start >= t1 || x.seq.b >= batch) x.there = false;
     else cut(x);
   };
-  // Parts live in shared memory: the one that the warp works on, and the one that its loads have come to.
-  __shared__ Part parts[kWarps], parts_ahead[kWarps];
   Part &now = parts[warp], &ahead = parts_ahead[warp];
   if (lane == 0) {
     Part x;
-    open(x, first_seq[warp], first_base[warp]);
+    x.seq = now.seq;
+    x.start = x.seq.base;
     x.unit = static_cast<int>((t0 - x.start) / (x.seq.tiles + kRowsUnitCost));
     x.start += static_cast<int64_t>(x.unit) * (x.seq.tiles + kRowsUnitCost);
     cut(x);
@@ -624,7 +624,8 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
 }
 
 // What a row's records add up to.  CTA (b, y) has rows of sequence b: D / 4 threads a row, kSplits times, which deal its records out; four are asked for before the first is used.
-// Four or sixteen: rows of 592 records (4 sequences on 16384, 2 KV heads) took the whole call from 30 to 50 us with four.
+// Four, or sixteen where rows have more than 40: 4 sequences on 16384 with 2 KV heads, the whole call, 50 us with four and shares of any size (592 records a row), 23 with sixteen and
+// kRowsMinShare.
 // A part whose scores are all -inf weighs nothing beside another.
 struct Join {
   pages::Cache cache;
@@ -660,7 +661,9 @@ __device__ __forceinline__ Pieces pieces(const Records& rec, int tile_tokens, ui
   }
   const int2 cut = __ldcg(rec.cut + cut0 + static_cast<int64_t>(head) * rec.units + unit);
   Pieces x;
-  x.n = max(cut.y, 1);
+  // a kernel that gave up a wait has left some places unwritten: nothing is read by those
+  const bool there = cut.x >= 0 && cut.y >= 0 && cut.x < rec.shares && cut.y <= rec.shares - cut.x;
+  x.n = there ? max(cut.y, 1) : 0;
   x.step = 2 * held * REC;
   const float* place = rec.part + (static_cast<int64_t>(cut.x) * (2 * held) + r) * REC;
   x.first = cut.y == 0 ? rec.whole + static_cast<int64_t>(row) * REC : place + held * REC;

@@ -93,7 +93,7 @@ struct Params {
   int32_t tokens;      // of a tile: 128 / group
   int32_t run_log2;    // positions of a page's box
   float scale_log2;
-  int32_t prefix;      // attention_paged.cuh: Keys
+  int32_t prefix;      // attention_paged_rows.cuh: Keys
   int32_t large;
   const int32_t* prefix_table;
   Records records;

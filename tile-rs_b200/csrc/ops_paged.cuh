@@ -320,7 +320,7 @@ inline int32_t attention_cross_rows(std::string* err, const paged::Params& p, co
   if (st != TSM100_OK) return st;
   PrefixArgs more = {};
   more.rest.whole = space.floats(whole), more.rest.part = space.floats(part), more.rest.cut = space.places(cuts);
-  more.rest.units = static_cast<int32_t>(units);
+  more.rest.units = static_cast<int32_t>(units), more.rest.shares = static_cast<int32_t>(ctas * L::kWarps);
   paged::Join join = join_of(p);
   join.all = 1, join.rest = more.rest, join.rest_held = L::kHeld;
   st = attention_rows_launch<T, kI8, D, kWide, paged::kAll>(err, p, more, q, s);
@@ -380,6 +380,8 @@ inline int32_t attention_prefix_launch(std::string* err, const paged::Params& p,
   join.shared.cut = space.places(heads * shared_units), join.rest.cut = space.places(heads * p.step.batch * rest_units);
   join.rest_large.cut = space.places(heads * p.step.batch * large_units);
   join.shared.units = static_cast<int32_t>(shared_units), join.rest.units = static_cast<int32_t>(rest_units), join.rest_large.units = static_cast<int32_t>(large_units);
+  join.rest.shares = static_cast<int32_t>(ctas) * (wide ? pg::RowsTile<kI8, D, true>::kWarps : pg::RowsTile<kI8, D, false>::kWarps);
+  join.shared.shares = plan.shared_tc ? static_cast<int32_t>(ctas) : join.rest.shares, join.rest_large.shares = static_cast<int32_t>(ctas);
   more.shared = join.shared, more.rest = join.rest;
   if (plan.shared_tc) {
     st = attention_paged_tc_launch<T, kI8, D, pg::kShared>(err, p, plan.run_log2, q, o, s, more);
