@@ -430,7 +430,7 @@ int32_t tsm100_quantise_rows(tsm100_device_t dev, const tsm100_quantise_rows_des
 
 /* Product in 8 bits, C[m,n] = (sum_k a[m,k] w[n,k]) * a_scales[m] * w_scales[n]: a [M][K] and w [N][K] are whole numbers (any int8), with a
  * step for every row of each (what tsm100_add_rms_norm and tsm100_quantise_rows leave).  The sums are exact (32-bit whole numbers, K < 131072), their
- * scaling is f32 and C is rounded once to dtype, so results do not depend on how the work is dealt out.  A row whose step is NaN is NaN.  lda / ldw / ldc
+ * scaling is f32 and C is rounded once to dtype, so results do not depend on how the work is dealt out.  A row whose step is NaN is NaN (K = 0: zeros, the steps are not read).  lda / ldw / ldc
  * are row pitches in elements, 0 = packed.  Operands whose rows do not start on 16-byte boundaries are copied to scratch (above). */
 typedef struct {
   int32_t dtype; /* of C: TSM100_F32 | TSM100_F16 | TSM100_BF16 */

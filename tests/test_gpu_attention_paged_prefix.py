@@ -277,6 +277,24 @@ def test_what_is_outside_is_reported(dev, pkg, held):
             assert dev.status() == 0
 
 
+@pytest.mark.parametrize("held", ["bf16", "i8"])
+@pytest.mark.parametrize("news,group,page", [((1, 1, 1), 4, 16), ((3, 1, 0), 4, 16), ((3, 40, 9), 4, 16), ((3, 40, 9), 5, 3)])
+def test_any_number_of_new_tokens_allowed(dev, pkg, news, group, page, held):
+    """max_new as large as it goes takes no memory by itself: the same result, bit for bit, as with the call's tokens."""
+    cache = Sharing(pkg, 31, list(zip(news, (90, 700, 33))), 2, 64, page, "bf16", held, 7)
+    q = u.normal(u.gen(32), (cache.tokens, 2 * group, 64)).bfloat16()
+    got = []
+    for most in (cache.tokens, 2**31 - 1):
+        batch = pkg.hal.PagedBatch(3, cache.tokens, most, 0, cache.pitch, u.ptr(cache.table), u.ptr(cache.lens), u.ptr(cache.starts))
+        o = torch.full_like(q, 55.0)
+        dev.attention_paged_prefix(cache.view(), batch, pkg.capi.BF16, 2 * group, cache.shared * cache.page, u.ptr(cache.prefix), u.ptr(q), u.ptr(o), stream=u.stream())
+        torch.cuda.synchronize()
+        assert dev.status() == 0
+        got.append(o)
+    assert torch.equal(*got)
+    check(cache, q, got[0])
+
+
 def test_refusals(dev, pkg):
     capi, hal = pkg.capi, pkg.hal
     x = torch.zeros(4096, device=u.GPU)

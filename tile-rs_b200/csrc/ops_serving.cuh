@@ -142,6 +142,9 @@ inline int32_t attention_paged(std::string* err, const tsm100_paged_kv* kv, cons
   return attention_paged_any(err, p, d->dtype == TSM100_BF16, kv->dtype == TSM100_I8, q, o, static_cast<cudaStream_t>(stream));
 }
 
+// Records, and routes, by max_new: no sequence has more tokens than the call, whatever the caller allows.
+inline void bound_new(paged::Params* p) { p->step.max_new = std::min(p->step.max_new, p->step.tokens); }
+
 inline int32_t attention_paged_cross(std::string* err, const tsm100_paged_kv* kv, const tsm100_paged_batch* b, const tsm100_attention_paged_desc* d, const void* q,
                                      void* o, uint32_t* status, void* stream) {
   if (!d) return op_fail(err, TSM100_ERR_INVALID, "attention_paged_cross: null descriptor");
@@ -151,6 +154,7 @@ inline int32_t attention_paged_cross(std::string* err, const tsm100_paged_kv* kv
   if (st != TSM100_OK || nothing) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = d->dtype == TSM100_BF16;
+  bound_new(&p);
   return kv->dtype == TSM100_I8 ? attention_cross_held<true>(err, p, bf16, q, o, s) : attention_cross_held<false>(err, p, bf16, q, o, s);
 }
 
@@ -170,11 +174,12 @@ inline int32_t attention_paged_prefix(std::string* err, const tsm100_paged_kv* k
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = d->dtype == TSM100_BF16, i8 = kv->dtype == TSM100_I8;
   if (d->prefix_len == 0) return attention_paged_any(err, p, bf16, i8, q, o, s);
+  bound_new(&p);
   PrefixPlan plan;
   plan.run_log2 = page_run_log2(kv->page_size, 7);
   const bool tc = paged_fits_tcgen05(p.group, i8, plan.run_log2);
   plan.shared_tc = tc && route::prefix_on_tcgen05(static_cast<int64_t>(b->tokens) * p.group, d->prefix_len, kv->heads_kv, kv->head_dim, i8);
-  plan.rest_tc = tc && static_cast<int64_t>(b->max_new) * p.group > route::kPrefixFewRows;
+  plan.rest_tc = tc && static_cast<int64_t>(p.step.max_new) * p.group > route::kPrefixFewRows;
   PrefixArgs more = {};
   more.large = plan.rest_tc ? static_cast<int32_t>(route::kPrefixFewRows) : 0;
   more.prefix = d->prefix_len, more.table = d->prefix;
