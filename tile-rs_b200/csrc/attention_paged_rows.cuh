@@ -23,8 +23,11 @@ enum Keys { kPast, kAll, kShared, kRest, kBoth };
 // kAll, kRest and kBoth here, kAll, kShared and kRest on tcgen05.  The last three leave records, which attention_paged_join_kernel puts together; here kAll does too.
 __host__ __device__ constexpr bool leaves_records(Keys k) { return k == kShared || k == kRest || k == kBoth; }
 
-// Records of rows: D numbers of O, not normalised, the logarithm to base 2 of what the weights were taken against, their sum, two unused.  A unit (or block) of rows that one
+// Records of rows: D numbers of O, not normalised, the logarithm to base 2 of what the weights were taken against, their sum, six unused, so that rows start on the 32 bytes
+// that memory is written by (with two and stores of 16 bytes 64 sequences behind 16384 positions in 8 bits took 104.0 us, so 101.6).  A unit (or block) of rows that one
 // share has all of leaves them in `whole`, by token and head; one that is cut, in the shares' places, which `cut` tells by the unit.
+template <int D>
+constexpr int kRecord = D + 8;
 struct Records {
   float* whole;       // [tokens][heads_q]
   float* part;        // [share][2][held], of a unit that began in an earlier share, of one that goes on in the next
@@ -82,7 +85,7 @@ struct RowsTile {
   static constexpr int kRowBytes = kI8 ? D : 2 * D;
   static constexpr int kPos = kBytes / kRowBytes;         // 16, 32 or 64 positions
   static constexpr int kSlots = kWide ? 6 : 4;            // per warp
-  static constexpr int kRec = D + 4;                      // floats of a row's record
+  static constexpr int kRec = kRecord<D>;                 // floats of a row's record
   static constexpr int kScales = kI8 ? kPos * 4 : 0;      // bytes beside a slot
   static constexpr int kSmem = kWarps * kSlots * (kBytes + kScales) + kWarps * kSlots * 8 + 1024;
   static_assert(kSmem + 2048 + 160 * kWarps <= 227 * 1024, "shared memory of one CTA, with what is declared in the kernel");
@@ -649,7 +652,7 @@ struct Pieces {
 // (Tokens times heads fit 31 bits, so the rows of a KV head and all of them do.)
 template <int D>
 __device__ __forceinline__ Pieces pieces(const Records& rec, int tile_tokens, uint32_t held, int64_t cut0, uint32_t head, uint32_t group, uint32_t token, uint32_t h, uint32_t row) {
-  constexpr uint32_t REC = D + 4;
+  constexpr uint32_t REC = kRecord<D>;
   uint32_t unit, r;
   if (tile_tokens > 0) {
     unit = token / (2 * tile_tokens);

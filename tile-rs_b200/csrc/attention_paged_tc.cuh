@@ -764,7 +764,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
         [[maybe_unused]] uint16_t* orow = o + row * D;
         [[maybe_unused]] float* record = nullptr;
         if constexpr (leaves_records(kKeysSeen))
-          record = whole ? p.records.whole + (row_ok ? row : 0) * (D + 4) : p.records.part + (rec * 256 + g * kTileRows + r) * (D + 4);
+          record = whole ? p.records.whole + (row_ok ? row : 0) * kRecord<D> : p.records.part + (rec * 256 + g * kTileRows + r) * kRecord<D>;
 #pragma unroll 1
         for (int q = 0; q < D / 32; ++q) {
           uint32_t ov[32];
@@ -778,9 +778,7 @@ attention_paged_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gr
           if constexpr (leaves_records(kKeysSeen)) {
             if (row_ok) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                reinterpret_cast<float4*>(record + q * 32)[i] =
-                    make_float4(__uint_as_float(ov[4 * i]), __uint_as_float(ov[4 * i + 1]), __uint_as_float(ov[4 * i + 2]), __uint_as_float(ov[4 * i + 3]));
+              for (int i = 0; i < 4; ++i) ptx::st_global_v8(record + q * 32 + i * 8, ov + i * 8);
             }
           } else if (whole) {
             if (row_ok) {

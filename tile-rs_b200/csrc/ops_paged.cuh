@@ -352,7 +352,7 @@ struct PrefixPlan {
 template <typename T, bool kI8, int D>
 inline int32_t attention_prefix_launch(std::string* err, const paged::Params& p, const PrefixPlan& plan, PrefixArgs more, const void* q, void* o, cudaStream_t s) {
   namespace pg = paged;
-  constexpr size_t REC = D + 4;
+  constexpr size_t REC = pg::kRecord<D>;
   int sms = 0;
   int32_t st = sm_count(err, &sms);
   if (st != TSM100_OK) return st;

@@ -408,6 +408,11 @@ __device__ __forceinline__ void tcgen05_mma_i8_ss_pair(uint32_t d_tmem, uint64_t
       : "memory");
 }
 
+// 32 bytes, on a boundary of as many.
+__device__ __forceinline__ void st_global_v8(void* to, const uint32_t* x) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
+}
+
 // ---------------------------------------------------------------------------
 // tcgen05.mma descriptors
 // ---------------------------------------------------------------------------
