@@ -149,9 +149,10 @@ int32_t tsm100_launch(tsm100_module_t mod, const char* name, uint32_t blocks, vo
  *   more than 16, else up to 2.5 MB;
  *   tsm100_gemm_w4, more than 64 rows in 8 bits: 2 bytes per element of A; more than 1024 rows in 16 bits, N >= 2048 and K >= 512: 2 per element of W,
  *   and of C where its rows do not start on 16-byte boundaries;
- *   tsm100_attention_paged_cross: as tsm100_attention_paged for more than 16 rows, else 4 (d + 8) bytes for each token and query head, and up to 20 MB for heads of 128, 10 MB for 64;
- *   tsm100_attention_paged_prefix: 8 (d + 8) bytes for each token and query head and 20 MB (10 for heads of 64), 40 (21) more where the prefix has many rows, and as many again
- *   where a sequence has more than 64;
+ *   tsm100_attention_paged_cross: as tsm100_attention_paged for more than 16 rows, else 4 (d + 8) bytes for each token and query head, and up to 21 MB for heads of 128, 11 MB for 64,
+ *   and 8 bytes for every 8 rows that a sequence may have, by max_new and by the call's tokens, of each sequence and KV head;
+ *   tsm100_attention_paged_prefix: 8 (d + 8) bytes for each token and query head and 21 MB (11 for heads of 64), 41 (22) more where the prefix has many rows, and as many again
+ *   where a sequence has more than 64; places of 8 bytes as there;
  *   tsm100_gemm_i8, rows of a or w that do not start on 16-byte boundaries: a copy of a, of w, or of both.
  * It is taken and returned on the caller's stream, from a pool of the library's own on each device (the device's default
  * memory pool is neither used nor changed).  The pool keeps up to 1/16 of the device's memory for later calls and gives it
