@@ -417,7 +417,8 @@ typedef struct {
 int32_t tsm100_gemm_w4(tsm100_device_t dev, const tsm100_gemm_w4_desc* desc, const void* a, const float* a_scales, const uint8_t* w,
                        const void* w_scales, const uint8_t* w_zeros, void* c, void* stream);
 
-/* Rows as whole numbers and steps, where no norm before a product leaves them: v = x, or with `up` v = silu(x) * up, silu(x) = x / (1 + exp(-x)), in f32;
+/* Rows as whole numbers and steps, where no norm before a product leaves them: v = x, or with `up` v = silu(x) * up, silu(x) = x / (1 + exp(-x)), in f32
+ * (off by 2^-20 of v and, where x is negative, another |x| 2^-23.6 of it at most; below x = -88.7, where exp(-x) overflows, v is 0);
  * y[rows][cols] = the whole numbers of v, scales[rows] their steps.  x and up have `pitch` elements from row to row (0: cols), so that gate and up may
  * lie side by side in the rows of one product; y is packed.  No overlap of y with x or up.  Rows may start anywhere. */
 typedef struct {

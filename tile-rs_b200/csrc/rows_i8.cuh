@@ -37,13 +37,15 @@ __device__ __forceinline__ float row_max(uint32_t top, uint32_t* red) {
   top = (threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0u;
   return __uint_as_float(__reduce_max_sync(0xffffffffu, top));
 }
-// silu(x) * up, within 2^-20 of it where x is above -16 (and ten units more below the largest of any row that has an x above 0): the exponential and the reciprocal are the
-// approximate ones, 2^-22 and 2^-23 off, because exact ones are twenty more instructions and 8192 rows of 14336 bf16 took 170 us with them, 119 so (4.9 TB/s).
+// silu(x) * up, off by 2^-20 of itself and for a negative x another |x| 2^-23.6 of itself at most: x * log2(e) is rounded to f32 (|x| 1.25 2^-24 of the exponential, with the constant), the
+// exponential and the reciprocal are the approximate ones, 2^-22 and 2^-23 off, because exact ones are twenty more instructions and 8192 rows of 14336 bf16 took 170 us with them,
+// 114 so (5.1 TB/s).  rcp.approx makes 0 of results below 2^-126, which 1 / (1 + exp(-x)) is from x = -87.3 down while exp(-x) is finite (-88.7): so it is
+// taken of 2^-32 (1 + exp(-x)), and 2^-32 times that still has 21 bits there.  Further down the exponential overflows and the value is 0, as the formula's is in f32.
 __device__ __forceinline__ float gated(float x, float up) {
   const float e = ptx::ex2_approx(x * -1.4426950408889634f);
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return x * r * up;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(e, 0x1p-32f, 0x1p-32f)));
+  return x * (r * 0x1p-32f) * up;
 }
 
 // Every row on 16-byte boundaries (y: on as many bytes as a vector has elements); VPT vectors a thread, a warp a row (kWarp) or a CTA of as many warps as the row fills.
