@@ -458,7 +458,7 @@ typedef struct {
 
 /* Sequences of uneven length, side by side: tokens starts[b] .. starts[b+1]-1 of the call are the last ones of sequence b, which has
  * lens[b] positions with them; position p of it lies in page table[b][p / page_size].  The arrays are in device memory and are read when the call's
- * kernels run.  A sequence with more positions than its row of the table has room for, more than max_new tokens, or more tokens than
+ * kernels run.  A sequence with more positions than its row of the table has room for (or than 2^31 - 4096), more than max_new tokens, or more tokens than
  * positions, is left out; what a table entry outside 0 .. pages-1 stands for is not written, and a result that reads it means nothing.  Nothing
  * outside the buffers is touched, other sequences are served, and the next tsm100_stream_synchronize, or operator on host memory, answers TSM100_ERR_INVALID (status
  * 0x2000|site).  Tokens from starts[batch] on belong to no sequence and are left alone. */

@@ -13,6 +13,8 @@ namespace tsm100 {
 namespace pages {
 
 constexpr uint32_t kStatusOutside = 0x2000u;  // | site: a page, a position or a sequence outside what the call described
+// Positions of a sequence at most: kernels add a tile, a warp's copies or what a block costs (up to 1984) to positions in 32 bits.
+constexpr int32_t kMostPositions = 0x7fffffff - 4095;
 
 struct Cache {
   int32_t heads, d, page_size;
@@ -38,7 +40,7 @@ __device__ __forceinline__ bool sequence(const Batch& s, int64_t page_size, int 
   count = s.starts[b + 1] - first;
   len = s.lens[b];
   if (count == 0) return false;
-  if (first < 0 || count < 0 || count > s.max_new || first > s.tokens - count || len < (kOwn ? count : 0) || len > page_size * s.pitch) {
+  if (first < 0 || count < 0 || count > s.max_new || first > s.tokens - count || len < (kOwn ? count : 0) || len > kMostPositions || len > page_size * s.pitch) {
     report(status, site);
     return false;
   }
