@@ -268,9 +268,12 @@ inline int32_t attention_rows_launch(std::string* err, const paged::Params& base
 // `records`: about how many a row has.
 template <typename T, int D>
 inline int32_t attention_join_launch(std::string* err, const paged::Join& join, int64_t records, void* o, cudaStream_t s) {
+  int sms = 0;
+  const int32_t st = sm_count(err, &sms);
+  if (st != TSM100_OK) return st;
   auto go = [&](auto kern, int splits, int threads) {
-    const int64_t at_once = threads / (D / 4) / splits, ys = (static_cast<int64_t>(join.step.max_new) * join.heads_q + at_once - 1) / at_once;
-    const dim3 grid(static_cast<unsigned>(join.step.batch), static_cast<unsigned>(std::min<int64_t>(ys, 64)));
+    const int64_t at_once = threads / (D / 4) / splits, rows = static_cast<int64_t>(join.step.max_new) * join.heads_q;
+    const dim3 grid(static_cast<unsigned>(join.step.batch), static_cast<unsigned>(route::join_ctas(rows, at_once, join.step.batch, 1024 / threads, sms)));
     return cuda_ok(err, launch_chained(kern, grid, threads, 0, s, 0, static_cast<T*>(o), join), "attention_paged_join_kernel launch");
   };
   return records > 40 ? go(paged::attention_paged_join_kernel<T, D, 16>, 16, paged::kJoinThreads<16>) : go(paged::attention_paged_join_kernel<T, D, 4>, 4, paged::kJoinThreads<4>);

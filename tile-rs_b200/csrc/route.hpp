@@ -343,6 +343,11 @@ inline bool prefix_on_tcgen05(int64_t rows, int64_t prefix, int heads_kv, int he
 }
 // Rows of a sequence's own tokens beyond which its own positions are tcgen05's.
 constexpr int64_t kPrefixFewRows = 64;
+// CTAs that join the records of a sequence, of up to `rows` rows, `at_once` to a CTA and pass: 64, no more, so that many sequences' CTAs begin and end seldom, but all that the SMs hold where there are
+// few sequences (with 64 in any case one of 2048 tokens and 32 heads on 4096 positions took 1473 us, 356 so; one of 512 381 and 110; two of 4096 3447 and 1475).
+inline int64_t join_ctas(int64_t rows, int64_t at_once, int64_t batch, int ctas_per_sm, int sms) {
+  return std::min(div_up(rows, at_once), std::max<int64_t>(64, div_up(static_cast<int64_t>(ctas_per_sm) * sms, batch)));
+}
 
 // Rotary embedding: how many heads a thread walks through (`blocks` blocks of 256 threads for one head group).  Few tokens: groups of four
 // heads or more, as many as make two blocks per SM; the angles are computed once per group.  With a block for every second SM that
