@@ -134,7 +134,8 @@ inline int32_t attention_paged_tc_launch(std::string* err, const paged::Params& 
     const size_t rows = static_cast<size_t>(ctas) * 2 * 256, part = rows * D * sizeof(float), ml = rows * sizeof(float2);
     uint8_t* ws = nullptr;
     st = take_scratch(err, reinterpret_cast<void**>(&ws), part + ml + ctas * sizeof(int4), s);
-    if (st == kNoScratch) return op_fail(err, TSM100_ERR_MEMORY, "attention_paged: no device memory for partial results");
+    if (st == kNoScratch)
+      return op_fail(err, TSM100_ERR_MEMORY, kKeys == paged::kAll ? "attention_paged_cross: no device memory for partial results" : "attention_paged: no device memory for partial results");
     if (st != TSM100_OK) return st;
     p.part = reinterpret_cast<float4*>(ws);
     p.part_ml = reinterpret_cast<float2*>(ws + part);
@@ -308,7 +309,7 @@ inline paged::Join join_of(const paged::Params& p) {
   return x;
 }
 
-// Every token against all positions of its sequence (serving_cross.cu).
+// Every token against all positions of its sequence (serving_cross_16bit.cu, serving_cross_i8.cu).
 template <typename T, bool kI8, int D, bool kWide>
 inline int32_t attention_cross_rows(std::string* err, const paged::Params& p, const void* q, void* o, cudaStream_t s) {
   using L = paged::RowsTile<kI8, D, kWide>;
