@@ -527,6 +527,8 @@ attention_paged_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
             for (int n = 0; n < NB; ++n) s[j][n][2 * h] *= x, s[j][n][2 * h + 1] *= x;
           }
       }
+      // Rounded to what the products take, 16 bits: the tensor core's other types are slower, and results are 1.67e-3 to 1.78e-3 from 64 bits in bf16, whose own rounding is 1.65e-3, and
+      // 2.1e-4 to 2.3e-4 in f16 (2.07e-4).  The sums above are of what was not rounded.
       uint32_t pb[N16][NB][2], rest[kTwoParts ? N16 : 1][NB][2];
 #pragma unroll
       for (int j = 0; j < N16; ++j)
