@@ -14,6 +14,8 @@
 //     probabilities, so that nothing but the probabilities is rounded (with K and V times their steps rounded, errors were 1.6 times as large), and those to f16, whatever q's type
 //     is.  They keep their bits by a power of two that follows the largest step and is taken out again with the sum.
 //     (Sums of queries times whole numbers are f32 before K's step comes to them: queries end at 2^114.)
+//   * Probabilities are rounded to 16 bits, which P V takes them in; their sum is of unrounded ones.  Cross attention in f16 is 2.5e-4 from 64 bits where rounding the result alone
+//     makes 2.1e-4, on a shared prefix in bf16 1.8e-3 to 2.0e-3 where it makes 1.65e-3.
 // Bound: the tensor core and the exponentials, as there.
 #pragma once
 
